@@ -114,6 +114,29 @@ SIGNATURES = [
                                      c_longlong, c_int, c_int, c_int, c_void_p, c_void_p,
                                      c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                      c_void_p, c_int, c_void_p]),
+    ("b2a_page_plan", c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
+    ("b2a_rope_append_paged", c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p,
+                                      c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_int, c_int, c_longlong, c_int, c_void_p, c_int, c_int,
+                                      c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    ("b2a_tree_decode_workspace_bytes", c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    ("b2a_tree_decode", c_int, [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_longlong,
+                                c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int,
+                                c_int, c_int, c_int, c_float, c_int, c_void_p]),
+    ("b2a_constrain_logits_workspace_bytes", c_size_t, [c_int, c_int]),
+    ("b2a_constrain_logits", c_int, [c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int,
+                                     c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    ("b2a_tree_commit", c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_longlong, c_int, c_void_p, c_void_p, c_int, c_longlong, c_int,
+                                c_int, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
 ]
 
 _lib = None

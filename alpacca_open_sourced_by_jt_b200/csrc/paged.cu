@@ -1,0 +1,567 @@
+// A paged KV cache for many requests: block tables and slot maps built on the
+// GPU, RoPE + append by slot, and the commit of a draft tree's accepted path.
+
+#include <limits.h>
+
+#include <type_traits>
+
+#include "b2a_common.cuh"
+
+namespace b2a {
+namespace paged {
+
+constexpr int kMaxNodes = B2A_TREE_MAX_NODES;
+
+// ---------------------------------------------------------------------------
+// Block tables, slot map, positions (b2a_page_plan)
+// ---------------------------------------------------------------------------
+// All of it follows from three prefix sums over the requests (tokens, pages
+// to take, pages to give back).  Every CTA forms them itself (a few
+// microseconds for hundreds of requests, and no second launch), then writes
+// its share: a warp per request for table entries and returned pages, a
+// thread per 4 tokens for the slot map.  Pages taken come from the ring's
+// head and pages given back go to its tail: the two regions do not meet
+// while free and held pages together fit the ring, so CTAs need no order.
+constexpr int kPlanThreads = 256;
+constexpr int kPlanTokens = kPlanThreads * 4;  // tokens of a CTA
+
+struct Plan {
+  const int *lens, *add, *parents, *held;
+  int* table;
+  long long table_stride;
+  int* ring;
+  const int* state;
+  int *held_out, *state_out, *cu, *seq, *pos, *slot;
+  int B, max_tokens, max_pages, page_shift, ring_size;
+};
+
+// Tokens, pages wanted from the ring and pages given back of request b.
+__device__ __forceinline__ void plan_request(const Plan& p, int b, int& n, int& need, int& back,
+                                             bool& fits) {
+  const int add = p.add[b], len = p.lens[b], held = p.held[b];
+  const bool bad = len < 0 || held < 0 || held > p.max_pages;
+  n = add < 0 ? 0 : min(add, p.max_tokens + 1);
+  const long long want = (static_cast<long long>(len) + n + (1 << p.page_shift) - 1) >> p.page_shift;
+  fits = add >= 0 && !bad && want <= p.max_pages;
+  need = fits ? max(0, static_cast<int>(want) - held) : 0;
+  back = add < 0 && !bad ? held : 0;
+  if (bad) set_dev_error(B2A_ERR_POSITION, b);
+}
+
+__device__ __forceinline__ int clamp_int(long long x) {
+  return x > INT_MAX ? INT_MAX : static_cast<int>(x);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_constant__ Plan p) {
+  pdl_wait();
+  extern __shared__ int psm[];
+  int* s_cu = psm;               // [B + 1] tokens before request b
+  int* s_need = s_cu + p.B + 1;  // [B + 1] pages taken before request b
+  int* s_back = s_need + p.B + 1;  // [B + 1] pages given back before request b
+  __shared__ long long s_part[3][kPlanThreads / 32];
+  __shared__ long long s_run[3];
+  __shared__ int s_par[kPlanTokens + kMaxNodes];
+  __shared__ int s_taken;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int kWarps = kPlanThreads / 32;
+  const int gw = blockIdx.x * kWarps + warp, n_warps = gridDim.x * kWarps;
+  // (kept inside the ring whatever the state holds)
+  const int head = static_cast<int>(static_cast<unsigned>(p.state[0]) % static_cast<unsigned>(p.ring_size));
+  const int count = min(max(p.state[1], 0), p.ring_size);
+  if (tid < 3) s_run[tid] = 0;
+  if (tid == 0) s_taken = 0;
+  __syncthreads();
+  // the prefix sums, kPlanThreads requests at a time
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int n = 0, need = 0, back = 0;
+    bool fits = false;
+    if (b < p.B) plan_request(p, b, n, need, back, fits);
+    long long v[3] = {n, need, back}, inc[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      inc[k] = v[k];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, inc[k], o);
+        if (lane >= o) inc[k] += x;
+      }
+      if (lane == 31) s_part[k][warp] = inc[k];
+    }
+    __syncthreads();
+    long long before[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      before[k] = s_run[k];
+      for (int w = 0; w < warp; ++w) before[k] += s_part[k][w];
+      before[k] += inc[k] - v[k];
+    }
+    if (b < p.B) {
+      s_cu[b] = clamp_int(before[0]);
+      s_need[b] = clamp_int(before[1]);
+      const long long upto = before[1] + need;
+      const bool served = fits && (need == 0 || upto <= count);
+      if (served && need > 0) atomicMax(&s_taken, static_cast<int>(upto));
+      if (blockIdx.x == 0) {
+        p.cu[b] = clamp_int(before[0]);
+        p.held_out[b] = p.add[b] < 0 ? p.held[b] - back : p.held[b] + (served ? need : 0);
+      }
+      s_back[b] = clamp_int(before[2]);
+    }
+    __syncthreads();
+    if (tid < 3) {
+      long long t = s_run[tid];
+      for (int w = 0; w < kWarps; ++w) t += s_part[tid][w];
+      s_run[tid] = t;
+    }
+    __syncthreads();
+  }
+  const int total = clamp_int(s_run[0]);
+  if (tid == 0) {
+    s_cu[p.B] = total;
+    s_need[p.B] = clamp_int(s_run[1]);
+    s_back[p.B] = clamp_int(s_run[2]);
+    if (blockIdx.x == 0) {
+      p.cu[p.B] = total;
+      p.state_out[0] = static_cast<int>((static_cast<long long>(head) + s_taken) % p.ring_size);
+      p.state_out[1] = clamp_int(static_cast<long long>(count) - s_taken + s_run[2]);
+      if (total > p.max_tokens) set_dev_error(B2A_ERR_POSITION, total);
+    }
+  }
+  __syncthreads();
+  // new table entries, and pages given back
+  for (int b = gw; b < p.B; b += n_warps) {
+    const int back = s_back[b + 1] - s_back[b];
+    for (int j = lane; j < back; j += 32)
+      p.ring[(static_cast<long long>(head) + count + s_back[b] + j) % p.ring_size] =
+          p.table[b * p.table_stride + j];
+    const int lo = s_need[b], need = s_need[b + 1] - lo;
+    if (need == 0 || s_need[b + 1] > count) continue;
+    const int held = p.held[b];
+    for (int k = lane; k < need; k += 32)
+      p.table[b * p.table_stride + held + k] = p.ring[(static_cast<long long>(head) + lo + k) % p.ring_size];
+  }
+  // tokens
+  const int t0 = blockIdx.x * kPlanTokens;
+  if (t0 >= p.max_tokens) return;
+  auto find = [&](int t) {  // the request that holds token t < total
+    int lo = 0, hi = p.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_cu[mid] <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  };
+  int par0 = 0;
+  if (p.parents) {
+    // the tile's parents, from the first node of the tree that it cuts
+    const int end = min(min(t0 + kPlanTokens, p.max_tokens), total);
+    if (t0 < total) par0 = max(s_cu[find(t0)], t0 - kMaxNodes);
+    for (int i = tid; par0 + i < end; i += kPlanThreads) s_par[i] = p.parents[par0 + i];
+    __syncthreads();
+  }
+  const int first = t0 + tid * 4;
+  int b = first < total ? find(first) : 0;
+  int sq[4], ps[4], sl[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int t = first + e;
+    sq[e] = -1;
+    ps[e] = 0;
+    sl[e] = -1;
+    if (t >= total || t >= p.max_tokens) continue;
+    while (t >= s_cu[b + 1]) ++b;
+    const int i = t - s_cu[b];
+    const int len = p.lens[b], held = p.held[b];
+    int depth = i;
+    if (p.parents) {
+      depth = 0;
+      int at = i;
+      const int base = s_cu[b] - par0;
+      if (i >= kMaxNodes) {
+        set_dev_error(B2A_ERR_POSITION, b);
+      } else {
+        while (true) {
+          const int up = s_par[base + at];
+          if (up < 0 || up >= at) {
+            if (up != -1) set_dev_error(B2A_ERR_POSITION, b);
+            break;
+          }
+          at = up;
+          ++depth;
+        }
+      }
+    }
+    sq[e] = b;
+    ps[e] = len + depth;
+    const int lo = s_need[b], need = s_need[b + 1] - lo;
+    int n_, need_, back_;
+    bool fits;
+    plan_request(p, b, n_, need_, back_, fits);
+    if (fits && (need == 0 || s_need[b + 1] <= count)) {
+      const int row = len + i, pg = row >> p.page_shift;
+      const int page = pg < held ? p.table[b * p.table_stride + pg]
+                                 : p.ring[(static_cast<long long>(head) + lo + pg - held) % p.ring_size];
+      sl[e] = (page << p.page_shift) + (row & ((1 << p.page_shift) - 1));
+    }
+  }
+  if (first + 3 < p.max_tokens) {
+    *reinterpret_cast<int4*>(p.seq + first) = make_int4(sq[0], sq[1], sq[2], sq[3]);
+    *reinterpret_cast<int4*>(p.pos + first) = make_int4(ps[0], ps[1], ps[2], ps[3]);
+    *reinterpret_cast<int4*>(p.slot + first) = make_int4(sl[0], sl[1], sl[2], sl[3]);
+  } else {
+    for (int e = 0; e < 4; ++e)
+      if (first + e < p.max_tokens) {
+        p.seq[first + e] = sq[e];
+        p.pos[first + e] = ps[e];
+        p.slot[first + e] = sl[e];
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// RoPE + append by slot (b2a_rope_append_paged)
+// ---------------------------------------------------------------------------
+// One element pair per thread and step; products and sums are rounded one by
+// one, as rope_append.cu does.
+template <typename TS, typename TK, typename TQ>
+__global__ void __launch_bounds__(256) rope_paged_kernel(
+    const TS* __restrict__ q, long long q_stride, const TS* __restrict__ k, long long k_stride,
+    const TS* __restrict__ v, long long v_stride, const float* __restrict__ bq,
+    const float* __restrict__ bk, const float* __restrict__ bv, const float* __restrict__ cos_tab,
+    const float* __restrict__ sin_tab, int tab_rows, const int* __restrict__ pos,
+    const int* __restrict__ slots, TK* __restrict__ k_pool, TK* __restrict__ v_pool,
+    int page_shift, long long page_stride, long long n_slots, TQ* __restrict__ q_out, int H,
+    int KV, int D, int n_rot, int neox) {
+  pdl_wait();
+  const int i = blockIdx.x;
+  const int p = pos[i];
+  const int slot = slots[i];
+  if (p < 0 || p >= tab_rows || slot >= n_slots) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) set_dev_error(B2A_ERR_POSITION, i);
+    return;
+  }
+  const int half = n_rot >> 1;
+  const size_t row = slot < 0 ? 0 : static_cast<size_t>(slot >> page_shift) * page_stride +
+                                        static_cast<size_t>(slot & ((1 << page_shift) - 1)) * KV * D;
+  const int per = D >> 1;
+  for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < (H + 2 * KV) * per;
+       u += gridDim.y * blockDim.x) {
+    const int head = u / per, t = u - head * per;
+    const bool is_q = head < H, is_v = head >= H + KV;
+    const int h = is_q ? head : (is_v ? head - H - KV : head - H);
+    if (!is_q && slot < 0) continue;
+    const TS* src = is_q ? q + i * q_stride + h * D : (is_v ? v + i * v_stride : k + i * k_stride) + h * D;
+    const float* bias = is_q ? bq : (is_v ? bv : bk);
+    int a = 2 * t, b = 2 * t + 1;
+    const bool turn = !is_v && t < half;
+    if (turn && neox) {
+      a = t;
+      b = t + half;
+    }
+    float x0 = ld_elem(src + a), x1 = ld_elem(src + b);
+    if (bias) {
+      x0 = __fadd_rn(x0, bias[h * D + a]);
+      x1 = __fadd_rn(x1, bias[h * D + b]);
+    }
+    float y0 = x0, y1 = x1;
+    if (turn) {
+      const float c = cos_tab[static_cast<size_t>(p) * half + t];
+      const float s = sin_tab[static_cast<size_t>(p) * half + t];
+      y0 = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
+      y1 = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
+    }
+    if (is_q) {
+      TQ* dst = q_out + (static_cast<size_t>(i) * H + h) * D;
+      st_elem(dst + a, y0);
+      st_elem(dst + b, y1);
+    } else {
+      TK* dst = (is_v ? v_pool : k_pool) + row + h * D;
+      st_elem(dst + a, y0);
+      st_elem(dst + b, y1);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Accepted path and row moves (b2a_tree_commit)
+// ---------------------------------------------------------------------------
+// From the root, the path goes on to the first child whose token is the
+// node's pick.  Warp 0 of every CTA walks it (each step is one ballot over
+// the request's nodes), then each thread moves one 16-byte column of the
+// path's rows, in path order: the row at depth d comes from node path[d] >= d,
+// so no row is overwritten before it was read.
+constexpr int kCommitThreads = 256;
+
+struct Commit {
+  const int *picks, *tokens, *parents, *cu, *lens, *table;
+  long long table_stride;
+  unsigned char *k, *v;
+  long long layer_bytes, page_bytes;
+  int row_bytes, n_layers, n_pages, page_shift;  // page_shift < 0: one block per sequence
+  int max_len, n_tok, max_nodes;
+  int *path, *accepted, *next, *lens_out;
+};
+
+__global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __grid_constant__ Commit c) {
+  pdl_wait();
+  __shared__ int s_path[kMaxNodes];
+  __shared__ long long s_src[kMaxNodes], s_dst[kMaxNodes];
+  __shared__ int s_n;
+  const int b = blockIdx.y;
+  const int lane = threadIdx.x & 31;
+  const int c0 = c.cu[b], n = c.cu[b + 1] - c0, len = c.lens[b];
+  const bool bad = n < 0 || n > c.max_nodes || c0 < 0 || c0 + n > c.n_tok || len < 0 ||
+                   len > c.max_len - n;
+  if (threadIdx.x < 32) {
+    int par[kMaxNodes / 32], tok[kMaxNodes / 32];
+#pragma unroll
+    for (int w = 0; w < kMaxNodes / 32; ++w) {
+      const int j = w * 32 + lane;
+      const bool in = !bad && j < n;
+      par[w] = in ? (c.parents ? c.parents[c0 + j] : j - 1) : -2;
+      tok[w] = in ? c.tokens[c0 + j] : 0;
+    }
+    int len_path = 0, cur = 0, last = -1;
+    if (!bad && n > 0) {
+      while (true) {
+        if (lane == 0) s_path[len_path] = cur;
+        ++len_path;
+        last = c.picks[c0 + cur];
+        int nxt = -1;
+#pragma unroll
+        for (int w = 0; w < kMaxNodes / 32; ++w) {
+          const int j = w * 32 + lane;
+          const unsigned hit = __ballot_sync(0xffffffffu, par[w] == cur && j > cur && tok[w] == last);
+          if (nxt < 0 && hit) nxt = w * 32 + __ffs(hit) - 1;
+        }
+        if (nxt < 0) break;
+        cur = nxt;
+      }
+    }
+    __syncwarp();
+    if (blockIdx.x == 0) {
+      for (int d = lane; d < c.max_nodes; d += 32)
+        c.path[static_cast<size_t>(b) * c.max_nodes + d] = d < len_path ? s_path[d] : -1;
+      if (lane == 0) {
+        c.accepted[b] = len_path;
+        c.next[b] = last;
+        c.lens_out[b] = len + len_path;
+        if (bad) set_dev_error(B2A_ERR_POSITION, b);
+      }
+    }
+    for (int d = lane; d < len_path; d += 32) {
+      const int from = len + s_path[d], to = len + d;
+      long long src = -1, dst = -1;
+      if (from != to) {
+        if (c.page_shift < 0) {
+          src = b * c.page_bytes + static_cast<long long>(from) * c.row_bytes;
+          dst = b * c.page_bytes + static_cast<long long>(to) * c.row_bytes;
+        } else {
+          const int pf = c.table[b * c.table_stride + (from >> c.page_shift)];
+          const int pt = c.table[b * c.table_stride + (to >> c.page_shift)];
+          const int mask = (1 << c.page_shift) - 1;
+          if (pf < 0 || pf >= c.n_pages || pt < 0 || pt >= c.n_pages) {
+            set_dev_error(B2A_ERR_POSITION, b);
+          } else {
+            src = pf * c.page_bytes + static_cast<long long>(from & mask) * c.row_bytes;
+            dst = pt * c.page_bytes + static_cast<long long>(to & mask) * c.row_bytes;
+          }
+        }
+      }
+      s_src[d] = src;
+      s_dst[d] = dst;
+    }
+    if (lane == 0) s_n = len_path;
+  }
+  __syncthreads();
+  const int m = s_n;
+  const int chunks = c.row_bytes >> 4;
+  const int cols = c.n_layers * 2 * chunks;
+  for (int u = blockIdx.x * kCommitThreads + threadIdx.x; u < cols; u += gridDim.x * kCommitThreads) {
+    const int row = u / chunks, at = u - row * chunks;
+    unsigned char* base = ((row & 1) ? c.v : c.k) + (row >> 1) * c.layer_bytes + at * 16;
+    for (int d = 0; d < m; ++d) {
+      if (s_src[d] < 0) continue;
+      const uint4 x = *reinterpret_cast<const uint4*>(base + s_src[d]);
+      *reinterpret_cast<uint4*>(base + s_dst[d]) = x;
+    }
+  }
+}
+
+}  // namespace paged
+}  // namespace b2a
+
+// ===========================================================================
+// Host side
+// ===========================================================================
+namespace {
+
+namespace PG = b2a::paged;
+
+template <typename TS, typename TK, typename TQ>
+cudaError_t rope_paged_launch(const void* q, long long qs, const void* k, long long ks,
+                              const void* v, long long vs, const float* bq, const float* bk,
+                              const float* bv, const float* cos_tab, const float* sin_tab,
+                              int tab_rows, const int* pos, const int* slots, void* kp, void* vp,
+                              int shift, long long page_stride, long long n_slots, void* qo,
+                              int n_tok, int H, int KV, int D, int n_rot, int neox,
+                              cudaStream_t st) {
+  const int pairs = (H + 2 * KV) * (D / 2);
+  const int gy = (pairs + 255) / 256;
+  return b2a_host::launch(PG::rope_paged_kernel<TS, TK, TQ>, dim3(n_tok, gy), dim3(256), 0, st,
+                          static_cast<const TS*>(q), qs, static_cast<const TS*>(k), ks,
+                          static_cast<const TS*>(v), vs, bq, bk, bv, cos_tab, sin_tab, tab_rows,
+                          pos, slots, static_cast<TK*>(kp), static_cast<TK*>(vp), shift,
+                          page_stride, n_slots, static_cast<TQ*>(qo), H, KV, D, n_rot, neox);
+}
+
+// Calls f with a null pointer of the element type of a dtype code.
+template <typename F>
+auto with_type(int dtype, F&& f) {
+  if (dtype == B2A_F16) return f(static_cast<__half*>(nullptr));
+  if (dtype == B2A_BF16) return f(static_cast<__nv_bfloat16*>(nullptr));
+  return f(static_cast<float*>(nullptr));
+}
+
+}  // namespace
+
+extern "C" {
+
+int b2a_page_plan(const int* lens_dev, const int* add_dev, const int* parents_dev,
+                  const int* held_dev, int* held_out_dev, int* table_dev, long long table_stride,
+                  int* ring_dev, int ring_size, const int* ring_state_dev,
+                  int* ring_state_out_dev, int* cu_dev, int* seq_dev, int* pos_dev, int* slot_dev,
+                  int B, int max_tokens, int max_pages, int page_rows, void* stream) {
+  if (!lens_dev || !add_dev || !held_dev || !held_out_dev || !table_dev || !ring_dev ||
+      !ring_state_dev || !ring_state_out_dev || !cu_dev || !seq_dev || !pos_dev || !slot_dev)
+    return fail(B2A_ERR_ARG, "page_plan: null pointer argument");
+  if (B <= 0 || max_tokens < 0 || max_pages <= 0 || ring_size <= 0)
+    return fail(B2A_ERR_ARG, "page_plan: sizes must be positive (B=%d max_tokens=%d max_pages=%d ring=%d)",
+                B, max_tokens, max_pages, ring_size);
+  if (B > B2A_PLAN_MAX_REQUESTS)
+    return fail(B2A_ERR_UNSUPPORTED, "page_plan: %d requests > %d", B, B2A_PLAN_MAX_REQUESTS);
+  if (!power_of_two(page_rows))
+    return fail(B2A_ERR_SHAPE, "page_plan: page_rows %d is not a power of two", page_rows);
+  if (table_stride < max_pages)
+    return fail(B2A_ERR_SHAPE, "page_plan: table_stride %lld < max_pages %d", table_stride, max_pages);
+  if (held_dev == held_out_dev || ring_state_dev == ring_state_out_dev)
+    return fail(B2A_ERR_ARG, "page_plan: held and ring_state need output buffers of their own");
+  if (static_cast<long long>(ring_size) * page_rows > INT_MAX)
+    return fail(B2A_ERR_UNSUPPORTED, "page_plan: %d pages of %d rows exceed 32-bit slots", ring_size, page_rows);
+  if (!b2a_host::aligned16(seq_dev) || !b2a_host::aligned16(pos_dev) || !b2a_host::aligned16(slot_dev))
+    return fail(B2A_ERR_ALIGN, "page_plan: seq, pos and slot must be 16-byte aligned");
+  PG::Plan p = {lens_dev, add_dev, parents_dev, held_dev, table_dev, table_stride, ring_dev,
+                ring_state_dev, held_out_dev, ring_state_out_dev, cu_dev, seq_dev, pos_dev,
+                slot_dev, B, max_tokens, max_pages, log2_of(page_rows), ring_size};
+  constexpr int kWarps = PG::kPlanThreads / 32;
+  int grid = (max_tokens + PG::kPlanTokens - 1) / PG::kPlanTokens;
+  if (grid < (B + kWarps - 1) / kWarps) grid = (B + kWarps - 1) / kWarps;
+  const int smem = 3 * (B + 1) * static_cast<int>(sizeof(int));
+  const cudaError_t e = b2a_host::launch(PG::page_plan_kernel, dim3(grid), dim3(PG::kPlanThreads),
+                                         smem, static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "page_plan launch");
+}
+
+int b2a_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
+                          long long k_tok_stride, const void* v, long long v_tok_stride,
+                          int in_dtype, const float* bq, const float* bk, const float* bv,
+                          const float* cos_tab, const float* sin_tab, int tab_rows,
+                          const int* pos_dev, const int* slot_dev, void* k_pool, void* v_pool,
+                          int n_pages, int page_rows, long long page_stride, int kv_dtype,
+                          void* q_out, int q_out_dtype, int n_tok, int H, int KV, int D, int n_rot,
+                          int style, void* stream) {
+  if (!q || !k || !v || !cos_tab || !sin_tab || !pos_dev || !slot_dev || !k_pool || !v_pool || !q_out)
+    return fail(B2A_ERR_ARG, "rope_append_paged: null pointer argument");
+  if (n_tok < 0 || H <= 0 || KV <= 0 || D <= 0 || tab_rows <= 0 || n_pages <= 0)
+    return fail(B2A_ERR_ARG, "rope_append_paged: sizes must be positive (n_tok=%d H=%d KV=%d D=%d)",
+                n_tok, H, KV, D);
+  if (D % 2 != 0 || D > 256) return fail(B2A_ERR_UNSUPPORTED, "rope_append_paged: head_dim %d", D);
+  if (n_rot < 0 || n_rot % 2 != 0 || n_rot > D)
+    return fail(B2A_ERR_SHAPE, "rope_append_paged: n_rot %d (even, at most D=%d)", n_rot, D);
+  if (style != B2A_ROPE_NORM && style != B2A_ROPE_NEOX)
+    return fail(B2A_ERR_ARG, "rope_append_paged: style %d", style);
+  const int es = b2a_host::elem_size(in_dtype);
+  if (es == 0 || b2a_host::elem_size(kv_dtype) == 0 || b2a_host::elem_size(q_out_dtype) == 0)
+    return fail(B2A_ERR_DTYPE, "rope_append_paged: dtypes %d, %d, %d", in_dtype, kv_dtype, q_out_dtype);
+  if (!power_of_two(page_rows))
+    return fail(B2A_ERR_SHAPE, "rope_append_paged: page_rows %d is not a power of two", page_rows);
+  const long long page_elems = static_cast<long long>(page_rows) * KV * D;
+  if (page_stride == 0) page_stride = page_elems;
+  if (page_stride < page_elems)
+    return fail(B2A_ERR_SHAPE, "rope_append_paged: page_stride %lld < page_rows*KV*D %lld", page_stride, page_elems);
+  if (q_tok_stride < static_cast<long long>(H) * D || k_tok_stride < static_cast<long long>(KV) * D ||
+      v_tok_stride < static_cast<long long>(KV) * D)
+    return fail(B2A_ERR_SHAPE, "rope_append_paged: token strides overlap the rows");
+  if (n_tok == 0) return B2A_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long n_slots = static_cast<long long>(n_pages) * page_rows;
+  const cudaError_t e = with_type(in_dtype, [&](auto* ts) {
+    return with_type(kv_dtype, [&](auto* tk) {
+      return with_type(q_out_dtype, [&](auto* tq) {
+        using TS = typename std::remove_pointer<decltype(ts)>::type;
+        using TK = typename std::remove_pointer<decltype(tk)>::type;
+        using TQ = typename std::remove_pointer<decltype(tq)>::type;
+        return rope_paged_launch<TS, TK, TQ>(q, q_tok_stride, k, k_tok_stride, v, v_tok_stride, bq,
+                                             bk, bv, cos_tab, sin_tab, tab_rows, pos_dev, slot_dev,
+                                             k_pool, v_pool, log2_of(page_rows), page_stride,
+                                             n_slots, q_out, n_tok, H, KV, D, n_rot,
+                                             style == B2A_ROPE_NEOX, st);
+      });
+    });
+  });
+  return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "rope_append_paged launch");
+}
+
+int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* parents_dev,
+                    const int* cu_dev, const int* lens_dev, const int* table_dev,
+                    long long table_stride, int table_width, void* k_cache, void* v_cache,
+                    int n_layers, long long layer_stride, int n_pages, int page_rows,
+                    long long page_stride, int KV, int D, int dtype, int B, int n_tok,
+                    int max_nodes, int max_len, int* path_dev, int* accepted_dev, int* next_dev,
+                    int* lens_out_dev, void* stream) {
+  if (!picks_dev || !tokens_dev || !cu_dev || !lens_dev || !k_cache || !v_cache || !path_dev ||
+      !accepted_dev || !next_dev || !lens_out_dev)
+    return fail(B2A_ERR_ARG, "tree_commit: null pointer argument");
+  if (n_layers <= 0 || n_pages <= 0 || page_rows <= 0 || KV <= 0 || D <= 0 || B <= 0 || n_tok < 0 || max_len <= 0)
+    return fail(B2A_ERR_ARG, "tree_commit: sizes must be positive");
+  if (max_nodes <= 0 || max_nodes > B2A_TREE_MAX_NODES)
+    return fail(B2A_ERR_ARG, "tree_commit: max_nodes %d (1..%d)", max_nodes, B2A_TREE_MAX_NODES);
+  if (B > 65535) return fail(B2A_ERR_UNSUPPORTED, "tree_commit: %d requests > 65535", B);
+  if (lens_out_dev == lens_dev)
+    return fail(B2A_ERR_ARG, "tree_commit: lens_out needs a buffer of its own");
+  const int es = b2a_host::elem_size(dtype);
+  if (es == 0) return fail(B2A_ERR_DTYPE, "tree_commit: dtype %d", dtype);
+  const long long page_elems = static_cast<long long>(page_rows) * KV * D;
+  if (page_stride == 0) page_stride = page_elems;
+  if (page_stride < page_elems || (n_layers > 1 && layer_stride < page_stride * (n_pages - 1) + page_elems))
+    return fail(B2A_ERR_SHAPE, "tree_commit: page or layer strides overlap");
+  if (table_dev) {
+    if (!power_of_two(page_rows))
+      return fail(B2A_ERR_SHAPE, "tree_commit: page_rows %d is not a power of two", page_rows);
+    if (table_width <= 0 || table_stride < table_width ||
+        static_cast<long long>(table_width) * page_rows < max_len)
+      return fail(B2A_ERR_SHAPE, "tree_commit: a table row of %d pages (stride %lld) does not hold max_len %d rows",
+                  table_width, table_stride, max_len);
+  } else if (n_pages < B || page_rows < max_len) {
+    return fail(B2A_ERR_SHAPE, "tree_commit: %d blocks of %d rows for %d sequences of up to %d",
+                n_pages, page_rows, B, max_len);
+  }
+  const long long row_bytes = static_cast<long long>(KV) * D * es;
+  if (!b2a_host::aligned16(k_cache) || !b2a_host::aligned16(v_cache) || row_bytes % 16 != 0 ||
+      (page_stride * es) % 16 != 0 || (n_layers > 1 && (layer_stride * es) % 16 != 0))
+    return fail(B2A_ERR_ALIGN, "tree_commit: caches, rows and strides must be 16-byte aligned");
+  PG::Commit c = {picks_dev, tokens_dev, parents_dev, cu_dev, lens_dev, table_dev, table_stride,
+                  static_cast<unsigned char*>(k_cache), static_cast<unsigned char*>(v_cache),
+                  n_layers > 1 ? layer_stride * es : 0, page_stride * es, static_cast<int>(row_bytes),
+                  n_layers, n_pages, table_dev ? log2_of(page_rows) : -1, max_len, n_tok, max_nodes,
+                  path_dev, accepted_dev, next_dev, lens_out_dev};
+  const long long cols = static_cast<long long>(n_layers) * 2 * (row_bytes / 16);
+  const long long gx = (cols + PG::kCommitThreads - 1) / PG::kCommitThreads;
+  const cudaError_t e = b2a_host::launch(PG::tree_commit_kernel, dim3(static_cast<unsigned>(gx < 64 ? gx : 64), B),
+                                         dim3(PG::kCommitThreads), 0, static_cast<cudaStream_t>(stream), c);
+  return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "tree_commit launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,227 @@
+// Work division of the tree attention over a cache (tree_decode.cu,
+// tree_wide.cu): what every kernel of it shares.
+//
+// The work is a list of items (request, KV head, block of query rows), each
+// as long as its request's key tiles.  Lengths live on the device, so the
+// division is made there: the list's tiles are numbered through and CTA c of
+// G takes tiles [c * chunk, (c + 1) * chunk), chunk = ceil(total / G).  Every
+// CTA so streams the same number of tiles whatever the lengths, and at most
+// one item is cut at each CTA boundary.  An item wholly inside one CTA's
+// range is finished there; the parts of a cut item go to the workspace and
+// tree_merge_kernel joins them.  CTA c writes at most two parts: slot 2c for
+// an item that began before its range and ends in it, slot 2c + 1 for one
+// that goes on past its range.
+#pragma once
+
+#include "b2a_common.cuh"
+
+namespace b2a {
+namespace tree {
+
+constexpr int kMaxNodes = B2A_TREE_MAX_NODES;  // nodes of one request's tree
+constexpr int kWords = kMaxNodes / 32;         // words of an ancestor mask
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// The requests, as the kernels see them.
+struct Batch {
+  const int* lens;     // cached rows before the tree
+  const int* cu;       // [B + 1] first node of each request
+  const int* parents;  // [n_tok] or null: a chain
+  const int* table;    // [B][table_stride] pages, or null: request b's block is page b
+  long long table_stride;
+  int B, n_tok, max_nodes, max_len, n_pages, page_shift;
+  int H, KV, group;
+  int rows_per_block;  // query rows of an item
+  int tile;            // keys per tile
+  int by_item;         // CTAs take whole items (no parts)
+  int min_units;       // least tiles of a CTA's range
+};
+
+// Nodes and cache rows of request b; a request whose numbers are out of
+// bounds has none (recorded).
+__device__ __forceinline__ void request(const Batch& bt, int b, int& n, int& len) {
+  const int c0 = bt.cu[b], c1 = bt.cu[b + 1];
+  len = bt.lens[b];
+  n = c1 - c0;
+  if (n < 0 || n > bt.max_nodes || c0 < 0 || c1 > bt.n_tok || len < 0 ||
+      len > bt.max_len - n) {
+    set_dev_error(B2A_ERR_POSITION, b);
+    n = 0;
+    len = 0;
+  }
+}
+
+__device__ __forceinline__ int blocks_of(const Batch& bt, int n) {
+  return (n * bt.group + bt.rows_per_block - 1) / bt.rows_per_block;
+}
+
+__device__ __forceinline__ long long units_of(const Batch& bt, int n, int len) {
+  if (n == 0) return 0;
+  const long long items = static_cast<long long>(bt.KV) * blocks_of(bt, n);
+  return bt.by_item ? items : items * ((len + n + bt.tile - 1) / bt.tile);
+}
+
+// Start of a CTA's range.
+struct Start {
+  long long off;    // units into request b
+  long long left;   // units of this CTA
+  long long chunk;  // units per CTA
+  int b;
+};
+
+// Warp-collective: the range of CTA c of G.
+__device__ __forceinline__ Start locate(const Batch& bt, int c, int G) {
+  const int lane = threadIdx.x & 31;
+  long long total = 0;
+  for (int b = lane; b < bt.B; b += 32) {
+    int n, len;
+    request(bt, b, n, len);
+    total += units_of(bt, n, len);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  Start s;
+  s.chunk = (total + G - 1) / G;
+  if (s.chunk < bt.min_units) s.chunk = bt.min_units;
+  const long long first = s.chunk * c;
+  s.left = total - first;
+  if (s.left > s.chunk) s.left = s.chunk;
+  s.b = bt.B;
+  s.off = 0;
+  if (s.left <= 0) {
+    s.left = 0;
+    return s;
+  }
+  long long run = 0;
+  for (int b0 = 0; b0 < bt.B; b0 += 32) {
+    int n = 0, len = 0;
+    if (b0 + lane < bt.B) request(bt, b0 + lane, n, len);
+    const long long u = units_of(bt, n, len);
+    long long inc = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    const long long lo = run + inc - u;
+    const unsigned hit = __ballot_sync(0xffffffffu, first >= lo && first < lo + u);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      s.b = b0 + src;
+      s.off = first - __shfl_sync(0xffffffffu, lo, src);
+      return s;
+    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  s.left = 0;  // not reached
+  return s;
+}
+
+struct Item {
+  int b, kvh, blk;
+  int n, len;     // the request's nodes and cached rows
+  int t0, t1;     // this CTA's key tiles of the item
+  int tiles;      // the item's key tiles
+  int node0;      // row of the request's node 0 in q and out
+};
+
+// Walks the items of a CTA's range; every role of a CTA walks the same ones.
+struct Walker {
+  long long off, left;
+  int b, n, len;
+  __device__ __forceinline__ void start(const Batch& bt, const Start& s) {
+    off = s.off;
+    left = s.left;
+    b = s.b;
+    if (left > 0) request(bt, b, n, len);
+  }
+  __device__ __forceinline__ bool next(const Batch& bt, Item& it) {
+    while (left > 0) {
+      const long long u = units_of(bt, n, len);
+      if (off >= u) {
+        off -= u;
+        if (++b >= bt.B) return false;
+        request(bt, b, n, len);
+        continue;
+      }
+      it.b = b;
+      it.n = n;
+      it.len = len;
+      it.tiles = (len + n + bt.tile - 1) / bt.tile;
+      const int per = bt.by_item ? 1 : it.tiles;
+      const int idx = static_cast<int>(off / per);
+      const int at = static_cast<int>(off - static_cast<long long>(idx) * per);
+      int take = per - at;
+      if (take > left) take = static_cast<int>(left);
+      it.t0 = bt.by_item ? 0 : at;
+      it.t1 = bt.by_item ? it.tiles : at + take;
+      const int blks = blocks_of(bt, n);
+      it.kvh = idx / blks;
+      it.blk = idx - it.kvh * blks;
+      it.node0 = bt.cu[b];
+      off += take;
+      left -= take;
+      return true;
+    }
+    return false;
+  }
+};
+
+// Ancestor masks of a request's nodes (bit j of node i's: i sees node j),
+// written by threads tid of nt to anc[node][kWords]; par holds the parents
+// (synchronise before and after).  A parent that is not an earlier node is
+// recorded and ends the path.
+__device__ __forceinline__ void ancestor_masks(const int* par, bool chain, int n,
+                                               uint32_t (*anc)[kWords], int tid, int nt,
+                                               int where) {
+  for (int i = tid; i < n; i += nt) {
+    uint32_t m[kWords];
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) m[w] = 0u;
+    if (chain) {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        const int k = i + 1 - w * 32;  // bits of this word
+        m[w] = k >= 32 ? 0xffffffffu : (k > 0 ? (1u << k) - 1u : 0u);
+      }
+    } else {
+      int p = i;
+      while (true) {
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+          if ((p >> 5) == w) m[w] |= 1u << (p & 31);
+        const int up = par[p];
+        if (up < 0 || up >= p) {
+          if (up != -1) set_dev_error(B2A_ERR_POSITION, where);
+          break;
+        }
+        p = up;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) anc[i][w] = m[w];
+  }
+}
+
+// Page (outer tensor-map coordinate) that holds cache row `row` of request
+// b; a page outside the pool is recorded and answered with n_pages, which
+// TMA reads as zeros.
+__device__ __forceinline__ int page_of(const Batch& bt, int b, int row) {
+  if (bt.table == nullptr) return b;
+  const int pg = bt.table[b * bt.table_stride + (row >> bt.page_shift)];
+  if (pg < 0 || pg >= bt.n_pages) {
+    set_dev_error(B2A_ERR_POSITION, b);
+    return bt.n_pages;
+  }
+  return pg;
+}
+
+// Part slot of an item in CTA c's range, or -1 if the item is whole in it.
+__device__ __forceinline__ int part_slot(const Item& it, int c) {
+  if (it.t0 == 0 && it.t1 == it.tiles) return -1;
+  return 2 * c + (it.t1 < it.tiles ? 1 : 0);
+}
+
+}  // namespace tree
+}  // namespace b2a

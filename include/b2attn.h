@@ -480,6 +480,158 @@ int b2a_gemm_qkv_rope_q8(const void* a, long long lda, const void* codes, long l
 int b2a_q8_dequant(const void* codes, long long ldq, const void* scales, long long lds,
                    void* out, long long ldo, int dtype, int rows, int cols, void* stream);
 
+/* ---- many requests: a paged cache, drafted token trees -------------------
+ *
+ * No reference counterpart (the reference serves one sequence per Model from
+ * one contiguous block per layer, alpaccaroo/model.py:867-870).  A step of a
+ * serving loop runs
+ *   b2a_page_plan          block tables, slots and positions of its tokens
+ *   per layer: b2a_rope_append_paged, b2a_tree_decode
+ *   b2a_constrain_logits   on the LM head's rows
+ *   b2a_tree_commit        the accepted path's K/V rows into place, all layers
+ *
+ * Pools: K and V caches as [n_pages][page_rows][KV][D], pages page_stride
+ * elements apart (0: dense).  Row r of request b is row r % page_rows of page
+ * table[b * table_stride + r / page_rows]; page_rows is a power of two.  Slot
+ * s of a pool is row s % page_rows of page s / page_rows.  With a NULL table
+ * (b2a_tree_decode, b2a_tree_commit) page b is request b's whole block: the
+ * layout b2a_decode reads, any page_rows.
+ *
+ * Trees: the step's tokens (nodes) of all requests lie behind one another;
+ * request b has nodes cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]), at most
+ * max_nodes <= B2A_TREE_MAX_NODES.  parents int32 [n_tok]: the node's parent
+ * as an index inside its request, smaller than its own, -1 for a root; NULL
+ * is a chain (node i follows node i - 1).  Node i's K/V rows stand at cache
+ * row len + i, its RoPE position is len + its depth.  Prompt chunks are
+ * chains.  Arrays sized n_tok may hold padding rows from cu[B] on (captured
+ * steps); what each entry does with them is stated.
+ *
+ * A device-side number out of bounds (a length, a node count, a parent, a
+ * page) records B2A_ERR_POSITION; the request, or the row, is left out. */
+#define B2A_TREE_MAX_NODES 128
+#define B2A_PLAN_MAX_REQUESTS 2048
+
+/* Block tables, slot map and positions of a step, from request lengths.
+ *   lens, add, held  int32 [B]: cached rows, tokens to add (-1: the request
+ *                    ends and gives its pages back), pages in its table
+ *   parents          int32 [max_tokens] trees of the added tokens, or NULL
+ *   table            int32 [B][table_stride], in place: new pages are entered
+ *                    behind the held ones
+ *   ring, ring_state the free pages: int32 [ring_size] pages, of which count
+ *                    from head on are free; state = (head, count).  Taken
+ *                    from the head, given back at the tail, in place; a ring
+ *                    as large as the pool never overwrites a free page
+ *   held_out, ring_state_out  the numbers after the step (other buffers than
+ *                    held and ring_state: the call can then be repeated)
+ *   cu               int32 [B + 1]
+ *   seq, pos, slot   int32 [max_tokens], 16-byte aligned: a token's request,
+ *                    RoPE position and slot; padding rows get -1, 0, -1
+ * Pages go to the requests in order: request b is served if the pages wanted
+ * up to and including its own are there (or it wants none) and its rows fit
+ * max_pages; else it keeps what it holds and its tokens' slots are -1. */
+int b2a_page_plan(const int* lens_dev, const int* add_dev, const int* parents_dev,
+                  const int* held_dev, int* held_out_dev, int* table_dev, long long table_stride,
+                  int* ring_dev, int ring_size, const int* ring_state_dev,
+                  int* ring_state_out_dev, int* cu_dev, int* seq_dev, int* pos_dev, int* slot_dev,
+                  int B, int max_tokens, int max_pages, int page_rows, void* stream);
+
+/* b2a_rope_append into a paged cache, position and cache row apart:
+ *   q, k, v   rows of in_dtype (F32, F16, BF16), token strides in elements
+ *   q_out     [n_tok][H][D] of q_out_dtype: q (+ bq) rotated at pos
+ *   k_pool, v_pool  of kv_dtype: slot of the token gets k (+ bk) rotated and
+ *             v (+ bv); a negative slot stores nothing (q is still rotated)
+ * Rotation, tables, bias, styles and rounding as b2a_rope_append; dims from
+ * n_rot on pass through.  A position outside the table or a slot past the
+ * pool records B2A_ERR_POSITION and writes nothing for that token.  The
+ * tokens' slots differ. */
+int b2a_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
+                          long long k_tok_stride, const void* v, long long v_tok_stride,
+                          int in_dtype, const float* bq, const float* bk, const float* bv,
+                          const float* cos_tab, const float* sin_tab, int tab_rows,
+                          const int* pos_dev, const int* slot_dev, void* k_pool, void* v_pool,
+                          int n_pages, int page_rows, long long page_stride, int kv_dtype,
+                          void* q_out, int q_out_dtype, int n_tok, int H, int KV, int D, int n_rot,
+                          int style, void* stream);
+
+/* Attention of the nodes over the cache: node i of request b reads rows
+ * 0 .. lens[b] - 1, its ancestors' rows and its own,
+ *   out = softmax(scale q.K^T) . V,  lse = natural log-sum-exp of the scores.
+ *   q, k_cache, v_cache, out  one type; q [n_tok] rows of [H][D] q_tok_stride
+ *             apart (0: dense), out [n_tok][H][D]; D 64, 128 or 256; head h
+ *             reads KV head h / (H / KV), H / KV <= 128
+ *   lens      int32 [B]: cached rows without the nodes' own
+ *   lse_out   f32 [n_tok][H] or NULL
+ *   max_len   host bound on lens[b] + nodes (<= table_width * page_rows, or
+ *             page_rows without a table); paged caches: page_rows >= 16
+ * Padding rows of out become 0 (lse -inf).  16-bit types: tensor cores, f32
+ * scores, sums and accumulators, the weights rounded to the type for the
+ * product with V.  F32: f32 products and sums.  One node per request is a
+ * batched decode step. */
+size_t b2a_tree_decode_workspace_bytes(int max_nodes, int H, int KV, int D, int dtype);
+int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
+                    const void* v_cache, int n_pages, int page_rows, long long page_stride,
+                    const int* table_dev, long long table_stride, int table_width,
+                    const int* lens_dev, const int* cu_dev, const int* parents_dev, void* out,
+                    float* lse_out, void* workspace, size_t workspace_bytes, int B, int n_tok,
+                    int max_nodes, int H, int KV, int D, int dtype, float scale, int max_len,
+                    void* stream);
+
+/* Penalties, biases and grammar masks on the nodes' logits rows, and each
+ * row's greedy pick.  For token v of the row of node t of request b:
+ *   x = logits + bias (if v is among the request's bias ids)
+ *   c = times v is in the request's output history or on t's path (t's own
+ *       token and its ancestors')
+ *   c > 0 or v in the prompt part:  x = x > 0 ? x / repetition : x * repetition
+ *   c > 0:                          x = x - frequency * c - presence
+ *   mask bit v of the row is 0:     x = -inf
+ * each step rounded to f32; out gets x in out_dtype (may be logits itself),
+ * picks the lowest v of the largest x, -1 where no x is above -inf.
+ *   logits, out  [n_rows][V] with row strides, F32, F16 or BF16
+ *   tokens       int32 [n_rows] the nodes' tokens, or NULL (no path)
+ *   hist, hist_start, prompt_len  int32: request b's history is hist[
+ *                hist_start[b] .. hist_start[b + 1]), prompt_len[b] tokens of
+ *                prompt first (NULL: none); the tree's tokens are not in it.
+ *                hist NULL: no history; n_hist its size
+ *   repetition, presence, frequency  f32 [B], NULL: 1, 0, 0
+ *   bias_start, bias_ids, bias       request b's entries bias_start[b] ..
+ *                bias_start[b + 1]; the last entry of an id counts.  bias
+ *                NULL: none; n_bias the arrays' size
+ *   mask         bit v % 32 of word v / 32 of the row, or NULL
+ * Tokens outside [0, V) in the lists are ignored.  Padding rows: pick -1, out
+ * untouched. */
+size_t b2a_constrain_logits_workspace_bytes(int n_rows, int V);
+int b2a_constrain_logits(const void* logits, long long row_stride, int in_dtype, void* out,
+                         long long out_row_stride, int out_dtype, int* picks_dev,
+                         const int* cu_dev, const int* parents_dev, const int* tokens_dev,
+                         const int* hist_dev, const int* hist_start_dev, int n_hist,
+                         const int* prompt_len_dev, const float* repetition_dev,
+                         const float* presence_dev, const float* frequency_dev,
+                         const int* bias_start_dev, const int* bias_ids_dev,
+                         const float* bias_dev, int n_bias, const unsigned int* mask_dev,
+                         long long mask_row_stride, int B, int n_rows, int max_nodes, int V,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* The accepted path of each tree, and its K/V rows moved into place.  The
+ * path begins at node 0 and goes from a node to its first child whose token
+ * is the node's pick.
+ *   picks, tokens  int32 [n_tok]: the model's token after each node, the
+ *                  node's own token
+ *   k_cache, v_cache  n_layers caches layer_stride elements apart (dtype for
+ *                  the element size): row lens[b] + path[d] of every layer is
+ *                  copied to row lens[b] + d
+ *   path       int32 [B][max_nodes], -1 behind the path
+ *   accepted   int32 [B] nodes on the path (0 for a request without nodes)
+ *   next       int32 [B] the pick of the path's last node (-1 without nodes)
+ *   lens_out   int32 [B] lens + accepted (another buffer than lens)
+ * max_len as in b2a_tree_decode. */
+int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* parents_dev,
+                    const int* cu_dev, const int* lens_dev, const int* table_dev,
+                    long long table_stride, int table_width, void* k_cache, void* v_cache,
+                    int n_layers, long long layer_stride, int n_pages, int page_rows,
+                    long long page_stride, int KV, int D, int dtype, int B, int n_tok,
+                    int max_nodes, int max_len, int* path_dev, int* accepted_dev, int* next_dev,
+                    int* lens_out_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
