@@ -122,7 +122,7 @@ SIGNATURES = [
                                       c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                       c_int, c_int, c_longlong, c_int, c_void_p, c_int, c_int,
                                       c_int, c_int, c_int, c_int, c_int, c_void_p]),
-    ("b2a_tree_decode_workspace_bytes", c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    ("b2a_tree_decode_workspace_bytes", c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     ("b2a_tree_decode", c_int, [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_longlong,
                                 c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int,

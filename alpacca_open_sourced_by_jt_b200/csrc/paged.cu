@@ -33,6 +33,7 @@ struct Plan {
   const int* state;
   int *held_out, *state_out, *cu, *seq, *pos, *slot;
   int B, max_tokens, max_pages, page_shift, ring_size;
+  bool whole;  // seq, pos and slot take 16-byte stores
 };
 
 // Tokens, pages wanted from the ring and pages given back of request b.
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
       sl[e] = (page << p.page_shift) + (row & ((1 << p.page_shift) - 1));
     }
   }
-  if (first + 3 < p.max_tokens) {
+  if (p.whole && first + 3 < p.max_tokens) {
     *reinterpret_cast<int4*>(p.seq + first) = make_int4(sq[0], sq[1], sq[2], sq[3]);
     *reinterpret_cast<int4*>(p.pos + first) = make_int4(ps[0], ps[1], ps[2], ps[3]);
     *reinterpret_cast<int4*>(p.slot + first) = make_int4(sl[0], sl[1], sl[2], sl[3]);
@@ -450,11 +451,10 @@ int b2a_page_plan(const int* lens_dev, const int* add_dev, const int* parents_de
     return fail(B2A_ERR_ARG, "page_plan: held and ring_state need output buffers of their own");
   if (static_cast<long long>(ring_size) * page_rows > INT_MAX)
     return fail(B2A_ERR_UNSUPPORTED, "page_plan: %d pages of %d rows exceed 32-bit slots", ring_size, page_rows);
-  if (!b2a_host::aligned16(seq_dev) || !b2a_host::aligned16(pos_dev) || !b2a_host::aligned16(slot_dev))
-    return fail(B2A_ERR_ALIGN, "page_plan: seq, pos and slot must be 16-byte aligned");
   PG::Plan p = {lens_dev, add_dev, parents_dev, held_dev, table_dev, table_stride, ring_dev,
                 ring_state_dev, held_out_dev, ring_state_out_dev, cu_dev, seq_dev, pos_dev,
-                slot_dev, B, max_tokens, max_pages, log2_of(page_rows), ring_size};
+                slot_dev, B, max_tokens, max_pages, log2_of(page_rows), ring_size,
+                b2a_host::aligned16(seq_dev) && b2a_host::aligned16(pos_dev) && b2a_host::aligned16(slot_dev)};
   constexpr int kWarps = PG::kPlanThreads / 32;
   int grid = (max_tokens + PG::kPlanTokens - 1) / PG::kPlanTokens;
   if (grid < (B + kWarps - 1) / kWarps) grid = (B + kWarps - 1) / kWarps;

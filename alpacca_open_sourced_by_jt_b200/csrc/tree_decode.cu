@@ -46,7 +46,7 @@ constexpr int kRows = 64;
 constexpr int kConsumers = 8;
 constexpr int kMmaThreads = (kConsumers + 1) * 32;
 
-template <int D, int NT>
+template <int D, int NT, bool kByRows>
 struct MmaCfg {
   static constexpr int kBoxes = D / 64;
   static constexpr int kBoxBytes = kRows * 128;
@@ -56,7 +56,10 @@ struct MmaCfg {
   static constexpr int kState = (D / 16 * NT * 4 + NT * 4) * 32 * 4;
   static constexpr int kMerge = 4 * kState;
   static constexpr int kFit = (232448 - 1024 - 4096 - kMerge) / kStageBytes;
-  static constexpr int kStages = kFit > 10 ? 10 : kFit;
+  // Without kByRows a stage must always belong to the same half of the warps:
+  // a warp that skipped a stage's last use could not tell its phase by the
+  // parity.  An even ring keeps tile parity and stage parity together.
+  static constexpr int kStages = kFit > 10 ? 10 : (kByRows ? kFit : kFit & ~1);
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kMerge;
   static_assert(kStages >= 2, "ring");
 };
@@ -67,7 +70,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
     const __grid_constant__ Batch bt, const T* __restrict__ q, long long q_stride,
     T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o,
     float* __restrict__ part_ml, int piece_rows, float sscale) {
-  using C = MmaCfg<D, NT>;
+  using C = MmaCfg<D, NT, kByRows>;
   constexpr int KS = D / 16;
   constexpr int RB = kByRows ? 16 * NT : 8 * NT;
   extern __shared__ uint8_t smem_raw[];
@@ -809,6 +812,11 @@ int tree_rows_per_block(int dtype, int rows) {
   return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
 }
 
+// Keys of a tile, and whether CTAs take whole items: for short contexts one
+// launch without parts to join costs less than cutting the items.
+int tree_tile(int dtype, int D) { return dtype == B2A_F32 && D > 128 ? 32 : TR::kRows; }
+bool tree_by_item(int max_len, int tile) { return (max_len + tile - 1) / tile <= 8; }
+
 struct TreeArgs {
   const void *q, *k, *v;
   long long q_stride, page_stride;
@@ -852,7 +860,7 @@ int tree_map(CUtensorMap* m, const TreeArgs& a, const void* base, int box_rows) 
 template <typename T, int D, int NT, bool kByRows>
 int tree_mma(const TreeArgs& a) {
   auto kern = TR::tree_mma_kernel<T, D, NT, kByRows>;
-  constexpr int smem = TR::MmaCfg<D, NT>::kSmem;
+  constexpr int smem = TR::MmaCfg<D, NT, kByRows>::kSmem;
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_smem(kern, smem, done);
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "cudaFuncSetAttribute(tree_decode)");
@@ -913,8 +921,9 @@ bool power_of_two(int x) { return x > 0 && (x & (x - 1)) == 0; }
 
 extern "C" {
 
-size_t b2a_tree_decode_workspace_bytes(int max_nodes, int H, int KV, int D, int dtype) {
+size_t b2a_tree_decode_workspace_bytes(int max_nodes, int H, int KV, int D, int dtype, int max_len) {
   if (max_nodes <= 0 || H <= 0 || KV <= 0 || D <= 0 || H % KV != 0) return 0;
+  if (tree_by_item(max_len, tree_tile(dtype, D))) return 0;
   const int rb = tree_rows_per_block(dtype, max_nodes * (H / KV));
   return tree_part_o_bytes(D, rb) +
          static_cast<size_t>(2) * b2a_host::sm_count() * rb * 2 * sizeof(float);
@@ -971,22 +980,20 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
   TreeArgs a = {};
   const int rows = max_nodes * group;
   const int rb = tree_rows_per_block(dtype, rows);
-  const int tile = dtype == B2A_F32 && D > 128 ? 32 : TR::kRows;
+  const int tile = tree_tile(dtype, D);
   a.bt = TR::Batch{lens_dev, cu_dev, parents_dev, table_dev, table_stride, B, n_tok, max_nodes,
                    max_len, n_pages, table_dev ? log2_of(page_rows) : 0, H, KV, group, rb, tile, 0, 1};
-  // Short contexts: whole items per CTA (one launch, no parts to join) cost
-  // less than cutting them.  Else the tiles are cut evenly over the SMs, at
-  // least 4 to a CTA.
+  // The tiles are cut evenly over the SMs, at least 4 to a CTA.
   const long long max_tiles = (max_len + tile - 1) / tile;
   const long long items = static_cast<long long>(B) * KV * ((rows + rb - 1) / rb);
-  a.bt.by_item = max_tiles <= 8 ? 1 : 0;
+  a.bt.by_item = tree_by_item(max_len, tile) ? 1 : 0;
   a.bt.min_units = a.bt.by_item ? 1 : 4;
   const long long units = a.bt.by_item ? items : (items * max_tiles + 3) / 4;
   const int sms = b2a_host::sm_count();
   a.grid = static_cast<int>(units < sms ? units : sms);
   a.merge = !a.bt.by_item;
   if (a.merge) {
-    const size_t need = b2a_tree_decode_workspace_bytes(max_nodes, H, KV, D, dtype);
+    const size_t need = b2a_tree_decode_workspace_bytes(max_nodes, H, KV, D, dtype, max_len);
     if (!workspace || workspace_bytes < need)
       return fail(B2A_ERR_WORKSPACE, "tree_decode: workspace %zu bytes < %zu needed", workspace_bytes, need);
   }

@@ -23,41 +23,80 @@ of bounds are recorded (`_lib.device_error`).
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
 import torch
 
 from . import _lib, device
-from .device import _code, _need, _ptr, _stream
+from .device import _code
 
 MAX_NODES = 128      # B2A_TREE_MAX_NODES
 MAX_REQUESTS = 2048  # B2A_PLAN_MAX_REQUESTS
 
 
+def _bad(msg: str):
+    raise _lib.B2AShapeError(_lib.ERR_SHAPE, msg)
+
+
+# The checks below run before every launch of a serving step: messages are
+# only built when a check fails.
+
 def _i32(name: str, t: torch.Tensor, n: int | None = None):
-    _need(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and
-          (n is None or t.numel() == n),
-          f"{name} must be a contiguous CUDA int32 tensor" + (f" of {n}" if n is not None else ""))
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous() or (
+            n is not None and t.numel() != n):
+        _bad(f"{name} must be a contiguous CUDA int32 tensor" + ("" if n is None else f" of {n}"))
+
+
+def _i32_rows(name: str, t: torch.Tensor | None, n: int):
+    """The address of a per-node array that covers n rows (None: a null pointer)."""
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous() or t.numel() < n:
+        _bad(f"{name} must be a contiguous CUDA int32 tensor of at least {n}")
+    return t.data_ptr()
+
+
+def _f32(name: str, t: torch.Tensor | None, n: int):
+    """The address of an f32 array of n (None: a null pointer)."""
+    if t is None:
+        return None
+    if t.dtype is not torch.float32 or not t.is_cuda or not t.is_contiguous() or t.numel() != n:
+        _bad(f"{name} must be a contiguous CUDA f32 tensor of {n}")
+    return t.data_ptr()
 
 
 def _table(table, B: int):
-    """(stride, width) of a block table (B, max_pages), rows of unit stride."""
+    """(address, stride, width) of a block table (B, max_pages), rows of unit stride."""
     if table is None:
-        return 0, 0
-    _need(table.dtype == torch.int32 and table.is_cuda and table.dim() == 2 and
-          table.shape[0] == B and table.stride(1) == 1,
-          "table must be a CUDA int32 tensor (B, max_pages)")
-    return (table.stride(0) if B > 1 else table.shape[1]), table.shape[1]
+        return None, 0, 0
+    shape, stride = table.shape, table.stride()
+    if table.dtype is not torch.int32 or not table.is_cuda or len(shape) != 2 or shape[0] != B or (
+            stride[1] != 1):
+        _bad("table must be a CUDA int32 tensor (B, max_pages)")
+    return table.data_ptr(), (stride[0] if B > 1 else shape[1]), shape[1]
 
 
-def _pool(k: torch.Tensor, v: torch.Tensor):
-    """(n_pages, page_rows, page_stride, KV, D) of a K and V pool."""
-    _need(k.is_cuda and v.is_cuda and k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and
-          k.stride() == v.stride(), "k and v pools (n_pages, page_rows, KV, D) of one type and layout")
-    P, R, KV, D = k.shape
-    _need(k[0].is_contiguous(), "each page must be contiguous")
-    return P, R, (k.stride(0) if P > 1 else R * KV * D), KV, D
+def _pool(k: torch.Tensor, v: torch.Tensor, dims: int = 4):
+    """(shape, strides) of a K and V pool, (n_pages, page_rows, KV, D) with
+    contiguous pages; dims 5: (L, ...), a layer stride in front."""
+    shape, stride = k.shape, k.stride()
+    if not k.is_cuda or not v.is_cuda or len(shape) != dims or v.shape != shape or (
+            v.dtype is not k.dtype or v.stride() != stride):
+        _bad("k and v pools (n_pages, page_rows, KV, D) of one type and layout")
+    R, KV, D = shape[-3:]
+    if stride[-1] != 1 or stride[-2] != D or (R > 1 and stride[-3] != KV * D):
+        _bad("each page must be contiguous")
+    return shape, stride
+
+
+def _stream(stream, t: torch.Tensor):
+    """The caller's stream, or t's device's current one (its raw handle: a
+    torch.cuda.Stream object costs microseconds a call)."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return device._stream(stream)
 
 
 class PagePlan(NamedTuple):
@@ -90,27 +129,26 @@ def page_plan(lens: torch.Tensor, add: torch.Tensor, held: torch.Tensor, table: 
     _i32("held", held, B)
     _i32("ring", ring)
     _i32("ring_state", ring_state, 2)
-    stride, width = _table(table, B)
+    tptr, tstride, width = _table(table, B)
     if parents is not None:
         _i32("parents", parents, max_tokens)
     if out is None:
-        # one allocation: five int32 arrays, the three per-token ones 16-byte aligned
-        n = (max_tokens + 3) & ~3
-        buf = torch.empty(3 * n + 2 * B + 3, dtype=torch.int32, device=lens.device)
-        out = PagePlan(buf[3 * n:3 * n + B + 1], buf[:max_tokens], buf[n:n + max_tokens],
-                       buf[2 * n:2 * n + max_tokens], buf[3 * n + B + 1:3 * n + 2 * B + 1],
-                       buf[3 * n + 2 * B + 1:])
+        seq, pos, slots, cu, held_out, state_out = torch.empty(
+            3 * max_tokens + 2 * B + 3, dtype=torch.int32, device=lens.device).split_with_sizes(
+                (max_tokens, max_tokens, max_tokens, B + 1, B, 2))
+        out = PagePlan(cu, seq, pos, slots, held_out, state_out)
     else:
-        _i32("out.cu", out.cu, B + 1)
-        for name, t in (("seq", out.seq), ("positions", out.positions), ("slots", out.slots)):
+        cu, seq, pos, slots, held_out, state_out = out
+        _i32("out.cu", cu, B + 1)
+        for name, t in (("seq", seq), ("positions", pos), ("slots", slots)):
             _i32("out." + name, t, max_tokens)
-        _i32("out.held", out.held, B)
-        _i32("out.ring_state", out.ring_state, 2)
+        _i32("out.held", held_out, B)
+        _i32("out.ring_state", state_out, 2)
     _lib.check(_lib.load().b2a_page_plan(
-        _ptr(lens), _ptr(add), _ptr(parents), _ptr(held), _ptr(out.held), _ptr(table), stride,
-        _ptr(ring), ring.numel(), _ptr(ring_state), _ptr(out.ring_state), _ptr(out.cu),
-        _ptr(out.seq), _ptr(out.positions), _ptr(out.slots), B, int(max_tokens), width,
-        int(page_rows), _stream(stream)))
+        lens.data_ptr(), add.data_ptr(), None if parents is None else parents.data_ptr(),
+        held.data_ptr(), held_out.data_ptr(), tptr, tstride, ring.data_ptr(), ring.numel(),
+        ring_state.data_ptr(), state_out.data_ptr(), cu.data_ptr(), seq.data_ptr(), pos.data_ptr(),
+        slots.data_ptr(), B, max_tokens, width, page_rows, _stream(stream, lens)))
     return out
 
 
@@ -125,47 +163,51 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     int32 as page_plan writes them: the rotary position and the pool row are
     apart, a negative slot stores nothing.  Returns q_out (n, H, D), in the
     pools' type unless given."""
-    _need(q.dim() == 3 and k.dim() == 3 and k.shape == v.shape and q.dtype == k.dtype == v.dtype and
-          q.is_cuda and k.is_cuda and v.is_cuda, "q (n,H,D), k/v (n,KV,D) CUDA tensors of one type")
-    n, H, D = q.shape
-    P, R, pstride, KV, Dp = _pool(k_pool, v_pool)
-    _need(k.shape == (n, KV, D) and Dp == D, "k/v rows do not match the pools")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _need(t.stride(2) == 1 and t.stride(1) == D, f"{name} rows must be contiguous per token")
+    (P, R, KV, D), pstride = _pool(k_pool, v_pool)
+    dt, qs, ks, vs = q.dtype, q.stride(), k.stride(), v.stride()
+    n, H, Dq = q.shape
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and k.dtype is dt and v.dtype is dt and
+            Dq == D and k.shape == (n, KV, D) and v.shape == (n, KV, D)):
+        _bad("q (n, H, D), k and v (n, KV, D): CUDA tensors of one type, as the pools' rows")
+    if qs[2] != 1 or qs[1] != D or ks[2] != 1 or ks[1] != D or vs[2] != 1 or vs[1] != D:
+        _bad("q, k and v rows must be contiguous per token")
     _i32("positions", positions, n)
     _i32("slots", slots, n)
-    device._cuda_contig("cos_tab", cos_tab)
-    device._cuda_contig("sin_tab", sin_tab)
+    rows, half = cos_tab.shape
     if n_rot is None:
-        n_rot = 2 * cos_tab.shape[1]
-    _need(cos_tab.shape == sin_tab.shape and cos_tab.shape[1] * 2 == n_rot and
-          cos_tab.dtype == sin_tab.dtype == torch.float32, "cos/sin tables f32 (rows, n_rot/2)")
-    for name, t, m in (("bq", bq, H), ("bk", bk, KV), ("bv", bv, KV)):
-        if t is not None:
-            device._cuda_contig(name, t)
-            _need(t.dtype == torch.float32 and t.numel() == m * D, f"{name} f32 ({m}, D)")
+        n_rot = 2 * half
+    if half * 2 != n_rot:
+        _bad("cos/sin tables f32 (rows, n_rot/2)")
+    cos, sin = _f32("cos_tab", cos_tab, rows * half), _f32("sin_tab", sin_tab, rows * half)
     if q_out is None:
-        q_out = torch.empty((n, H, D), dtype=k_pool.dtype, device=q.device)
-    else:
-        device._cuda_contig("q_out", q_out)
-        _need(q_out.numel() == n * H * D, "q_out (n, H, D)")
-
-    def stride(t, m):
-        return t.stride(0) if n > 1 else m * D
-
+        q_out = k_pool.new_empty((n, H, D))
+    elif not q_out.is_cuda or not q_out.is_contiguous() or q_out.numel() != n * H * D:
+        _bad("q_out must be a contiguous CUDA tensor (n, H, D)")
     _lib.check(_lib.load().b2a_rope_append_paged(
-        _ptr(q), stride(q, H), _ptr(k), stride(k, KV), _ptr(v), stride(v, KV), _code(q.dtype),
-        _ptr(bq), _ptr(bk), _ptr(bv), _ptr(cos_tab), _ptr(sin_tab), cos_tab.shape[0],
-        _ptr(positions), _ptr(slots), _ptr(k_pool), _ptr(v_pool), P, R, pstride,
-        _code(k_pool.dtype), _ptr(q_out), _code(q_out.dtype), n, H, KV, D, int(n_rot),
-        device._STYLE[style], _stream(stream)))
+        q.data_ptr(), qs[0] if n > 1 else H * D, k.data_ptr(), ks[0] if n > 1 else KV * D,
+        v.data_ptr(), vs[0] if n > 1 else KV * D, _code(dt), _f32("bq", bq, H * D),
+        _f32("bk", bk, KV * D), _f32("bv", bv, KV * D), cos, sin, rows, positions.data_ptr(),
+        slots.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), P, R,
+        pstride[0] if P > 1 else R * KV * D, _code(k_pool.dtype), q_out.data_ptr(),
+        _code(q_out.dtype), n, H, KV, D, n_rot, device._STYLE[style], _stream(stream, q)))
     return q_out
 
 
+@functools.lru_cache(maxsize=256)
+def _tree_bytes(device_index, max_nodes, n_head, n_kv, head_dim, code, max_len) -> int:
+    return _lib.load().b2a_tree_decode_workspace_bytes(max_nodes, n_head, n_kv, head_dim, code, max_len)
+
+
+@functools.lru_cache(maxsize=256)
+def _logits_bytes(n_rows, vocab) -> int:
+    return _lib.load().b2a_constrain_logits_workspace_bytes(n_rows, vocab)
+
+
 def tree_decode_workspace(max_nodes: int, n_head: int, n_kv: int, head_dim: int,
-                          dtype: torch.dtype, dev) -> torch.Tensor:
+                          dtype: torch.dtype, max_len: int, dev) -> torch.Tensor:
     """Allocate (via torch) a workspace big enough for b2a_tree_decode."""
-    n = _lib.load().b2a_tree_decode_workspace_bytes(max_nodes, n_head, n_kv, head_dim, _code(dtype))
+    n = _lib.load().b2a_tree_decode_workspace_bytes(max_nodes, n_head, n_kv, head_dim, _code(dtype),
+                                                    max_len)
     return torch.empty(max(int(n), 16), dtype=torch.uint8, device=dev)
 
 
@@ -183,37 +225,37 @@ def tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, len
     max_len bounds lens + nodes (default: what the table or the block holds).
     Returns out (n, H, D) in q's type, padding rows zero; lse (n, H) f32
     receives the natural-log log-sum-exp if given."""
-    _need(q.dim() == 3 and q.is_cuda and q.stride(2) == 1 and q.stride(1) == q.shape[2],
-          "q must be a CUDA tensor (n, H, D), contiguous per token")
-    n, H, D = q.shape
-    P, R, pstride, KV, Dp = _pool(k_pool, v_pool)
-    _need(Dp == D and k_pool.dtype == q.dtype, "the pools must have q's head_dim and type")
+    (P, R, KV, D), pstride = _pool(k_pool, v_pool)
+    dt, qs = q.dtype, q.stride()
+    n, H, Dq = q.shape
+    if not q.is_cuda or qs[2] != 1 or qs[1] != D or Dq != D or k_pool.dtype is not dt:
+        _bad("q must be a CUDA tensor (n, H, D), contiguous per token, in the pools' type")
     B = lens.numel()
     _i32("lens", lens)
     _i32("cu", cu, B + 1)
-    if parents is not None:
-        _i32("parents", parents)
-        _need(parents.numel() >= n, "parents must cover q's rows")
-    tstride, width = _table(table, B)
+    pptr = _i32_rows("parents", parents, n)
+    tptr, tstride, width = _table(table, B)
     if max_len is None:
         max_len = width * R if table is not None else R
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
     if out is None:
-        out = torch.empty((n, H, D), dtype=q.dtype, device=q.device)
-    else:
-        device._cuda_contig("out", out)
-        _need(out.shape == (n, H, D) and out.dtype == q.dtype, "out (n, H, D) in q's type")
-    if lse is not None:
-        device._cuda_contig("lse", lse)
-        _need(lse.dtype == torch.float32 and lse.numel() == n * H, "lse must be f32 (n, H)")
+        out = q.new_empty((n, H, D))
+    elif not out.is_cuda or not out.is_contiguous() or out.shape != (n, H, D) or out.dtype is not dt:
+        _bad("out must be a contiguous CUDA tensor (n, H, D) in q's type")
+    lib = _lib.load()
+    code = _code(dt)
     if workspace is None:
-        workspace = tree_decode_workspace(max_nodes, H, KV, D, q.dtype, q.device)
-    _lib.check(_lib.load().b2a_tree_decode(
-        _ptr(q), q.stride(0) if n > 1 else H * D, _ptr(k_pool), _ptr(v_pool), P, R, pstride,
-        _ptr(table), tstride, width, _ptr(lens), _ptr(cu), _ptr(parents), _ptr(out), _ptr(lse),
-        _ptr(workspace), workspace.numel() * workspace.element_size(), B, n, int(max_nodes), H, KV,
-        D, _code(q.dtype), float(scale), int(max_len), _stream(stream)))
+        ws_bytes = _tree_bytes(q.device.index, max_nodes, H, KV, D, code, max_len)
+        # (held until the launch below: the allocator hands it out again in stream order)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    else:
+        ws_bytes = workspace.numel() * workspace.element_size()
+    _lib.check(lib.b2a_tree_decode(
+        q.data_ptr(), qs[0] if n > 1 else H * D, k_pool.data_ptr(), v_pool.data_ptr(), P, R,
+        pstride[0] if P > 1 else R * KV * D, tptr, tstride, width, lens.data_ptr(), cu.data_ptr(),
+        pptr, out.data_ptr(), _f32("lse", lse, n * H),
+        None if workspace is None else workspace.data_ptr(), ws_bytes, B, n,
+        max_nodes, H, KV, D, code, 1.0 / math.sqrt(D) if scale is None else scale, max_len,
+        _stream(stream, q)))
     return out
 
 
@@ -235,57 +277,53 @@ def constrain_logits(logits: torch.Tensor, cu: torch.Tensor, parents: torch.Tens
     int32: bit v % 32 of word v / 32 allows token v.  Returns (out, picks): out
     defaults to a new f32 tensor (pass out=logits for in place); picks (n,)
     int32, -1 where nothing can be picked."""
-    _need(logits.dim() == 2 and logits.is_cuda and logits.stride(1) == 1, "logits CUDA (n, V)")
     n, V = logits.shape
+    ls = logits.stride()
+    if not logits.is_cuda or ls[1] != 1:
+        _bad("logits must be a CUDA tensor (n, V), unit stride along V")
     B = cu.numel() - 1
     _i32("cu", cu)
-    for name, t in (("parents", parents), ("tokens", tokens)):
-        if t is not None:
-            _i32(name, t)
-            _need(t.numel() >= n, f"{name} must cover the rows")
+    n_hist = n_bias = mstride = 0
+    hptr = sptr = bsptr = biptr = mptr = None
     if hist is not None:
-        _i32("hist", hist)
-        _need(hist_start is not None, "hist needs hist_start")
-        _i32("hist_start", hist_start, B + 1)
-    if prompt_lens is not None:
-        _i32("prompt_lens", prompt_lens, B)
-    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if t is not None:
-            device._cuda_contig(name, t)
-            _need(t.dtype == torch.float32 and t.numel() == B, f"{name} f32 (B,)")
+        if hist_start is None:
+            _bad("hist needs hist_start")
+        n_hist = hist.numel()
+        hptr, sptr = _i32_rows("hist", hist, 0), _i32_rows("hist_start", hist_start, B + 1)
     if bias is not None:
-        _need(bias_start is not None and bias_ids is not None, "bias needs bias_start and bias_ids")
-        _i32("bias_start", bias_start, B + 1)
-        _i32("bias_ids", bias_ids, bias.numel())
-        device._cuda_contig("bias", bias)
-        _need(bias.dtype == torch.float32, "bias f32")
+        if bias_start is None or bias_ids is None:
+            _bad("bias needs bias_start and bias_ids")
+        n_bias = bias.numel()
+        bsptr, biptr = _i32_rows("bias_start", bias_start, B + 1), _i32_rows("bias_ids", bias_ids, n_bias)
     if mask is not None:
-        _need(mask.dtype in (torch.int32, torch.uint32) and mask.is_cuda and mask.dim() == 2 and
-              mask.shape[0] == n and mask.stride(1) == 1 and mask.shape[1] * 32 >= V,
-              "mask int32 (n, V / 32) words")
+        mshape, mstride = mask.shape, mask.stride()
+        if mask.dtype not in (torch.int32, torch.uint32) or not mask.is_cuda or len(mshape) != 2 or (
+                mshape[0] != n or mstride[1] != 1 or mshape[1] * 32 < V):
+            _bad("mask must be a CUDA int32 tensor (n, V / 32) of words")
+        mptr, mstride = mask.data_ptr(), (mstride[0] if n > 1 else mshape[1])
     if out is None:
         out = torch.empty((n, V), dtype=torch.float32, device=logits.device)
-    _need(out.shape == (n, V) and out.is_cuda and out.stride(1) == 1, "out CUDA (n, V)")
+    os = out.stride()
+    if not out.is_cuda or out.shape != (n, V) or os[1] != 1:
+        _bad("out must be a CUDA tensor (n, V), unit stride along V")
+    lib = _lib.load()
+    if workspace is None:
+        ws_bytes = _logits_bytes(n, V)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
+    else:
+        ws_bytes = workspace.numel() * workspace.element_size()
     if picks is None:
         picks = torch.empty(n, dtype=torch.int32, device=logits.device)
     else:
         _i32("picks", picks, n)
-    lib = _lib.load()
-    if workspace is None:
-        workspace = torch.empty(max(lib.b2a_constrain_logits_workspace_bytes(n, V), 16),
-                                dtype=torch.uint8, device=logits.device)
-
-    def stride(t, w):
-        return t.stride(0) if n > 1 else w
-
     _lib.check(lib.b2a_constrain_logits(
-        _ptr(logits), stride(logits, V), _code(logits.dtype), _ptr(out), stride(out, V),
-        _code(out.dtype), _ptr(picks), _ptr(cu), _ptr(parents), _ptr(tokens), _ptr(hist),
-        _ptr(hist_start), 0 if hist is None else hist.numel(), _ptr(prompt_lens),
-        _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_start), _ptr(bias_ids),
-        _ptr(bias), 0 if bias is None else bias.numel(), _ptr(mask),
-        0 if mask is None else stride(mask, mask.shape[1]), B, n, int(max_nodes), V,
-        _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(stream)))
+        logits.data_ptr(), ls[0] if n > 1 else V, _code(logits.dtype), out.data_ptr(),
+        os[0] if n > 1 else V, _code(out.dtype), picks.data_ptr(), cu.data_ptr(),
+        _i32_rows("parents", parents, n), _i32_rows("tokens", tokens, n), hptr, sptr, n_hist,
+        _i32_rows("prompt_lens", prompt_lens, B), _f32("repetition", repetition, B),
+        _f32("presence", presence, B), _f32("frequency", frequency, B), bsptr, biptr,
+        _f32("bias", bias, n_bias), n_bias, mptr, mstride, B, n, max_nodes, V,
+        workspace.data_ptr(), ws_bytes, _stream(stream, logits)))
     return out, picks
 
 
@@ -309,35 +347,31 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     own.  Pools (L, n_pages, page_rows, KV, D) for all layers at once, or one
     layer's 4-D pool; table, lens, cu, parents as in tree_decode (table None:
     (L, B, n_ctx, KV, D) blocks)."""
-    if k_pool.dim() == 4:
-        k_pool, v_pool = k_pool.unsqueeze(0), v_pool.unsqueeze(0)
-    _need(k_pool.dim() == 5 and k_pool.shape == v_pool.shape and k_pool.stride() == v_pool.stride(),
-          "pools (L, n_pages, page_rows, KV, D)")
-    L = k_pool.shape[0]
-    P, R, pstride, KV, D = _pool(k_pool[0], v_pool[0])
+    dims = k_pool.dim()
+    shape, stride = _pool(k_pool, v_pool, 5 if dims == 5 else 4)
+    P, R, KV, D = shape[-4:]
+    L = shape[0] if dims == 5 else 1
     B, n = lens.numel(), tokens.numel()
     _i32("lens", lens)
     _i32("cu", cu, B + 1)
-    _i32("tokens", tokens)
-    _i32("picks", picks)
-    _need(picks.numel() >= n, "picks must cover the tokens")
-    if parents is not None:
-        _i32("parents", parents)
-        _need(parents.numel() >= n, "parents must cover the tokens")
-    tstride, width = _table(table, B)
+    tptr, tstride, width = _table(table, B)
     if max_len is None:
         max_len = width * R if table is not None else R
     if out is None:
-        buf = torch.empty(B * (max_nodes + 3), dtype=torch.int32, device=lens.device)
-        m = B * max_nodes
-        out = Commit(buf[:m].view(B, max_nodes), buf[m:m + B], buf[m + B:m + 2 * B], buf[m + 2 * B:])
+        path, accepted, nxt, lens_out = torch.empty(
+            B * (max_nodes + 3), dtype=torch.int32,
+            device=lens.device).split_with_sizes((B * max_nodes, B, B, B))
+        out = Commit(path.view(B, max_nodes), accepted, nxt, lens_out)
     else:
-        _i32("out.path", out.path, B * max_nodes)
-        for name, t in (("accepted", out.accepted), ("next_token", out.next_token), ("lens", out.lens)):
+        path, accepted, nxt, lens_out = out
+        _i32("out.path", path, B * max_nodes)
+        for name, t in (("accepted", accepted), ("next_token", nxt), ("lens", lens_out)):
             _i32("out." + name, t, B)
     _lib.check(_lib.load().b2a_tree_commit(
-        _ptr(picks), _ptr(tokens), _ptr(parents), _ptr(cu), _ptr(lens), _ptr(table), tstride, width,
-        _ptr(k_pool), _ptr(v_pool), L, k_pool.stride(0) if L > 1 else 0, P, R, pstride, KV, D,
-        _code(k_pool.dtype), B, n, int(max_nodes), int(max_len), _ptr(out.path), _ptr(out.accepted),
-        _ptr(out.next_token), _ptr(out.lens), _stream(stream)))
+        _i32_rows("picks", picks, n), _i32_rows("tokens", tokens, n),
+        _i32_rows("parents", parents, n), cu.data_ptr(), lens.data_ptr(), tptr, tstride, width,
+        k_pool.data_ptr(), v_pool.data_ptr(), L, stride[0] if L > 1 else 0, P, R,
+        stride[-4] if P > 1 else R * KV * D, KV, D, _code(k_pool.dtype), B, n, max_nodes, max_len,
+        path.data_ptr(), accepted.data_ptr(), nxt.data_ptr(), lens_out.data_ptr(),
+        _stream(stream, lens)))
     return out

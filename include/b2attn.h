@@ -524,8 +524,8 @@ int b2a_q8_dequant(const void* codes, long long ldq, const void* scales, long lo
  *   held_out, ring_state_out  the numbers after the step (other buffers than
  *                    held and ring_state: the call can then be repeated)
  *   cu               int32 [B + 1]
- *   seq, pos, slot   int32 [max_tokens], 16-byte aligned: a token's request,
- *                    RoPE position and slot; padding rows get -1, 0, -1
+ *   seq, pos, slot   int32 [max_tokens]: a token's request, RoPE position and
+ *                    slot; padding rows get -1, 0, -1
  * Pages go to the requests in order: request b is served if the pages wanted
  * up to and including its own are there (or it wants none) and its rows fit
  * max_pages; else it keeps what it holds and its tokens' slots are -1. */
@@ -565,9 +565,10 @@ int b2a_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
  *             page_rows without a table); paged caches: page_rows >= 16
  * Padding rows of out become 0 (lse -inf).  16-bit types: tensor cores, f32
  * scores, sums and accumulators, the weights rounded to the type for the
- * product with V.  F32: f32 products and sums.  One node per request is a
+ * product with V.  F32: f32 products and sums.  Short contexts need no workspace
+ * (0 bytes, NULL).  One node per request is a
  * batched decode step. */
-size_t b2a_tree_decode_workspace_bytes(int max_nodes, int H, int KV, int D, int dtype);
+size_t b2a_tree_decode_workspace_bytes(int max_nodes, int H, int KV, int D, int dtype, int max_len);
 int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
                     const void* v_cache, int n_pages, int page_rows, long long page_stride,
                     const int* table_dev, long long table_stride, int table_width,

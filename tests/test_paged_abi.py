@@ -60,7 +60,6 @@ BAD = [
     ("page_plan", dict(held_out=P), _lib.ERR_ARG),
     ("page_plan", dict(state_out=P), _lib.ERR_ARG),
     ("page_plan", dict(ring_size=1 << 28), _lib.ERR_UNSUPPORTED),
-    ("page_plan", dict(pos=P + 4), _lib.ERR_ALIGN),
     ("rope_append_paged", dict(q=None), _lib.ERR_ARG),
     ("rope_append_paged", dict(n_tok=-1), _lib.ERR_ARG),
     ("rope_append_paged", dict(D=63), _lib.ERR_UNSUPPORTED),
@@ -126,7 +125,8 @@ def test_refusals(lib, name, kw, code):
 
 def test_workspace_sizes(lib):
     # two parts per SM of the item's rows: (o, m, l) in f32
-    assert lib.b2a_tree_decode_workspace_bytes(8, 32, 8, 128, F16) >= 2 * 32 * 130 * 4
-    assert lib.b2a_tree_decode_workspace_bytes(0, 32, 8, 128, F16) == 0
+    assert lib.b2a_tree_decode_workspace_bytes(8, 32, 8, 128, F16, 4096) >= 2 * 32 * 130 * 4
+    assert lib.b2a_tree_decode_workspace_bytes(8, 32, 8, 128, F16, 64) == 0
+    assert lib.b2a_tree_decode_workspace_bytes(0, 32, 8, 128, F16, 4096) == 0
     assert lib.b2a_constrain_logits_workspace_bytes(10, 128256) >= 10 * 8
     assert lib.b2a_constrain_logits_workspace_bytes(0, 5) == 0

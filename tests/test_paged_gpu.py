@@ -140,6 +140,44 @@ def test_attention_cut_items(cuda_dev, dt, nodes):
     assert torch.equal(out, s.run())  # and a rerun is bit-identical
 
 
+@pytest.mark.parametrize("dt,D", [("bf16", 64), ("f16", 128), ("bf16", 256), ("f32", 128)])
+@pytest.mark.parametrize("T", [1, 2, 4, 8, 16, 40])
+def test_attention_many_tiles(cuda_dev, dt, D, T):
+    """Every CTA's range is many tiles long: the tile ring goes round several
+    times for each count of query rows (4 to 160).  The definition in 64 bits is
+    evaluated on the device."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, paged
+    g = torch.Generator("cuda").manual_seed(T + D)
+    B, H, KV, page = 12, 16, 4, 32
+    lens = [2500 + 17 * b for b in range(B)]
+    rows = [n + T for n in lens]
+    rng = np.random.default_rng(T)
+    table, pages = ref.deal_pages(rows, page, rng)
+    k = torch.randn((pages, page, KV, D), device=cuda_dev, generator=g).to(TDT[dt])
+    v = torch.randn((pages, page, KV, D), device=cuda_dev, generator=g).to(TDT[dt])
+    q = torch.randn((B * T, H, D), device=cuda_dev, generator=g).to(TDT[dt])
+    trees = [ref.random_tree(T, rng) for _ in range(B)]
+    out = paged.tree_decode(q, k, v, i32(lens, cuda_dev), i32(np.arange(B + 1) * T, cuda_dev),
+                            i32(sum(trees, []), cuda_dev), table=i32(table, cuda_dev), max_nodes=T,
+                            max_len=max(rows))
+    _lib.raise_device_error()
+    for b in range(B):
+        at = torch.from_numpy(table[b, :-(-rows[b] // page)]).long().to(cuda_dev)
+        kb = k[at].flatten(0, 1)[:rows[b]].double().repeat_interleave(H // KV, 1)
+        vb = v[at].flatten(0, 1)[:rows[b]].double().repeat_interleave(H // KV, 1)
+        s = torch.einsum("thd,rhd->htr", q[b * T:(b + 1) * T].double(), kb) / math.sqrt(D)
+        blind = torch.ones((T, T), dtype=torch.bool)
+        for i in range(T):
+            blind[i, ref.chain_of(trees[b], i)] = False
+        s[:, :, lens[b]:].masked_fill_(blind.to(cuda_dev), -math.inf)
+        p = torch.softmax(s, -1)
+        o = torch.einsum("htr,rhd->thd", p, vb)
+        w = torch.einsum("htr,rhd->thd", p, vb.abs())
+        u = UNIT[dt] if dt != "f32" else 0.0
+        err = (out[b * T:(b + 1) * T].double() - o).abs()
+        assert (err <= u * (o.abs() + w) + 2e-4 * w + 1e-7).all(), b
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("page", [0, 16, 128])
 def test_attention_never_written_rows_do_not_leak(cuda_dev, dt, page):
@@ -173,7 +211,7 @@ def test_attention_padding_rows_and_graph(cuda_dev):
     par[:10] = s.dev["parents"]
     out = torch.full((n, 8, 128), float("nan"), device=cuda_dev).to(torch.bfloat16)
     lse = torch.zeros((n, 8), device=cuda_dev)
-    ws = paged.tree_decode_workspace(8, 8, 2, 128, torch.bfloat16, cuda_dev)
+    ws = paged.tree_decode_workspace(8, 8, 2, 128, torch.bfloat16, 928, cuda_dev)
     d = s.dev
 
     def step():
