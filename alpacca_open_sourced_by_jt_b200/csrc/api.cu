@@ -59,7 +59,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 int make_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int rank, void* base,
               const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-              CUtensorMapSwizzle swizzle) {
+              CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   PFN_encodeTiled fn = get_encode_fn();
   if (!fn) return fail(B2A_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
   cuuint64_t d[5];
@@ -73,7 +73,7 @@ int make_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int rank, void* base,
   }
   for (int i = 0; i < rank - 1; ++i) s[i] = strides_bytes[i];
   CUresult r = fn(out, dtype, (cuuint32_t)rank, base, d, s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(B2A_ERR_ARG, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
   return B2A_OK;
 }

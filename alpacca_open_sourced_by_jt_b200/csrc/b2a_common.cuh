@@ -122,6 +122,16 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+
 // L2 prefetch of one tile of a 3-D tensor map (no shared memory, no mbarrier);
 // same coordinate rules as tma_load_3d.
 __device__ __forceinline__ void tma_prefetch_l2_3d(const CUtensorMap* map, int c0, int c1, int c2) {
@@ -235,7 +245,8 @@ int cuda_fail(cudaError_t e, const char* what);
 // bytes for dims 1..rank-1.
 int make_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int rank, void* base,
               const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-              CUtensorMapSwizzle swizzle);
+              CUtensorMapSwizzle swizzle,
+              CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 
 int elem_size(int dtype);
 bool aligned16(const void* p);

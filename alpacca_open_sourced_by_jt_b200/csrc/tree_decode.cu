@@ -16,6 +16,7 @@
 // and tree_merge_kernel joins the parts of items cut between CTAs.
 
 #include <math.h>
+#include <stdlib.h>
 
 #include <atomic>
 
@@ -29,8 +30,8 @@ namespace tree {
 // 16-bit caches, few rows: warp-level MMAs
 // ---------------------------------------------------------------------------
 // One persistent CTA per SM.  A producer warp streams 64-row K and V tiles
-// into a ring with TMA: one box per page piece and 64 columns, each issued by
-// a lane of its own (a tile of 16-row pages takes 4 pieces x D/64 boxes x 2).
+// into a ring with TMA: one box per page piece (all columns of its rows), each
+// issued by a lane of its own (a tile of 16-row pages takes 4 pieces x 2).
 // Eight consumer warps run the decode kernel's fragments (decode.cu):
 // S^T = K.Q^T with the query rows on the MMA's N axis, online softmax on the
 // accumulators, O^T += V^T.P^T.  A warp takes 16 keys of a tile:
@@ -49,8 +50,7 @@ constexpr int kMmaThreads = (kConsumers + 1) * 32;
 template <int D, int NT, bool kByRows>
 struct MmaCfg {
   static constexpr int kBoxes = D / 64;
-  static constexpr int kBoxBytes = kRows * 128;
-  static constexpr int kTileBytes = kBoxes * kBoxBytes;
+  static constexpr int kTileBytes = kBoxes * kRows * 128;
   static constexpr int kStageBytes = 2 * kTileBytes;
   // four warps' states (o, m, l) while the warps of a CTA are joined
   static constexpr int kState = (D / 16 * NT * 4 + NT * 4) * 32 * 4;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
                                              ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    const Start s = locate(bt, blockIdx.x, gridDim.x);
+    const Start s = locate(bt, blockIdx.x / bt.KV);
     if (lane == 0) s_start = s;
   } else if (warp == kConsumers && lane == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
   }
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int kvh = blockIdx.x % bt.KV;
   Walker wk;
   wk.start(bt, s_start);
   Item it;
@@ -103,32 +104,39 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
   if (warp == kConsumers) {
     // ---------------- producer warp ---------------------------------------
     const int pieces = kRows / piece_rows;
-    const int kv = lane & 1, box = (lane >> 1) % C::kBoxes, piece = (lane >> 1) / C::kBoxes;
+    const int kv = lane & 1, piece = lane >> 1;
     const bool mine = piece < pieces;
+    const int bytes = piece_rows * D * 2;  // of one piece: all its columns
     const CUtensorMap* map = kv ? &tmV : &tmK;
     if (lane < 2) tma_prefetch_desc(map);
     uint32_t seq = 0;
     bool ok = true;
     while (ok && wk.next(bt, it)) {
       const int rows = it.len + it.n;
+      // the page of the next tile is looked up while this one waits for room
+      auto page_at = [&](int t) {
+        const int row = t * kRows + piece * piece_rows;
+        return mine && t < it.t1 && row < rows ? page_of(bt, it.b, row) : 0;
+      };
+      int next_pg = page_at(it.t0);
       for (int t = it.t0; t < it.t1; ++t, ++seq) {
         const int row = t * kRows + piece * piece_rows;
         const bool live = mine && row < rows;
-        const int pg = live ? page_of(bt, it.b, row) : 0;
+        const int pg = next_pg;
+        next_pg = page_at(t + 1);
         const int in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
         const int n_live = __popc(__ballot_sync(0xffffffffu, live));
         const int s = seq % C::kStages;
         if (lane == 0) {
           if (seq >= C::kStages)
             ok = mbar_wait(&empty_bar[s], ((seq / C::kStages) & 1) ^ 1, 0x31000 | s);
-          if (ok) mbar_arrive_expect_tx(&full_bar[s], n_live * piece_rows * 128);
+          if (ok) mbar_arrive_expect_tx(&full_bar[s], n_live * bytes);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         if (live)
-          tma_load_4d(smem + s * C::kStageBytes + kv * C::kTileBytes + box * C::kBoxBytes +
-                          piece * piece_rows * 128,
-                      map, &full_bar[s], box * 64, it.kvh, in_page, pg);
+          tma_load_5d(smem + s * C::kStageBytes + kv * C::kTileBytes + piece * bytes, map,
+                      &full_bar[s], 0, in_page, 0, kvh, pg);
       }
     }
     return;
@@ -148,9 +156,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
   const int slice = warp & 3, half = warp >> 2;
   const uint32_t ring = smem_u32(smem);
   float* merge = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
-  const int a_row = slice * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;  // K (non-trans)
+  // A tile is [piece][64-column box][row of the piece][128 bytes]; a warp's 16
+  // rows lie in one piece.
+  const int box_bytes = piece_rows * 128;
+  const int slice_at = (slice * 16 / piece_rows) * piece_rows * D * 2 +
+                       (slice * 16 % piece_rows) * 128;
+  const int a_row = (lane & 7) + ((lane >> 3) & 1) * 8;  // K (non-trans)
   const int a_khalf = lane >> 4;
-  const int v_row = slice * 16 + (lane & 7) + ((lane >> 4) << 3);     // V (trans)
+  const int v_row = (lane & 7) + ((lane >> 4) << 3);     // V (trans)
   const int v_dhalf = (lane >> 3) & 1;
   uint32_t seq = 0;
   int anc_of = -1;   // the request whose masks are in shared memory
@@ -175,7 +188,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
       const int r = row_lo + nt * 8 + g;
       const bool valid = r < R;
       const int node = valid ? r / bt.group : 0;
-      const int head = it.kvh * bt.group + (valid ? r - node * bt.group : 0);
+      const int head = kvh * bt.group + (valid ? r - node * bt.group : 0);
       const T* qr = q + (it.node0 + node) * q_stride + head * D;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -205,7 +218,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
         dead = !__all_sync(0xffffffffu,
                            mbar_wait(&full_bar[s], (seq / C::kStages) & 1, 0x32000 | s));
       if (dead) continue;
-      const uint32_t kt = ring + s * C::kStageBytes;
+      const uint32_t kt = ring + s * C::kStageBytes + slice_at;
       const uint32_t vt = kt + C::kTileBytes;
 
       // Rows past the request's last hold anything (a pool's old rows, or
@@ -215,11 +228,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
       const bool partial = slice0 + 16 > rows;
       if (partial) {
         const int first_bad = max(rows - slice0, 0);
-        uint8_t* vslice = smem + s * C::kStageBytes + C::kTileBytes;
+        uint8_t* vslice = smem + s * C::kStageBytes + C::kTileBytes + slice_at;
         for (int idx = lane; idx < (16 - first_bad) * C::kBoxes * 8; idx += 32) {
-          const int row = slice * 16 + first_bad + idx / (C::kBoxes * 8);
+          const int row = first_bad + idx / (C::kBoxes * 8);
           const int rem = idx % (C::kBoxes * 8);
-          *reinterpret_cast<uint4*>(vslice + (rem >> 3) * C::kBoxBytes + sw128_off(row, rem & 7)) =
+          *reinterpret_cast<uint4*>(vslice + (rem >> 3) * box_bytes + sw128_off(row, rem & 7)) =
               make_uint4(0u, 0u, 0u, 0u);
         }
         __syncwarp();
@@ -231,7 +244,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         uint32_t a[4];
-        ldsm_x4(kt + (ks >> 2) * C::kBoxBytes + sw128_off(a_row, ((ks & 3) << 1) + a_khalf), a[0],
+        ldsm_x4(kt + (ks >> 2) * box_bytes + sw128_off(a_row, ((ks & 3) << 1) + a_khalf), a[0],
                 a[1], a[2], a[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(sc[nt], a, qf[nt][ks]);
@@ -286,7 +299,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
       for (int mt = 0; mt < KS; ++mt) {
         uint32_t a[4];
         const int dchunk = 2 * mt + v_dhalf;
-        ldsm_x4_trans(vt + (dchunk >> 3) * C::kBoxBytes + sw128_off(v_row, dchunk & 7), a[0], a[1],
+        ldsm_x4_trans(vt + (dchunk >> 3) * box_bytes + sw128_off(v_row, dchunk & 7), a[0], a[1],
                       a[2], a[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(o[mt][nt], a, pb[nt]);
@@ -394,7 +407,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
       for (int i = threadIdx.x; i < live * (D / 8); i += kConsumers * 32) {
         const int r = i / (D / 8), d = (i - r * (D / 8)) * 8;
         const int rr = it.blk * RB + r, node = rr / bt.group;
-        const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + it.kvh * bt.group + (rr - node * bt.group);
+        const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + kvh * bt.group + (rr - node * bt.group);
         const float* x = fin + r * kPad + d;
         uint4 u;
         u.x = MmaOp<T>::pack(x[0], x[1]);
@@ -450,7 +463,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
   float* ps = qs + C::kQ;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 0) {
-    const Start s = locate(bt, blockIdx.x, gridDim.x);
+    const Start s = locate(bt, blockIdx.x / bt.KV);
     if (lane == 0) s_start = s;
   }
   __syncthreads();
@@ -462,6 +475,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
       if (lse && lane == 0) lse[r] = -INFINITY;
     }
   }
+  const int kvh = blockIdx.x % bt.KV;
   Walker wk;
   wk.start(bt, s_start);
   Item it;
@@ -482,7 +496,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
       const int rr = it.blk * kF32Rows + r;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (rr < R) {
-        const int node = rr / bt.group, head = it.kvh * bt.group + rr - node * bt.group;
+        const int node = rr / bt.group, head = kvh * bt.group + rr - node * bt.group;
         x = *reinterpret_cast<const float4*>(q + (it.node0 + node) * q_stride + head * D + d);
       }
       *reinterpret_cast<float4*>(qs + r * C::kKStride + d) = x;
@@ -508,7 +522,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
           in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
         }
         const size_t src = live ? static_cast<size_t>(pg) * page_stride +
-                                      (static_cast<size_t>(in_page) * bt.KV + it.kvh) * D + d
+                                      (static_cast<size_t>(in_page) * bt.KV + kvh) * D + d
                                 : 0;
         const int bytes = live ? 16 : 0;  // rows past the end are filled with zeros
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
@@ -649,7 +663,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
         }
       } else {
         const int gr = it.blk * kF32Rows + rr, node = gr / bt.group;
-        const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + it.kvh * bt.group + (gr - node * bt.group);
+        const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + kvh * bt.group + (gr - node * bt.group);
         const float f = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int c = 0; c < kCols; ++c) out[row * D + oc + c * 128] = o[r][c] * f;
@@ -664,18 +678,18 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
 // ---------------------------------------------------------------------------
 // Block (c, y) looks at the last item of CTA c's range: if the item goes on
 // past the range and does not begin before it, its parts are CTA c's slot
-// 2c + 1, the same slot of every CTA the item fills, and slot 2e of the CTA e
-// where it ends.  One warp per query row.
+// 2c + 1, the same slot of every later CTA of the head that the item fills,
+// and slot 2e of the CTA e where it ends.  One warp per query row.
 constexpr int kMergeWarps = 8;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
     const __grid_constant__ Batch bt, const float* __restrict__ part_o,
-    const float* __restrict__ part_ml, T* __restrict__ out, float* __restrict__ lse, int G) {
+    const float* __restrict__ part_ml, T* __restrict__ out, float* __restrict__ lse) {
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x;
-  const Start s = locate(bt, c, G);
+  const int c = blockIdx.x, kvh = c % bt.KV;
+  const Start s = locate(bt, c / bt.KV);
   if (s.left < s.chunk) return;  // an empty range, or the list's last
   // the item that holds the range's last tile
   int b = s.b, n, len;
@@ -689,21 +703,19 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
     u = units_of(bt, n, len);
   }
   const int tiles = (len + n + bt.tile - 1) / bt.tile;
-  const int idx = static_cast<int>(off / tiles);
-  const int at = static_cast<int>(off - static_cast<long long>(idx) * tiles);
+  const int blk = static_cast<int>(off / tiles);
+  const int at = static_cast<int>(off - static_cast<long long>(blk) * tiles);
   const int after = tiles - 1 - at;  // tiles past the range
   if (after == 0 || at >= s.chunk) return;
-  const int whole = static_cast<int>(after / s.chunk);  // later CTAs the item fills
+  const int whole = static_cast<int>(after / s.chunk);  // later ranges the item fills
   const int rest = static_cast<int>(after - whole * s.chunk);
   const int parts = 1 + whole + (rest > 0 ? 1 : 0);
   const int RB = bt.rows_per_block;
-  const int blks = blocks_of(bt, n);
-  const int kvh = idx / blks, blk = idx - kvh * blks;
   const int live = min(RB, n * bt.group - blk * RB);
   const int node0 = bt.cu[b];
   // A part that ends exactly with its CTA's range is that CTA's slot 2e.
   auto slot = [&](int i) {
-    return 2 * (c + i) + ((i == parts - 1) ? 0 : 1);
+    return 2 * (c + i * bt.KV) + ((i == parts - 1) ? 0 : 1);
   };
   for (int r = blockIdx.y * kMergeWarps + warp; r < live; r += gridDim.y * kMergeWarps) {
     float M = -INFINITY;
@@ -806,16 +818,28 @@ cudaError_t allow_smem(K kern, int smem, std::atomic<unsigned long long>& done) 
   return e;
 }
 
-// Query rows of an item, by type and by the most rows a KV head can have.
-int tree_rows_per_block(int dtype, int rows) {
-  if (dtype == B2A_F32) return TR::kF32Rows;
-  return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
+// Which kernel, by type and by the most rows a KV head can have.
+enum TreeKernel { kTreeF32, kTreeMma, kTreeWide };
+
+TreeKernel tree_kernel(int dtype, int rows, int D) {
+  if (dtype == B2A_F32) return kTreeF32;
+  if (getenv("B2A_TREE_NARROW")) return kTreeMma;
+  return rows <= (D > 128 ? 8 : 16) ? kTreeMma : kTreeWide;
 }
 
-// Keys of a tile, and whether CTAs take whole items: for short contexts one
-// launch without parts to join costs less than cutting the items.
-int tree_tile(int dtype, int D) { return dtype == B2A_F32 && D > 128 ? 32 : TR::kRows; }
-bool tree_by_item(int max_len, int tile) { return (max_len + tile - 1) / tile <= 8; }
+// Query rows of an item, keys of a tile, and whether CTAs take whole items
+// (short contexts: one launch without parts to join costs less than cutting).
+int tree_rows_per_block(TreeKernel k, int rows, int group) {
+  if (k == kTreeF32) return TR::kF32Rows;
+  if (k == kTreeWide) return TR::kWideM / group * group;
+  return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
+}
+int tree_tile(TreeKernel k, int D) {
+  if (k == kTreeF32) return D > 128 ? 32 : 64;
+  if (k == kTreeWide) return D > 128 ? 64 : 128;
+  return TR::kRows;
+}
+bool tree_by_item(int max_len) { return max_len <= 512; }
 
 struct TreeArgs {
   const void *q, *k, *v;
@@ -823,6 +847,7 @@ struct TreeArgs {
   void* out;
   float *lse, *part_o, *part_ml;
   int D, dtype, page_rows, grid;
+  TreeKernel kernel;
   float sscale;
   bool merge;
   TR::Batch bt;
@@ -837,24 +862,28 @@ int tree_merge(const TreeArgs& a) {
                                       dim3(TR::kMergeWarps * 32), 0, a.st, a.bt,
                                       const_cast<const float*>(a.part_o),
                                       const_cast<const float*>(a.part_ml),
-                                      static_cast<T*>(a.out), a.lse, a.grid);
+                                      static_cast<T*>(a.out), a.lse);
   return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "tree_decode merge launch");
 }
 
-// Tensor map of a pool: columns, KV heads, rows of a page, pages.
-int tree_map(CUtensorMap* m, const TreeArgs& a, const void* base, int box_rows) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(a.D), static_cast<uint64_t>(a.bt.KV),
-                            static_cast<uint64_t>(a.page_rows),
-                            static_cast<uint64_t>(a.bt.n_pages)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(a.D) * 2,
-                               static_cast<uint64_t>(a.bt.KV) * a.D * 2,
+// Tensor map of a pool for boxes of box_rows rows x box_cols x 64 columns,
+// written as [64-column box][row][128 bytes]: 64 columns, rows of a page, column
+// boxes, KV heads, pages.  L2 fetches no more than a row of one head (128
+// bytes for D = 64): the next head's bytes are another CTA's.
+int tree_map(CUtensorMap* m, const TreeArgs& a, const void* base, int box_rows, int box_cols) {
+  const uint64_t dims[5] = {64, static_cast<uint64_t>(a.page_rows), static_cast<uint64_t>(a.D / 64),
+                            static_cast<uint64_t>(a.bt.KV), static_cast<uint64_t>(a.bt.n_pages)};
+  const uint64_t strides[4] = {static_cast<uint64_t>(a.bt.KV) * a.D * 2, 128,
+                               static_cast<uint64_t>(a.D) * 2,
                                static_cast<uint64_t>(a.page_stride) * 2};
-  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(box_rows), 1};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(box_rows), static_cast<uint32_t>(box_cols), 1, 1};
   return b2a_host::make_tmap(m,
                              a.dtype == B2A_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                             4, const_cast<void*>(base), dims, strides, box,
-                             CU_TENSOR_MAP_SWIZZLE_128B);
+                             5, const_cast<void*>(base), dims, strides, box,
+                             CU_TENSOR_MAP_SWIZZLE_128B,
+                             a.D > 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                      : CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 template <typename T, int D, int NT, bool kByRows>
@@ -866,8 +895,8 @@ int tree_mma(const TreeArgs& a) {
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "cudaFuncSetAttribute(tree_decode)");
   const int piece = a.bt.table && a.page_rows < TR::kRows ? a.page_rows : TR::kRows;
   CUtensorMap tk, tv;
-  int rc = tree_map(&tk, a, a.k, piece);
-  if (rc == B2A_OK) rc = tree_map(&tv, a, a.v, piece);
+  int rc = tree_map(&tk, a, a.k, piece, D / 64);
+  if (rc == B2A_OK) rc = tree_map(&tv, a, a.v, piece, D / 64);
   if (rc) return rc;
   e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kMmaThreads), smem, a.st, tk, tv, a.bt,
                        static_cast<const T*>(a.q), a.q_stride, static_cast<T*>(a.out), a.lse,
@@ -877,7 +906,38 @@ int tree_mma(const TreeArgs& a) {
 }
 
 template <typename T, int D>
+int tree_wide(const TreeArgs& a) {
+  auto kern = TR::tree_wide_kernel<T, D>;
+  using C = TR::WideCfg<D>;
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_smem(kern, C::kSmem, done);
+  if (e != cudaSuccess) return b2a_host::cuda_fail(e, "cudaFuncSetAttribute(tree_wide)");
+  const int piece = a.bt.table && a.page_rows < C::kBN ? a.page_rows : C::kBN;
+  const int cols = piece == C::kBN ? D / 64 : 1;
+  CUtensorMap tq, tk, tv;
+  int rc = tree_map(&tk, a, a.k, piece, cols);
+  if (rc == B2A_OK) rc = tree_map(&tv, a, a.v, piece, cols);
+  // q as nodes of [H][D]: a box is the rows of one KV head's group x the
+  // block's nodes
+  const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.bt.H),
+                            static_cast<uint64_t>(a.bt.n_tok)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(D) * 2, static_cast<uint64_t>(a.q_stride) * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(a.bt.group),
+                           static_cast<uint32_t>(a.bt.rows_per_block / a.bt.group)};
+  if (rc == B2A_OK)
+    rc = b2a_host::make_tmap(&tq, a.dtype == B2A_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                             3, const_cast<void*>(a.q), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kWideThreads), C::kSmem, a.st, tq, tk, tv, a.bt,
+                       static_cast<T*>(a.out), a.lse, a.part_o, a.part_ml, piece, a.sscale);
+  if (e != cudaSuccess) return b2a_host::cuda_fail(e, "tree_wide launch");
+  return tree_merge<T, D>(a);
+}
+
+template <typename T, int D>
 int tree_16bit(const TreeArgs& a) {
+  if (a.kernel == kTreeWide) return tree_wide<T, D>(a);
   if (a.bt.rows_per_block == 8) return tree_mma<T, D, 1, false>(a);
   if (a.bt.rows_per_block == 16) return tree_mma<T, D, 2, false>(a);
   return tree_mma<T, D, 2, true>(a);
@@ -900,13 +960,19 @@ int tree_f32(const TreeArgs& a) {
 
 template <int D>
 int tree_dispatch(const TreeArgs& a) {
-  if (a.dtype == B2A_F32) return tree_f32<D>(a);
+  if (a.kernel == kTreeF32) return tree_f32<D>(a);
   if (a.dtype == B2A_BF16) return tree_16bit<__nv_bfloat16, D>(a);
   return tree_16bit<__half, D>(a);
 }
 
-size_t tree_part_o_bytes(int D, int rows_per_block) {
-  return static_cast<size_t>(2) * b2a_host::sm_count() * rows_per_block * D * sizeof(float);
+// CTAs of a grid of teams: as many whole teams as there are SMs for.
+int tree_ctas(int KV) {
+  const int teams = b2a_host::sm_count() / KV;
+  return (teams > 0 ? teams : 1) * KV;
+}
+
+size_t tree_part_o_bytes(int D, int KV, int rows_per_block) {
+  return static_cast<size_t>(2) * tree_ctas(KV) * rows_per_block * D * sizeof(float);
 }
 
 int log2_of(int x) {
@@ -923,10 +989,10 @@ extern "C" {
 
 size_t b2a_tree_decode_workspace_bytes(int max_nodes, int H, int KV, int D, int dtype, int max_len) {
   if (max_nodes <= 0 || H <= 0 || KV <= 0 || D <= 0 || H % KV != 0) return 0;
-  if (tree_by_item(max_len, tree_tile(dtype, D))) return 0;
-  const int rb = tree_rows_per_block(dtype, max_nodes * (H / KV));
-  return tree_part_o_bytes(D, rb) +
-         static_cast<size_t>(2) * b2a_host::sm_count() * rb * 2 * sizeof(float);
+  if (tree_by_item(max_len)) return 0;
+  const int rows = max_nodes * (H / KV);
+  const int rb = tree_rows_per_block(tree_kernel(dtype, rows, D), rows, H / KV);
+  return tree_part_o_bytes(D, KV, rb) + static_cast<size_t>(2) * tree_ctas(KV) * rb * 2 * sizeof(float);
 }
 
 int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
@@ -979,18 +1045,20 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
 
   TreeArgs a = {};
   const int rows = max_nodes * group;
-  const int rb = tree_rows_per_block(dtype, rows);
-  const int tile = tree_tile(dtype, D);
+  a.kernel = tree_kernel(dtype, rows, D);
+  const int rb = tree_rows_per_block(a.kernel, rows, group);
+  const int tile = tree_tile(a.kernel, D);
   a.bt = TR::Batch{lens_dev, cu_dev, parents_dev, table_dev, table_stride, B, n_tok, max_nodes,
-                   max_len, n_pages, table_dev ? log2_of(page_rows) : 0, H, KV, group, rb, tile, 0, 1};
-  // The tiles are cut evenly over the SMs, at least 4 to a CTA.
+                   max_len, n_pages, table_dev ? log2_of(page_rows) : 0, H, KV, group, rb, tile, 0, 1, 1};
+  // A head's tiles are cut evenly over the teams, at least 4 to a CTA.
   const long long max_tiles = (max_len + tile - 1) / tile;
-  const long long items = static_cast<long long>(B) * KV * ((rows + rb - 1) / rb);
-  a.bt.by_item = tree_by_item(max_len, tile) ? 1 : 0;
+  const long long items = static_cast<long long>(B) * ((rows + rb - 1) / rb);
+  a.bt.by_item = tree_by_item(max_len) ? 1 : 0;
   a.bt.min_units = a.bt.by_item ? 1 : 4;
   const long long units = a.bt.by_item ? items : (items * max_tiles + 3) / 4;
-  const int sms = b2a_host::sm_count();
-  a.grid = static_cast<int>(units < sms ? units : sms);
+  const int teams = tree_ctas(KV) / KV;
+  a.bt.teams = static_cast<int>(units < teams ? units : teams);
+  a.grid = a.bt.teams * KV;
   a.merge = !a.bt.by_item;
   if (a.merge) {
     const size_t need = b2a_tree_decode_workspace_bytes(max_nodes, H, KV, D, dtype, max_len);
@@ -1005,7 +1073,7 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
   a.out = out;
   a.lse = lse_out;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + tree_part_o_bytes(D, rb)) : nullptr;
+  a.part_ml = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + tree_part_o_bytes(D, KV, rb)) : nullptr;
   a.D = D;
   a.dtype = dtype;
   a.page_rows = page_rows;

@@ -1,16 +1,19 @@
 // Work division of the tree attention over a cache (tree_decode.cu,
 // tree_wide.cu): what every kernel of it shares.
 //
-// The work is a list of items (request, KV head, block of query rows), each
-// as long as its request's key tiles.  Lengths live on the device, so the
-// division is made there: the list's tiles are numbered through and CTA c of
-// G takes tiles [c * chunk, (c + 1) * chunk), chunk = ceil(total / G).  Every
-// CTA so streams the same number of tiles whatever the lengths, and at most
-// one item is cut at each CTA boundary.  An item wholly inside one CTA's
-// range is finished there; the parts of a cut item go to the workspace and
-// tree_merge_kernel joins them.  CTA c writes at most two parts: slot 2c for
-// an item that began before its range and ends in it, slot 2c + 1 for one
-// that goes on past its range.
+// The grid is teams x KV heads: CTA c reads KV head c % KV, and the KV CTAs of
+// a team do the same work for their heads side by side, so the rows of a cache
+// page (all heads of a token behind one another) are read together.  A head's
+// work is a list of items (request, block of query rows), each as long as its
+// request's key tiles.  Lengths live on the device, so the division is made
+// there: the list's tiles are numbered through and team i takes tiles
+// [i * chunk, (i + 1) * chunk), chunk = ceil(total / teams) or a least number
+// of tiles where that is more.  Every CTA so streams the same number of tiles
+// whatever the lengths, and at most one item is cut at each boundary.  An item
+// wholly inside one range is finished there; the parts of a cut item go to the
+// workspace and tree_merge_kernel joins them.  CTA c writes at most two parts:
+// slot 2c for an item that began before its range and ends in it, slot 2c + 1
+// for one that goes on past its range.
 #pragma once
 
 #include "b2a_common.cuh"
@@ -35,7 +38,8 @@ struct Batch {
   int rows_per_block;  // query rows of an item
   int tile;            // keys per tile
   int by_item;         // CTAs take whole items (no parts)
-  int min_units;       // least tiles of a CTA's range
+  int min_units;       // least tiles of a range
+  int teams;           // ranges a head's list is cut into
 };
 
 // Nodes and cache rows of request b; a request whose numbers are out of
@@ -58,20 +62,20 @@ __device__ __forceinline__ int blocks_of(const Batch& bt, int n) {
 
 __device__ __forceinline__ long long units_of(const Batch& bt, int n, int len) {
   if (n == 0) return 0;
-  const long long items = static_cast<long long>(bt.KV) * blocks_of(bt, n);
+  const long long items = blocks_of(bt, n);
   return bt.by_item ? items : items * ((len + n + bt.tile - 1) / bt.tile);
 }
 
-// Start of a CTA's range.
+// Start of a team's range.
 struct Start {
   long long off;    // units into request b
-  long long left;   // units of this CTA
-  long long chunk;  // units per CTA
+  long long left;   // units of this team
+  long long chunk;  // units per team
   int b;
 };
 
-// Warp-collective: the range of CTA c of G.
-__device__ __forceinline__ Start locate(const Batch& bt, int c, int G) {
+// Warp-collective: the range of one team.
+__device__ __forceinline__ Start locate(const Batch& bt, int team) {
   const int lane = threadIdx.x & 31;
   long long total = 0;
   for (int b = lane; b < bt.B; b += 32) {
@@ -82,9 +86,9 @@ __device__ __forceinline__ Start locate(const Batch& bt, int c, int G) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   Start s;
-  s.chunk = (total + G - 1) / G;
+  s.chunk = (total + bt.teams - 1) / bt.teams;
   if (s.chunk < bt.min_units) s.chunk = bt.min_units;
-  const long long first = s.chunk * c;
+  const long long first = s.chunk * team;
   s.left = total - first;
   if (s.left > s.chunk) s.left = s.chunk;
   s.b = bt.B;
@@ -119,7 +123,7 @@ __device__ __forceinline__ Start locate(const Batch& bt, int c, int G) {
 }
 
 struct Item {
-  int b, kvh, blk;
+  int b, blk;
   int n, len;     // the request's nodes and cached rows
   int t0, t1;     // this CTA's key tiles of the item
   int tiles;      // the item's key tiles
@@ -150,15 +154,12 @@ struct Walker {
       it.len = len;
       it.tiles = (len + n + bt.tile - 1) / bt.tile;
       const int per = bt.by_item ? 1 : it.tiles;
-      const int idx = static_cast<int>(off / per);
-      const int at = static_cast<int>(off - static_cast<long long>(idx) * per);
+      it.blk = static_cast<int>(off / per);
+      const int at = static_cast<int>(off - static_cast<long long>(it.blk) * per);
       int take = per - at;
       if (take > left) take = static_cast<int>(left);
       it.t0 = bt.by_item ? 0 : at;
       it.t1 = bt.by_item ? it.tiles : at + take;
-      const int blks = blocks_of(bt, n);
-      it.kvh = idx / blks;
-      it.blk = idx - it.kvh * blks;
       it.node0 = bt.cu[b];
       off += take;
       left -= take;
