@@ -15,6 +15,7 @@
 //   tree_f32_kernel   f32 caches, f32 FMAs
 // and tree_merge_kernel joins the parts of items cut between CTAs.
 
+#include <limits.h>
 #include <math.h>
 #include <stdlib.h>
 
@@ -29,9 +30,9 @@ namespace tree {
 // ---------------------------------------------------------------------------
 // 16-bit caches, few rows: warp-level MMAs
 // ---------------------------------------------------------------------------
-// One persistent CTA per SM.  A producer warp streams 64-row K and V tiles
-// into a ring with TMA: one box per page piece (all columns of its rows), each
-// issued by a lane of its own (a tile of 16-row pages takes 4 pieces x 2).
+// One persistent CTA per SM.  Producer warps stream 64-row K and V tiles into a
+// ring with TMA: one box per page piece, all columns of its rows (a tile of
+// 16-row pages takes 4 pieces x 2).
 // Eight consumer warps run the decode kernel's fragments (decode.cu):
 // S^T = K.Q^T with the query rows on the MMA's N axis, online softmax on the
 // accumulators, O^T += V^T.P^T.  A warp takes 16 keys of a tile:
@@ -45,7 +46,8 @@ namespace tree {
 // pre-scaled: the scale goes onto the f32 scores.
 constexpr int kRows = 64;
 constexpr int kConsumers = 8;
-constexpr int kMmaThreads = (kConsumers + 1) * 32;
+constexpr int kProducers = 4;
+constexpr int kMmaThreads = (kConsumers + kProducers) * 32;
 
 template <int D, int NT, bool kByRows>
 struct MmaCfg {
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
     if (lane == 0) s_start = s;
   } else if (warp == kConsumers && lane == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], min(kProducers, 2 * (kRows / piece_rows)));
       mbar_init(&empty_bar[s], kByRows ? kConsumers : kConsumers / 2);
     }
     fence_mbar_init();
@@ -101,42 +103,51 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
   wk.start(bt, s_start);
   Item it;
 
-  if (warp == kConsumers) {
-    // ---------------- producer warp ---------------------------------------
-    const int pieces = kRows / piece_rows;
-    const int kv = lane & 1, piece = lane >> 1;
-    const bool mine = piece < pieces;
-    const int bytes = piece_rows * D * 2;  // of one piece: all its columns
-    const CUtensorMap* map = kv ? &tmV : &tmK;
-    if (lane < 2) tma_prefetch_desc(map);
-    uint32_t seq = 0;
-    bool ok = true;
-    while (ok && wk.next(bt, it)) {
-      const int rows = it.len + it.n;
-      // the page of the next tile is looked up while this one waits for room
-      auto page_at = [&](int t) {
-        const int row = t * kRows + piece * piece_rows;
-        return mine && t < it.t1 && row < rows ? page_of(bt, it.b, row) : 0;
-      };
-      int next_pg = page_at(it.t0);
-      for (int t = it.t0; t < it.t1; ++t, ++seq) {
-        const int row = t * kRows + piece * piece_rows;
-        const bool live = mine && row < rows;
-        const int pg = next_pg;
-        next_pg = page_at(t + 1);
-        const int in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
-        const int n_live = __popc(__ballot_sync(0xffffffffu, live));
-        const int s = seq % C::kStages;
-        if (lane == 0) {
-          if (seq >= C::kStages)
-            ok = mbar_wait(&empty_bar[s], ((seq / C::kStages) & 1) ^ 1, 0x31000 | s);
-          if (ok) mbar_arrive_expect_tx(&full_bar[s], n_live * bytes);
+  if (warp >= kConsumers) {
+    // ---------------- producer warps --------------------------------------
+    // A TMA issue takes a thread about a hundred cycles (its operands move to
+    // uniform registers), so the boxes of a tile, K and V of each page piece,
+    // are dealt to the producer warps; each warp's first lane issues its own.
+    const int p = warp - kConsumers;
+    const int boxes = 2 * (kRows / piece_rows);
+    const int bytes = piece_rows * D * 2;
+    if (p < boxes && lane == 0) {
+      const CUtensorMap* map = (p & 1) ? &tmV : &tmK;
+      tma_prefetch_desc(map);
+      uint8_t* dst = smem + (p & 1) * C::kTileBytes;
+      uint32_t s = 0, round = 0;
+      bool ok = true;
+      while (ok && wk.next(bt, it)) {
+        const int rows = it.len + it.n;
+        // the pages of the next tile are looked up while this one waits for room
+        const int at0 = (p >> 1) * piece_rows, at1 = at0 + (kProducers / 2) * piece_rows;
+        auto entry = [&](int t, int at) {
+          const int row = t * kRows + at;
+          return t < it.t1 && at < kRows && row < rows ? table_entry(bt, it.b, row) : 0;
+        };
+        int pg0 = entry(it.t0, at0), pg1 = entry(it.t0, at1);
+        for (int t = it.t0; t < it.t1; ++t) {
+          const int row0 = t * kRows + at0, row1 = t * kRows + at1;
+          const bool live0 = row0 < rows, live1 = at1 < kRows && row1 < rows;
+          const int now0 = live0 ? checked_page(bt, it.b, pg0) : 0;
+          const int now1 = live1 ? checked_page(bt, it.b, pg1) : 0;
+          pg0 = entry(t + 1, at0);
+          pg1 = entry(t + 1, at1);
+          if (round > 0 && !mbar_wait(&empty_bar[s], (round & 1) ^ 1, 0x31000 | s)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full_bar[s], (live0 ? bytes : 0) + (live1 ? bytes : 0));
+          const int mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
+          uint8_t* at = dst + s * C::kStageBytes + (p >> 1) * bytes;
+          if (live0) tma_load_5d(at, map, &full_bar[s], 0, row0 & mask, 0, kvh, now0);
+          if (live1)
+            tma_load_5d(at + (kProducers / 2) * bytes, map, &full_bar[s], 0, row1 & mask, 0, kvh, now1);
+          if (++s == C::kStages) {
+            s = 0;
+            ++round;
+          }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
-        if (live)
-          tma_load_5d(smem + s * C::kStageBytes + kv * C::kTileBytes + piece * bytes, map,
-                      &full_bar[s], 0, in_page, 0, kvh, pg);
       }
     }
     return;
@@ -517,8 +528,8 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
         int pg = 0, in_page = 0;
         bool live = row < rows;
         if (live) {
-          pg = page_of(bt, it.b, row);
-          live = bt.table == nullptr || pg < bt.n_pages;
+          pg = checked_page(bt, it.b, table_entry(bt, it.b, row));
+          live = pg < bt.n_pages;
           in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
         }
         const size_t src = live ? static_cast<size_t>(pg) * page_stride +

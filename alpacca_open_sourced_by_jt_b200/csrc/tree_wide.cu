@@ -17,11 +17,12 @@
 // tiles relative to the last maximum it used; they meet at the item's end.
 // Warps whose 32 rows hold no query do nothing but pass the barriers.
 //
-// 320 threads: warp 0 TMA producer (a lane per box: page piece x 64 columns, or
-// a whole tile where a page holds it), warp 1 TMEM owner and MMA issuer, warps
-// 2-9 softmax (TMEM lane quarter = warp % 4).  About 200 registers a thread
-// without moving any between warps.
+// 384 threads: warp 0 TMA producer of Q and K, warp 2 of V (a box per page
+// piece and 64 columns, or one per tile where a page holds it), warp 1 TMEM
+// owner and MMA issuer, warps 4-11 softmax (TMEM lane quarter = warp % 4).
 // TMEM: S0 [0, BN), S1 [BN, 2 BN), O [2 BN, 2 BN + D).
+
+#include <limits.h>
 
 #include "b2a_common.cuh"
 #include "tree_work.cuh"
@@ -43,7 +44,7 @@ using prefill::tc_st32;
 using prefill::tc_wait_ld;
 using prefill::tc_wait_st;
 
-constexpr int kWideThreads = 320;
+constexpr int kWideThreads = 384;
 constexpr int kWideM = 128;
 
 template <int D>
@@ -118,61 +119,60 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
   wk.start(bt, s_start);
   Item it;
 
-  if (warp == 0) {
-    // ------------------------------ TMA producer ---------------------------
-    const int boxes = piece_rows == BN ? 1 : D / 64;  // boxes of a page piece
-    const int pieces = BN / piece_rows;
-    const int box = lane % boxes, piece = lane / boxes;
-    const bool mine = piece < pieces;
-    const int bytes = piece_rows * 128 * (piece_rows == BN ? D / 64 : 1);
-    if (lane == 0) tma_prefetch_desc(&tmQ);
-    if (lane == 1) tma_prefetch_desc(&tmK);
-    if (lane == 2) tma_prefetch_desc(&tmV);
-    uint32_t seq = 0, qcnt = 0;
-    bool ok = true;
-    while (ok && wk.next(bt, it)) {
-      const int rows = it.len + it.n;
-      auto page_at = [&](int t) {
-        const int row = t * BN + piece * piece_rows;
-        return mine && t < it.t1 && row < rows ? page_of(bt, it.b, row) : 0;
-      };
-      int next_pg = page_at(it.t0);
-      if (lane == 0) {
-        if (qcnt > 0) ok = mbar_wait(&bar_qe, (qcnt - 1) & 1, 0x33000);
-        if (ok) {
+  if (warp == 0 || warp == 2) {
+    // ------------------------------ TMA producers --------------------------
+    // one lane per warp issues: warp 0 loads Q and K, warp 2 loads V
+    const int kv = warp >> 1;
+    const CUtensorMap* map = kv ? &tmV : &tmK;
+    const bool whole = piece_rows == BN;  // a page holds a tile: one box for it
+    const int bytes = piece_rows * 128 * (whole ? D / 64 : 1);
+    if (lane == 0) {
+      if (kv == 0) tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(map);
+      uint32_t seq = kv, qcnt = 0;  // K tiles take the ring's even numbers, V tiles the odd ones
+      bool ok = true;
+      const int mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
+      while (ok && wk.next(bt, it)) {
+        const int rows = it.len + it.n;
+        int next_pg = table_entry(bt, it.b, it.t0 * BN);
+        if (kv == 0) {
+          if (qcnt > 0 && !mbar_wait(&bar_qe, (qcnt - 1) & 1, 0x33000)) break;
           mbar_arrive_expect_tx(&bar_qf, (D / 64) * bt.rows_per_block * 128);
 #pragma unroll
           for (int b = 0; b < D / 64; ++b)
             tma_load_3d(smem + b * C::kBoxQ, &tmQ, &bar_qf, b * 64, kvh * bt.group,
                         it.node0 + it.blk * block_nodes);
+          ++qcnt;
         }
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      ++qcnt;
-      for (int t = it.t0; ok && t < it.t1; ++t) {
-        const int row = t * BN + piece * piece_rows;
-        const bool live = mine && row < rows;
-        const int pg = next_pg;
-        next_pg = page_at(t + 1);
-        const int in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
-        const int n_live = __popc(__ballot_sync(0xffffffffu, live));
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++seq) {
+        for (int t = it.t0; t < it.t1; ++t, seq += 2) {
+          const int row0 = t * BN;
+          const int pieces = (min(BN, rows - row0) + piece_rows - 1) / piece_rows;  // with rows
           const int slot = seq % kSlots;
-          if (lane == 0) {
-            if (seq >= kSlots)
-              ok = mbar_wait(&bar_empty[slot], ((seq / kSlots) & 1) ^ 1, 0x34000 | slot);
-            if (ok) mbar_arrive_expect_tx(&bar_full[slot], n_live * bytes);
+          if (seq >= kSlots && !mbar_wait(&bar_empty[slot], ((seq / kSlots) & 1) ^ 1, 0x34000 | slot)) {
+            ok = false;
+            break;
           }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          if (live)
-            tma_load_5d(smem + C::kRing + slot * C::kTileKV + box * C::kBoxKV +
-                            piece * piece_rows * 128,
-                        kv ? &tmV : &tmK, &bar_full[slot], 0, in_page, box, kvh, pg);
+          uint8_t* dst = smem + C::kRing + slot * C::kTileKV;
+          mbar_arrive_expect_tx(&bar_full[slot], pieces * bytes * (whole ? 1 : D / 64));
+          if (whole) {
+            const int pg = checked_page(bt, it.b, next_pg);
+            if (t + 1 < it.t1) next_pg = table_entry(bt, it.b, row0 + BN);
+            tma_load_5d(dst, map, &bar_full[slot], 0, row0 & mask, 0, kvh, pg);
+          } else {
+            for (int i = 0; i < pieces; ++i) {
+              const int pg = checked_page(bt, it.b, next_pg);
+              const int row = row0 + i * piece_rows, next = row + piece_rows;
+              if (next < rows && next < it.t1 * BN) next_pg = table_entry(bt, it.b, next);
+#pragma unroll
+              for (int b = 0; b < D / 64; ++b)
+                tma_load_5d(dst + b * C::kBoxKV + i * piece_rows * 128, map, &bar_full[slot], 0,
+                            row & mask, b, kvh, pg);
+            }
+          }
         }
       }
     }
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------ MMA issuer -----------------------------
     if (lane == 0) {
@@ -235,9 +235,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp >= 4) {
     // ------------------------------ softmax ----------------------------------
-    const int w = (warp - 2) >> 2;                 // warpgroup: tiles jj % 2 == w
+    const int w = (warp - 4) >> 2;                 // warpgroup: tiles jj % 2 == w
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;             // row of the block == TMEM lane
     const uint32_t tl = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
     // rows past the last node (the padding of a captured step) become zeros
     if (blockIdx.x == 0) {
       const long long first = static_cast<long long>(max(bt.cu[bt.B], 0)) * bt.H;
-      for (long long i = first + warp - 2; i < static_cast<long long>(bt.n_tok) * bt.H; i += 8) {
+      for (long long i = first + warp - 4; i < static_cast<long long>(bt.n_tok) * bt.H; i += 8) {
         for (int d = lane; d < D; d += 32) st_elem(out + i * D + d, 0.f);
         if (lse && lane == 0) lse[i] = -INFINITY;
       }
@@ -267,9 +267,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
       if (it.t1 * BN > it.len && anc_of != it.b) {
         asm volatile("bar.sync 1, 256;");
         if (bt.parents)
-          for (int i = threadIdx.x - 64; i < it.n; i += 256) s_par[i] = bt.parents[it.node0 + i];
+          for (int i = threadIdx.x - 128; i < it.n; i += 256) s_par[i] = bt.parents[it.node0 + i];
         asm volatile("bar.sync 1, 256;");
-        ancestor_masks(s_par, bt.parents == nullptr, it.n, s_anc, threadIdx.x - 64, 256, it.b);
+        ancestor_masks(s_par, bt.parents == nullptr, it.n, s_anc, threadIdx.x - 128, 256, it.b);
         asm volatile("bar.sync 1, 256;");
         anc_of = it.b;
       }

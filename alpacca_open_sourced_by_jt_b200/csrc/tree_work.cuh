@@ -205,17 +205,19 @@ __device__ __forceinline__ void ancestor_masks(const int* par, bool chain, int n
   }
 }
 
-// Page (outer tensor-map coordinate) that holds cache row `row` of request
-// b; a page outside the pool is recorded and answered with n_pages, which
-// TMA reads as zeros.
-__device__ __forceinline__ int page_of(const Batch& bt, int b, int row) {
-  if (bt.table == nullptr) return b;
-  const int pg = bt.table[b * bt.table_stride + (row >> bt.page_shift)];
-  if (pg < 0 || pg >= bt.n_pages) {
-    set_dev_error(B2A_ERR_POSITION, b);
-    return bt.n_pages;
-  }
-  return pg;
+// Page (outer tensor-map coordinate) that holds cache row `row` of request b,
+// as the table has it.  The check is apart from the load, so that a producer
+// can look a page up one tile ahead without waiting for it.
+__device__ __forceinline__ int table_entry(const Batch& bt, int b, int row) {
+  return bt.table ? __ldg(bt.table + b * bt.table_stride + (row >> bt.page_shift)) : b;
+}
+
+// A page outside the pool is recorded and answered with n_pages, which TMA
+// reads as zeros.
+__device__ __forceinline__ int checked_page(const Batch& bt, int b, int pg) {
+  if (pg >= 0 && pg < bt.n_pages) return pg;
+  set_dev_error(B2A_ERR_POSITION, b);
+  return bt.n_pages;
 }
 
 // Part slot of an item in CTA c's range, or -1 if the item is whole in it.
