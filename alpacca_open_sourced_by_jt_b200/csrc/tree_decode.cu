@@ -925,23 +925,13 @@ int tree_wide(const TreeArgs& a) {
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "cudaFuncSetAttribute(tree_wide)");
   const int piece = a.bt.table && a.page_rows < C::kBN ? a.page_rows : C::kBN;
   const int cols = piece == C::kBN ? D / 64 : 1;
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tk, tv;
   int rc = tree_map(&tk, a, a.k, piece, cols);
   if (rc == B2A_OK) rc = tree_map(&tv, a, a.v, piece, cols);
-  // q as nodes of [H][D]: a box is the rows of one KV head's group x the
-  // block's nodes
-  const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.bt.H),
-                            static_cast<uint64_t>(a.bt.n_tok)};
-  const uint64_t strides[2] = {static_cast<uint64_t>(D) * 2, static_cast<uint64_t>(a.q_stride) * 2};
-  const uint32_t box[3] = {64, static_cast<uint32_t>(a.bt.group),
-                           static_cast<uint32_t>(a.bt.rows_per_block / a.bt.group)};
-  if (rc == B2A_OK)
-    rc = b2a_host::make_tmap(&tq, a.dtype == B2A_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                             3, const_cast<void*>(a.q), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kWideThreads), C::kSmem, a.st, tq, tk, tv, a.bt,
-                       static_cast<T*>(a.out), a.lse, a.part_o, a.part_ml, piece, a.sscale);
+  e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kWideThreads), C::kSmem, a.st, tk, tv, a.bt,
+                       static_cast<const T*>(a.q), a.q_stride, static_cast<T*>(a.out), a.lse,
+                       a.part_o, a.part_ml, piece, a.sscale);
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "tree_wide launch");
   return tree_merge<T, D>(a);
 }
