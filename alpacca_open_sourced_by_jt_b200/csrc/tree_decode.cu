@@ -17,7 +17,6 @@
 
 #include <limits.h>
 #include <math.h>
-#include <stdlib.h>
 
 #include <atomic>
 
@@ -35,11 +34,9 @@ namespace tree {
 // 16-row pages takes 4 pieces x 2).
 // Eight consumer warps run the decode kernel's fragments (decode.cu):
 // S^T = K.Q^T with the query rows on the MMA's N axis, online softmax on the
-// accumulators, O^T += V^T.P^T.  A warp takes 16 keys of a tile:
-//   kByRows = false (up to 8 NT rows): warps 0-3 take the even tiles, 4-7 the
-//     odd ones, every warp all the rows;
-//   kByRows = true (up to 32 rows): warps 0-3 take rows 0-15 of every tile,
-//     4-7 rows 16-31.
+// accumulators, O^T += V^T.P^T.  Warps 0-3 take the even
+// tiles, 4-7 the odd ones; a warp takes 16 keys of a tile and all the query rows
+// (up to 8 NT).
 // P is rounded to the cache's type for the second product (its error, one
 // part in 2^8 or 2^11 of each weight, is what the output's own rounding
 // makes); scores, maxima, sums and accumulators are f32.  Q is not
@@ -49,7 +46,7 @@ constexpr int kConsumers = 8;
 constexpr int kProducers = 4;
 constexpr int kMmaThreads = (kConsumers + kProducers) * 32;
 
-template <int D, int NT, bool kByRows>
+template <int D, int NT>
 struct MmaCfg {
   static constexpr int kBoxes = D / 64;
   static constexpr int kTileBytes = kBoxes * kRows * 128;
@@ -58,23 +55,23 @@ struct MmaCfg {
   static constexpr int kState = (D / 16 * NT * 4 + NT * 4) * 32 * 4;
   static constexpr int kMerge = 4 * kState;
   static constexpr int kFit = (232448 - 1024 - 4096 - kMerge) / kStageBytes;
-  // Without kByRows a stage must always belong to the same half of the warps:
-  // a warp that skipped a stage's last use could not tell its phase by the
-  // parity.  An even ring keeps tile parity and stage parity together.
-  static constexpr int kStages = kFit > 10 ? 10 : (kByRows ? kFit : kFit & ~1);
+  // A stage must always belong to the same half of the warps: a warp that
+  // skipped a stage's last use could not tell its phase by the parity.  An even
+  // ring keeps tile parity and stage parity together.
+  static constexpr int kStages = kFit > 10 ? 10 : kFit & ~1;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kMerge;
   static_assert(kStages >= 2, "ring");
 };
 
-template <typename T, int D, int NT, bool kByRows>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
     const __grid_constant__ Batch bt, const T* __restrict__ q, long long q_stride,
     T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o,
     float* __restrict__ part_ml, int piece_rows, float sscale) {
-  using C = MmaCfg<D, NT, kByRows>;
+  using C = MmaCfg<D, NT>;
   constexpr int KS = D / 16;
-  constexpr int RB = kByRows ? 16 * NT : 8 * NT;
+  constexpr int RB = 8 * NT;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[C::kStages];
   __shared__ __align__(8) uint64_t empty_bar[C::kStages];
@@ -87,18 +84,17 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
                                              ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    const Start s = locate(bt, blockIdx.x / bt.KV);
+    const Start s = locate(bt, team_of(bt, blockIdx.x));
     if (lane == 0) s_start = s;
   } else if (warp == kConsumers && lane == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full_bar[s], min(kProducers, 2 * (kRows / piece_rows)));
-      mbar_init(&empty_bar[s], kByRows ? kConsumers : kConsumers / 2);
+      mbar_init(&empty_bar[s], kConsumers / 2);
     }
     fence_mbar_init();
   }
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int kvh = blockIdx.x % bt.KV;
   Walker wk;
   wk.start(bt, s_start);
   Item it;
@@ -140,9 +136,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
           mbar_arrive_expect_tx(&full_bar[s], (live0 ? bytes : 0) + (live1 ? bytes : 0));
           const int mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
           uint8_t* at = dst + s * C::kStageBytes + (p >> 1) * bytes;
-          if (live0) tma_load_5d(at, map, &full_bar[s], 0, row0 & mask, 0, kvh, now0);
+          if (live0) tma_load_5d(at, map, &full_bar[s], 0, row0 & mask, 0, it.kvh, now0);
           if (live1)
-            tma_load_5d(at + (kProducers / 2) * bytes, map, &full_bar[s], 0, row1 & mask, 0, kvh, now1);
+            tma_load_5d(at + (kProducers / 2) * bytes, map, &full_bar[s], 0, row1 & mask, 0, it.kvh, now1);
           if (++s == C::kStages) {
             s = 0;
             ++round;
@@ -182,7 +178,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
 
   while (wk.next(bt, it)) {
     const int R = it.n * bt.group;
-    const int row_lo = it.blk * RB + (kByRows ? half * 8 * NT : 0);  // this warp's rows
+    const int row_lo = it.blk * RB;
     if (it.t1 * kRows > it.len && anc_of != it.b) {
       asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32));
       if (bt.parents)
@@ -199,7 +195,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
       const int r = row_lo + nt * 8 + g;
       const bool valid = r < R;
       const int node = valid ? r / bt.group : 0;
-      const int head = kvh * bt.group + (valid ? r - node * bt.group : 0);
+      const int head = it.kvh * bt.group + (valid ? r - node * bt.group : 0);
       const T* qr = q + (it.node0 + node) * q_stride + head * D;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -223,7 +219,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
     const int rows = it.len + it.n;
 
     for (int t = it.t0; t < it.t1; ++t, ++seq) {
-      if (!kByRows && (seq & 1u) != static_cast<uint32_t>(half)) continue;
+      if ((seq & 1u) != static_cast<uint32_t>(half)) continue;
       const int s = seq % C::kStages;
       if (!dead)
         dead = !__all_sync(0xffffffffu,
@@ -335,10 +331,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
     // in each round the upper half of the remaining warps hands its state to
     // the lower half
 #pragma unroll
-    for (int left = kByRows ? 2 : 4; left > 0; left >>= 1) {
-      const int rank = kByRows ? slice : warp;
-      const int box = kByRows ? half * 2 + (rank & (left - 1)) : (rank & (left - 1));
-      float* st = merge + box * (C::kState / 4) + lane;
+    for (int left = 4; left > 0; left >>= 1) {
+      const int rank = warp;
+      float* st = merge + (rank & (left - 1)) * (C::kState / 4) + lane;
       if (rank >= left && rank < 2 * left) {
 #pragma unroll
         for (int mt = 0; mt < KS; ++mt)
@@ -385,13 +380,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
     float* fml = merge + RB * kPad;    // [RB][2]
     static_assert((RB * (D + 4) + 2 * RB) * 4 <= C::kMerge, "final rows fit the merge buffer");
     const int slot = part_slot(it, blockIdx.x);
-    if (kByRows ? slice == 0 : warp == 0) {
-      const int c0 = kByRows ? half * 8 * NT : 0;
+    if (warp == 0) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int r = c0 + nt * 8 + 2 * t4 + c;
+          const int r = nt * 8 + 2 * t4 + c;
           const float f = slot >= 0 ? 1.f : (l[nt][c] > 0.f ? 1.f / l[nt][c] : 0.f);
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt) {
@@ -418,7 +412,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
       for (int i = threadIdx.x; i < live * (D / 8); i += kConsumers * 32) {
         const int r = i / (D / 8), d = (i - r * (D / 8)) * 8;
         const int rr = it.blk * RB + r, node = rr / bt.group;
-        const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + kvh * bt.group + (rr - node * bt.group);
+        const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + it.kvh * bt.group + (rr - node * bt.group);
         const float* x = fin + r * kPad + d;
         uint4 u;
         u.x = MmaOp<T>::pack(x[0], x[1]);
@@ -474,7 +468,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
   float* ps = qs + C::kQ;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 0) {
-    const Start s = locate(bt, blockIdx.x / bt.KV);
+    const Start s = locate(bt, team_of(bt, blockIdx.x));
     if (lane == 0) s_start = s;
   }
   __syncthreads();
@@ -486,7 +480,6 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
       if (lse && lane == 0) lse[r] = -INFINITY;
     }
   }
-  const int kvh = blockIdx.x % bt.KV;
   Walker wk;
   wk.start(bt, s_start);
   Item it;
@@ -507,7 +500,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
       const int rr = it.blk * kF32Rows + r;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (rr < R) {
-        const int node = rr / bt.group, head = kvh * bt.group + rr - node * bt.group;
+        const int node = rr / bt.group, head = it.kvh * bt.group + rr - node * bt.group;
         x = *reinterpret_cast<const float4*>(q + (it.node0 + node) * q_stride + head * D + d);
       }
       *reinterpret_cast<float4*>(qs + r * C::kKStride + d) = x;
@@ -533,7 +526,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
           in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
         }
         const size_t src = live ? static_cast<size_t>(pg) * page_stride +
-                                      (static_cast<size_t>(in_page) * bt.KV + kvh) * D + d
+                                      (static_cast<size_t>(in_page) * bt.KV + it.kvh) * D + d
                                 : 0;
         const int bytes = live ? 16 : 0;  // rows past the end are filled with zeros
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
@@ -674,7 +667,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
         }
       } else {
         const int gr = it.blk * kF32Rows + rr, node = gr / bt.group;
-        const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + kvh * bt.group + (gr - node * bt.group);
+        const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + it.kvh * bt.group + (gr - node * bt.group);
         const float f = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int c = 0; c < kCols; ++c) out[row * D + oc + c * 128] = o[r][c] * f;
@@ -689,8 +682,8 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
 // ---------------------------------------------------------------------------
 // Block (c, y) looks at the last item of CTA c's range: if the item goes on
 // past the range and does not begin before it, its parts are CTA c's slot
-// 2c + 1, the same slot of every later CTA of the head that the item fills,
-// and slot 2e of the CTA e where it ends.  One warp per query row.
+// 2c + 1, the same slot of its fellows in the later teams that the item fills,
+// and slot 2e of the one, e, where it ends.  One warp per query row.
 constexpr int kMergeWarps = 8;
 
 template <typename T, int D>
@@ -699,8 +692,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
     const float* __restrict__ part_ml, T* __restrict__ out, float* __restrict__ lse) {
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x, kvh = c % bt.KV;
-  const Start s = locate(bt, c / bt.KV);
+  const int c = blockIdx.x;
+  const Start s = locate(bt, team_of(bt, c));
   if (s.left < s.chunk) return;  // an empty range, or the list's last
   // the item that holds the range's last tile
   int b = s.b, n, len;
@@ -714,10 +707,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
     u = units_of(bt, n, len);
   }
   const int tiles = (len + n + bt.tile - 1) / bt.tile;
-  const int blk = static_cast<int>(off / tiles);
-  const int at = static_cast<int>(off - static_cast<long long>(blk) * tiles);
+  const int idx = static_cast<int>(off / tiles);
+  const int at = static_cast<int>(off - static_cast<long long>(idx) * tiles);
   const int after = tiles - 1 - at;  // tiles past the range
-  if (after == 0 || at >= s.chunk) return;
+  int kvh, blk;
+  if (after == 0 || at >= s.chunk || !member_item(bt, c, idx, blocks_of(bt, n), kvh, blk)) return;
   const int whole = static_cast<int>(after / s.chunk);  // later ranges the item fills
   const int rest = static_cast<int>(after - whole * s.chunk);
   const int parts = 1 + whole + (rest > 0 ? 1 : 0);
@@ -726,7 +720,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
   const int node0 = bt.cu[b];
   // A part that ends exactly with its CTA's range is that CTA's slot 2e.
   auto slot = [&](int i) {
-    return 2 * (c + i * bt.KV) + ((i == parts - 1) ? 0 : 1);
+    return 2 * (c + i * bt.m_heads * bt.m_blks) + ((i == parts - 1) ? 0 : 1);
   };
   for (int r = blockIdx.y * kMergeWarps + warp; r < live; r += gridDim.y * kMergeWarps) {
     float M = -INFINITY;
@@ -834,7 +828,6 @@ enum TreeKernel { kTreeF32, kTreeMma, kTreeWide };
 
 TreeKernel tree_kernel(int dtype, int rows, int D) {
   if (dtype == B2A_F32) return kTreeF32;
-  if (getenv("B2A_TREE_NARROW")) return kTreeMma;
   return rows <= (D > 128 ? 8 : 16) ? kTreeMma : kTreeWide;
 }
 
@@ -843,7 +836,7 @@ TreeKernel tree_kernel(int dtype, int rows, int D) {
 int tree_rows_per_block(TreeKernel k, int rows, int group) {
   if (k == kTreeF32) return TR::kF32Rows;
   if (k == kTreeWide) return TR::kWideM / group * group;
-  return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
+  return rows <= 8 ? 8 : 16;
 }
 int tree_tile(TreeKernel k, int D) {
   if (k == kTreeF32) return D > 128 ? 32 : 64;
@@ -851,6 +844,7 @@ int tree_tile(TreeKernel k, int D) {
   return TR::kRows;
 }
 bool tree_by_item(int max_len) { return max_len <= 512; }
+int max_rows_blocks(int rows, int rows_per_block) { return (rows + rows_per_block - 1) / rows_per_block; }
 
 struct TreeArgs {
   const void *q, *k, *v;
@@ -897,10 +891,10 @@ int tree_map(CUtensorMap* m, const TreeArgs& a, const void* base, int box_rows, 
                                       : CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
-template <typename T, int D, int NT, bool kByRows>
+template <typename T, int D, int NT>
 int tree_mma(const TreeArgs& a) {
-  auto kern = TR::tree_mma_kernel<T, D, NT, kByRows>;
-  constexpr int smem = TR::MmaCfg<D, NT, kByRows>::kSmem;
+  auto kern = TR::tree_mma_kernel<T, D, NT>;
+  constexpr int smem = TR::MmaCfg<D, NT>::kSmem;
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_smem(kern, smem, done);
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "cudaFuncSetAttribute(tree_decode)");
@@ -925,13 +919,23 @@ int tree_wide(const TreeArgs& a) {
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "cudaFuncSetAttribute(tree_wide)");
   const int piece = a.bt.table && a.page_rows < C::kBN ? a.page_rows : C::kBN;
   const int cols = piece == C::kBN ? D / 64 : 1;
-  CUtensorMap tk, tv;
+  CUtensorMap tq, tk, tv;
   int rc = tree_map(&tk, a, a.k, piece, cols);
   if (rc == B2A_OK) rc = tree_map(&tv, a, a.v, piece, cols);
+  // q as nodes of [H][D]: a box is the rows of one KV head's group x the
+  // block's nodes
+  const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.bt.H),
+                            static_cast<uint64_t>(a.bt.n_tok)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(D) * 2, static_cast<uint64_t>(a.q_stride) * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(a.bt.group),
+                           static_cast<uint32_t>(a.bt.rows_per_block / a.bt.group)};
+  if (rc == B2A_OK)
+    rc = b2a_host::make_tmap(&tq, a.dtype == B2A_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                             3, const_cast<void*>(a.q), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kWideThreads), C::kSmem, a.st, tk, tv, a.bt,
-                       static_cast<const T*>(a.q), a.q_stride, static_cast<T*>(a.out), a.lse,
-                       a.part_o, a.part_ml, piece, a.sscale);
+  e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kWideThreads), C::kSmem, a.st, tq, tk, tv, a.bt,
+                       static_cast<T*>(a.out), a.lse, a.part_o, a.part_ml, piece, a.sscale);
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "tree_wide launch");
   return tree_merge<T, D>(a);
 }
@@ -939,9 +943,10 @@ int tree_wide(const TreeArgs& a) {
 template <typename T, int D>
 int tree_16bit(const TreeArgs& a) {
   if (a.kernel == kTreeWide) return tree_wide<T, D>(a);
-  if (a.bt.rows_per_block == 8) return tree_mma<T, D, 1, false>(a);
-  if (a.bt.rows_per_block == 16) return tree_mma<T, D, 2, false>(a);
-  return tree_mma<T, D, 2, true>(a);
+  if constexpr (D <= 128) {
+    if (a.bt.rows_per_block == 16) return tree_mma<T, D, 2>(a);
+  }
+  return tree_mma<T, D, 1>(a);
 }
 
 template <int D>
@@ -966,10 +971,12 @@ int tree_dispatch(const TreeArgs& a) {
   return tree_16bit<__half, D>(a);
 }
 
-// CTAs of a grid of teams: as many whole teams as there are SMs for.
+// Most CTAs of a grid of teams (a team has a CTA per KV head, or up to
+// kTreeBlocks).
+constexpr int kTreeBlocks = 8;
 int tree_ctas(int KV) {
-  const int teams = b2a_host::sm_count() / KV;
-  return (teams > 0 ? teams : 1) * KV;
+  const int sms = b2a_host::sm_count();
+  return KV > sms ? KV : sms;
 }
 
 size_t tree_part_o_bytes(int D, int KV, int rows_per_block) {
@@ -1050,16 +1057,28 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
   const int rb = tree_rows_per_block(a.kernel, rows, group);
   const int tile = tree_tile(a.kernel, D);
   a.bt = TR::Batch{lens_dev, cu_dev, parents_dev, table_dev, table_stride, B, n_tok, max_nodes,
-                   max_len, n_pages, table_dev ? log2_of(page_rows) : 0, H, KV, group, rb, tile, 0, 1, 1};
-  // A head's tiles are cut evenly over the teams, at least 4 to a CTA.
+                   max_len, n_pages, table_dev ? log2_of(page_rows) : 0, H, KV, group, rb, tile, 0, 1, 1, 1, 1};
+  // Side by side in a team: the KV heads, or, where a request has several
+  // blocks of query rows, those (as many as the average request has; one with
+  // more goes round again).  16 x 32K rows, bf16, 32/8 x 128, 128 nodes (4
+  // blocks): MEASURED_TEAMS
+  const long long avg_rows = static_cast<long long>(n_tok) * group / B;
+  long long blks = (avg_rows + rb / 2) / rb;
+  if (blks > (max_rows_blocks(rows, rb))) blks = max_rows_blocks(rows, rb);
+  if (blks > kTreeBlocks) blks = (blks + (blks + kTreeBlocks - 1) / kTreeBlocks - 1) / ((blks + kTreeBlocks - 1) / kTreeBlocks);
+  a.bt.m_blks = blks > 1 && a.kernel == kTreeWide ? static_cast<int>(blks) : 1;
+  a.bt.m_heads = a.bt.m_blks > 1 ? 1 : KV;
+  const int members = a.bt.m_heads * a.bt.m_blks;
+  // A list's tiles are cut evenly over the teams, at least 4 to a team.
   const long long max_tiles = (max_len + tile - 1) / tile;
-  const long long items = static_cast<long long>(B) * ((rows + rb - 1) / rb);
+  const long long items = static_cast<long long>(B) * (KV / a.bt.m_heads) *
+                          ((max_rows_blocks(rows, rb) + a.bt.m_blks - 1) / a.bt.m_blks);
   a.bt.by_item = tree_by_item(max_len) ? 1 : 0;
   a.bt.min_units = a.bt.by_item ? 1 : 4;
   const long long units = a.bt.by_item ? items : (items * max_tiles + 3) / 4;
-  const int teams = tree_ctas(KV) / KV;
+  const int teams = b2a_host::sm_count() > members ? b2a_host::sm_count() / members : 1;
   a.bt.teams = static_cast<int>(units < teams ? units : teams);
-  a.grid = a.bt.teams * KV;
+  a.grid = a.bt.teams * members;
   a.merge = !a.bt.by_item;
   if (a.merge) {
     const size_t need = b2a_tree_decode_workspace_bytes(max_nodes, H, KV, D, dtype, max_len);

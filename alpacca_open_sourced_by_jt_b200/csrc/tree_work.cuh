@@ -1,10 +1,11 @@
 // Work division of the tree attention over a cache (tree_decode.cu,
 // tree_wide.cu): what every kernel of it shares.
 //
-// The grid is teams x KV heads: CTA c reads KV head c % KV, and the KV CTAs of
-// a team do the same work for their heads side by side, so the rows of a cache
-// page (all heads of a token behind one another) are read together.  A head's
-// work is a list of items (request, block of query rows), each as long as its
+// The grid is teams of CTAs that read the same cache rows side by side:
+// either a CTA per KV head (a page holds all heads of a token behind one
+// another), for one block of query rows per request, or a CTA per block of
+// query rows of one KV head, so that the blocks' second and later reads of a
+// tile hit L2.  What a team works on is a list of items, each as long as its
 // request's key tiles.  Lengths live on the device, so the division is made
 // there: the list's tiles are numbered through and team i takes tiles
 // [i * chunk, (i + 1) * chunk), chunk = ceil(total / teams) or a least number
@@ -39,7 +40,9 @@ struct Batch {
   int tile;            // keys per tile
   int by_item;         // CTAs take whole items (no parts)
   int min_units;       // least tiles of a range
-  int teams;           // ranges a head's list is cut into
+  int teams;           // ranges the list is cut into
+  int m_heads;         // KV heads side by side in a team: KV or 1
+  int m_blks;          // blocks of query rows side by side
 };
 
 // Nodes and cache rows of request b; a request whose numbers are out of
@@ -62,7 +65,8 @@ __device__ __forceinline__ int blocks_of(const Batch& bt, int n) {
 
 __device__ __forceinline__ long long units_of(const Batch& bt, int n, int len) {
   if (n == 0) return 0;
-  const long long items = blocks_of(bt, n);
+  const long long items = static_cast<long long>(bt.KV / bt.m_heads) *
+                          ((blocks_of(bt, n) + bt.m_blks - 1) / bt.m_blks);
   return bt.by_item ? items : items * ((len + n + bt.tile - 1) / bt.tile);
 }
 
@@ -123,12 +127,29 @@ __device__ __forceinline__ Start locate(const Batch& bt, int team) {
 }
 
 struct Item {
-  int b, blk;
+  int b, kvh, blk;
   int n, len;     // the request's nodes and cached rows
   int t0, t1;     // this CTA's key tiles of the item
   int tiles;      // the item's key tiles
   int node0;      // row of the request's node 0 in q and out
 };
+
+// KV head and block of a team's item `idx` of a request with `blks` blocks,
+// for CTA c of the grid; false if this CTA has no block in it.
+__device__ __forceinline__ bool member_item(const Batch& bt, int c, int idx, int blks, int& kvh,
+                                            int& blk) {
+  const int member = c % (bt.m_heads * bt.m_blks);
+  const int hm = member % bt.m_heads, bm = member / bt.m_heads;
+  const int rounds = (blks + bt.m_blks - 1) / bt.m_blks;
+  const int hl = idx / rounds;
+  kvh = bt.m_heads > 1 ? hm : hl;
+  blk = (idx - hl * rounds) * bt.m_blks + bm;
+  return blk < blks;
+}
+
+__device__ __forceinline__ int team_of(const Batch& bt, int c) {
+  return c / (bt.m_heads * bt.m_blks);
+}
 
 // Walks the items of a CTA's range; every role of a CTA walks the same ones.
 struct Walker {
@@ -154,8 +175,8 @@ struct Walker {
       it.len = len;
       it.tiles = (len + n + bt.tile - 1) / bt.tile;
       const int per = bt.by_item ? 1 : it.tiles;
-      it.blk = static_cast<int>(off / per);
-      const int at = static_cast<int>(off - static_cast<long long>(it.blk) * per);
+      const int idx = static_cast<int>(off / per);
+      const int at = static_cast<int>(off - static_cast<long long>(idx) * per);
       int take = per - at;
       if (take > left) take = static_cast<int>(left);
       it.t0 = bt.by_item ? 0 : at;
@@ -163,7 +184,7 @@ struct Walker {
       it.node0 = bt.cu[b];
       off += take;
       left -= take;
-      return true;
+      if (member_item(bt, blockIdx.x, idx, blocks_of(bt, n), it.kvh, it.blk)) return true;
     }
     return false;
   }
