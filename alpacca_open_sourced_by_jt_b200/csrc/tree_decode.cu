@@ -1064,7 +1064,8 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
   // blocks): MEASURED_TEAMS
   const long long avg_rows = static_cast<long long>(n_tok) * group / B;
   long long blks = (avg_rows + rb / 2) / rb;
-  if (blks > (max_rows_blocks(rows, rb))) blks = max_rows_blocks(rows, rb);
+  const int most = max_rows_blocks(rows, rb);
+  if (blks > most || 4 * blks >= 3 * most) blks = most;
   if (blks > kTreeBlocks) blks = (blks + (blks + kTreeBlocks - 1) / kTreeBlocks - 1) / ((blks + kTreeBlocks - 1) / kTreeBlocks);
   a.bt.m_blks = blks > 1 && a.kernel == kTreeWide ? static_cast<int>(blks) : 1;
   a.bt.m_heads = a.bt.m_blks > 1 ? 1 : KV;

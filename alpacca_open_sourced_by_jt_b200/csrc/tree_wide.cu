@@ -9,21 +9,21 @@
 // columns as 16-bit pairs (the schedule of prefill_head.cu).
 //
 // A thread's part of a tile (128 exponentials, and the waits and TMEM traffic
-// around them) takes longer than the tensor core's, so two warpgroups take the
-// key tiles in turn and three S buffers keep both supplied: while they work on
-// tiles j and j + 1, QK(j + 2) is done, and PV(j) frees its buffer for
-// QK(j + 3).  What ties the warpgroups is the running maximum: the warp of tile
-// j publishes its rows' maximum before its exponentials, and the other
-// warpgroup's warp of the same rows goes on from there with tile j + 1.  Each
-// keeps the sum of its own tiles relative to the last maximum it used; they
-// meet at the item's end.  Warps whose 32 rows hold no query only pass the
-// barriers.  (Both warpgroups on every tile, half of its keys each: their
-// exponentials then fall together on one SFU and wait together for the next
-// tile, 2000 cycles a tile.)
+// around them) takes two to three times the tensor core's, so three warpgroups
+// take the key tiles in turn, each with an S buffer of its own: while they work
+// on tiles j to j + 2, PV(j) frees its buffer for QK(j + 3).  What ties the
+// warpgroups is the running maximum: the warp of tile j publishes its rows'
+// maximum before its exponentials, and the next warpgroup's warp of the same
+// rows goes on from there with tile j + 1.  Each keeps the sum of its own tiles
+// relative to the last maximum it used; they meet at the item's end.  S is read
+// from TMEM twice (maximum, exponentials) in 64-column steps of a loop rather
+// than held in 128 registers: that leaves room for the third warpgroup, and
+// code that stays in the instruction cache.  Warps whose 32 rows hold no query
+// only pass the barriers.
 //
-// 384 threads: warps 0 and 2 TMA producers (a box per page piece and 64
+// 512 threads: warps 0 and 2 TMA producers (a box per page piece and 64
 // columns, or one per tile where a page holds it), warp 1 TMEM owner and MMA
-// issuer, warps 4-11 softmax (TMEM lane quarter = warp % 4).
+// issuer, warps 4-15 softmax (TMEM lane quarter = warp % 4).
 // TMEM: S0 .. S2 (BN columns each), O (D columns).
 
 #include <limits.h>
@@ -48,34 +48,24 @@ using prefill::tc_st32;
 using prefill::tc_wait_ld;
 using prefill::tc_wait_st;
 
-constexpr int kWideThreads = 384;
+constexpr int kWideThreads = 512;
+constexpr int kWideGroups = 3;  // softmax warpgroups, each with an S buffer
 constexpr int kWideM = 128;
 constexpr int kMaxSlots = 16;
 
 struct WideShared {
   uint64_t bar_qf, bar_qe, bar_oe, bar_last;  // bar_last: an item's last PV
   uint64_t bar_full[kMaxSlots], bar_empty[kMaxSlots];
-  uint64_t bar_sf[3], bar_pf[3], bar_pv[2], bar_m[2][4];
+  uint64_t bar_sf[kWideGroups], bar_pf[kWideGroups], bar_pv[2], bar_m[kWideGroups][4];
   Start start;
   uint32_t tmem;
-  float m[2][kWideM], l[2][kWideM];  // maxima and sums between the warpgroups
+  float x[kWideGroups][kWideM];  // maxima, at an item's end sums, between the warpgroups
 };
-
-// One lane of the (converged) warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(p));
-  return p != 0;
-}
 
 template <int D>
 struct WideCfg {
   static constexpr int kBN = D > 128 ? 64 : 128;      // keys per tile
-  static constexpr int kS = 3;                        // S buffers
+  static constexpr int kS = kWideGroups;              // S buffers
   static constexpr int kBoxQ = kWideM * 128;          // 128 rows x 64 columns
   static constexpr int kBoxKV = kBN * 128;            // kBN rows x 64 columns
   static constexpr int kTileQ = (D / 64) * kBoxQ;
@@ -121,7 +111,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
   } else if (warp == 2 && lane == 0) {
     mbar_init(&sh.bar_qf, 1);
     mbar_init(&sh.bar_qe, 1);
-    mbar_init(&sh.bar_oe, 8);
+    mbar_init(&sh.bar_oe, 4 * kWideGroups);
     mbar_init(&sh.bar_last, 1);
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&bar_full[s], 1);
@@ -131,10 +121,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
       mbar_init(&sh.bar_sf[b], 1);
       mbar_init(&sh.bar_pf[b], 4);
     }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(&sh.bar_pv[w], 1);
+    for (int w = 0; w < kWideGroups; ++w)
       for (int i = 0; i < 4; ++i) mbar_init(&sh.bar_m[w][i], 1);
-    }
+    mbar_init(&sh.bar_pv[0], 1);
+    mbar_init(&sh.bar_pv[1], 1);
     fence_mbar_init();
   }
   tc_fence_before();
@@ -149,57 +139,78 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
   constexpr uint32_t kOCol = C::kS * BN;
   const int block_nodes = bt.rows_per_block / bt.group;
 
+  // a whole warp's wait on a barrier, with one answer for all lanes
+  auto arrived = [](uint64_t* bar, uint32_t parity, int where) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, where)) != 0;
+  };
+
   if (warp == 0 || warp == 2) {
     // ------------------------------ TMA producers --------------------------
-    // One lane per warp issues: warp 0 loads Q and K, warp 2 V, so that a K
-    // tile never queues behind a V tile whose slot is still in use.
-    const int p = warp >> 1;
+    // Warp 0 loads Q and K, warp 2 V, so that a K tile never queues behind a V
+    // tile whose slot is still in use.  Whole warps walk the loop and one
+    // elected lane issues (see the MMA issuer).
+    const int p = __shfl_sync(0xffffffffu, warp >> 1, 0);
     const CUtensorMap* map = p ? &tmV : &tmK;
-    const int boxes = piece_rows == BN ? 1 : D / 64;   // boxes of a page piece
-    const int bytes = piece_rows * 128 * (D / 64);     // of a piece
-    if (lane == 0) {
+    const bool whole = piece_rows == BN;
+    const int bytes = piece_rows * 128 * (D / 64);  // of a page piece
+    if (elect_one()) {
       if (p == 0) tma_prefetch_desc(&tmQ);
       tma_prefetch_desc(map);
-      uint32_t slot = p, round = 0, items = 0;  // K tiles in the even slots, V tiles in the odd ones
-      bool ok = true;
-      const int mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
-      while (ok && wk.next(bt, it)) {
-        const int rows = it.len + it.n;
-        int pg = table_entry(bt, it.b, it.t0 * BN);  // looked up one piece ahead
-        if (p == 0) {
-          if (items > 0 && !mbar_wait(&sh.bar_qe, (items - 1) & 1, 0x33000)) break;
+    }
+    uint32_t slot = p, round = 0, items = 0;  // K tiles in the even slots, V tiles in the odd ones
+    bool ok = true;
+    const int mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
+    while (ok && wk.next(bt, it)) {
+      const int rows = __shfl_sync(0xffffffffu, it.len + it.n, 0);
+      const int t0 = __shfl_sync(0xffffffffu, it.t0, 0), t1 = __shfl_sync(0xffffffffu, it.t1, 0);
+      const int kvh = __shfl_sync(0xffffffffu, it.kvh, 0);
+      const int pieces = (min(rows, t1 * BN) - t0 * BN + piece_rows - 1) / piece_rows;
+      // pages are looked up a warp's width of pieces at a time
+      const int lane_row = t0 * BN + lane * piece_rows;
+      int pgs = lane < pieces ? table_entry(bt, it.b, lane_row) : 0;
+      if (p == 0) {
+        if (items > 0) ok = arrived(&sh.bar_qe, (items - 1) & 1, 0x33000);
+        if (!ok) break;
+        const int node = __shfl_sync(0xffffffffu, it.node0 + it.blk * block_nodes, 0);
+        if (elect_one()) {
           mbar_arrive_expect_tx(&sh.bar_qf, (D / 64) * bt.rows_per_block * 128);
 #pragma unroll
           for (int b = 0; b < D / 64; ++b)
-            tma_load_3d(smem + b * C::kBoxQ, &tmQ, &sh.bar_qf, b * 64, it.kvh * bt.group,
-                        it.node0 + it.blk * block_nodes);
-          ++items;
+            tma_load_3d(smem + b * C::kBoxQ, &tmQ, &sh.bar_qf, b * 64, kvh * bt.group, node);
         }
-        const int row_end = min(rows, it.t1 * BN);
-        for (int t = it.t0; t < it.t1; ++t) {
-          const int row0 = t * BN;
-          const int end = min(row0 + BN, rows);
-          if (round > 0 && !mbar_wait(&bar_empty[slot], (round & 1) ^ 1, 0x34000 | slot)) {
-            ok = false;
-            break;
+        ++items;
+      }
+      int i = 0;  // piece of the item
+      for (int t = t0; t < t1; ++t) {
+        if (round > 0) ok = arrived(&bar_empty[slot], (round & 1) ^ 1, 0x34000);
+        if (!ok) break;
+        const int end = min(i + BN / piece_rows, pieces);
+        uint8_t* dst = smem + C::kRing + slot * C::kTileKV;
+        if (elect_one()) mbar_arrive_expect_tx(&bar_full[slot], (end - i) * bytes);
+        for (; i < end; ++i, dst += piece_rows * 128) {
+          const int pg = checked_page(bt, it.b, __shfl_sync(0xffffffffu, pgs, i & 31));
+          if ((i & 31) == 31) {
+            const int next = i + 1 + lane;
+            pgs = next < pieces ? table_entry(bt, it.b, t0 * BN + next * piece_rows) : 0;
           }
-          uint8_t* dst = smem + C::kRing + slot * C::kTileKV;
-          mbar_arrive_expect_tx(&bar_full[slot], (end - row0 + piece_rows - 1) / piece_rows * bytes);
-          for (int row = row0; row < end; row += piece_rows, dst += piece_rows * 128) {
-            const int now = checked_page(bt, it.b, pg);
-            if (row + piece_rows < row_end) pg = table_entry(bt, it.b, row + piece_rows);
-            for (int b = 0; b < boxes; ++b)
-              tma_load_5d(dst + b * C::kBoxKV, map, &bar_full[slot], 0, row & mask, b, it.kvh, now);
+          const int row = (t0 * BN + i * piece_rows) & mask;
+          if (elect_one()) {
+            if (whole) {
+              tma_load_5d(dst, map, &bar_full[slot], 0, row, 0, kvh, pg);
+            } else {
+#pragma unroll
+              for (int b = 0; b < D / 64; ++b)
+                tma_load_5d(dst + b * C::kBoxKV, map, &bar_full[slot], 0, row, b, kvh, pg);
+            }
           }
-          slot += 2;
-          if (slot >= kSlots) {
-            slot = p;
-            ++round;
-          }
+        }
+        slot += 2;
+        if (slot >= kSlots) {
+          slot = p;
+          ++round;
         }
       }
     }
-    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------ MMA issuer -----------------------------
     // The whole warp walks the loop and one elected lane issues.  Everything a
@@ -216,9 +227,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
     constexpr uint32_t kSlotStep = C::kTileKV >> 4;
     uint32_t kslot = 0, kround = 0, items = 0, pvg = 0;  // K(jj)'s slot; V(jj)'s is the next
     uint32_t pcnt = 0;  // bit b: parity of S buffer b's next P
-    auto arrived = [&](uint64_t* bar, uint32_t parity, int where) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, where)) != 0;
-    };
     // QK of a tile into S buffer sb, from ring slot `slot`
     auto qk = [&](uint32_t sb, uint32_t slot) {
       const uint64_t dk = dK0 + slot * kSlotStep;
@@ -256,11 +264,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
       uint32_t sb = 0;
       for (int jj = 0; ok && jj < n; ++jj) {
         const bool more = jj + C::kS < n;
-        // waits that do not depend on P(jj) come before the one that does
-        ok = arrived(&bar_full[vslot], vround, 0x39000);
-        if (ok && more) ok = arrived(&bar_full[kslot], kround, 0x35800);
+        // A wait takes some 150 cycles even where there is nothing to wait for;
+        // asked together, the three barriers (V, the next K, P) answer in one.
+        uint64_t *bv = &bar_full[vslot], *bk = &bar_full[more ? kslot : vslot], *bp = &sh.bar_pf[sb];
+        const uint32_t kpar = more ? kround : vround, ppar = (pcnt >> sb) & 1;
+        const bool v_in = mbar_test(bv, vround), k_in = mbar_test(bk, kpar), p_in = mbar_test(bp, ppar);
+        if (!__all_sync(0xffffffffu, v_in && k_in && p_in))
+          ok = arrived(bv, vround, 0x39000) && arrived(bk, kpar, 0x35800) && arrived(bp, ppar, 0x37000);
         if (ok && jj == 0 && items > 0) ok = arrived(&sh.bar_oe, (items - 1) & 1, 0x38000);
-        if (ok) ok = arrived(&sh.bar_pf[sb], (pcnt >> sb) & 1, 0x37000);
         pcnt ^= 1u << sb;
         if (!ok) break;
         tc_fence_after();
@@ -291,22 +302,25 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
     }
   } else if (warp >= 4) {
     // ------------------------------ softmax ----------------------------------
-    const int w = (warp - 4) >> 2;                 // warpgroup: tiles jj % 2 == w
+    const int w = (warp - 4) >> 2;                 // warpgroup: tiles jj % 3 == w, S buffer w
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;             // row of the block == TMEM lane
     const uint32_t tl = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint32_t scnt = 0;       // bit b: parity of S buffer b's next tile (all tiles of the CTA)
-    uint32_t mdone[2] = {0, 0};  // tiles each warpgroup has done
+    const uint32_t ts = tl + w * BN;
+    const int before_w = w == 0 ? kWideGroups - 1 : w - 1;  // whose tile comes before
+    uint32_t own = 0, theirs = 0;  // tiles this warpgroup and that one have done
     uint32_t pvbase = 0, kslot = 0, kround = 0, items = 0;
     bool dead = false;  // a wait ran out: no more waiting, the barriers go on
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity, where));
       return !dead;
     };
+    auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(128 * kWideGroups) : "memory"); };
     // rows past the last node (the padding of a captured step) become zeros
     if (blockIdx.x == 0) {
       const long long first = static_cast<long long>(max(bt.cu[bt.B], 0)) * bt.H;
-      for (long long i = first + warp - 4; i < static_cast<long long>(bt.n_tok) * bt.H; i += 8) {
+      for (long long i = first + warp - 4; i < static_cast<long long>(bt.n_tok) * bt.H;
+           i += 4 * kWideGroups) {
         for (int d = lane; d < D; d += 32) st_elem(out + i * D + d, 0.f);
         if (lse && lane == 0) lse[i] = -INFINITY;
       }
@@ -338,81 +352,87 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
           at = up;
         }
       }
+      // 32 scores whose first key is tree row j0 (negative: cached rows): bit j
+      // of the node's ancestors says whether it sees row j
+      auto hide = [&](float* s, int j0) {
+        if (j0 <= -32) return;
+        const int lo = j0 >> 5, sft = j0 & 31;  // floor
+        uint32_t a = lo < 0 ? 0xffffffffu : 0u, b = 0u;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          if (lo == i) a = anc[i];
+          if (lo + 1 == i) b = anc[i];
+        }
+        const uint32_t vis = sft ? (a >> sft) | (b << (32 - sft)) : a;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[e] = ((vis >> e) & 1u) ? s[e] : -INFINITY;
+      };
       float m = -INFINITY, l = 0.f;
-      int sb = 0;
-      for (int jj = 0; jj < n; ++jj) {
-        const uint32_t s_col = sb * BN;
-        uint64_t *sf = &sh.bar_sf[sb], *pf = &sh.bar_pf[sb];
-        const uint32_t sparity = (scnt >> sb) & 1;
-        scnt ^= 1u << sb;
-        if (++sb == C::kS) sb = 0;
-        if ((jj & 1) != w) continue;
+      for (int jj = w; jj < n; jj += kWideGroups) {
         const int t = it.t0 + jj;
-        const bool alive = wait(sf, sparity, 0x3A000);
+        const int tree0 = t * BN - it.len;  // tree row of the tile's first key
+        const bool tail = tree0 + BN > 0;
+        const bool alive = wait(&sh.bar_sf[w], own & 1, 0x3A000);
+        ++own;
         tc_fence_after();
         if (busy && alive) {
-          float s[BN];
+          float mxa = -INFINITY, mxb = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 64) {
+            float s[64];
+            tc_ld32(ts + c, s);
+            tc_ld32(ts + c + 32, s + 32);
+            tc_wait_ld();
+            if (tail) {
+              hide(s, tree0 + c);
+              hide(s + 32, tree0 + c + 32);
+            }
 #pragma unroll
-          for (int q32 = 0; q32 < BN / 32; ++q32) tc_ld32(tl + s_col + q32 * 32, s + q32 * 32);
-          tc_wait_ld();
-          if ((t + 1) * BN > it.len) {
-            // tree rows: bit j of the node's ancestors for key len + j
-#pragma unroll
-            for (int wd = 0; wd < BN / 32; ++wd) {
-              const int j0 = t * BN + wd * 32 - it.len;  // node of the word's first key
-              uint32_t vis = 0xffffffffu;
-              if (j0 > -32) {
-                const int lo = j0 >> 5, sft = j0 & 31;  // floor
-                uint32_t a = lo < 0 ? 0xffffffffu : 0u, b = 0u;
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                  if (lo == i) a = anc[i];
-                  if (lo + 1 == i) b = anc[i];
-                }
-                vis = sft ? (a >> sft) | (b << (32 - sft)) : a;
-              }
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                s[wd * 32 + e] = ((vis >> e) & 1u) ? s[wd * 32 + e] : -INFINITY;
+            for (int e = 0; e < 64; e += 4) {
+              mxa = fmaxf(mxa, fmaxf(s[e], s[e + 1]));
+              mxb = fmaxf(mxb, fmaxf(s[e + 2], s[e + 3]));
             }
           }
-          float mxa = -INFINITY, mxb = -INFINITY, mxc = -INFINITY, mxd = -INFINITY;
-#pragma unroll
-          for (int cc = 0; cc < BN; cc += 4) {
-            mxa = fmaxf(mxa, s[cc]);
-            mxb = fmaxf(mxb, s[cc + 1]);
-            mxc = fmaxf(mxc, s[cc + 2]);
-            mxd = fmaxf(mxd, s[cc + 3]);
-          }
-          const float mx = fmaxf(fmaxf(mxa, mxb), fmaxf(mxc, mxd)) * sscale;
+          const float mx = fmaxf(mxa, mxb) * sscale;
           // the reference maximum up to the tile before
           float before = -INFINITY;
           if (jj > 0) {
-            const uint32_t theirs = mdone[w ^ 1] + ((jj - 1) >> 1);
-            if (wait(&sh.bar_m[w ^ 1][quarter], theirs & 1, 0x3B000)) before = sh.m[w ^ 1][r];
+            const uint32_t idx = theirs + (w == 0 ? jj / kWideGroups - 1 : jj / kWideGroups);
+            if (wait(&sh.bar_m[before_w][quarter], idx & 1, 0x3B000)) before = sh.x[before_w][r];
           }
           // It only follows when a row's maximum grew by more than 2^8 (exact:
           // sums and O are relative to the same number).
           const bool grow = __any_sync(0xffffffffu, mx > before + prefill::kRescaleThreshold);
           const float now = grow ? fmaxf(before, mx) : before;
-          sh.m[w][r] = now;
+          sh.x[w][r] = now;
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.bar_m[w][quarter]);
           const float mref = (now == -INFINITY) ? 0.f : now;
           l *= (m == -INFINITY) ? 0.f : fast_exp2(m - mref);
           m = now;
           float suma = 0.f, sumb = 0.f;
-#pragma unroll
-          for (int qtr = 0; qtr < BN / 32; ++qtr) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float p0 = fast_exp2(fmaf(s[qtr * 32 + 2 * e], sscale, -mref));
-              const float p1 = fast_exp2(fmaf(s[qtr * 32 + 2 * e + 1], sscale, -mref));
-              if (e & 1) sumb += p0 + p1; else suma += p0 + p1;
-              pk[e] = Pack2<T>::run(p0, p1);
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 64) {
+            float s[64];
+            tc_ld32(ts + c, s);
+            tc_ld32(ts + c + 32, s + 32);
+            tc_wait_ld();
+            if (tail) {
+              hide(s, tree0 + c);
+              hide(s + 32, tree0 + c + 32);
             }
-            tc_st16(tl + s_col + qtr * 16, pk);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float p0 = fast_exp2(fmaf(s[h * 32 + 2 * e], sscale, -mref));
+                const float p1 = fast_exp2(fmaf(s[h * 32 + 2 * e + 1], sscale, -mref));
+                if (e & 1) sumb += p0 + p1; else suma += p0 + p1;
+                pk[e] = Pack2<T>::run(p0, p1);
+              }
+              tc_st16(ts + (c >> 1) + h * 16, pk);
+            }
           }
           tc_wait_st();
           l += suma + sumb;
@@ -422,7 +442,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
             if (wait(&sh.bar_pv[g & 1], (g >> 1) & 1, 0x3C000)) {
               const float alpha = (before == -INFINITY) ? 0.f : fast_exp2(before - mref);
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int cc = 0; cc < D / 32; ++cc) {
                 float o[32];
                 tc_ld32(tl + kOCol + cc * 32, o);
@@ -462,16 +482,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(pf);
+        if (lane == 0) mbar_arrive(&sh.bar_pf[w]);
       }
-      // ---------------- the item's end: both warpgroups' sums meet ----------
-      sh.l[w][r] = l;
-      sh.m[w][r] = m;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const float ma = sh.m[0][r], mb = sh.m[1][r];
-      const float M = fmaxf(ma, mb);
+      theirs += (n - before_w + kWideGroups - 1) / kWideGroups;
+      // ---------------- the item's end: the warpgroups' sums meet -----------
+      meet();  // the last tile's maximum is the one that O is relative to
+      const float M = sh.x[(n - 1) % kWideGroups][r];
       const float mref = (M == -INFINITY) ? 0.f : M;
-      const float L = sh.l[0][r] * fast_exp2(ma - mref) + sh.l[1][r] * fast_exp2(mb - mref);
+      meet();
+      sh.x[w][r] = (m == -INFINITY) ? 0.f : l * fast_exp2(m - mref);
+      meet();
+      const float L = (sh.x[0][r] + sh.x[1][r]) + sh.x[2][r];
       wait(&sh.bar_last, items & 1, 0x3E000);
       ++items;
       tc_fence_after();
@@ -480,10 +501,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
       const float f = L > 0.f ? 1.f / L : 0.f;
       float* po = part_o + (static_cast<size_t>(max(slot, 0)) * bt.rows_per_block + r) * D;
       if (busy && !dead) {
-        // each warpgroup writes half of the columns
-#pragma unroll
-        for (int cc = 0; cc < D / 64; ++cc) {
-          const int col = w * (D / 2) + cc * 32;
+        // the warpgroups write the columns in turn
+#pragma unroll 1
+        for (int col = w * 32; col < D; col += 32 * kWideGroups) {
           float o[32];
           tc_ld32(tl + kOCol + col, o);
           tc_wait_ld();
@@ -516,8 +536,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
           }
         }
       }
-      mdone[0] += (n + 1) >> 1;
-      mdone[1] += n >> 1;
       pvbase += n;
       kslot += 2 * (n % (kSlots / 2));
       kround ^= (n / (kSlots / 2)) & 1;
@@ -526,7 +544,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
         kround ^= 1;
       }
       tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // m, l and O are read
+      meet();  // the exchanged numbers and O are read
       if (lane == 0) mbar_arrive(&sh.bar_oe);
     }
   }
