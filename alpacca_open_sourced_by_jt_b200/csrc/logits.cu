@@ -182,41 +182,63 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     const TI* in = static_cast<const TI*>(a.in) + row * a.in_stride;
     TO* out = static_cast<TO*>(a.out) + row * a.out_stride;
     const uint32_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
-    unsigned long long best = 0ull;
-#pragma unroll 4
-    for (int i = tid * W; i < a.slice; i += kThreads * W) {
-      const int v0 = v_lo + i;
-      if (v0 >= v_hi) break;
-      const int live = min(W, v_hi - v0);
-      float x[W];
-      if (live == W) {
-        load_w<TI, W>(in + v0, x);
+    // a thread's tokens ascend, so only a larger value replaces its best
+    float top = -INFINITY;
+    int at = 0;
+    auto constrain = [&](float* x, int i, int v0, uint32_t bits) {
+      uint32_t w[W];
+      if constexpr (W == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(info + i);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
       } else {
-        for (int e = 0; e < W; ++e) x[e] = e < live ? ld_elem(in + v0 + e) : 0.f;
+        w[0] = info[i];
       }
-      const uint32_t bits = mask ? mask[v0 >> 5] >> (v0 & 31) : 0xffffffffu;
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        const uint32_t w = info[i + e];
-        if (w != 0u) {
-          if (w & kBias) x[e] = __fadd_rn(x[e], a.bias[e0 + bidx[i + e] - 1]);
-          const uint32_t c = w & kCount;
-          if (c != 0u || (w & kPrompt)) x[e] = x[e] > 0.f ? __fdiv_rn(x[e], rep) : __fmul_rn(x[e], rep);
+        if (w[e] != 0u) {
+          if (w[e] & kBias) x[e] = __fadd_rn(x[e], a.bias[e0 + bidx[i + e] - 1]);
+          const uint32_t c = w[e] & kCount;
+          if (c != 0u || (w[e] & kPrompt)) x[e] = x[e] > 0.f ? __fdiv_rn(x[e], rep) : __fmul_rn(x[e], rep);
           x[e] = __fsub_rn(x[e], __fmul_rn(freq, static_cast<float>(c)));
           if (c != 0u) x[e] = __fsub_rn(x[e], pres);
         }
         if (!((bits >> e) & 1u)) x[e] = -INFINITY;
-        if (e < live) {
-          const unsigned long long k = key_of(x[e], v0 + e);
-          best = k > best ? k : best;
+        if (x[e] > top) {
+          top = x[e];
+          at = v0 + e;
         }
       }
-      if (live == W) {
-        store_w<TO, W>(out + v0, x);
-      } else {
-        for (int e = 0; e < live; ++e) st_elem(out + v0 + e, x[e]);
+    };
+    constexpr int kPass = kThreads * W;    // tokens of one pass of the CTA
+    constexpr int kBatch = W == 4 ? 4 : 8;  // passes with their loads in flight
+    int i0 = 0;
+    for (; v_lo + i0 + kBatch * kPass <= v_hi; i0 += kBatch * kPass) {
+      float x[kBatch][W];
+      uint32_t bits[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int v0 = v_lo + i0 + k * kPass + tid * W;
+        load_w<TI, W>(in + v0, x[k]);
+        bits[k] = mask ? mask[v0 >> 5] >> (v0 & 31) : 0xffffffffu;
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = i0 + k * kPass + tid * W;
+        constrain(x[k], i, v_lo + i, bits[k]);
+        store_w<TO, W>(out + v_lo + i, x[k]);
       }
     }
+    for (int i = i0 + tid * W; v_lo + i < v_hi; i += kPass) {
+      const int v0 = v_lo + i, live = min(W, v_hi - v0);
+      float x[W];
+#pragma unroll
+      for (int e = 0; e < W; ++e) x[e] = e < live ? ld_elem(in + v0 + e) : -INFINITY;
+      constrain(x, i, v0, mask ? mask[v0 >> 5] >> (v0 & 31) : 0xffffffffu);
+#pragma unroll
+      for (int e = 0; e < W; ++e)
+        if (e < live) st_elem(out + v0 + e, x[e]);
+    }
+    unsigned long long best = key_of(top, at);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);

@@ -224,63 +224,223 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
 // ---------------------------------------------------------------------------
 // RoPE + append by slot (b2a_rope_append_paged)
 // ---------------------------------------------------------------------------
-// One element pair per thread and step; products and sums are rounded one by
-// one, as rope_append.cu does.
+// Bound by reading the projections and writing q and the pool.  Products and
+// sums are rounded one by one, as rope_append.cu does.  Two kernels:
+//   rope_paged_rows   rows in 16-byte aligned groups of 8 elements.  A thread
+//     keeps its 4 pairs' cosines and sines and goes over heads with them; the
+//     loads of kHeads heads are in flight at once.
+//   rope_paged_pairs  anything else (odd head or rotation widths, unaligned
+//     strides): one pair per thread and step.
+struct RopeArgs {
+  const void *q, *k, *v;
+  long long q_stride, k_stride, v_stride;
+  const float *bq, *bk, *bv, *cos_tab, *sin_tab;
+  const int *pos, *slots;
+  void *k_pool, *v_pool, *q_out;
+  long long page_stride, n_slots;
+  int tab_rows, page_shift, H, KV, D, n_rot, neox;
+};
+
+// The token's position and pool row (negative: not stored); false if the
+// token is left out.
+__device__ __forceinline__ bool rope_token(const RopeArgs& a, int i, int& p, long long& row) {
+  p = a.pos[i];
+  const int slot = a.slots[i];
+  if (p < 0 || p >= a.tab_rows || slot >= a.n_slots) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) set_dev_error(B2A_ERR_POSITION, i);
+    return false;
+  }
+  row = slot < 0 ? -1
+                 : static_cast<long long>(slot >> a.page_shift) * a.page_stride +
+                       static_cast<long long>(slot & ((1 << a.page_shift) - 1)) * a.KV * a.D;
+  return true;
+}
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* x) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = ld_elem(h + e);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  if constexpr (sizeof(T) == 4) {
+    load4(p, x);
+    load4(p + 4, x + 4);
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = ld_elem(h + e);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(MmaOp<T>::pack(x[0], x[1]), MmaOp<T>::pack(x[2], x[3]));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    store4(p, x);
+    store4(p + 4, x + 4);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(MmaOp<T>::pack(x[0], x[1]), MmaOp<T>::pack(x[2], x[3]),
+                                              MmaOp<T>::pack(x[4], x[5]), MmaOp<T>::pack(x[6], x[7]));
+  }
+}
+
+constexpr int kRopeThreads = 256;
+constexpr int kHeads = 3;  // heads of a thread with their loads in flight
+
 template <typename TS, typename TK, typename TQ>
-__global__ void __launch_bounds__(256) rope_paged_kernel(
-    const TS* __restrict__ q, long long q_stride, const TS* __restrict__ k, long long k_stride,
-    const TS* __restrict__ v, long long v_stride, const float* __restrict__ bq,
-    const float* __restrict__ bk, const float* __restrict__ bv, const float* __restrict__ cos_tab,
-    const float* __restrict__ sin_tab, int tab_rows, const int* __restrict__ pos,
-    const int* __restrict__ slots, TK* __restrict__ k_pool, TK* __restrict__ v_pool,
-    int page_shift, long long page_stride, long long n_slots, TQ* __restrict__ q_out, int H,
-    int KV, int D, int n_rot, int neox) {
+__global__ void __launch_bounds__(kRopeThreads) rope_paged_rows(const __grid_constant__ RopeArgs a) {
   pdl_wait();
   const int i = blockIdx.x;
-  const int p = pos[i];
-  const int slot = slots[i];
-  if (p < 0 || p >= tab_rows || slot >= n_slots) {
-    if (threadIdx.x == 0 && blockIdx.y == 0) set_dev_error(B2A_ERR_POSITION, i);
-    return;
+  int p;
+  long long row;
+  if (!rope_token(a, i, p, row)) return;
+  const int groups = a.D >> 3;              // groups of 8 elements (4 pairs) of a head
+  const int heads_at_once = kRopeThreads / groups;
+  const int g = threadIdx.x % groups, h0 = threadIdx.x / groups;
+  if (h0 >= heads_at_once) return;
+  const int half = a.n_rot >> 1;
+  const bool turned = 4 * g < half;         // the group's pairs rotate
+  // elements of the group: [lo, lo + 4) and [hi, hi + 4)
+  const bool split = a.neox && turned;
+  const int lo = split ? 4 * g : 8 * g, hi = split ? half + 4 * g : 8 * g + 4;
+  float c[4], s[4];
+  if (turned) {
+    load4(a.cos_tab + static_cast<size_t>(p) * half + 4 * g, c);
+    load4(a.sin_tab + static_cast<size_t>(p) * half + 4 * g, s);
   }
-  const int half = n_rot >> 1;
-  const size_t row = slot < 0 ? 0 : static_cast<size_t>(slot >> page_shift) * page_stride +
-                                        static_cast<size_t>(slot & ((1 << page_shift) - 1)) * KV * D;
-  const int per = D >> 1;
-  for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < (H + 2 * KV) * per;
-       u += gridDim.y * blockDim.x) {
-    const int head = u / per, t = u - head * per;
-    const bool is_q = head < H, is_v = head >= H + KV;
-    const int h = is_q ? head : (is_v ? head - H - KV : head - H);
-    if (!is_q && slot < 0) continue;
-    const TS* src = is_q ? q + i * q_stride + h * D : (is_v ? v + i * v_stride : k + i * k_stride) + h * D;
-    const float* bias = is_q ? bq : (is_v ? bv : bk);
-    int a = 2 * t, b = 2 * t + 1;
-    const bool turn = !is_v && t < half;
-    if (turn && neox) {
-      a = t;
-      b = t + half;
+  const int all = a.H + 2 * a.KV;
+  const int step = heads_at_once * gridDim.y;
+  for (int hb = blockIdx.y * heads_at_once + h0; hb < all; hb += kHeads * step) {
+    float x[kHeads][8];
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = hb + u * step;
+      if (h >= all || (row < 0 && h >= a.H)) continue;
+      const TS* src = h < a.H ? static_cast<const TS*>(a.q) + i * a.q_stride + h * a.D
+                    : h < a.H + a.KV ? static_cast<const TS*>(a.k) + i * a.k_stride + (h - a.H) * a.D
+                                     : static_cast<const TS*>(a.v) + i * a.v_stride + (h - a.H - a.KV) * a.D;
+      if (split && h < a.H + a.KV) {
+        load4(src + lo, x[u]);
+        load4(src + hi, x[u] + 4);
+      } else {
+        load8(src + 8 * g, x[u]);
+      }
     }
-    float x0 = ld_elem(src + a), x1 = ld_elem(src + b);
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = hb + u * step;
+      if (h >= all || (row < 0 && h >= a.H)) continue;
+      const bool is_v = h >= a.H + a.KV;
+      const bool part = split && !is_v;
+      const float* bias = h < a.H ? a.bq : (is_v ? a.bv : a.bk);
+      const int hh = h < a.H ? h : (is_v ? h - a.H - a.KV : h - a.H);
+      const int la = part ? lo : 8 * g, ha = part ? hi : 8 * g + 4;
+      if (bias) {
+        float b[8];
+        load4(bias + hh * a.D + la, b);
+        load4(bias + hh * a.D + ha, b + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[u][e] = __fadd_rn(x[u][e], b[e]);
+      }
+      if (turned && !is_v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = a.neox ? x[u][e] : x[u][2 * e];
+          const float x1 = a.neox ? x[u][e + 4] : x[u][2 * e + 1];
+          const float y0 = __fsub_rn(__fmul_rn(x0, c[e]), __fmul_rn(x1, s[e]));
+          const float y1 = __fadd_rn(__fmul_rn(x0, s[e]), __fmul_rn(x1, c[e]));
+          if (a.neox) {
+            x[u][e] = y0;
+            x[u][e + 4] = y1;
+          } else {
+            x[u][2 * e] = y0;
+            x[u][2 * e + 1] = y1;
+          }
+        }
+      }
+      if (h < a.H) {
+        TQ* dst = static_cast<TQ*>(a.q_out) + (static_cast<size_t>(i) * a.H + h) * a.D;
+        if (part) {
+          store4(dst + lo, x[u]);
+          store4(dst + hi, x[u] + 4);
+        } else {
+          store8(dst + 8 * g, x[u]);
+        }
+      } else {
+        TK* dst = static_cast<TK*>(is_v ? a.v_pool : a.k_pool) + row + hh * a.D;
+        if (part) {
+          store4(dst + lo, x[u]);
+          store4(dst + hi, x[u] + 4);
+        } else {
+          store8(dst + 8 * g, x[u]);
+        }
+      }
+    }
+  }
+}
+
+template <typename TS, typename TK, typename TQ>
+__global__ void __launch_bounds__(kRopeThreads) rope_paged_pairs(const __grid_constant__ RopeArgs a) {
+  pdl_wait();
+  const int i = blockIdx.x;
+  int p;
+  long long row;
+  if (!rope_token(a, i, p, row)) return;
+  const int half = a.n_rot >> 1, per = a.D >> 1;
+  for (int u = blockIdx.y * kRopeThreads + threadIdx.x; u < (a.H + 2 * a.KV) * per;
+       u += gridDim.y * kRopeThreads) {
+    const int head = u / per, t = u - head * per;
+    const bool is_q = head < a.H, is_v = head >= a.H + a.KV;
+    const int h = is_q ? head : (is_v ? head - a.H - a.KV : head - a.H);
+    if (!is_q && row < 0) continue;
+    const TS* src = (is_q ? static_cast<const TS*>(a.q) + i * a.q_stride
+                          : is_v ? static_cast<const TS*>(a.v) + i * a.v_stride
+                                 : static_cast<const TS*>(a.k) + i * a.k_stride) + h * a.D;
+    const float* bias = is_q ? a.bq : (is_v ? a.bv : a.bk);
+    int e0 = 2 * t, e1 = 2 * t + 1;
+    const bool turn = !is_v && t < half;
+    if (turn && a.neox) {
+      e0 = t;
+      e1 = t + half;
+    }
+    float x0 = ld_elem(src + e0), x1 = ld_elem(src + e1);
     if (bias) {
-      x0 = __fadd_rn(x0, bias[h * D + a]);
-      x1 = __fadd_rn(x1, bias[h * D + b]);
+      x0 = __fadd_rn(x0, bias[h * a.D + e0]);
+      x1 = __fadd_rn(x1, bias[h * a.D + e1]);
     }
     float y0 = x0, y1 = x1;
     if (turn) {
-      const float c = cos_tab[static_cast<size_t>(p) * half + t];
-      const float s = sin_tab[static_cast<size_t>(p) * half + t];
+      const float c = a.cos_tab[static_cast<size_t>(p) * half + t];
+      const float s = a.sin_tab[static_cast<size_t>(p) * half + t];
       y0 = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
       y1 = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
     }
     if (is_q) {
-      TQ* dst = q_out + (static_cast<size_t>(i) * H + h) * D;
-      st_elem(dst + a, y0);
-      st_elem(dst + b, y1);
+      TQ* dst = static_cast<TQ*>(a.q_out) + (static_cast<size_t>(i) * a.H + h) * a.D;
+      st_elem(dst + e0, y0);
+      st_elem(dst + e1, y1);
     } else {
-      TK* dst = (is_v ? v_pool : k_pool) + row + h * D;
-      st_elem(dst + a, y0);
-      st_elem(dst + b, y1);
+      TK* dst = static_cast<TK*>(is_v ? a.v_pool : a.k_pool) + row + h * a.D;
+      st_elem(dst + e0, y0);
+      st_elem(dst + e1, y1);
     }
   }
 }
@@ -316,20 +476,23 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __gri
   const bool bad = n < 0 || n > c.max_nodes || c0 < 0 || c0 + n > c.n_tok || len < 0 ||
                    len > c.max_len - n;
   if (threadIdx.x < 32) {
-    int par[kMaxNodes / 32], tok[kMaxNodes / 32];
+    int par[kMaxNodes / 32], tok[kMaxNodes / 32], pick[kMaxNodes / 32];
 #pragma unroll
     for (int w = 0; w < kMaxNodes / 32; ++w) {
       const int j = w * 32 + lane;
       const bool in = !bad && j < n;
       par[w] = in ? (c.parents ? c.parents[c0 + j] : j - 1) : -2;
       tok[w] = in ? c.tokens[c0 + j] : 0;
+      pick[w] = in ? c.picks[c0 + j] : 0;
     }
     int len_path = 0, cur = 0, last = -1;
     if (!bad && n > 0) {
       while (true) {
         if (lane == 0) s_path[len_path] = cur;
         ++len_path;
-        last = c.picks[c0 + cur];
+#pragma unroll
+        for (int w = 0; w < kMaxNodes / 32; ++w)
+          if (w == cur >> 5) last = __shfl_sync(0xffffffffu, pick[w], cur & 31);
         int nxt = -1;
 #pragma unroll
         for (int w = 0; w < kMaxNodes / 32; ++w) {
@@ -402,20 +565,29 @@ namespace {
 namespace PG = b2a::paged;
 
 template <typename TS, typename TK, typename TQ>
-cudaError_t rope_paged_launch(const void* q, long long qs, const void* k, long long ks,
-                              const void* v, long long vs, const float* bq, const float* bk,
-                              const float* bv, const float* cos_tab, const float* sin_tab,
-                              int tab_rows, const int* pos, const int* slots, void* kp, void* vp,
-                              int shift, long long page_stride, long long n_slots, void* qo,
-                              int n_tok, int H, int KV, int D, int n_rot, int neox,
-                              cudaStream_t st) {
-  const int pairs = (H + 2 * KV) * (D / 2);
-  const int gy = (pairs + 255) / 256;
-  return b2a_host::launch(PG::rope_paged_kernel<TS, TK, TQ>, dim3(n_tok, gy), dim3(256), 0, st,
-                          static_cast<const TS*>(q), qs, static_cast<const TS*>(k), ks,
-                          static_cast<const TS*>(v), vs, bq, bk, bv, cos_tab, sin_tab, tab_rows,
-                          pos, slots, static_cast<TK*>(kp), static_cast<TK*>(vp), shift,
-                          page_stride, n_slots, static_cast<TQ*>(qo), H, KV, D, n_rot, neox);
+cudaError_t rope_paged_launch(const PG::RopeArgs& a, int n_tok, cudaStream_t st) {
+  auto aligned = [](const void* p, long long stride, size_t es) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * static_cast<long long>(es) % 16 == 0;
+  };
+  const bool rows = a.D % 8 == 0 && a.n_rot % 8 == 0 && aligned(a.q, a.q_stride, sizeof(TS)) &&
+                    aligned(a.k, a.k_stride, sizeof(TS)) && aligned(a.v, a.v_stride, sizeof(TS)) &&
+                    aligned(a.q_out, 0, 2) && aligned(a.k_pool, a.page_stride, sizeof(TK)) &&
+                    aligned(a.v_pool, 0, 2) && aligned(a.cos_tab, 0, 4) && aligned(a.sin_tab, 0, 4) &&
+                    aligned(a.bq, 0, 4) && aligned(a.bk, 0, 4) && aligned(a.bv, 0, 4);
+  const int all = a.H + 2 * a.KV;
+  if (rows) {
+    // few tokens: a token's heads over more CTAs, until there are a few per SM
+    const int at_once = PG::kRopeThreads / (a.D / 8);
+    int gy = (all + at_once - 1) / at_once;
+    const int enough = (4 * b2a_host::sm_count() + n_tok - 1) / n_tok;
+    if (gy > enough) gy = enough;
+    return b2a_host::launch(PG::rope_paged_rows<TS, TK, TQ>, dim3(n_tok, gy),
+                            dim3(PG::kRopeThreads), 0, st, a);
+  }
+  const int pairs = all * (a.D / 2);
+  return b2a_host::launch(PG::rope_paged_pairs<TS, TK, TQ>,
+                          dim3(n_tok, (pairs + PG::kRopeThreads - 1) / PG::kRopeThreads),
+                          dim3(PG::kRopeThreads), 0, st, a);
 }
 
 // Calls f with a null pointer of the element type of a dtype code.
@@ -496,18 +668,17 @@ int b2a_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
     return fail(B2A_ERR_SHAPE, "rope_append_paged: token strides overlap the rows");
   if (n_tok == 0) return B2A_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const long long n_slots = static_cast<long long>(n_pages) * page_rows;
+  const PG::RopeArgs a = {q, k, v, q_tok_stride, k_tok_stride, v_tok_stride, bq, bk, bv, cos_tab,
+                          sin_tab, pos_dev, slot_dev, k_pool, v_pool, q_out, page_stride,
+                          static_cast<long long>(n_pages) * page_rows, tab_rows,
+                          log2_of(page_rows), H, KV, D, n_rot, style == B2A_ROPE_NEOX ? 1 : 0};
   const cudaError_t e = with_type(in_dtype, [&](auto* ts) {
     return with_type(kv_dtype, [&](auto* tk) {
       return with_type(q_out_dtype, [&](auto* tq) {
         using TS = typename std::remove_pointer<decltype(ts)>::type;
         using TK = typename std::remove_pointer<decltype(tk)>::type;
         using TQ = typename std::remove_pointer<decltype(tq)>::type;
-        return rope_paged_launch<TS, TK, TQ>(q, q_tok_stride, k, k_tok_stride, v, v_tok_stride, bq,
-                                             bk, bv, cos_tab, sin_tab, tab_rows, pos_dev, slot_dev,
-                                             k_pool, v_pool, log2_of(page_rows), page_stride,
-                                             n_slots, q_out, n_tok, H, KV, D, n_rot,
-                                             style == B2A_ROPE_NEOX, st);
+        return rope_paged_launch<TS, TK, TQ>(a, n_tok, st);
       });
     });
   });
