@@ -11,16 +11,18 @@
 // every operation rounded once to f32.  The pick is the lowest v of the
 // largest x (-1 where no x is above -inf).
 //
-// Bound by reading and writing the rows.  What a token needs besides its
-// logit is sparse, but looked up for every token: a CTA takes one slice of
-// the vocabulary of one request, builds that slice's counts in shared memory
-// from the history (integer atomics: the order does not matter), and then
-// streams the slice of several of the request's rows through, one 4-byte
-// word of shared memory per logit.  A node's path is added to the counts
-// before its row and taken off after it, which only happens (and only then
-// costs two barriers) where a drafted token falls into the slice.  Each warp
-// leaves its best (value, lowest token) as one ordered 64-bit key and a
-// second small kernel takes the rows' maxima.
+// Bound by reading and writing the rows.  The tokens that need more than a copy
+// and a mask are few, but evaluated where they stand they would hold up their
+// whole warp (a division each).  A CTA takes one slice of the vocabulary of one
+// request; from the history, the biases and the drafted tokens it builds, once
+// for several rows, the slice's counts in shared memory (integer atomics: the
+// order does not matter), a bit per token that is touched, and a list of the
+// touched tokens.  Each row is then streamed through with mask and maximum of
+// the untouched tokens while the next row's loads are in flight, and the list's
+// tokens are redone, one to a thread.  A node's path is added to the counts
+// before its row's list and taken off after it, where a drafted token falls
+// into the slice.  Each warp leaves its best (value, lowest token) as one
+// ordered 64-bit key and a second small kernel takes the rows' maxima.
 
 #include "b2a_common.cuh"
 
@@ -33,7 +35,8 @@ constexpr int kMaxNodes = B2A_TREE_MAX_NODES;
 constexpr int kWords = kMaxNodes / 32;
 constexpr uint32_t kPrompt = 0x80000000u;  // the token is in the prompt
 constexpr uint32_t kBias = 0x40000000u;    // the token has a bias
-constexpr uint32_t kCount = 0x3fffffffu;
+constexpr uint32_t kDraft = 0x20000000u;   // the token is drafted in the request's tree
+constexpr uint32_t kCount = 0x1fffffffu;
 
 struct Args {
   const void* in;
@@ -91,12 +94,15 @@ __device__ __forceinline__ void store_w(T* p, const float* x) {
 }
 
 template <typename TI, typename TO, int W>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 3) logits_kernel(const __grid_constant__ Args a) {
   pdl_wait();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(16) uint32_t lsm[];
   uint32_t* info = lsm;               // [slice] flags and counts
   uint32_t* bidx = lsm + a.slice;     // [slice] 1 + bias entry
+  uint32_t* touched = bidx + a.slice;  // [slice / 32] a bit per token with info
+  uint16_t* list = reinterpret_cast<uint16_t*>(touched + a.slice / 32);  // [slice] those tokens
+  __shared__ int s_list;              // how many
   __shared__ uint32_t s_anc[kMaxNodes][kWords];
   __shared__ int s_par[kMaxNodes], s_tok[kMaxNodes];
   __shared__ uint32_t s_in[kWords];   // the request's nodes whose token is in the slice
@@ -115,6 +121,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
   for (int i = tid * 4; i < 2 * a.slice; i += kThreads * 4)
     *reinterpret_cast<uint4*>(lsm + i) = make_uint4(0u, 0u, 0u, 0u);
   if (tid < kWords) s_in[tid] = 0u;
+  if (tid == 0) s_list = 0;
   if (tid < n) {
     s_par[tid] = a.parents ? a.parents[c0 + tid] : tid - 1;
     s_tok[tid] = a.tokens ? a.tokens[c0 + tid] : -1;
@@ -144,7 +151,10 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     }
   }
   if (tid < n) {
-    if (s_tok[tid] >= v_lo && s_tok[tid] < v_hi) atomicOr(&s_in[tid >> 5], 1u << (tid & 31));
+    if (s_tok[tid] >= v_lo && s_tok[tid] < v_hi) {
+      atomicOr(&s_in[tid >> 5], 1u << (tid & 31));
+      atomicOr(&info[s_tok[tid] - v_lo], kDraft);
+    }
     uint32_t m[kWords];
 #pragma unroll
     for (int w = 0; w < kWords; ++w) m[w] = 0u;
@@ -164,53 +174,58 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     for (int w = 0; w < kWords; ++w) s_anc[tid][w] = m[w];
   }
   __syncthreads();
+  for (int i = tid; i < a.slice; i += kThreads) {  // whole warps: the slice is a multiple of 32
+    const bool hit = info[i] != 0u;
+    const unsigned word = __ballot_sync(0xffffffffu, hit);
+    int at = 0;
+    if (lane == 0) {
+      touched[i >> 5] = word;
+      if (word) at = atomicAdd(&s_list, __popc(word));
+    }
+    at = __shfl_sync(0xffffffffu, at, 0);
+    if (hit) list[at + __popc(word & ((1u << lane) - 1u))] = static_cast<uint16_t>(i);
+  }
+  __syncthreads();
+  const int n_list = s_list;
 
   const float rep = a.repetition ? a.repetition[b] : 1.f;
   const float pres = a.presence ? a.presence[b] : 0.f;
   const float freq = a.frequency ? a.frequency[b] : 0.f;
+  constexpr int kPass = kThreads * W;     // tokens of one pass of the CTA
+  constexpr int kBatch = W == 4 ? 4 : 8;  // passes with their loads in flight
+  // a whole slice of one batch: the next row's loads go out before this row's work
+  const bool ahead = v_hi - v_lo == kBatch * kPass;
+  const TI* in0 = static_cast<const TI*>(a.in) + static_cast<size_t>(c0) * a.in_stride;
+  float next[kBatch][W];
+  if (ahead) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      load_w<TI, W>(in0 + t_lo * a.in_stride + v_lo + k * kPass + tid * W, next[k]);
+  }
   for (int t = t_lo; t < t_hi; ++t) {
     const size_t row = static_cast<size_t>(c0) + t;
     bool path = false;
 #pragma unroll
     for (int w = 0; w < kWords; ++w) path |= (s_anc[t][w] & s_in[w]) != 0u;
     const bool on_path = path && tid < n && ((s_anc[t][tid >> 5] & s_in[tid >> 5]) >> (tid & 31)) & 1u;
-    if (path) {
-      __syncthreads();
-      if (on_path) atomicAdd(&info[s_tok[tid] - v_lo], 1u);
-      __syncthreads();
-    }
     const TI* in = static_cast<const TI*>(a.in) + row * a.in_stride;
     TO* out = static_cast<TO*>(a.out) + row * a.out_stride;
     const uint32_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
     // a thread's tokens ascend, so only a larger value replaces its best
     float top = -INFINITY;
     int at = 0;
-    auto constrain = [&](float* x, int i, int v0, uint32_t bits) {
-      uint32_t w[W];
-      if constexpr (W == 4) {
-        const uint4 u = *reinterpret_cast<const uint4*>(info + i);
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-      } else {
-        w[0] = info[i];
-      }
+    auto keep = [&](float* x, int i, uint32_t bits) {  // mask, and best of the untouched
+      const uint32_t hit = touched[i >> 5] >> (i & 31);
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        if (w[e] != 0u) {
-          if (w[e] & kBias) x[e] = __fadd_rn(x[e], a.bias[e0 + bidx[i + e] - 1]);
-          const uint32_t c = w[e] & kCount;
-          if (c != 0u || (w[e] & kPrompt)) x[e] = x[e] > 0.f ? __fdiv_rn(x[e], rep) : __fmul_rn(x[e], rep);
-          x[e] = __fsub_rn(x[e], __fmul_rn(freq, static_cast<float>(c)));
-          if (c != 0u) x[e] = __fsub_rn(x[e], pres);
-        }
         if (!((bits >> e) & 1u)) x[e] = -INFINITY;
-        if (x[e] > top) {
+        if (x[e] > top && !((hit >> e) & 1u)) {
           top = x[e];
-          at = v0 + e;
+          at = v_lo + i + e;
         }
       }
     };
-    constexpr int kPass = kThreads * W;    // tokens of one pass of the CTA
-    constexpr int kBatch = W == 4 ? 4 : 8;  // passes with their loads in flight
+    auto allowed = [&](int v) { return mask ? mask[v >> 5] >> (v & 31) : 0xffffffffu; };
     int i0 = 0;
     for (; v_lo + i0 + kBatch * kPass <= v_hi; i0 += kBatch * kPass) {
       float x[kBatch][W];
@@ -218,13 +233,23 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int v0 = v_lo + i0 + k * kPass + tid * W;
-        load_w<TI, W>(in + v0, x[k]);
-        bits[k] = mask ? mask[v0 >> 5] >> (v0 & 31) : 0xffffffffu;
+        if (ahead) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) x[k][e] = next[k][e];
+        } else {
+          load_w<TI, W>(in + v0, x[k]);
+        }
+        bits[k] = allowed(v0);
+      }
+      if (ahead && t + 1 < t_hi) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          load_w<TI, W>(in + a.in_stride + v_lo + k * kPass + tid * W, next[k]);
       }
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int i = i0 + k * kPass + tid * W;
-        constrain(x[k], i, v_lo + i, bits[k]);
+        keep(x[k], i, bits[k]);
         store_w<TO, W>(out + v_lo + i, x[k]);
       }
     }
@@ -233,12 +258,32 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
       float x[W];
 #pragma unroll
       for (int e = 0; e < W; ++e) x[e] = e < live ? ld_elem(in + v0 + e) : -INFINITY;
-      constrain(x, i, v0, mask ? mask[v0 >> 5] >> (v0 & 31) : 0xffffffffu);
+      keep(x, i, allowed(v0));
 #pragma unroll
       for (int e = 0; e < W; ++e)
         if (e < live) st_elem(out + v0 + e, x[e]);
     }
     unsigned long long best = key_of(top, at);
+    if (n_list > 0) {
+      if (path) {
+        __syncthreads();  // the row before is done with the counts
+        if (on_path) atomicAdd(&info[s_tok[tid] - v_lo], 1u);
+      }
+      __syncthreads();  // the copies are written: the list's tokens go over them
+      for (int p = tid; p < n_list; p += kThreads) {
+        const int i = list[p], v = v_lo + i;
+        const uint32_t w = info[i], c = w & kCount;
+        float x = ld_elem(in + v);  // in place: the copy just written, or -inf where masked
+        if (w & kBias) x = __fadd_rn(x, a.bias[e0 + bidx[i] - 1]);
+        if (c != 0u || (w & kPrompt)) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+        x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(c)));
+        if (c != 0u) x = __fsub_rn(x, pres);
+        if (!(allowed(v) & 1u)) x = -INFINITY;
+        st_elem(out + v, x);
+        const unsigned long long k = key_of(x, v);
+        best = k > best ? k : best;
+      }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
@@ -298,7 +343,7 @@ int logits_slice(int V) {
 template <typename TI, typename TO>
 cudaError_t logits_launch(const LG::Args& a, int chunks, bool vec, cudaStream_t st) {
   const dim3 grid(a.slices, a.B, chunks);
-  const size_t smem = static_cast<size_t>(a.slice) * 8;
+  const size_t smem = static_cast<size_t>(a.slice) * (4 + 4 + 2) + a.slice / 8;
   if (vec) return b2a_host::launch(LG::logits_kernel<TI, TO, 4>, grid, dim3(LG::kThreads), smem, st, a);
   return b2a_host::launch(LG::logits_kernel<TI, TO, 1>, grid, dim3(LG::kThreads), smem, st, a);
 }

@@ -309,11 +309,8 @@ template <typename TS, typename TK, typename TQ>
 __global__ void __launch_bounds__(kRopeThreads) rope_paged_rows(const __grid_constant__ RopeArgs a) {
   pdl_wait();
   const int i = blockIdx.x;
-  int p;
-  long long row;
-  if (!rope_token(a, i, p, row)) return;
   const int groups = a.D >> 3;              // groups of 8 elements (4 pairs) of a head
-  const int heads_at_once = kRopeThreads / groups;
+  const int heads_at_once = blockDim.x / groups;
   const int g = threadIdx.x % groups, h0 = threadIdx.x / groups;
   if (h0 >= heads_at_once) return;
   const int half = a.n_rot >> 1;
@@ -322,10 +319,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_rows(const __grid_con
   const bool split = a.neox && turned;
   const int lo = split ? 4 * g : 8 * g, hi = split ? half + 4 * g : 8 * g + 4;
   float c[4], s[4];
-  if (turned) {
-    load4(a.cos_tab + static_cast<size_t>(p) * half + 4 * g, c);
-    load4(a.sin_tab + static_cast<size_t>(p) * half + 4 * g, s);
-  }
+  int p = -1;  // position, known once the first rows are on their way
+  long long row = -1;
   const int all = a.H + 2 * a.KV;
   const int step = heads_at_once * gridDim.y;
   for (int hb = blockIdx.y * heads_at_once + h0; hb < all; hb += kHeads * step) {
@@ -333,7 +328,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_rows(const __grid_con
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       const int h = hb + u * step;
-      if (h >= all || (row < 0 && h >= a.H)) continue;
+      if (h >= all) continue;
       const TS* src = h < a.H ? static_cast<const TS*>(a.q) + i * a.q_stride + h * a.D
                     : h < a.H + a.KV ? static_cast<const TS*>(a.k) + i * a.k_stride + (h - a.H) * a.D
                                      : static_cast<const TS*>(a.v) + i * a.v_stride + (h - a.H - a.KV) * a.D;
@@ -342,6 +337,13 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_rows(const __grid_con
         load4(src + hi, x[u] + 4);
       } else {
         load8(src + 8 * g, x[u]);
+      }
+    }
+    if (p < 0) {
+      if (!rope_token(a, i, p, row)) return;
+      if (turned) {
+        load4(a.cos_tab + static_cast<size_t>(p) * half + 4 * g, c);
+        load4(a.sin_tab + static_cast<size_t>(p) * half + 4 * g, s);
       }
     }
 #pragma unroll
@@ -576,13 +578,15 @@ cudaError_t rope_paged_launch(const PG::RopeArgs& a, int n_tok, cudaStream_t st)
                     aligned(a.bq, 0, 4) && aligned(a.bk, 0, 4) && aligned(a.bv, 0, 4);
   const int all = a.H + 2 * a.KV;
   if (rows) {
-    // few tokens: a token's heads over more CTAs, until there are a few per SM
-    const int at_once = PG::kRopeThreads / (a.D / 8);
-    int gy = (all + at_once - 1) / at_once;
+    // as many threads as give each kHeads heads; few tokens: a token's heads
+    // over more CTAs, until there are a few per SM
+    const int groups = a.D / 8;
+    int threads = ((all + PG::kHeads - 1) / PG::kHeads * groups + 31) / 32 * 32;
+    if (threads > PG::kRopeThreads) threads = PG::kRopeThreads;
+    int gy = (all + threads / groups - 1) / (threads / groups);
     const int enough = (4 * b2a_host::sm_count() + n_tok - 1) / n_tok;
     if (gy > enough) gy = enough;
-    return b2a_host::launch(PG::rope_paged_rows<TS, TK, TQ>, dim3(n_tok, gy),
-                            dim3(PG::kRopeThreads), 0, st, a);
+    return b2a_host::launch(PG::rope_paged_rows<TS, TK, TQ>, dim3(n_tok, gy), dim3(threads), 0, st, a);
   }
   const int pairs = all * (a.D / 2);
   return b2a_host::launch(PG::rope_paged_pairs<TS, TK, TQ>,

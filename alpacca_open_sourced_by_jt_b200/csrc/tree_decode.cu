@@ -431,22 +431,24 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
 // ---------------------------------------------------------------------------
 // f32 caches: f32 products and sums on the CUDA cores
 // ---------------------------------------------------------------------------
-// 128 threads, items of 16 query rows; K and V tiles arrive by cp.async into
-// two buffers.  Thread (i, j) forms the scores of 2 rows x kTile/16 keys, a
-// warp the softmax of 4 rows, a thread the output column(s) of its rows.
-constexpr int kF32Threads = 128;
+// 256 threads, items of 16 query rows, bound by the FMA pipe.  One K and one V
+// buffer, filled by cp.async: K(t + 1) loads while softmax and P.V of tile t
+// run, V(t + 1) while the scores of t + 1 do.  A thread forms the scores of 2
+// rows x kTile/32 keys (32 FMAs per 6 shared 16-byte reads, which the pipes do
+// in about the same time), a warp the softmax of 2 rows, a thread the output
+// column(s) of its rows.
+constexpr int kF32Threads = 256;
 constexpr int kF32Rows = 16;
 
 template <int D>
 struct F32Cfg {
-  static constexpr int kTile = D > 128 ? 32 : 64;
+  static constexpr int kTile = D > 128 ? 64 : 128;
   static constexpr int kKStride = D + 4;
   static constexpr int kK = kTile * kKStride;
   static constexpr int kV = kTile * D;
-  static constexpr int kStage = kK + kV;
   static constexpr int kQ = kF32Rows * kKStride;
   static constexpr int kP = kF32Rows * (kTile + 4);
-  static constexpr int kSmem = (2 * kStage + kQ + kP) * 4;
+  static constexpr int kSmem = (kK + kV + kQ + kP) * 4;
 };
 
 template <int D>
@@ -458,13 +460,16 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
   using C = F32Cfg<D>;
   constexpr int TILE = C::kTile;
   constexpr int PS = TILE + 4;
+  constexpr int kWarps = kF32Threads / 32;
   extern __shared__ __align__(16) float fsm[];
   __shared__ Start s_start;
   __shared__ int s_par[kMaxNodes];
   __shared__ uint32_t s_anc[kMaxNodes][kWords];
   __shared__ float s_m[kF32Rows], s_l[kF32Rows], s_alpha[kF32Rows];
   pdl_wait();
-  float* qs = fsm + 2 * C::kStage;
+  float* ks = fsm;
+  float* vs = ks + C::kK;
+  float* qs = vs + C::kV;
   float* ps = qs + C::kQ;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 0) {
@@ -475,7 +480,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x == 0) {
     const long long first = static_cast<long long>(max(bt.cu[bt.B], 0)) * bt.H;
-    for (long long r = first + warp; r < static_cast<long long>(bt.n_tok) * bt.H; r += kF32Threads / 32) {
+    for (long long r = first + warp; r < static_cast<long long>(bt.n_tok) * bt.H; r += kWarps) {
       for (int d = lane; d < D; d += 32) out[r * D + d] = 0.f;
       if (lse && lane == 0) lse[r] = -INFINITY;
     }
@@ -483,16 +488,39 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
   Walker wk;
   wk.start(bt, s_start);
   Item it;
-  constexpr int kCols = D > 128 ? D / 128 : 1;              // output columns of a thread
-  constexpr int kSplit = D < 128 ? 128 / D : 1;             // threads that share a column
-  constexpr int kORows = kF32Rows / kSplit;                 // rows of a thread
-  const int oc = tid % (D < 128 ? D : 128);
-  const int or0 = (tid / (D < 128 ? D : 128)) * kORows;
+  constexpr int kCols = D > kF32Threads ? D / kF32Threads : 1;  // output columns of a thread
+  constexpr int kShare = kF32Threads / (D / kCols);             // threads that share a column
+  constexpr int kORows = kF32Rows / kShare;                     // rows of a thread
+  const int oc = tid % (D / kCols);
+  const int or0 = (tid / (D / kCols)) * kORows;
 
   while (wk.next(bt, it)) {
     const int R = it.n * bt.group;
     const int rows = it.len + it.n;
-    __syncthreads();
+    // a K or V tile, rows past the end as zeros
+    auto load = [&](const float* src, float* dst, int stride, int t) {
+      for (int i = tid; i < TILE * (D / 4); i += kF32Threads) {
+        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+        const int row = t * TILE + r;
+        size_t at = 0;
+        int bytes = 0;
+        if (row < rows) {
+          const int pg = checked_page(bt, it.b, table_entry(bt, it.b, row));
+          if (pg < bt.n_pages) {
+            const int in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
+            at = static_cast<size_t>(pg) * page_stride +
+                 (static_cast<size_t>(in_page) * bt.KV + it.kvh) * D + d;
+            bytes = 16;
+          }
+        }
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * stride + d)),
+                     "l"(src + at), "r"(bytes) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();  // the item before is done with every buffer
+    load(kc, ks, C::kKStride, it.t0);
+    load(vc, vs, D, it.t0);
     if (bt.parents)
       for (int i = tid; i < it.n; i += kF32Threads) s_par[i] = bt.parents[it.node0 + i];
     for (int i = tid; i < kF32Rows * (D / 4); i += kF32Threads) {
@@ -512,57 +540,23 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
     __syncthreads();
     ancestor_masks(s_par, bt.parents == nullptr, it.n, s_anc, tid, kF32Threads, it.b);
 
-    auto load = [&](int t, int buf) {
-      float* kd = fsm + buf * C::kStage;
-      float* vd = kd + C::kK;
-      for (int i = tid; i < TILE * (D / 4); i += kF32Threads) {
-        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-        const int row = t * TILE + r;
-        int pg = 0, in_page = 0;
-        bool live = row < rows;
-        if (live) {
-          pg = checked_page(bt, it.b, table_entry(bt, it.b, row));
-          live = pg < bt.n_pages;
-          in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
-        }
-        const size_t src = live ? static_cast<size_t>(pg) * page_stride +
-                                      (static_cast<size_t>(in_page) * bt.KV + it.kvh) * D + d
-                                : 0;
-        const int bytes = live ? 16 : 0;  // rows past the end are filled with zeros
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                         smem_u32(kd + r * C::kKStride + d)), "l"(kc + src), "r"(bytes) : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(vd + r * D + d)),
-                     "l"(vc + src), "r"(bytes) : "memory");
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
     float o[kORows][kCols];
 #pragma unroll
     for (int r = 0; r < kORows; ++r)
 #pragma unroll
       for (int c = 0; c < kCols; ++c) o[r][c] = 0.f;
-    load(it.t0, 0);
     for (int t = it.t0; t < it.t1; ++t) {
-      const int buf = (t - it.t0) & 1;
-      if (t + 1 < it.t1) {
-        load(t + 1, buf ^ 1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      } else {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-      }
+      asm volatile("cp.async.wait_group 1;" ::: "memory");  // K(t); V(t) may be on its way
       __syncthreads();
-      const float* ks = fsm + buf * C::kStage;
-      const float* vs = ks + C::kK;
       {
-        constexpr int KN = TILE / 16;
+        constexpr int KN = TILE / 32;
         const int r0 = (tid & 7) * 2, k0 = tid >> 3;
         float acc[2][KN];
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
           for (int b = 0; b < KN; ++b) acc[a][b] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int d = 0; d < D; d += 4) {
           float4 qa[2];
 #pragma unroll
@@ -570,7 +564,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
             qa[a] = *reinterpret_cast<const float4*>(qs + (r0 + a) * C::kKStride + d);
 #pragma unroll
           for (int b = 0; b < KN; ++b) {
-            const float4 kk = *reinterpret_cast<const float4*>(ks + (k0 + 16 * b) * C::kKStride + d);
+            const float4 kk = *reinterpret_cast<const float4*>(ks + (k0 + 32 * b) * C::kKStride + d);
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
               acc[a][b] = fmaf(qa[a].x, kk.x, acc[a][b]);
@@ -584,17 +578,20 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
         for (int a = 0; a < 2; ++a)
 #pragma unroll
           for (int b = 0; b < KN; ++b) {
-            const int row = t * TILE + k0 + 16 * b;
+            const int row = t * TILE + k0 + 32 * b;
             const int r = it.blk * kF32Rows + r0 + a, j = row - it.len;
             bool see = j < 0;
             if (j >= 0 && j < it.n && r < R) see = (s_anc[r / bt.group][j >> 5] >> (j & 31)) & 1u;
-            ps[(r0 + a) * PS + k0 + 16 * b] = see ? acc[a][b] * sscale : -INFINITY;
+            ps[(r0 + a) * PS + k0 + 32 * b] = see ? acc[a][b] * sscale : -INFINITY;
           }
       }
       __syncthreads();
+      // K's buffer is free (an empty group keeps the count of groups)
+      if (t + 1 < it.t1) load(kc, ks, C::kKStride, t + 1);
+      else asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
-      for (int i = 0; i < kF32Rows / 4; ++i) {
-        const int r = warp * (kF32Rows / 4) + i;
+      for (int i = 0; i < kF32Rows / kWarps; ++i) {
+        const int r = warp * (kF32Rows / kWarps) + i;
         float x[TILE / 32], mx = -INFINITY;
 #pragma unroll
         for (int e = 0; e < TILE / 32; ++e) {
@@ -622,6 +619,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
           s_m[r] = mnew;
         }
       }
+      asm volatile("cp.async.wait_group 1;" ::: "memory");  // V(t)
       __syncthreads();
 #pragma unroll
       for (int r = 0; r < kORows; ++r) {
@@ -629,13 +627,13 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
 #pragma unroll
         for (int c = 0; c < kCols; ++c) o[r][c] *= al;
       }
-#pragma unroll 2
+#pragma unroll 4
       for (int k = 0; k < TILE; k += 4) {
         float v[4][kCols];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) v[e][c] = vs[(k + e) * D + oc + c * 128];
+          for (int c = 0; c < kCols; ++c) v[e][c] = vs[(k + e) * D + oc + c * kF32Threads];
 #pragma unroll
         for (int r = 0; r < kORows; ++r) {
           const float4 p = *reinterpret_cast<const float4*>(ps + (or0 + r) * PS + k);
@@ -649,7 +647,10 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
         }
       }
       __syncthreads();
+      if (t + 1 < it.t1) load(vc, vs, D, t + 1);
+      else asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     const int live = min(kF32Rows, R - it.blk * kF32Rows);
     const int slot = part_slot(it, blockIdx.x);
 #pragma unroll
@@ -660,7 +661,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
       if (slot >= 0) {
         float* po = part_o + (static_cast<size_t>(slot) * kF32Rows + rr) * D;
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) po[oc + c * 128] = o[r][c];
+        for (int c = 0; c < kCols; ++c) po[oc + c * kF32Threads] = o[r][c];
         if (oc == 0) {
           part_ml[(static_cast<size_t>(slot) * kF32Rows + rr) * 2] = s_m[rr];
           part_ml[(static_cast<size_t>(slot) * kF32Rows + rr) * 2 + 1] = l;
@@ -670,7 +671,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
         const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + it.kvh * bt.group + (gr - node * bt.group);
         const float f = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) out[row * D + oc + c * 128] = o[r][c] * f;
+        for (int c = 0; c < kCols; ++c) out[row * D + oc + c * kF32Threads] = o[r][c] * f;
         if (lse && oc == 0) lse[row] = l > 0.f ? (s_m[rr] + log2f(l)) * kLn2 : -INFINITY;
       }
     }
@@ -839,8 +840,7 @@ int tree_rows_per_block(TreeKernel k, int rows, int group) {
   return rows <= 8 ? 8 : 16;
 }
 int tree_tile(TreeKernel k, int D) {
-  if (k == kTreeF32) return D > 128 ? 32 : 64;
-  if (k == kTreeWide) return D > 128 ? 64 : 128;
+  if (k == kTreeF32 || k == kTreeWide) return D > 128 ? 64 : 128;
   return TR::kRows;
 }
 bool tree_by_item(int max_len) { return max_len <= 512; }
@@ -1070,13 +1070,14 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
   a.bt.m_blks = blks > 1 && a.kernel == kTreeWide ? static_cast<int>(blks) : 1;
   a.bt.m_heads = a.bt.m_blks > 1 ? 1 : KV;
   const int members = a.bt.m_heads * a.bt.m_blks;
-  // A list's tiles are cut evenly over the teams, at least 4 to a team.
+  // A list's tiles are cut evenly over the teams, at least 4 to a team (one of
+  // f32, where a tile is work enough).
   const long long max_tiles = (max_len + tile - 1) / tile;
   const long long items = static_cast<long long>(B) * (KV / a.bt.m_heads) *
                           ((max_rows_blocks(rows, rb) + a.bt.m_blks - 1) / a.bt.m_blks);
   a.bt.by_item = tree_by_item(max_len) ? 1 : 0;
-  a.bt.min_units = a.bt.by_item ? 1 : 4;
-  const long long units = a.bt.by_item ? items : (items * max_tiles + 3) / 4;
+  a.bt.min_units = a.bt.by_item || a.kernel == kTreeF32 ? 1 : 4;
+  const long long units = (items * (a.bt.by_item ? 1 : max_tiles) + a.bt.min_units - 1) / a.bt.min_units;
   const int teams = b2a_host::sm_count() > members ? b2a_host::sm_count() / members : 1;
   a.bt.teams = static_cast<int>(units < teams ? units : teams);
   a.grid = a.bt.teams * members;
