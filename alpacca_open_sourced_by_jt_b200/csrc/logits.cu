@@ -11,18 +11,21 @@
 // every operation rounded once to f32.  The pick is the lowest v of the
 // largest x (-1 where no x is above -inf).
 //
-// Bound by reading and writing the rows.  The tokens that need more than a copy
-// and a mask are few, but evaluated where they stand they would hold up their
-// whole warp (a division each).  A CTA takes one slice of the vocabulary of one
-// request; from the history, the biases and the drafted tokens it builds, once
-// for several rows, the slice's counts in shared memory (integer atomics: the
-// order does not matter), a bit per token that is touched, and a list of the
-// touched tokens.  Each row is then streamed through with mask and maximum of
-// the untouched tokens while the next row's loads are in flight, and the list's
-// tokens are redone, one to a thread.  A node's path is added to the counts
-// before its row's list and taken off after it, where a drafted token falls
-// into the slice.  Each warp leaves its best (value, lowest token) as one
-// ordered 64-bit key and a second small kernel takes the rows' maxima.
+// Bound by reading and writing the rows, if the few tokens that need more than
+// a copy and a mask are kept out of the way of the others.  A CTA takes one
+// slice of the vocabulary of one request; from the history, the biases and the
+// drafted tokens it builds, once for several rows, the slice's counts in shared
+// memory (integer atomics: the order does not matter) and, for each warp, the
+// list of the touched ones among the tokens it streams.  For each row a warp
+// evaluates its list first, one token to a lane, into shared memory, then
+// streams its part of the row through, 16 tokens a thread, taking the touched
+// ones from there, with the next row's loads in flight: no barrier of the CTA in
+// the loop.  A node's path is added to the counts before its row and taken off
+// after it by the warp that has the drafted token.  Each warp leaves its best
+// (value, lowest token) as one ordered 64-bit key and a second small kernel
+// takes the rows' maxima.  (1023 rows of 128256: divisions where the tokens
+// stand 280 us; one list per CTA and a barrier a row 378; now
+// 282, 3.7 TB/s.)
 
 #include "b2a_common.cuh"
 
@@ -31,6 +34,8 @@ namespace logits {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kEach = 16;                 // tokens of a thread
+constexpr int kSlice = kThreads * kEach;  // tokens of a CTA
 constexpr int kMaxNodes = B2A_TREE_MAX_NODES;
 constexpr int kWords = kMaxNodes / 32;
 constexpr uint32_t kPrompt = 0x80000000u;  // the token is in the prompt
@@ -52,16 +57,14 @@ struct Args {
   long long mask_stride;
   unsigned long long* best;  // [n_rows][slices * kWarps]
   int* picks;
-  int n_hist, n_bias, B, n_rows, max_nodes, V, slice, slices, rows_per_cta;
+  int n_hist, n_bias, B, n_rows, max_nodes, V, slices, rows_per_cta;
 };
 
-// A value's place in the order of floats, 0 for what cannot be picked (NaN,
-// -inf); ties go to the lowest token.
-__device__ __forceinline__ unsigned long long key_of(float x, int v) {
-  if (!(x > -INFINITY)) return 0ull;
+// A value's place in the order of floats, 0 for what cannot be picked (-inf).
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (!(x > -INFINITY)) return 0u;
   const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
-  const uint32_t o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return (static_cast<unsigned long long>(o) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
 template <typename T, int W>
@@ -69,10 +72,10 @@ __device__ __forceinline__ void load_w(const T* p, float* x) {
   if constexpr (W == 1) {
     x[0] = ld_elem(p);
   } else if constexpr (sizeof(T) == 4) {
-    const float4 f = __ldcs(reinterpret_cast<const float4*>(p));
+    const float4 f = *reinterpret_cast<const float4*>(p);
     x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
   } else {
-    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
     const T* h = reinterpret_cast<const T*>(&u);
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = ld_elem(h + e);
@@ -93,35 +96,61 @@ __device__ __forceinline__ void store_w(T* p, const float* x) {
   }
 }
 
+// W = 4: rows whose groups of 4 tokens are aligned; W = 1: any.
 template <typename TI, typename TO, int W>
 __global__ void __launch_bounds__(kThreads, 3) logits_kernel(const __grid_constant__ Args a) {
   pdl_wait();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(16) uint32_t lsm[];
-  uint32_t* info = lsm;               // [slice] flags and counts
-  uint32_t* bidx = lsm + a.slice;     // [slice] 1 + bias entry
-  uint32_t* touched = bidx + a.slice;  // [slice / 32] a bit per token with info
-  uint16_t* list = reinterpret_cast<uint16_t*>(touched + a.slice / 32);  // [slice] those tokens
-  __shared__ int s_list;              // how many
+  uint32_t* info = lsm;               // [kSlice] flags and counts
+  uint32_t* bidx = info + kSlice;     // [kSlice] 1 + bias entry
+  float* fixed = reinterpret_cast<float*>(bidx + kSlice);  // [kSlice] touched tokens' values
+  uint16_t* lists = reinterpret_cast<uint16_t*>(fixed + kSlice);  // [kWarps][kSlice / kWarps] their places
   __shared__ uint32_t s_anc[kMaxNodes][kWords];
   __shared__ int s_par[kMaxNodes], s_tok[kMaxNodes];
-  __shared__ uint32_t s_in[kWords];   // the request's nodes whose token is in the slice
+  __shared__ uint32_t s_in[kWarps][kWords];  // the nodes whose token is among the warp's
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int b = blockIdx.y;
+  // slices in the grid's slowest dimension: the first slices, where frequent
+  // tokens are and lists are long, start first
+  const int b = blockIdx.x, slice = blockIdx.z;
   const int c0 = a.cu[b];
   const int n = a.cu[b + 1] - c0;
   if (n < 0 || n > a.max_nodes || c0 < 0 || c0 + n > a.n_rows) {
     if (tid == 0) set_dev_error(B2A_ERR_POSITION, b);
     return;
   }
-  const int t_lo = blockIdx.z * a.rows_per_cta, t_hi = min(n, t_lo + a.rows_per_cta);
+  const int t_lo = blockIdx.y * a.rows_per_cta, t_hi = min(n, t_lo + a.rows_per_cta);
   if (t_lo >= t_hi) return;
-  const int v_lo = blockIdx.x * a.slice, v_hi = min(a.V, v_lo + a.slice);
+  const int v_lo = slice * kSlice, v_hi = min(a.V, v_lo + kSlice);
 
-  for (int i = tid * 4; i < 2 * a.slice; i += kThreads * 4)
+  // group k of this thread: W tokens from v_lo + k * kPass + tid * W on
+  constexpr int kGroups = kEach / W;
+  constexpr int kPass = kThreads * W;
+  const int len = v_hi - v_lo;
+  const TI* in = static_cast<const TI*>(a.in) + (static_cast<size_t>(c0) + t_lo) * a.in_stride + v_lo;
+  TO* out = static_cast<TO*>(a.out) + (static_cast<size_t>(c0) + t_lo) * a.out_stride + v_lo;
+  const uint32_t* mask =
+      a.mask ? a.mask + (static_cast<size_t>(c0) + t_lo) * a.mask_stride + (v_lo >> 5) : nullptr;
+  float next[kEach];
+  uint32_t next_mask[W == 4 ? kGroups : 1];
+  auto fetch = [&](const TI* src, const uint32_t* m) {
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const int i = k * kPass + tid * W;
+      if (i + W <= len) {
+        load_w<TI, W>(src + i, next + k * W);
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) next[k * W + e] = i + e < len ? ld_elem(src + i + e) : -INFINITY;
+      }
+      if constexpr (W == 4) next_mask[k] = m && i < len ? m[i >> 5] : 0xffffffffu;
+    }
+  };
+  fetch(in, mask);
+
+  for (int i = tid * 4; i < 2 * kSlice; i += kThreads * 4)
     *reinterpret_cast<uint4*>(lsm + i) = make_uint4(0u, 0u, 0u, 0u);
-  if (tid < kWords) s_in[tid] = 0u;
-  if (tid == 0) s_list = 0;
+  if (tid < kWarps * kWords) s_in[tid / kWords][tid % kWords] = 0u;
   if (tid < n) {
     s_par[tid] = a.parents ? a.parents[c0 + tid] : tid - 1;
     s_tok[tid] = a.tokens ? a.tokens[c0 + tid] : -1;
@@ -131,12 +160,20 @@ __global__ void __launch_bounds__(kThreads, 3) logits_kernel(const __grid_consta
     const int h0 = min(max(a.hist_start[b], 0), a.n_hist);
     const int h1 = min(max(a.hist_start[b + 1], h0), a.n_hist);
     const int p1 = h0 + (a.prompt_len ? min(max(a.prompt_len[b], 0), h1 - h0) : 0);
-#pragma unroll 4
-    for (int i = h0 + tid; i < h1; i += kThreads) {
-      const int v = a.hist[i];
-      if (v < v_lo || v >= v_hi) continue;
-      if (i < p1) atomicOr(&info[v - v_lo], kPrompt);
-      else atomicAdd(&info[v - v_lo], 1u);
+    // several loads a thread in flight: one at a time, a history of thousands
+    // took longer than the rows
+    constexpr int kLoads = 8;
+    for (int i0 = h0 + tid; i0 < h1; i0 += kLoads * kThreads) {
+      int v[kLoads];
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+        v[k] = i0 + k * kThreads < h1 ? a.hist[i0 + k * kThreads] : -1;
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k) {
+        if (v[k] < v_lo || v[k] >= v_hi) continue;
+        if (i0 + k * kThreads < p1) atomicOr(&info[v[k] - v_lo], kPrompt);
+        else atomicAdd(&info[v[k] - v_lo], 1u);
+      }
     }
   }
   int e0 = 0;
@@ -152,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 3) logits_kernel(const __grid_consta
   }
   if (tid < n) {
     if (s_tok[tid] >= v_lo && s_tok[tid] < v_hi) {
-      atomicOr(&s_in[tid >> 5], 1u << (tid & 31));
+      atomicOr(&s_in[(s_tok[tid] - v_lo) % kPass / (32 * W)][tid >> 5], 1u << (tid & 31));
       atomicOr(&info[s_tok[tid] - v_lo], kDraft);
     }
     uint32_t m[kWords];
@@ -174,126 +211,121 @@ __global__ void __launch_bounds__(kThreads, 3) logits_kernel(const __grid_consta
     for (int w = 0; w < kWords; ++w) s_anc[tid][w] = m[w];
   }
   __syncthreads();
-  for (int i = tid; i < a.slice; i += kThreads) {  // whole warps: the slice is a multiple of 32
-    const bool hit = info[i] != 0u;
-    const unsigned word = __ballot_sync(0xffffffffu, hit);
-    int at = 0;
-    if (lane == 0) {
-      touched[i >> 5] = word;
-      if (word) at = atomicAdd(&s_list, __popc(word));
+  // this thread's touched tokens (the same for all rows), and the warp's list
+  uint16_t* list = lists + warp * (kSlice / kWarps);
+  uint32_t hits = 0u;
+  int n_list = 0;
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k)
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const int i = k * kPass + tid * W + e;
+      const bool hit = info[i] != 0u;
+      const unsigned word = __ballot_sync(0xffffffffu, hit);
+      if (hit) {
+        hits |= 1u << (k * W + e);
+        list[n_list + __popc(word & ((1u << lane) - 1u))] = static_cast<uint16_t>(i);
+      }
+      n_list += __popc(word);
     }
-    at = __shfl_sync(0xffffffffu, at, 0);
-    if (hit) list[at + __popc(word & ((1u << lane) - 1u))] = static_cast<uint16_t>(i);
-  }
-  __syncthreads();
-  const int n_list = s_list;
+  __syncwarp();
 
   const float rep = a.repetition ? a.repetition[b] : 1.f;
   const float pres = a.presence ? a.presence[b] : 0.f;
   const float freq = a.frequency ? a.frequency[b] : 0.f;
-  constexpr int kPass = kThreads * W;     // tokens of one pass of the CTA
-  constexpr int kBatch = W == 4 ? 4 : 8;  // passes with their loads in flight
-  // a whole slice of one batch: the next row's loads go out before this row's work
-  const bool ahead = v_hi - v_lo == kBatch * kPass;
-  const TI* in0 = static_cast<const TI*>(a.in) + static_cast<size_t>(c0) * a.in_stride;
-  float next[kBatch][W];
-  if (ahead) {
+  // the list's first round of the next row is loaded one row ahead
+  const int mine = lane < n_list ? list[lane] : 0;
+  float ahead = lane < n_list ? ld_elem(in + mine) : 0.f;
+  unsigned long long* best_out =
+      a.best + ((static_cast<size_t>(c0) + t_lo) * a.slices + slice) * kWarps + warp;
+  // the counts change by `by` for the path of node t's tokens that are this warp's
+  auto count_path = [&](int t, uint32_t by) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      load_w<TI, W>(in0 + t_lo * a.in_stride + v_lo + k * kPass + tid * W, next[k]);
-  }
+    for (int w = 0; w < kWords; ++w)
+      if ((s_anc[t][w] & s_in[warp][w]) >> lane & 1u) atomicAdd(&info[s_tok[w * 32 + lane] - v_lo], by);
+    __syncwarp();
+  };
+  const bool drafts = (s_in[warp][0] | s_in[warp][1] | s_in[warp][2] | s_in[warp][3]) != 0u;
+  static_assert(kWords == 4, "drafts");
   for (int t = t_lo; t < t_hi; ++t) {
-    const size_t row = static_cast<size_t>(c0) + t;
-    bool path = false;
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) path |= (s_anc[t][w] & s_in[w]) != 0u;
-    const bool on_path = path && tid < n && ((s_anc[t][tid >> 5] & s_in[tid >> 5]) >> (tid & 31)) & 1u;
-    const TI* in = static_cast<const TI*>(a.in) + row * a.in_stride;
-    TO* out = static_cast<TO*>(a.out) + row * a.out_stride;
-    const uint32_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
-    // a thread's tokens ascend, so only a larger value replaces its best
-    float top = -INFINITY;
-    int at = 0;
-    auto keep = [&](float* x, int i, uint32_t bits) {  // mask, and best of the untouched
-      const uint32_t hit = touched[i >> 5] >> (i & 31);
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        if (!((bits >> e) & 1u)) x[e] = -INFINITY;
-        if (x[e] > top && !((hit >> e) & 1u)) {
-          top = x[e];
-          at = v_lo + i + e;
-        }
-      }
-    };
-    auto allowed = [&](int v) { return mask ? mask[v >> 5] >> (v & 31) : 0xffffffffu; };
-    int i0 = 0;
-    for (; v_lo + i0 + kBatch * kPass <= v_hi; i0 += kBatch * kPass) {
-      float x[kBatch][W];
-      uint32_t bits[kBatch];
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int v0 = v_lo + i0 + k * kPass + tid * W;
-        if (ahead) {
-#pragma unroll
-          for (int e = 0; e < W; ++e) x[k][e] = next[k][e];
-        } else {
-          load_w<TI, W>(in + v0, x[k]);
-        }
-        bits[k] = allowed(v0);
-      }
-      if (ahead && t + 1 < t_hi) {
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-          load_w<TI, W>(in + a.in_stride + v_lo + k * kPass + tid * W, next[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int i = i0 + k * kPass + tid * W;
-        keep(x[k], i, bits[k]);
-        store_w<TO, W>(out + v_lo + i, x[k]);
-      }
-    }
-    for (int i = i0 + tid * W; v_lo + i < v_hi; i += kPass) {
-      const int v0 = v_lo + i, live = min(W, v_hi - v0);
-      float x[W];
-#pragma unroll
-      for (int e = 0; e < W; ++e) x[e] = e < live ? ld_elem(in + v0 + e) : -INFINITY;
-      keep(x, i, allowed(v0));
-#pragma unroll
-      for (int e = 0; e < W; ++e)
-        if (e < live) st_elem(out + v0 + e, x[e]);
-    }
-    unsigned long long best = key_of(top, at);
     if (n_list > 0) {
-      if (path) {
-        __syncthreads();  // the row before is done with the counts
-        if (on_path) atomicAdd(&info[s_tok[tid] - v_lo], 1u);
-      }
-      __syncthreads();  // the copies are written: the list's tokens go over them
-      for (int p = tid; p < n_list; p += kThreads) {
-        const int i = list[p], v = v_lo + i;
+      if (drafts) count_path(t, 1u);
+      for (int p = lane; p < n_list; p += 32) {
+        const int i = list[p];
         const uint32_t w = info[i], c = w & kCount;
-        float x = ld_elem(in + v);  // in place: the copy just written, or -inf where masked
-        if (w & kBias) x = __fadd_rn(x, a.bias[e0 + bidx[i] - 1]);
-        if (c != 0u || (w & kPrompt)) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-        x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(c)));
-        if (c != 0u) x = __fsub_rn(x, pres);
-        if (!(allowed(v) & 1u)) x = -INFINITY;
-        st_elem(out + v, x);
-        const unsigned long long k = key_of(x, v);
-        best = k > best ? k : best;
+        float y = p == lane ? ahead : ld_elem(in + i);
+        if (w & kBias) y = __fadd_rn(y, a.bias[e0 + bidx[i] - 1]);
+        if (c != 0u || (w & kPrompt)) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+        y = __fsub_rn(y, __fmul_rn(freq, static_cast<float>(c)));
+        if (c != 0u) y = __fsub_rn(y, pres);
+        fixed[i] = y;
+      }
+      if (t + 1 < t_hi && lane < n_list) ahead = ld_elem(in + a.in_stride + mine);
+      __syncwarp();
+      if (drafts) count_path(t, 0xffffffffu);  // minus one
+    }
+    float x[kEach];
+    uint32_t allowed = 0u;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) x[e] = next[e];
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const int i = k * kPass + tid * W;
+      uint32_t word;
+      if constexpr (W == 4) word = next_mask[k];
+      else word = mask && i < len ? mask[i >> 5] : 0xffffffffu;
+      allowed |= ((word >> (i & 31)) & ((1u << W) - 1u)) << (k * W);
+    }
+    if (t + 1 < t_hi) fetch(in + a.in_stride, mask ? mask + a.mask_stride : nullptr);
+    if (hits != 0u) {
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        if (((hits >> (k * W)) & ((1u << W) - 1u)) == 0u) continue;
+        float f[W];
+        load_w<float, W>(fixed + k * kPass + tid * W, f);
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          if ((hits >> (k * W + e)) & 1u) x[k * W + e] = f[e];
       }
     }
+    if (allowed != (kEach == 32 ? 0xffffffffu : (1u << kEach) - 1u)) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
-      best = k > best ? k : best;
+      for (int e = 0; e < kEach; ++e)
+        if (!((allowed >> e) & 1u)) x[e] = -INFINITY;
     }
-    if (lane == 0) a.best[(row * a.slices + blockIdx.x) * kWarps + warp] = best;
-    if (path) {
-      __syncthreads();
-      if (on_path) atomicSub(&info[s_tok[tid] - v_lo], 1u);
+    float top = -INFINITY;  // (fmaxf passes NaN over: it cannot be picked)
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const int i = k * kPass + tid * W;
+#pragma unroll
+      for (int e = 0; e < W; ++e) top = fmaxf(top, x[k * W + e]);
+      if (i + W <= len) {
+        store_w<TO, W>(out + i, x + k * W);
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          if (i + e < len) st_elem(out + i + e, x[k * W + e]);
+      }
     }
+    // the warp's largest value, and the lowest token that has it
+    const uint32_t order = order_of(top);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, order);
+    uint32_t at = 0xffffffffu;
+    if (most != 0u && order == most) {
+#pragma unroll
+      for (int k = kGroups - 1; k >= 0; --k)
+#pragma unroll
+        for (int e = W - 1; e >= 0; --e)
+          if (x[k * W + e] == top) at = v_lo + k * kPass + tid * W + e;
+    }
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0)
+      *best_out = most ? (static_cast<unsigned long long>(most) << 32) | (0xffffffffu - at) : 0ull;
+    __syncwarp();  // the values are read: the next row's list may be evaluated
+    in += a.in_stride;
+    out += a.out_stride;
+    if (mask) mask += a.mask_stride;
+    best_out += static_cast<size_t>(a.slices) * kWarps;
   }
 }
 
@@ -334,18 +366,16 @@ namespace {
 
 namespace LG = b2a::logits;
 
-int logits_slice(int V) {
-  int s = 4096;
-  while (s > 1024 && s / 2 >= V) s /= 2;
-  return s;
-}
+int logits_slices(int V) { return (V + LG::kSlice - 1) / LG::kSlice; }
 
-template <typename TI, typename TO>
-cudaError_t logits_launch(const LG::Args& a, int chunks, bool vec, cudaStream_t st) {
-  const dim3 grid(a.slices, a.B, chunks);
-  const size_t smem = static_cast<size_t>(a.slice) * (4 + 4 + 2) + a.slice / 8;
-  if (vec) return b2a_host::launch(LG::logits_kernel<TI, TO, 4>, grid, dim3(LG::kThreads), smem, st, a);
-  return b2a_host::launch(LG::logits_kernel<TI, TO, 1>, grid, dim3(LG::kThreads), smem, st, a);
+template <typename TI, typename TO, int W>
+cudaError_t logits_launch(const LG::Args& a, int chunks, cudaStream_t st) {
+  auto kern = LG::logits_kernel<TI, TO, W>;
+  constexpr int smem = LG::kSlice * (4 + 4 + 4 + 2);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = allow_smem(kern, smem, done);
+  if (e != cudaSuccess) return e;
+  return b2a_host::launch(kern, dim3(a.B, chunks, a.slices), dim3(LG::kThreads), smem, st, a);
 }
 
 }  // namespace
@@ -354,8 +384,7 @@ extern "C" {
 
 size_t b2a_constrain_logits_workspace_bytes(int n_rows, int V) {
   if (n_rows <= 0 || V <= 0) return 0;
-  const int s = logits_slice(V);
-  return static_cast<size_t>(n_rows) * ((V + s - 1) / s) * LG::kWarps * 8;
+  return static_cast<size_t>(n_rows) * logits_slices(V) * LG::kWarps * 8;
 }
 
 int b2a_constrain_logits(const void* logits, long long row_stride, int in_dtype, void* out,
@@ -418,9 +447,8 @@ int b2a_constrain_logits(const void* logits, long long row_stride, int in_dtype,
   a.n_rows = n_rows;
   a.max_nodes = max_nodes;
   a.V = V;
-  a.slice = logits_slice(V);
-  a.slices = (V + a.slice - 1) / a.slice;
-  a.rows_per_cta = 8;
+  a.slices = logits_slices(V);
+  a.rows_per_cta = 16;
   const int chunks = (max_nodes + a.rows_per_cta - 1) / a.rows_per_cta;
   // 4 logits per access where every row starts on such a boundary
   auto fits = [](const void* p, long long stride, int es) {
@@ -432,7 +460,7 @@ int b2a_constrain_logits(const void* logits, long long row_stride, int in_dtype,
     return with_type(out_dtype, [&](auto* to) {
       using TI = typename std::remove_pointer<decltype(ti)>::type;
       using TO = typename std::remove_pointer<decltype(to)>::type;
-      return logits_launch<TI, TO>(a, chunks, vec, st);
+      return vec ? logits_launch<TI, TO, 4>(a, chunks, st) : logits_launch<TI, TO, 1>(a, chunks, st);
     });
   });
   if (e == cudaSuccess)
