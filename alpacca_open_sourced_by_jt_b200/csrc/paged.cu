@@ -612,7 +612,8 @@ int b2a_page_plan(const int* lens_dev, const int* add_dev, const int* parents_de
                   int* ring_state_out_dev, int* cu_dev, int* seq_dev, int* pos_dev, int* slot_dev,
                   int B, int max_tokens, int max_pages, int page_rows, void* stream) {
   if (!lens_dev || !add_dev || !held_dev || !held_out_dev || !table_dev || !ring_dev ||
-      !ring_state_dev || !ring_state_out_dev || !cu_dev || !seq_dev || !pos_dev || !slot_dev)
+      !ring_state_dev || !ring_state_out_dev || !cu_dev ||
+      (max_tokens > 0 && (!seq_dev || !pos_dev || !slot_dev)))
     return fail(B2A_ERR_ARG, "page_plan: null pointer argument");
   if (B <= 0 || max_tokens < 0 || max_pages <= 0 || ring_size <= 0)
     return fail(B2A_ERR_ARG, "page_plan: sizes must be positive (B=%d max_tokens=%d max_pages=%d ring=%d)",

@@ -525,7 +525,7 @@ int b2a_q8_dequant(const void* codes, long long ldq, const void* scales, long lo
  *                    held and ring_state: the call can then be repeated)
  *   cu               int32 [B + 1]
  *   seq, pos, slot   int32 [max_tokens]: a token's request, RoPE position and
- *                    slot; padding rows get -1, 0, -1
+ *                    slot; padding rows get -1, 0, -1 (NULL if max_tokens is 0)
  * Pages go to the requests in order: request b is served if the pages wanted
  * up to and including its own are there (or it wants none) and its rows fit
  * max_pages; else it keeps what it holds and its tokens' slots are -1. */
