@@ -824,7 +824,13 @@ cudaError_t allow_smem(K kern, int smem, std::atomic<unsigned long long>& done) 
   return e;
 }
 
-// Which kernel, by type and by the most rows a KV head can have.
+// Which kernel, by type and by the most rows a KV head can have.  16 x 32K rows,
+// bf16, pages of 64, tree_mma against tree_wide, us: D = 64, 4 rows 223 / 243, 16
+// rows 244 / 244; D = 128, 4 rows 355 / 356, 16 rows 346 / 358; D = 256, 8 rows
+// 202 / 210 (16 rows do not fit tree_mma's registers: 295 / 213).  From 17 rows on
+// tree_mma would read shared memory once more per 16 rows: 32 rows of D = 128
+// took 445 / 365.  In short contexts tree_wide's set-up shows too: one request of
+// 64 rows 7.0 / 9.7, 16 of 1024 24 / 37.
 enum TreeKernel { kTreeF32, kTreeMma, kTreeWide };
 
 TreeKernel tree_kernel(int dtype, int rows, int D) {
@@ -832,8 +838,7 @@ TreeKernel tree_kernel(int dtype, int rows, int D) {
   return rows <= (D > 128 ? 8 : 16) ? kTreeMma : kTreeWide;
 }
 
-// Query rows of an item, keys of a tile, and whether CTAs take whole items
-// (short contexts: one launch without parts to join costs less than cutting).
+// Query rows of an item and keys of a tile.
 int tree_rows_per_block(TreeKernel k, int rows, int group) {
   if (k == kTreeF32) return TR::kF32Rows;
   if (k == kTreeWide) return TR::kWideM / group * group;
@@ -843,7 +848,18 @@ int tree_tile(TreeKernel k, int D) {
   if (k == kTreeF32 || k == kTreeWide) return D > 128 ? 64 : 128;
   return TR::kRows;
 }
-bool tree_by_item(int max_len) { return max_len <= 512; }
+// Whole items per CTA, one launch without parts to join, or items cut evenly
+// over the CTAs.  Cutting costs some 12 us (division of the work by tiles, the
+// parts, the second kernel).  Whole against cut, 32/8 heads x 64, f16, pages of
+// 16, us: 1 request of 512 rows 9.3 / 12.2, of 1024 12.1 / 12.6, of 2048 18.8 /
+// 13.2; 4 of 1024 12.4 / 15.8, of 4000 32 / 21; 16 of 1024 12.6 / 24.6, of 4000
+// 35 / 43; 64 of 200 to 2047 55 / 76, of 4000 122 / 127.  So: short contexts, and
+// middling ones where the items alone nearly fill the SMs.
+bool tree_always_whole(int max_len) { return max_len <= 1024; }
+bool tree_by_item(int max_len, int B, int KV) {
+  return tree_always_whole(max_len) ||
+         (max_len <= 4096 && static_cast<long long>(B) * KV * 4 >= 3LL * b2a_host::sm_count());
+}
 int max_rows_blocks(int rows, int rows_per_block) { return (rows + rows_per_block - 1) / rows_per_block; }
 
 struct TreeArgs {
@@ -997,7 +1013,7 @@ extern "C" {
 
 size_t b2a_tree_decode_workspace_bytes(int max_nodes, int H, int KV, int D, int dtype, int max_len) {
   if (max_nodes <= 0 || H <= 0 || KV <= 0 || D <= 0 || H % KV != 0) return 0;
-  if (tree_by_item(max_len)) return 0;
+  if (tree_always_whole(max_len)) return 0;
   const int rows = max_nodes * (H / KV);
   const int rb = tree_rows_per_block(tree_kernel(dtype, rows, D), rows, H / KV);
   return tree_part_o_bytes(D, KV, rb) + static_cast<size_t>(2) * tree_ctas(KV) * rb * 2 * sizeof(float);
@@ -1059,9 +1075,11 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
   a.bt = TR::Batch{lens_dev, cu_dev, parents_dev, table_dev, table_stride, B, n_tok, max_nodes,
                    max_len, n_pages, table_dev ? log2_of(page_rows) : 0, H, KV, group, rb, tile, 0, 1, 1, 1, 1};
   // Side by side in a team: the KV heads, or, where a request has several
-  // blocks of query rows, those (as many as the average request has; one with
-  // more goes round again).  16 x 32K rows, bf16, 32/8 x 128, 128 nodes (4
-  // blocks): MEASURED_TEAMS
+  // blocks of query rows, those (as many as the average request has, or as the
+  // largest where that is not much more; a request with more goes round again).
+  // 16 x 32K rows, bf16, 32/8 heads x 128, 128 nodes (4 blocks): 1465 us with the
+  // heads side by side (every block reads K and V from HBM again), 1170 with the
+  // blocks.
   const long long avg_rows = static_cast<long long>(n_tok) * group / B;
   long long blks = (avg_rows + rb / 2) / rb;
   const int most = max_rows_blocks(rows, rb);
@@ -1075,7 +1093,7 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
   const long long max_tiles = (max_len + tile - 1) / tile;
   const long long items = static_cast<long long>(B) * (KV / a.bt.m_heads) *
                           ((max_rows_blocks(rows, rb) + a.bt.m_blks - 1) / a.bt.m_blks);
-  a.bt.by_item = tree_by_item(max_len) ? 1 : 0;
+  a.bt.by_item = tree_by_item(max_len, B, KV) ? 1 : 0;
   a.bt.min_units = a.bt.by_item || a.kernel == kTreeF32 ? 1 : 4;
   const long long units = (items * (a.bt.by_item ? 1 : max_tiles) + a.bt.min_units - 1) / a.bt.min_units;
   const int teams = b2a_host::sm_count() > members ? b2a_host::sm_count() / members : 1;

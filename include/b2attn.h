@@ -565,8 +565,8 @@ int b2a_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
  *             page_rows without a table); paged caches: page_rows >= 16
  * Padding rows of out become 0 (lse -inf).  16-bit types: tensor cores, f32
  * scores, sums and accumulators, the weights rounded to the type for the
- * product with V.  F32: f32 products and sums.  Short contexts need no workspace
- * (0 bytes, NULL).  One node per request is a
+ * product with V.  F32: f32 products and sums.  Short contexts (max_len up to
+ * 1024) need no workspace (0 bytes, NULL).  One node per request is a
  * batched decode step. */
 size_t b2a_tree_decode_workspace_bytes(int max_nodes, int H, int KV, int D, int dtype, int max_len);
 int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
