@@ -16,6 +16,11 @@ Layers:
   qwen35_layer                Qwen35 full-attention layer step on the device
   decode_chain, prefill_chain whole decode token / prefill chunk of a Q8_0 llama
                               model on the device
+  paged                       many requests over one paged cache: page plan, append by
+                              slot, attention of drafted token trees, logits
+                              constraints, commit of accepted paths
+  draft_step                  a llama step that runs them: verify draft trees of many
+                              requests
 """
 from . import _lib  # noqa: F401
 from ._lib import B2AError, B2AShapeError, B2ADeviceError  # noqa: F401
