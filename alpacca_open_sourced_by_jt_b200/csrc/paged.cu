@@ -228,7 +228,9 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
 // sums are rounded one by one, as rope_append.cu does.  Two kernels:
 //   rope_paged_rows   rows in 16-byte aligned groups of 8 elements.  A thread
 //     keeps its 4 pairs' cosines and sines and goes over heads with them; the
-//     loads of kHeads heads are in flight at once.
+//     loads of kHeads heads are in flight at once, before the position is known.
+//     8 CTAs per SM go over the tokens (8191 tokens, 32/8 heads x 64, f16: 27.8 us;
+//     a CTA per token 29.7; one pair per thread and step 83).
 //   rope_paged_pairs  anything else (odd head or rotation widths, unaligned
 //     strides): one pair per thread and step.
 struct RopeArgs {
@@ -238,7 +240,7 @@ struct RopeArgs {
   const int *pos, *slots;
   void *k_pool, *v_pool, *q_out;
   long long page_stride, n_slots;
-  int tab_rows, page_shift, H, KV, D, n_rot, neox;
+  int tab_rows, page_shift, H, KV, D, n_rot, neox, n_tok;
 };
 
 // The token's position and pool row (negative: not stored); false if the
@@ -308,7 +310,6 @@ constexpr int kHeads = 3;  // heads of a thread with their loads in flight
 template <typename TS, typename TK, typename TQ>
 __global__ void __launch_bounds__(kRopeThreads) rope_paged_rows(const __grid_constant__ RopeArgs a) {
   pdl_wait();
-  const int i = blockIdx.x;
   const int groups = a.D >> 3;              // groups of 8 elements (4 pairs) of a head
   const int heads_at_once = blockDim.x / groups;
   const int g = threadIdx.x % groups, h0 = threadIdx.x / groups;
@@ -318,81 +319,83 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_rows(const __grid_con
   // elements of the group: [lo, lo + 4) and [hi, hi + 4)
   const bool split = a.neox && turned;
   const int lo = split ? 4 * g : 8 * g, hi = split ? half + 4 * g : 8 * g + 4;
-  float c[4], s[4];
-  int p = -1;  // position, known once the first rows are on their way
-  long long row = -1;
   const int all = a.H + 2 * a.KV;
   const int step = heads_at_once * gridDim.y;
-  for (int hb = blockIdx.y * heads_at_once + h0; hb < all; hb += kHeads * step) {
-    float x[kHeads][8];
+  for (int i = blockIdx.x; i < a.n_tok; i += gridDim.x) {
+    float c[4], s[4];
+    int p = -1;  // position, known once the first rows are on their way
+    long long row = -1;
+    for (int hb = blockIdx.y * heads_at_once + h0; hb < all; hb += kHeads * step) {
+      float x[kHeads][8];
 #pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const int h = hb + u * step;
-      if (h >= all) continue;
-      const TS* src = h < a.H ? static_cast<const TS*>(a.q) + i * a.q_stride + h * a.D
-                    : h < a.H + a.KV ? static_cast<const TS*>(a.k) + i * a.k_stride + (h - a.H) * a.D
-                                     : static_cast<const TS*>(a.v) + i * a.v_stride + (h - a.H - a.KV) * a.D;
-      if (split && h < a.H + a.KV) {
-        load4(src + lo, x[u]);
-        load4(src + hi, x[u] + 4);
-      } else {
-        load8(src + 8 * g, x[u]);
+      for (int u = 0; u < kHeads; ++u) {
+        const int h = hb + u * step;
+        if (h >= all) continue;
+        const TS* src = h < a.H ? static_cast<const TS*>(a.q) + i * a.q_stride + h * a.D
+                      : h < a.H + a.KV ? static_cast<const TS*>(a.k) + i * a.k_stride + (h - a.H) * a.D
+                                       : static_cast<const TS*>(a.v) + i * a.v_stride + (h - a.H - a.KV) * a.D;
+        if (split && h < a.H + a.KV) {
+          load4(src + lo, x[u]);
+          load4(src + hi, x[u] + 4);
+        } else {
+          load8(src + 8 * g, x[u]);
+        }
       }
-    }
-    if (p < 0) {
-      if (!rope_token(a, i, p, row)) return;
-      if (turned) {
-        load4(a.cos_tab + static_cast<size_t>(p) * half + 4 * g, c);
-        load4(a.sin_tab + static_cast<size_t>(p) * half + 4 * g, s);
+      if (p < 0) {
+        if (!rope_token(a, i, p, row)) break;
+        if (turned) {
+          load4(a.cos_tab + static_cast<size_t>(p) * half + 4 * g, c);
+          load4(a.sin_tab + static_cast<size_t>(p) * half + 4 * g, s);
+        }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const int h = hb + u * step;
-      if (h >= all || (row < 0 && h >= a.H)) continue;
-      const bool is_v = h >= a.H + a.KV;
-      const bool part = split && !is_v;
-      const float* bias = h < a.H ? a.bq : (is_v ? a.bv : a.bk);
-      const int hh = h < a.H ? h : (is_v ? h - a.H - a.KV : h - a.H);
-      const int la = part ? lo : 8 * g, ha = part ? hi : 8 * g + 4;
-      if (bias) {
-        float b[8];
-        load4(bias + hh * a.D + la, b);
-        load4(bias + hh * a.D + ha, b + 4);
+      for (int u = 0; u < kHeads; ++u) {
+        const int h = hb + u * step;
+        if (h >= all || (row < 0 && h >= a.H)) continue;
+        const bool is_v = h >= a.H + a.KV;
+        const bool part = split && !is_v;
+        const float* bias = h < a.H ? a.bq : (is_v ? a.bv : a.bk);
+        const int hh = h < a.H ? h : (is_v ? h - a.H - a.KV : h - a.H);
+        const int la = part ? lo : 8 * g, ha = part ? hi : 8 * g + 4;
+        if (bias) {
+          float b[8];
+          load4(bias + hh * a.D + la, b);
+          load4(bias + hh * a.D + ha, b + 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[u][e] = __fadd_rn(x[u][e], b[e]);
-      }
-      if (turned && !is_v) {
+          for (int e = 0; e < 8; ++e) x[u][e] = __fadd_rn(x[u][e], b[e]);
+        }
+        if (turned && !is_v) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x0 = a.neox ? x[u][e] : x[u][2 * e];
-          const float x1 = a.neox ? x[u][e + 4] : x[u][2 * e + 1];
-          const float y0 = __fsub_rn(__fmul_rn(x0, c[e]), __fmul_rn(x1, s[e]));
-          const float y1 = __fadd_rn(__fmul_rn(x0, s[e]), __fmul_rn(x1, c[e]));
-          if (a.neox) {
-            x[u][e] = y0;
-            x[u][e + 4] = y1;
-          } else {
-            x[u][2 * e] = y0;
-            x[u][2 * e + 1] = y1;
+          for (int e = 0; e < 4; ++e) {
+            const float x0 = a.neox ? x[u][e] : x[u][2 * e];
+            const float x1 = a.neox ? x[u][e + 4] : x[u][2 * e + 1];
+            const float y0 = __fsub_rn(__fmul_rn(x0, c[e]), __fmul_rn(x1, s[e]));
+            const float y1 = __fadd_rn(__fmul_rn(x0, s[e]), __fmul_rn(x1, c[e]));
+            if (a.neox) {
+              x[u][e] = y0;
+              x[u][e + 4] = y1;
+            } else {
+              x[u][2 * e] = y0;
+              x[u][2 * e + 1] = y1;
+            }
           }
         }
-      }
-      if (h < a.H) {
-        TQ* dst = static_cast<TQ*>(a.q_out) + (static_cast<size_t>(i) * a.H + h) * a.D;
-        if (part) {
-          store4(dst + lo, x[u]);
-          store4(dst + hi, x[u] + 4);
+        if (h < a.H) {
+          TQ* dst = static_cast<TQ*>(a.q_out) + (static_cast<size_t>(i) * a.H + h) * a.D;
+          if (part) {
+            store4(dst + lo, x[u]);
+            store4(dst + hi, x[u] + 4);
+          } else {
+            store8(dst + 8 * g, x[u]);
+          }
         } else {
-          store8(dst + 8 * g, x[u]);
-        }
-      } else {
-        TK* dst = static_cast<TK*>(is_v ? a.v_pool : a.k_pool) + row + hh * a.D;
-        if (part) {
-          store4(dst + lo, x[u]);
-          store4(dst + hi, x[u] + 4);
-        } else {
-          store8(dst + 8 * g, x[u]);
+          TK* dst = static_cast<TK*>(is_v ? a.v_pool : a.k_pool) + row + hh * a.D;
+          if (part) {
+            store4(dst + lo, x[u]);
+            store4(dst + hi, x[u] + 4);
+          } else {
+            store8(dst + 8 * g, x[u]);
+          }
         }
       }
     }
@@ -586,7 +589,9 @@ cudaError_t rope_paged_launch(const PG::RopeArgs& a, int n_tok, cudaStream_t st)
     int gy = (all + threads / groups - 1) / (threads / groups);
     const int enough = (4 * b2a_host::sm_count() + n_tok - 1) / n_tok;
     if (gy > enough) gy = enough;
-    return b2a_host::launch(PG::rope_paged_rows<TS, TK, TQ>, dim3(n_tok, gy), dim3(threads), 0, st, a);
+    const int resident = 8 * b2a_host::sm_count();
+    return b2a_host::launch(PG::rope_paged_rows<TS, TK, TQ>, dim3(n_tok < resident ? n_tok : resident, gy),
+                            dim3(threads), 0, st, a);
   }
   const int pairs = all * (a.D / 2);
   return b2a_host::launch(PG::rope_paged_pairs<TS, TK, TQ>,
@@ -676,7 +681,7 @@ int b2a_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
   const PG::RopeArgs a = {q, k, v, q_tok_stride, k_tok_stride, v_tok_stride, bq, bk, bv, cos_tab,
                           sin_tab, pos_dev, slot_dev, k_pool, v_pool, q_out, page_stride,
                           static_cast<long long>(n_pages) * page_rows, tab_rows,
-                          log2_of(page_rows), H, KV, D, n_rot, style == B2A_ROPE_NEOX ? 1 : 0};
+                          log2_of(page_rows), H, KV, D, n_rot, style == B2A_ROPE_NEOX ? 1 : 0, n_tok};
   const cudaError_t e = with_type(in_dtype, [&](auto* ts) {
     return with_type(kv_dtype, [&](auto* tk) {
       return with_type(q_out_dtype, [&](auto* tq) {

@@ -77,8 +77,10 @@ int b2a_selftest_wait_timeout(void* stream);
 
 /* Launch mode of the calling thread's later launches; returns the previous
  * flags.  B2A_LAUNCH_PDL launches b2a_rope_append, b2a_imrope_append,
- * b2a_decode (both kernels), b2a_lse_combine, b2a_gemm and b2a_gemm_qkv_rope as
- * programmatic dependents of the kernel before them on the stream: each
+ * b2a_decode (both kernels), b2a_lse_combine, b2a_gemm, b2a_gemm_qkv_rope and
+ * the paged-cache entries (which wait for that kernel before they read
+ * anything) as programmatic dependents of the kernel before them on the
+ * stream: each
  * starts while that kernel drains and waits for it (griddepcontrol.wait)
  * before reading what it wrote.  The decode's K/V rows below the newest
  * (row len - 1 of each sequence) are streamed before that wait, and every
