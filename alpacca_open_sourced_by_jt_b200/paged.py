@@ -19,7 +19,9 @@ MAX_NODES nodes.  Rows from cu[B] on are padding (captured steps).
 
 As in `device`, every function checks its arguments on the host, makes one
 C-ABI call and never synchronises; numbers that live on the device and are out
-of bounds are recorded (`_lib.device_error`).
+of bounds are recorded (`_lib.device_error`).  A call runs on the current stream,
+or on `stream` (a torch.cuda.Stream or a raw handle), which its new outputs then
+belong to.
 """
 from __future__ import annotations
 
@@ -91,12 +93,19 @@ def _pool(k: torch.Tensor, v: torch.Tensor, dims: int = 4):
     return shape, stride
 
 
-def _stream(stream, t: torch.Tensor):
-    """The caller's stream, or t's device's current one (its raw handle: a
-    torch.cuda.Stream object costs microseconds a call)."""
-    if stream is None:
-        return torch._C._cuda_getCurrentRawStream(t.device.index)
-    return device._stream(stream)
+def _stream(t: torch.Tensor):
+    """The current stream of t's device (its raw handle: a torch.cuda.Stream
+    object costs microseconds a call)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _on(stream):
+    """A call's `stream` as the current one: what the call allocates then belongs
+    to the stream that uses it, and a workspace given back at the call's end is
+    not handed to another stream while the kernel still runs."""
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(int(stream))
+    return torch.cuda.stream(stream)
 
 
 class PagePlan(NamedTuple):
@@ -123,6 +132,10 @@ def page_plan(lens: torch.Tensor, add: torch.Tensor, held: torch.Tensor, table: 
     pages in the ring.  parents (max_tokens,) gives tree nodes their depth's
     position, None a chain's.  A request the ring cannot serve keeps its pages
     and its tokens' slots are -1."""
+    if stream is not None:
+        with _on(stream):
+            return page_plan(lens, add, held, table, ring, ring_state, page_rows=page_rows,
+                             max_tokens=max_tokens, parents=parents, out=out)
     B = lens.numel()
     _i32("lens", lens)
     _i32("add", add, B)
@@ -148,7 +161,7 @@ def page_plan(lens: torch.Tensor, add: torch.Tensor, held: torch.Tensor, table: 
         lens.data_ptr(), add.data_ptr(), None if parents is None else parents.data_ptr(),
         held.data_ptr(), held_out.data_ptr(), tptr, tstride, ring.data_ptr(), ring.numel(),
         ring_state.data_ptr(), state_out.data_ptr(), cu.data_ptr(), seq.data_ptr(), pos.data_ptr(),
-        slots.data_ptr(), B, max_tokens, width, page_rows, _stream(stream, lens)))
+        slots.data_ptr(), B, max_tokens, width, page_rows, _stream(lens)))
     return out
 
 
@@ -163,6 +176,11 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     int32 as page_plan writes them: the rotary position and the pool row are
     apart, a negative slot stores nothing.  Returns q_out (n, H, D), in the
     pools' type unless given."""
+    if stream is not None:
+        with _on(stream):
+            return rope_append(q, k, v, positions, slots, cos_tab, sin_tab, k_pool=k_pool,
+                               v_pool=v_pool, n_rot=n_rot, style=style, q_out=q_out, bq=bq, bk=bk,
+                               bv=bv)
     (P, R, KV, D), pstride = _pool(k_pool, v_pool)
     dt, qs, ks, vs = q.dtype, q.stride(), k.stride(), v.stride()
     n, H, Dq = q.shape
@@ -189,7 +207,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
         _f32("bk", bk, KV * D), _f32("bv", bv, KV * D), cos, sin, rows, positions.data_ptr(),
         slots.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), P, R,
         pstride[0] if P > 1 else R * KV * D, _code(k_pool.dtype), q_out.data_ptr(),
-        _code(q_out.dtype), n, H, KV, D, n_rot, device._STYLE[style], _stream(stream, q)))
+        _code(q_out.dtype), n, H, KV, D, n_rot, device._STYLE[style], _stream(q)))
     return q_out
 
 
@@ -225,6 +243,11 @@ def tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, len
     max_len bounds lens + nodes (default: what the table or the block holds).
     Returns out (n, H, D) in q's type, padding rows zero; lse (n, H) f32
     receives the natural-log log-sum-exp if given."""
+    if stream is not None:
+        with _on(stream):
+            return tree_decode(q, k_pool, v_pool, lens, cu, parents, table=table,
+                               max_nodes=max_nodes, max_len=max_len, scale=scale, out=out, lse=lse,
+                               workspace=workspace)
     (P, R, KV, D), pstride = _pool(k_pool, v_pool)
     dt, qs = q.dtype, q.stride()
     n, H, Dq = q.shape
@@ -255,7 +278,7 @@ def tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, len
         pptr, out.data_ptr(), _f32("lse", lse, n * H),
         None if workspace is None else workspace.data_ptr(), ws_bytes, B, n,
         max_nodes, H, KV, D, code, 1.0 / math.sqrt(D) if scale is None else scale, max_len,
-        _stream(stream, q)))
+        _stream(q)))
     return out
 
 
@@ -277,6 +300,13 @@ def constrain_logits(logits: torch.Tensor, cu: torch.Tensor, parents: torch.Tens
     int32: bit v % 32 of word v / 32 allows token v.  Returns (out, picks): out
     defaults to a new f32 tensor (pass out=logits for in place); picks (n,)
     int32, -1 where nothing can be picked."""
+    if stream is not None:
+        with _on(stream):
+            return constrain_logits(
+                logits, cu, parents, tokens, max_nodes=max_nodes, hist=hist, hist_start=hist_start,
+                prompt_lens=prompt_lens, repetition=repetition, presence=presence,
+                frequency=frequency, bias_start=bias_start, bias_ids=bias_ids, bias=bias, mask=mask,
+                out=out, picks=picks, workspace=workspace)
     n, V = logits.shape
     ls = logits.stride()
     if not logits.is_cuda or ls[1] != 1:
@@ -323,7 +353,7 @@ def constrain_logits(logits: torch.Tensor, cu: torch.Tensor, parents: torch.Tens
         _i32_rows("prompt_lens", prompt_lens, B), _f32("repetition", repetition, B),
         _f32("presence", presence, B), _f32("frequency", frequency, B), bsptr, biptr,
         _f32("bias", bias, n_bias), n_bias, mptr, mstride, B, n, max_nodes, V,
-        workspace.data_ptr(), ws_bytes, _stream(stream, logits)))
+        workspace.data_ptr(), ws_bytes, _stream(logits)))
     return out, picks
 
 
@@ -347,8 +377,12 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     own.  Pools (L, n_pages, page_rows, KV, D) for all layers at once, or one
     layer's 4-D pool; table, lens, cu, parents as in tree_decode (table None:
     (L, B, n_ctx, KV, D) blocks)."""
+    if stream is not None:
+        with _on(stream):
+            return tree_commit(picks, tokens, parents, cu, lens, k_pool, v_pool, table=table,
+                               max_nodes=max_nodes, max_len=max_len, out=out)
     dims = k_pool.dim()
-    shape, stride = _pool(k_pool, v_pool, 5 if dims == 5 else 4)
+    shape, strides = _pool(k_pool, v_pool, 5 if dims == 5 else 4)
     P, R, KV, D = shape[-4:]
     L = shape[0] if dims == 5 else 1
     B, n = lens.numel(), tokens.numel()
@@ -370,8 +404,8 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     _lib.check(_lib.load().b2a_tree_commit(
         _i32_rows("picks", picks, n), _i32_rows("tokens", tokens, n),
         _i32_rows("parents", parents, n), cu.data_ptr(), lens.data_ptr(), tptr, tstride, width,
-        k_pool.data_ptr(), v_pool.data_ptr(), L, stride[0] if L > 1 else 0, P, R,
-        stride[-4] if P > 1 else R * KV * D, KV, D, _code(k_pool.dtype), B, n, max_nodes, max_len,
+        k_pool.data_ptr(), v_pool.data_ptr(), L, strides[0] if L > 1 else 0, P, R,
+        strides[-4] if P > 1 else R * KV * D, KV, D, _code(k_pool.dtype), B, n, max_nodes, max_len,
         path.data_ptr(), accepted.data_ptr(), nxt.data_ptr(), lens_out.data_ptr(),
-        _stream(stream, lens)))
+        _stream(lens)))
     return out

@@ -642,3 +642,24 @@ def test_other_stream(cuda_dev):
                                 max_nodes=5, max_len=2005)
     side.synchronize()
     assert torch.equal(out, want)
+
+
+def test_stream_argument_owns_what_the_call_allocates(cuda_dev):
+    """A call given a busy side stream: its output and workspace come from that
+    stream, so work queued on the current stream afterwards cannot be handed the
+    same memory while the kernels still wait."""
+    from alpacca_open_sourced_by_jt_b200 import paged
+    s = Setup(cuda_dev, "bf16", 64, 8, 2, [5000, 40], [5, 2], 16, seed=1)
+    want = s.run()
+    d = s.dev
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        out = paged.tree_decode(s.q, s.k, s.v, d["lens"], d["cu"], d["parents"], table=d["table"],
+                                max_nodes=5, max_len=5005, stream=stream)
+        junk = [torch.full((1 << 16,), 7.0, device=cuda_dev) for _ in range(64)]
+        side.synchronize()
+        assert torch.equal(out, want)
+        del junk
