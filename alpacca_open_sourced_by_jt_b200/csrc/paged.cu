@@ -157,10 +157,11 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
     return lo;
   };
   int par0 = 0;
-  if (p.parents) {
-    // the tile's parents, from the first node of the tree that it cuts
+  if (p.parents && t0 < total) {
+    // the tile's parents, from the first node of the tree that it cuts: at most
+    // kMaxNodes before the tile (a tile of padding has none)
     const int end = min(min(t0 + kPlanTokens, p.max_tokens), total);
-    if (t0 < total) par0 = max(s_cu[find(t0)], t0 - kMaxNodes);
+    par0 = max(s_cu[find(t0)], t0 - kMaxNodes);
     for (int i = tid; par0 + i < end; i += kPlanThreads) s_par[i] = p.parents[par0 + i];
     __syncthreads();
   }
