@@ -46,7 +46,8 @@ __device__ __forceinline__ void plan_request(const Plan& p, int b, int& n, int& 
   n = add < 0 ? 0 : min(add, p.max_tokens + 1);
   const long long want = (static_cast<long long>(len) + n + (1 << p.page_shift) - 1) >> p.page_shift;
   fits = add >= 0 && !bad && want <= p.max_pages;
-  need = fits ? max(0, static_cast<int>(want) - held) : 0;
+  // (no tokens, no pages: the lens of a request that ended may still be there)
+  need = fits && n > 0 ? max(0, static_cast<int>(want) - held) : 0;
   back = add < 0 && !bad ? held : 0;
   if (bad) set_dev_error(B2A_ERR_POSITION, b);
 }

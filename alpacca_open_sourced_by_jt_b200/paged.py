@@ -127,8 +127,9 @@ def page_plan(lens: torch.Tensor, add: torch.Tensor, held: torch.Tensor, table: 
     (b2a_page_plan).
 
     lens, add, held (B,) int32: cached rows, tokens to add (-1 ends the
-    request), pages held.  table (B, max_pages) and ring (pages of the pool)
-    are updated in place; ring_state (2,) int32 is (head, count) of the free
+    request, 0 leaves it as it is), pages held.  lens is not written: set an
+    ended request's to 0 before its place goes to a new one.  table (B,
+    max_pages) and ring (pages of the pool) are updated in place; ring_state (2,) int32 is (head, count) of the free
     pages in the ring.  parents (max_tokens,) gives tree nodes their depth's
     position, None a chain's.  A request the ring cannot serve keeps its pages
     and its tokens' slots are -1."""

@@ -515,7 +515,10 @@ int b2a_q8_dequant(const void* codes, long long ldq, const void* scales, long lo
 
 /* Block tables, slot map and positions of a step, from request lengths.
  *   lens, add, held  int32 [B]: cached rows, tokens to add (-1: the request
- *                    ends and gives its pages back), pages in its table
+ *                    ends and gives its pages back; 0: nothing, it takes no
+ *                    pages), pages in its table.  lens is read only: whoever
+ *                    gives the place of an ended request to a new one sets its
+ *                    lens to 0 first
  *   parents          int32 [max_tokens] trees of the added tokens, or NULL
  *   table            int32 [B][table_stride], in place: new pages are entered
  *                    behind the held ones

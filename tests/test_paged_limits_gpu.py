@@ -56,3 +56,19 @@ def test_page_plan_trees_with_whole_tiles_of_padding(cuda_dev, total, max_tokens
                state=p.ring_state)
     for key, x in got.items():
         assert np.array_equal(x.cpu().numpy(), np.asarray(want[key])), key
+
+
+def test_page_plan_ended_request_takes_no_pages(cuda_dev):
+    """After a request ends, its lens still stands (commit returns it unchanged):
+    steps that add nothing to it leave the ring alone."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, paged
+    lens, held = i32([100, 20], cuda_dev), i32([7, 2], cuda_dev)
+    table = i32([[0, 1, 2, 3, 4, 5, 6, -1], [7, 8, -1, -1, -1, -1, -1, -1]], cuda_dev)
+    ring, state = i32(range(12), cuda_dev), i32([9, 3], cuda_dev)
+    for add, want_held, want_state in (([-1, 1], [0, 2], [9, 10]), ([0, 1], [0, 2], [9, 10]),
+                                       ([0, 0], [0, 2], [9, 10]), ([0, 13], [0, 3], [10, 9])):
+        p = paged.page_plan(lens, i32(add, cuda_dev), held, table, ring, state, page_rows=16, max_tokens=16)
+        _lib.raise_device_error()
+        held, state = p.held, p.ring_state
+        assert held.tolist() == want_held and state.tolist() == want_state
+    assert p.slots[:13].tolist() == [table[1, r // 16].item() * 16 + r % 16 for r in range(20, 33)]
