@@ -153,15 +153,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
   }
 
   // ---------------- consumer warps ----------------------------------------
-  // rows past the last node (the padding of a captured step) become zeros
-  if (blockIdx.x == 0) {
-    const long long first = static_cast<long long>(max(bt.cu[bt.B], 0)) * bt.H;
-    for (long long r = first + threadIdx.x / 32; r < static_cast<long long>(bt.n_tok) * bt.H;
-         r += kConsumers) {
-      for (int d = lane; d < D; d += 32) st_elem(out + r * D + d, 0.f);
-      if (lse && lane == 0) lse[r] = -INFINITY;
-    }
-  }
+  zero_unwritten<T, D>(bt, s_start.left_out, out, lse, warp, kConsumers);
   const int g = lane >> 2, t4 = lane & 3;
   const int slice = warp & 3, half = warp >> 2;
   const uint32_t ring = smem_u32(smem);
@@ -482,13 +474,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
   }
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (blockIdx.x == 0) {
-    const long long first = static_cast<long long>(max(bt.cu[bt.B], 0)) * bt.H;
-    for (long long r = first + warp; r < static_cast<long long>(bt.n_tok) * bt.H; r += kWarps) {
-      for (int d = lane; d < D; d += 32) out[r * D + d] = 0.f;
-      if (lse && lane == 0) lse[r] = -INFINITY;
-    }
-  }
+  zero_unwritten<float, D>(bt, s_start.left_out, out, lse, warp, kWarps);
   Walker wk;
   wk.start(bt, s_start);
   Item it;

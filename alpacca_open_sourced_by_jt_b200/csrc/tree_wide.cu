@@ -320,15 +320,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
       return !dead;
     };
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(128 * kWideGroups) : "memory"); };
-    // rows past the last node (the padding of a captured step) become zeros
-    if (blockIdx.x == 0) {
-      const long long first = static_cast<long long>(max(bt.cu[bt.B], 0)) * bt.H;
-      for (long long i = first + warp - 4; i < static_cast<long long>(bt.n_tok) * bt.H;
-           i += 4 * kWideGroups) {
-        for (int d = lane; d < D; d += 32) st_elem(out + i * D + d, 0.f);
-        if (lse && lane == 0) lse[i] = -INFINITY;
-      }
-    }
+    zero_unwritten<T, D>(bt, sh.start.left_out, out, lse, warp - 4, 4 * kWideGroups);
     while (wk.next(bt, it)) {
       const int n = it.t1 - it.t0;
       const int rows = it.len + it.n;

@@ -56,9 +56,9 @@ struct Batch {
   int m_blks;          // blocks of query rows side by side
 };
 
-// Nodes and cache rows of request b; a request whose numbers are out of
-// bounds has none (recorded).
-__device__ __forceinline__ void request(const Batch& bt, int b, int& n, int& len) {
+// Nodes and cache rows of request b; false for a request that is left out: one
+// whose numbers are out of bounds (recorded) has no nodes and no rows.
+__device__ __forceinline__ bool request(const Batch& bt, int b, int& n, int& len) {
   const int c0 = bt.cu[b], c1 = bt.cu[b + 1];
   len = bt.lens[b];
   n = c1 - c0;
@@ -67,7 +67,9 @@ __device__ __forceinline__ void request(const Batch& bt, int b, int& n, int& len
     set_dev_error(B2A_ERR_POSITION, b);
     n = 0;
     len = 0;
+    return false;
   }
+  return true;
 }
 
 __device__ __forceinline__ int blocks_of(const Batch& bt, int n) {
@@ -87,20 +89,23 @@ struct Start {
   long long left;   // units of this team
   long long chunk;  // units per team
   int b;
+  bool left_out;  // some request is left out
 };
 
 // Warp-collective: the range of one team.
 __device__ __forceinline__ Start locate(const Batch& bt, int team) {
   const int lane = threadIdx.x & 31;
   long long total = 0;
+  bool out = false;
   for (int b = lane; b < bt.B; b += 32) {
     int n, len;
-    request(bt, b, n, len);
+    out |= !request(bt, b, n, len);
     total += units_of(bt, n, len);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   Start s;
+  s.left_out = __any_sync(0xffffffffu, out) != 0;
   s.chunk = (total + bt.teams - 1) / bt.teams;
   if (s.chunk < bt.min_units) s.chunk = bt.min_units;
   const long long first = s.chunk * team;
@@ -200,6 +205,40 @@ struct Walker {
     return false;
   }
 };
+
+// Rows [lo, hi) of out become zeros, their lse -inf, by thread i0 of step.
+template <typename T, int D>
+__device__ __forceinline__ void zero_rows(T* out, float* lse, long long lo, long long hi,
+                                          long long i0, long long step) {
+  constexpr int kGroups = D * sizeof(T) / 16;
+  for (long long i = lo * kGroups + i0; i < hi * kGroups; i += step)
+    reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (lse)
+    for (long long i = lo + i0; i < hi; i += step) lse[i] = -INFINITY;
+}
+
+// The rows that no item writes become zeros: those past the last node (the
+// padding of a captured step) and those of requests left out.  Called by warp
+// `warp` of `warps` of every CTA.
+template <typename T, int D>
+__device__ __forceinline__ void zero_unwritten(const Batch& bt, bool left_out, T* out, float* lse,
+                                               int warp, int warps) {
+  const int lane = threadIdx.x & 31;
+  const long long i0 = (static_cast<long long>(blockIdx.x) * warps + warp) * 32 + lane;
+  const long long step = static_cast<long long>(gridDim.x) * warps * 32;
+  zero_rows<T, D>(out, lse, static_cast<long long>(max(bt.cu[bt.B], 0)) * bt.H,
+                  static_cast<long long>(bt.n_tok) * bt.H, i0, step);
+  if (!left_out) return;
+  for (int b0 = 0; b0 < bt.B; b0 += 32) {
+    int n, len;
+    unsigned out_here = __ballot_sync(0xffffffffu, b0 + lane < bt.B && !request(bt, b0 + lane, n, len));
+    for (; out_here; out_here &= out_here - 1) {
+      const int b = b0 + __ffs(out_here) - 1;
+      zero_rows<T, D>(out, lse, static_cast<long long>(max(bt.cu[b], 0)) * bt.H,
+                      static_cast<long long>(min(bt.cu[b + 1], bt.n_tok)) * bt.H, i0, step);
+    }
+  }
+}
 
 // Ancestor masks of a request's nodes (bit j of node i's: i sees node j),
 // written by threads tid of nt to anc[node][kWords]; par holds the parents

@@ -242,8 +242,8 @@ def tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, len
     and parents (n,) the trees (None: chains).  Node i reads the cached rows,
     its ancestors' rows and its own, which stand at rows lens[b] + node.
     max_len bounds lens + nodes (default: what the table or the block holds).
-    Returns out (n, H, D) in q's type, padding rows zero; lse (n, H) f32
-    receives the natural-log log-sum-exp if given."""
+    Returns out (n, H, D) in q's type, padding rows and those of requests left
+    out zero; lse (n, H) f32 receives the natural-log log-sum-exp if given."""
     if stream is not None:
         with _on(stream):
             return tree_decode(q, k_pool, v_pool, lens, cu, parents, table=table,

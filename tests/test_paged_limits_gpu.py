@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from tests import paged_ref as ref
+from tests.paged_ref import TDT
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +73,63 @@ def test_page_plan_ended_request_takes_no_pages(cuda_dev):
         held, state = p.held, p.ring_state
         assert held.tolist() == want_held and state.tolist() == want_state
     assert p.slots[:13].tolist() == [table[1, r // 16].item() * 16 + r % 16 for r in range(20, 33)]
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+def attend(dev, dt, D, H, KV, lens, cu, parents, q, k, v, table, max_nodes, max_len, fill=float("nan")):
+    """tree_decode into buffers that hold NaN: (out, lse, device error code)."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, paged
+    out = torch.full((q.shape[0], H, D), fill, device=dev).to(TDT[dt])
+    lse = torch.full((q.shape[0], H), fill, device=dev)
+    paged.tree_decode(q, k, v, i32(lens, dev), i32(cu, dev), None if parents is None else i32(parents, dev),
+                      table=None if table is None else i32(table, dev), max_nodes=max_nodes,
+                      max_len=max_len, out=out, lse=lse)
+    return out, lse, _lib.device_error(clear=True)[0]
+
+
+@pytest.mark.parametrize("dt,D,H,KV,n", [("bf16", 64, 8, 2, 3), ("f16", 128, 16, 2, 20), ("bf16", 256, 16, 1, 9),
+                                         ("f32", 128, 8, 2, 5)])
+@pytest.mark.parametrize("max_len", [640, 6000])
+def test_attention_rows_of_requests_left_out_are_zero(cuda_dev, dt, D, H, KV, n, max_len):
+    """Too long, too many nodes, nodes past the arrays: recorded, their rows (and the
+    padding behind the last node) are zeros, never what the memory held."""
+    from alpacca_open_sourced_by_jt_b200 import _lib
+    rng = np.random.default_rng(D + n)
+    B, page = 40, 32
+    nodes = [n] * B
+    lens = rng.integers(0, max_len - n + 1, B).tolist()
+    table, pages = ref.deal_pages([a + n for a in lens], page, rng)
+    cu = (np.arange(B + 1) * n).tolist()
+    g = torch.Generator("cuda").manual_seed(n)
+    k = torch.randn((pages, page, KV, D), device=cuda_dev, generator=g).to(TDT[dt])
+    v = torch.randn((pages, page, KV, D), device=cuda_dev, generator=g).to(TDT[dt])
+    q = torch.randn((B * n + 7, H, D), device=cuda_dev, generator=g).to(TDT[dt])
+    table = np.concatenate([table, np.full((B, -(-max_len // page)), -1)], 1)
+    args = (q, k, v, table, n, max_len)
+    good, lse0, code = attend(cuda_dev, dt, D, H, KV, lens, cu, None, *args)
+    assert code == 0 and torch.isfinite(good).all()
+    assert (good[B * n:] == 0).all() and torch.isneginf(lse0[B * n:]).all()
+
+    bad_lens = list(lens)
+    for b in (0, 33, 38):  # one row too long, below zero, far too long
+        bad_lens[b] = {0: max_len - n + 1, 33: -1, 38: 2 ** 31 - 1}[b]
+    out, lse, code = attend(cuda_dev, dt, D, H, KV, bad_lens, cu, None, *args)
+    assert code == _lib.ERR_POSITION
+    for b in range(B):
+        rows = slice(cu[b], cu[b + 1])
+        if b in (0, 33, 38):
+            assert (out[rows] == 0).all() and torch.isneginf(lse[rows]).all(), b
+        else:
+            assert (out[rows].float() - good[rows].float()).abs().max() < 2e-2, b
+    # request 5 takes request 6's nodes too (one too many), the last ends past the arrays
+    odd = list(cu)
+    odd[6] += 1
+    odd[B] = B * n + 8
+    out, lse, code = attend(cuda_dev, dt, D, H, KV, lens, odd, None, *args)
+    assert code == _lib.ERR_POSITION
+    for rows in (slice(odd[5], odd[6]), slice(odd[B - 1], B * n + 7)):
+        assert (out[rows] == 0).all() and torch.isneginf(lse[rows]).all()
+    assert torch.isfinite(out).all()
