@@ -140,10 +140,13 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
       p.ring[(static_cast<long long>(head) + count + s_back[b] + j) % p.ring_size] =
           p.table[b * p.table_stride + j];
     const int lo = s_need[b], need = s_need[b + 1] - lo;
-    if (need == 0 || s_need[b + 1] > count) continue;
-    const int held = p.held[b];
+    // a request that is not served has -1 where its pages would be: the entries
+    // may hold pages of an earlier request that are others' by now
+    const bool served = s_need[b + 1] <= count;
+    const int held = need > 0 ? p.held[b] : 0;
     for (int k = lane; k < need; k += 32)
-      p.table[b * p.table_stride + held + k] = p.ring[(static_cast<long long>(head) + lo + k) % p.ring_size];
+      p.table[b * p.table_stride + held + k] =
+          served ? p.ring[(static_cast<long long>(head) + lo + k) % p.ring_size] : -1;
   }
   // tokens
   const int t0 = blockIdx.x * kPlanTokens;
@@ -458,7 +461,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_pairs(const __grid_co
 // Accepted path and row moves (b2a_tree_commit)
 // ---------------------------------------------------------------------------
 // From the root, the path goes on to the first child whose token is the
-// node's pick.  Warp 0 of every CTA walks it (each step is one ballot over
+// node's pick.  A request that the plan did not serve (its last row has no page)
+// has no path.  Warp 0 of every CTA walks it (each step is one ballot over
 // the request's nodes), then each thread moves one 16-byte column of the
 // path's rows, in path order: the row at depth d comes from node path[d] >= d,
 // so no row is overwritten before it was read.  Latency-bound: 16 layers, one
@@ -485,18 +489,21 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __gri
   const int c0 = c.cu[b], n = c.cu[b + 1] - c0, len = c.lens[b];
   const bool bad = n < 0 || n > c.max_nodes || c0 < 0 || c0 + n > c.n_tok || len < 0 ||
                    len > c.max_len - n;
+  const bool served = !bad && n > 0 &&
+                      (c.page_shift < 0 ||
+                       c.table[b * c.table_stride + ((len + n - 1) >> c.page_shift)] != -1);
   if (threadIdx.x < 32) {
     int par[kMaxNodes / 32], tok[kMaxNodes / 32], pick[kMaxNodes / 32];
 #pragma unroll
     for (int w = 0; w < kMaxNodes / 32; ++w) {
       const int j = w * 32 + lane;
-      const bool in = !bad && j < n;
+      const bool in = served && j < n;
       par[w] = in ? (c.parents ? c.parents[c0 + j] : j - 1) : -2;
       tok[w] = in ? c.tokens[c0 + j] : 0;
       pick[w] = in ? c.picks[c0 + j] : 0;
     }
     int len_path = 0, cur = 0, last = -1;
-    if (!bad && n > 0) {
+    if (served) {
       while (true) {
         if (lane == 0) s_path[len_path] = cur;
         ++len_path;

@@ -56,8 +56,9 @@ struct Batch {
   int m_blks;          // blocks of query rows side by side
 };
 
-// Nodes and cache rows of request b; false for a request that is left out: one
-// whose numbers are out of bounds (recorded) has no nodes and no rows.
+// Nodes and cache rows of request b; false for a request that is left out (no
+// nodes and no rows): its numbers are out of bounds (recorded), or its last row
+// has no page, -1 in the table, where the plan could not serve it (no error).
 __device__ __forceinline__ bool request(const Batch& bt, int b, int& n, int& len) {
   const int c0 = bt.cu[b], c1 = bt.cu[b + 1];
   len = bt.lens[b];
@@ -65,11 +66,13 @@ __device__ __forceinline__ bool request(const Batch& bt, int b, int& n, int& len
   if (n < 0 || n > bt.max_nodes || c0 < 0 || c1 > bt.n_tok || len < 0 ||
       len > bt.max_len - n) {
     set_dev_error(B2A_ERR_POSITION, b);
-    n = 0;
-    len = 0;
-    return false;
+  } else if (n == 0 || !bt.table ||
+             __ldg(bt.table + b * bt.table_stride + ((len + n - 1) >> bt.page_shift)) != -1) {
+    return true;
   }
-  return true;
+  n = 0;
+  len = 0;
+  return false;
 }
 
 __device__ __forceinline__ int blocks_of(const Batch& bt, int n) {

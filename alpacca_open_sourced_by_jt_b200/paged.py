@@ -131,8 +131,9 @@ def page_plan(lens: torch.Tensor, add: torch.Tensor, held: torch.Tensor, table: 
     ended request's to 0 before its place goes to a new one.  table (B,
     max_pages) and ring (pages of the pool) are updated in place; ring_state (2,) int32 is (head, count) of the free
     pages in the ring.  parents (max_tokens,) gives tree nodes their depth's
-    position, None a chain's.  A request the ring cannot serve keeps its pages
-    and its tokens' slots are -1."""
+    position, None a chain's.  A request the ring cannot serve keeps its pages;
+    its tokens' slots and the table entries of the pages it wanted are -1, and
+    tree_decode and tree_commit leave it out of the step."""
     if stream is not None:
         with _on(stream):
             return page_plan(lens, add, held, table, ring, ring_state, page_rows=page_rows,
@@ -377,7 +378,8 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     picks, tokens (n,) int32: the model's token after each node and the node's
     own.  Pools (L, n_pages, page_rows, KV, D) for all layers at once, or one
     layer's 4-D pool; table, lens, cu, parents as in tree_decode (table None:
-    (L, B, n_ctx, KV, D) blocks)."""
+    (L, B, n_ctx, KV, D) blocks).  A request left out (page_plan could not serve
+    it) has accepted 0, next_token -1, its lens as it was, and moves no rows."""
     if stream is not None:
         with _on(stream):
             return tree_commit(picks, tokens, parents, cu, lens, k_pool, v_pool, table=table,

@@ -509,7 +509,10 @@ int b2a_q8_dequant(const void* codes, long long ldq, const void* scales, long lo
  * steps); what each entry does with them is stated.
  *
  * A device-side number out of bounds (a length, a node count, a parent, a
- * page) records B2A_ERR_POSITION; the request, or the row, is left out. */
+ * page) records B2A_ERR_POSITION; the request, or the row, is left out.  A
+ * request whose last row (len + nodes - 1) has table entry -1 was not served
+ * by the plan: b2a_tree_decode and b2a_tree_commit leave it out, which is no
+ * error. */
 #define B2A_TREE_MAX_NODES 128
 #define B2A_PLAN_MAX_REQUESTS 2048
 
@@ -533,7 +536,9 @@ int b2a_q8_dequant(const void* codes, long long ldq, const void* scales, long lo
  *                    slot; padding rows get -1, 0, -1 (NULL if max_tokens is 0)
  * Pages go to the requests in order: request b is served if the pages wanted
  * up to and including its own are there (or it wants none) and its rows fit
- * max_pages; else it keeps what it holds and its tokens' slots are -1. */
+ * max_pages; else it keeps what it holds, its tokens' slots are -1 and so are
+ * the table entries of the pages it wanted, by which b2a_tree_decode and
+ * b2a_tree_commit leave it out of the step. */
 int b2a_page_plan(const int* lens_dev, const int* add_dev, const int* parents_dev,
                   const int* held_dev, int* held_out_dev, int* table_dev, long long table_stride,
                   int* ring_dev, int ring_size, const int* ring_state_dev,
@@ -627,8 +632,9 @@ int b2a_constrain_logits(const void* logits, long long row_stride, int in_dtype,
  *                  the element size): row lens[b] + path[d] of every layer is
  *                  copied to row lens[b] + d
  *   path       int32 [B][max_nodes], -1 behind the path
- *   accepted   int32 [B] nodes on the path (0 for a request without nodes)
- *   next       int32 [B] the pick of the path's last node (-1 without nodes)
+ *   accepted   int32 [B] nodes on the path (0 for a request without nodes or
+ *              left out: nothing of it moves)
+ *   next       int32 [B] the pick of the path's last node (-1 without a path)
  *   lens_out   int32 [B] lens + accepted (another buffer than lens)
  * max_len as in b2a_tree_decode. */
 int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* parents_dev,

@@ -133,3 +133,102 @@ def test_attention_rows_of_requests_left_out_are_zero(cuda_dev, dt, D, H, KV, n,
     for rows in (slice(odd[5], odd[6]), slice(odd[B - 1], B * n + 7)):
         assert (out[rows] == 0).all() and torch.isneginf(lse[rows]).all()
     assert torch.isfinite(out).all()
+
+
+# ---------------------------------------------------------------------------
+# steps of a serving loop
+# ---------------------------------------------------------------------------
+
+def serving_loop(dev, dt, others_only):
+    """Four requests over ten pages of 16 rows, four steps.  Request 3 ends in the
+    second step; in the third its place goes to a new one that finds one page of
+    two, while requests 1 and 2 have taken pages it gave back.  With others_only the
+    new request comes one step later.  Returns per step what each request has: K and V
+    rows, attention rows, plan, commit."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, device, paged
+    L, H, KV, D, page, n_pages, max_len = 2, 4, 2, 64, 16, 10, 128
+    k = torch.zeros((L, n_pages, page, KV, D), device=dev).to(TDT[dt])
+    v = torch.zeros_like(k)
+    table = torch.zeros((4, max_len // page), dtype=torch.int32, device=dev)
+    ring, state = i32([7, 2, 9, 4, 0, 1, 8, 3, 6, 5], dev), i32([0, n_pages], dev)
+    lens, held = i32([0, 0, 0, 0], dev), i32([0, 0, 0, 0], dev)
+    cos, sin = device.rope_tables(max_len, D, 10000.0, device=dev)
+    star = [-1] + [0] * 19
+    wide = [-1, 0, 0, 1, 2, 2, 4, 5]
+    chains = [[i - 1 for i in range(n)] for n in (30, 45, 10, 40)]
+    new = None if others_only else star
+    steps = [chains, [[-1, 0, 0]] * 3 + ["end"], [wide] * 3 + [new], [[-1, 0, 0]] * 3 + [star[:10]]]
+    seen = []
+    for at, trees in enumerate(steps):
+        if at == 2:
+            lens[3] = 0
+        add = [-1 if t == "end" else 0 if t is None else len(t) for t in trees]
+        nodes = [max(a, 0) for a in add]
+        flat = [p for t in trees if t is not None and t != "end" for p in t]
+        n = len(flat)
+        plan = paged.page_plan(lens, i32(add, dev), held, table, ring, state, page_rows=page,
+                               max_tokens=n, parents=i32(flat, dev))
+        # a request's rows are its own whatever else is in the step
+        rows = [torch.randn((m, H + 2 * KV, D), device=dev,
+                            generator=torch.Generator("cuda").manual_seed(100 * at + b))
+                for b, m in enumerate(nodes)]
+        qkv = torch.cat(rows)
+        att = []
+        for li in range(L):
+            q = paged.rope_append(qkv[:, :H], qkv[:, H:H + KV], qkv[:, H + KV:], plan.positions, plan.slots,
+                                  cos, sin, k_pool=k[li], v_pool=v[li])
+            att.append(paged.tree_decode(q, k[li], v[li], lens, plan.cu, i32(flat, dev), table=table,
+                                         max_nodes=max(nodes), max_len=max_len))
+        # the path goes to a node's last child (chains: on to the end)
+        tokens, picks = [], []
+        for t in trees:
+            if t is None or t == "end":
+                continue
+            tokens += list(range(len(t)))
+            kids = [[j for j in range(len(t)) if t[j] == i] for i in range(len(t))]
+            picks += [c[-1] if c else 999 for c in kids]
+        c = paged.tree_commit(i32(picks, dev), i32(tokens, dev), i32(flat, dev), plan.cu, lens, k, v,
+                              table=table, max_nodes=max(nodes), max_len=max_len)
+        _lib.raise_device_error()
+        lens, held, state = c.lens, plan.held, plan.ring_state
+        cu = plan.cu.tolist()
+        cache = []
+        for b in range(4):
+            r = torch.arange(lens[b].item() if held[b] > 0 else 0, device=dev)
+            where = (slice(None), table[b].long()[r // page], r % page)
+            cache.append((k[where].clone(), v[where].clone()))
+        seen.append(dict(cache=cache, att=[[a[cu[b]:cu[b + 1]] for a in att] for b in range(4)],
+                         slots=[plan.slots[cu[b]:cu[b + 1]].tolist() for b in range(4)],
+                         accepted=c.accepted.tolist(), next=c.next_token.tolist(), path=c.path.tolist(),
+                         lens=lens.tolist(), held=held.tolist(), state=state.tolist(), table=table.tolist()))
+    return seen
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_request_without_pages_is_left_out_of_the_step(cuda_dev, dt):
+    """Plan, append, attention and commit, step by step: the request that finds no
+    pages changes nothing of the others' rows, and nothing of its own is counted."""
+    full, others = serving_loop(cuda_dev, dt, False), serving_loop(cuda_dev, dt, True)
+    assert full[0]["lens"] == [30, 45, 10, 40] and full[1]["held"] == [3, 3, 1, 0]
+    step = full[2]
+    assert step["held"] == [3, 4, 2, 0] and step["state"][1] == 1  # two wanted, one there
+    assert step["slots"][3] == [-1] * 20 and step["accepted"][:3] == [4, 4, 4]
+    for b in range(3):
+        for x, y in zip(step["cache"][b], others[2]["cache"][b]):
+            assert torch.equal(x, y), b
+    assert step["accepted"][3] == 0 and step["next"][3] == -1 and step["lens"][3] == 0
+    assert set(step["path"][3]) == {-1} and step["table"][3][:2] == [-1, -1]
+    for a in step["att"][3]:
+        assert a.shape[0] == 20 and (a == 0).all()
+    for at in range(4):
+        for key in ("accepted", "next", "lens", "held", "state"):
+            assert full[at][key] == others[at][key], (at, key)
+        for b in range(3):
+            for x, y in zip(full[at]["cache"][b], others[at]["cache"][b]):
+                assert torch.equal(x, y), (at, b)
+            for x, y in zip(full[at]["att"][b], others[at]["att"][b]):
+                assert (x.float() - y.float()).abs().max() < 2e-2, (at, b)
+    # one step later there is a page for ten nodes
+    assert full[3]["held"][3] == 1 and full[3]["accepted"][3] == 2 and full[3]["lens"][3] == 2
+    for x, y in zip(full[3]["cache"][3], others[3]["cache"][3]):
+        assert torch.equal(x, y)
