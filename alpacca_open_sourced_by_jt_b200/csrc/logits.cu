@@ -60,6 +60,15 @@ struct Args {
   int n_hist, n_bias, B, n_rows, max_nodes, V, slices, rows_per_cta;
 };
 
+// The rows of request b; false for one that is left out (recorded by the first
+// kernel): both kernels ask here, since the second reads what the first wrote.
+__device__ __forceinline__ bool request_rows(const Args& a, int b, int& c0, int& n) {
+  c0 = a.cu[b];
+  const int c1 = a.cu[b + 1];
+  n = c1 - c0;
+  return c0 >= 0 && c1 >= c0 && c1 <= a.n_rows && n <= a.max_nodes;
+}
+
 // A value's place in the order of floats, 0 for what cannot be picked (-inf).
 __device__ __forceinline__ uint32_t order_of(float x) {
   if (!(x > -INFINITY)) return 0u;
@@ -113,9 +122,8 @@ __global__ void __launch_bounds__(kThreads, 3) logits_kernel(const __grid_consta
   // slices in the grid's slowest dimension: the first slices, where frequent
   // tokens are and lists are long, start first
   const int b = blockIdx.x, slice = blockIdx.z;
-  const int c0 = a.cu[b];
-  const int n = a.cu[b + 1] - c0;
-  if (n < 0 || n > a.max_nodes || c0 < 0 || c0 + n > a.n_rows) {
+  int c0, n;
+  if (!request_rows(a, b, c0, n)) {
     if (tid == 0) set_dev_error(B2A_ERR_POSITION, b);
     return;
   }
@@ -335,12 +343,13 @@ __global__ void __launch_bounds__(kThreads) logits_pick_kernel(const __grid_cons
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (row >= a.n_rows) return;
-  // rows of no request (padding), or of one with too many nodes, have no pick
-  int before = 0;
-  for (int b = lane; b < a.B; b += 32) before += a.cu[b + 1] <= row ? 1 : 0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  const bool good = before < a.B && a.cu[before] <= row && a.cu[before + 1] - a.cu[before] <= a.max_nodes;
+  // rows of no request (padding), or of one that is left out, have no pick
+  bool mine = false;
+  for (int b = lane; b < a.B; b += 32) {
+    int c0, n;
+    mine |= request_rows(a, b, c0, n) && row >= c0 && row < c0 + n;
+  }
+  const bool good = __any_sync(0xffffffffu, mine) != 0;
   unsigned long long best = 0ull;
   const int k = a.slices * kWarps;
   if (good)

@@ -609,8 +609,8 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
  *                bias_start[b + 1]; the last entry of an id counts.  bias
  *                NULL: none; n_bias the arrays' size
  *   mask         bit v % 32 of word v / 32 of the row, or NULL
- * Tokens outside [0, V) in the lists are ignored.  Padding rows: pick -1, out
- * untouched. */
+ * Tokens outside [0, V) in the lists are ignored.  Padding rows and the rows
+ * of a request left out: pick -1, out untouched. */
 size_t b2a_constrain_logits_workspace_bytes(int n_rows, int V);
 int b2a_constrain_logits(const void* logits, long long row_stride, int in_dtype, void* out,
                          long long out_row_stride, int out_dtype, int* picks_dev,

@@ -136,6 +136,30 @@ def test_attention_rows_of_requests_left_out_are_zero(cuda_dev, dt, D, H, KV, n,
 
 
 # ---------------------------------------------------------------------------
+# logits
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cu,left_out", [([0, 3, 5, 9], [2]), ([0, 6, 7, 8], [0]), ([-1, 2, 4, 8], [0]),
+                                         ([0, 2, 40, 41], [1, 2]), ([0, 9, 1, 2], [0, 1])])
+def test_logits_rows_of_requests_left_out_have_no_pick(cuda_dev, cu, left_out):
+    """Nodes past the arrays, too many of them, starts out of order: recorded, and no
+    pick comes from memory that nothing of this call wrote."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, paged
+    n, V = 8, 9000
+    x = torch.randn((n, V), device=cuda_dev, generator=torch.Generator("cuda").manual_seed(len(left_out)))
+    for byte in (0xff, 0x7f):
+        ws = torch.full((paged._logits_bytes(n, V),), byte, dtype=torch.uint8, device=cuda_dev)
+        _, picks = paged.constrain_logits(x, i32(cu, cuda_dev), None, None, max_nodes=5, workspace=ws)
+        assert _lib.device_error(clear=True)[0] == _lib.ERR_POSITION
+        want = [-1] * n
+        for b in range(3):
+            if b not in left_out:
+                for r in range(cu[b], cu[b + 1]):
+                    want[r] = int(x[r].argmax())
+        assert picks.tolist() == want
+
+
+# ---------------------------------------------------------------------------
 # steps of a serving loop
 # ---------------------------------------------------------------------------
 
