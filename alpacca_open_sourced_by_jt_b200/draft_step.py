@@ -34,7 +34,8 @@ from .prefill_chain import ChunkPrefill, _dequant
 
 class DraftStep:
     """`requests` slots over a pool of n_pages pages of page_rows rows per
-    layer (f16 or bf16), at most max_len rows a request."""
+    layer (f16 or bf16), at most max_len rows a request (prompts and trees that
+    pass it are refused)."""
 
     def __init__(self, model: LlamaQ8, requests: int, n_pages: int, *, page_rows: int = 64,
                  max_len: int = 4096, dtype: torch.dtype = torch.float16):
@@ -53,10 +54,24 @@ class DraftStep:
         self.ring_state = torch.tensor([0, n_pages], **i32)
         self.lens = torch.zeros(requests, **i32)
         self.held = torch.zeros(requests, **i32)
+        self._rows = [0] * requests  # lens, as the host knows them
         self.cos, self.sin = device.rope_tables(max_len, m.D, m.rope_base, device=dev)
         self.w = [dict(qkv=_dequant(ly["wqkv"], dtype), wo=_dequant(ly["wo"], dtype),
                        gu=ChunkPrefill._gate_up(_dequant(ly["wgu"], dtype), m.F),
                        down=_dequant(ly["w_down"], dtype)) for ly in m.layers]
+
+    def _check(self, sequences):
+        """Refuse what the kernels would leave out: a count of requests that is not
+        this step's, tokens outside the vocabulary, rows past max_len."""
+        if len(sequences) != self.B:
+            raise _lib.B2AShapeError(_lib.ERR_SHAPE, f"{len(sequences)} requests for {self.B}")
+        for b, ids in enumerate(sequences):
+            if self._rows[b] + len(ids) > self.max_len:
+                raise _lib.B2AShapeError(
+                    _lib.ERR_SHAPE, f"request {b}: {self._rows[b]} cached rows and {len(ids)} tokens "
+                    f"exceed max_len {self.max_len}")
+            if not all(0 <= t < self.m.V for t in ids):
+                raise _lib.B2AShapeError(_lib.ERR_ARG, f"request {b}: a token outside [0, {self.m.V})")
 
     def _norm(self, x, w):
         h = torch.empty(x.shape, dtype=self.dt, device=x.device)
@@ -97,7 +112,9 @@ class DraftStep:
     def prefill(self, prompts):
         """Append prompts (a list of ids per request, empty: none) to the
         requests; returns each request's pick after its last token (-1: no
-        prompt) as a list."""
+        prompt) as a list.  Where pages run out between chunks, the chunks before
+        are in the cache (`lens` says how far each request came)."""
+        self._check(prompts)
         last = [-1] * self.B
         done = [0] * self.B
         while any(done[b] < len(p) for b, p in enumerate(prompts)):
@@ -107,6 +124,7 @@ class DraftStep:
             logits, plan = self._forward(add, tokens, None)
             _, picks = paged.constrain_logits(logits, plan.cu, None, None, max_nodes=max(add), out=logits)
             self.lens = self.lens + torch.tensor(add, dtype=torch.int32, device=self.m.device)
+            self._rows = [r + a for r, a in zip(self._rows, add)]
             picks, at = picks.tolist(), 0
             for b, c in enumerate(chunk):
                 at += len(c)
@@ -121,6 +139,15 @@ class DraftStep:
         history, penalty, bias and mask arguments of paged.constrain_logits.
         Returns per request the tokens that are new: the accepted drafts and the
         model's own next token (None without a tree)."""
+        self._check([() if t is None else t[0] for t in trees])
+        for b, t in enumerate(trees):
+            if t is None:
+                continue
+            if not 0 < len(t[0]) <= paged.MAX_NODES or len(t[1]) != len(t[0]):
+                raise _lib.B2AShapeError(
+                    _lib.ERR_SHAPE, f"request {b}: a tree needs 1 to {paged.MAX_NODES} tokens, each with a parent")
+            if not all(-1 <= p < i for i, p in enumerate(t[1])):
+                raise _lib.B2AShapeError(_lib.ERR_ARG, f"request {b}: a parent that is not an earlier node")
         add = [0 if t is None else len(t[0]) for t in trees]
         flat = [x for t in trees if t is not None for x in t[0]]
         par = [x for t in trees if t is not None for x in t[1]]
@@ -134,6 +161,7 @@ class DraftStep:
                               self.v_pool, table=self.table, max_nodes=max(add), max_len=self.max_len)
         self.lens = c.lens
         path, accepted, nxt = c.path.tolist(), c.accepted.tolist(), c.next_token.tolist()
+        self._rows = [r + a for r, a in zip(self._rows, accepted)]
         return [None if t is None else [t[0][i] for i in path[b][1:accepted[b]]] + [nxt[b]]
                 for b, t in enumerate(trees)]
 
@@ -147,3 +175,4 @@ class DraftStep:
         self.held, self.ring_state = plan.held, plan.ring_state
         gone = torch.tensor([b in requests for b in range(self.B)], device=dev)
         self.lens = torch.where(gone, 0, self.lens).int()
+        self._rows = [0 if b in requests else r for b, r in enumerate(self._rows)]
