@@ -714,7 +714,7 @@ int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* pare
                     long long page_stride, int KV, int D, int dtype, int B, int n_tok,
                     int max_nodes, int max_len, int* path_dev, int* accepted_dev, int* next_dev,
                     int* lens_out_dev, void* stream) {
-  if (!picks_dev || !tokens_dev || !cu_dev || !lens_dev || !k_cache || !v_cache || !path_dev ||
+  if ((n_tok > 0 && (!picks_dev || !tokens_dev)) || !cu_dev || !lens_dev || !k_cache || !v_cache || !path_dev ||
       !accepted_dev || !next_dev || !lens_out_dev)
     return fail(B2A_ERR_ARG, "tree_commit: null pointer argument");
   if (n_layers <= 0 || n_pages <= 0 || page_rows <= 0 || KV <= 0 || D <= 0 || B <= 0 || n_tok < 0 || max_len <= 0)

@@ -148,6 +148,8 @@ class DraftStep:
                     _lib.ERR_SHAPE, f"request {b}: a tree needs 1 to {paged.MAX_NODES} tokens, each with a parent")
             if not all(-1 <= p < i for i, p in enumerate(t[1])):
                 raise _lib.B2AShapeError(_lib.ERR_ARG, f"request {b}: a parent that is not an earlier node")
+        if all(t is None for t in trees):
+            return [None] * self.B
         add = [0 if t is None else len(t[0]) for t in trees]
         flat = [x for t in trees if t is not None for x in t[0]]
         par = [x for t in trees if t is not None for x in t[1]]

@@ -203,6 +203,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
         q_out = k_pool.new_empty((n, H, D))
     elif not q_out.is_cuda or not q_out.is_contiguous() or q_out.numel() != n * H * D:
         _bad("q_out must be a contiguous CUDA tensor (n, H, D)")
+    if n == 0:  # (an empty tensor has no address)
+        return q_out
     _lib.check(_lib.load().b2a_rope_append_paged(
         q.data_ptr(), qs[0] if n > 1 else H * D, k.data_ptr(), ks[0] if n > 1 else KV * D,
         v.data_ptr(), vs[0] if n > 1 else KV * D, _code(dt), _f32("bq", bq, H * D),
@@ -266,6 +268,8 @@ def tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, len
         out = q.new_empty((n, H, D))
     elif not out.is_cuda or not out.is_contiguous() or out.shape != (n, H, D) or out.dtype is not dt:
         _bad("out must be a contiguous CUDA tensor (n, H, D) in q's type")
+    if n == 0:
+        return out
     lib = _lib.load()
     code = _code(dt)
     if workspace is None:
@@ -348,6 +352,8 @@ def constrain_logits(logits: torch.Tensor, cu: torch.Tensor, parents: torch.Tens
         picks = torch.empty(n, dtype=torch.int32, device=logits.device)
     else:
         _i32("picks", picks, n)
+    if n == 0:
+        return out, picks
     _lib.check(lib.b2a_constrain_logits(
         logits.data_ptr(), ls[0] if n > 1 else V, _code(logits.dtype), out.data_ptr(),
         os[0] if n > 1 else V, _code(out.dtype), picks.data_ptr(), cu.data_ptr(),

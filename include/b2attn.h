@@ -627,7 +627,7 @@ int b2a_constrain_logits(const void* logits, long long row_stride, int in_dtype,
  * path begins at node 0 and goes from a node to its first child whose token
  * is the node's pick.
  *   picks, tokens  int32 [n_tok]: the model's token after each node, the
- *                  node's own token
+ *                  node's own token (NULL if n_tok is 0)
  *   k_cache, v_cache  n_layers caches layer_stride elements apart (dtype for
  *                  the element size): row lens[b] + path[d] of every layer is
  *                  copied to row lens[b] + d

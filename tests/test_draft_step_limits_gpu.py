@@ -62,3 +62,13 @@ def test_tokens_parents_and_counts_are_refused(cuda_dev):
     assert s.ring_state.tolist() == free and s.lens.tolist() == [2, 1]
     assert len(s.verify([([1] * 128, [-1] + [0] * 127), ([4], [-1])])) == 2
     _lib.raise_device_error()
+
+
+def test_step_of_no_trees(cuda_dev):
+    from alpacca_open_sourced_by_jt_b200 import _lib
+    s = make(cuda_dev, requests=2, n_pages=8, page_rows=16, max_len=64)
+    assert s.verify([None, None]) == [None, None] and s.prefill([[], []]) == [-1, -1]
+    first = s.prefill([[5, 6], []])
+    assert s.verify([None, None]) == [None, None] and s.lens.tolist() == [2, 0]
+    assert len(s.verify([([first[0]], [-1]), None])[0]) == 1
+    _lib.raise_device_error()

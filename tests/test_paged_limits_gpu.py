@@ -256,3 +256,36 @@ def test_request_without_pages_is_left_out_of_the_step(cuda_dev, dt):
     assert full[3]["held"][3] == 1 and full[3]["accepted"][3] == 2 and full[3]["lens"][3] == 2
     for x, y in zip(full[3]["cache"][3], others[3]["cache"][3]):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("paged_cache", [True, False])
+def test_step_without_nodes(cuda_dev, paged_cache):
+    """All requests idle: every entry takes tensors of no rows."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, device, paged
+    B, H, KV, D, page = 3, 8, 2, 64, 32
+    none = i32([], cuda_dev)
+    lens, held = i32([20, 0, 32], cuda_dev), i32([1, 0, 1], cuda_dev)
+    table = i32([[4, -1], [-1, -1], [0, -1]], cuda_dev)
+    ring, state = i32(range(5), cuda_dev), i32([1, 3], cuda_dev)
+    k = torch.randn((5, page, KV, D), device=cuda_dev)
+    v = torch.randn_like(k)
+    k0, v0 = k.clone(), v.clone()
+    cos, sin = device.rope_tables(64, D, 10000.0, device=cuda_dev)
+    plan = paged.page_plan(lens, i32([0, 0, 0], cuda_dev), held, table, ring, state, page_rows=page,
+                           max_tokens=0, parents=none)
+    assert plan.cu.tolist() == [0] * (B + 1) and plan.held.tolist() == [1, 0, 1]
+    assert plan.ring_state.tolist() == [1, 3] and plan.slots.numel() == 0
+    rows = torch.empty((0, H + 2 * KV, D), device=cuda_dev)
+    q = paged.rope_append(rows[:, :H], rows[:, H:H + KV], rows[:, H + KV:], plan.positions, plan.slots, cos,
+                          sin, k_pool=k, v_pool=v)
+    t = table if paged_cache else None
+    att = paged.tree_decode(q, k, v, lens, plan.cu, none, table=t, max_nodes=1,
+                            lse=torch.empty((0, H), device=cuda_dev))
+    assert q.shape == att.shape == (0, H, D)
+    out, picks = paged.constrain_logits(torch.empty((0, 500), device=cuda_dev), plan.cu, none, none, max_nodes=1)
+    assert out.shape == (0, 500) and picks.shape == (0,)
+    c = paged.tree_commit(picks, none, none, plan.cu, lens, k, v, table=t, max_nodes=1)
+    assert c.accepted.tolist() == [0] * B and c.next_token.tolist() == [-1] * B
+    assert c.lens.tolist() == [20, 0, 32] and (c.path == -1).all()
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+    _lib.raise_device_error()
