@@ -70,8 +70,8 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
     const __grid_constant__ Batch bt, const T* __restrict__ q, long long q_stride,
-    T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o,
-    float* __restrict__ part_ml, int piece_rows, float sscale) {
+    const T* __restrict__ vc, long long page_stride, T* __restrict__ out, float* __restrict__ lse,
+    float* __restrict__ part_o, float* __restrict__ part_ml, int piece_rows, float sscale) {
   using C = MmaCfg<D, NT>;
   constexpr int KS = D / 16;
   constexpr int RB = 8 * NT;
@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
   __shared__ __align__(8) uint64_t full_bar[C::kStages];
   __shared__ __align__(8) uint64_t empty_bar[C::kStages];
   __shared__ Start s_start;
+  __shared__ int s_special;  // the item's tree rows held infinities or NaN
   __shared__ int s_par[kMaxNodes];
   __shared__ uint32_t s_anc[kMaxNodes][kWords];
 
@@ -95,6 +96,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
       mbar_init(&empty_bar[s], kConsumers / 2);
     }
     fence_mbar_init();
+    s_special = 0;
   }
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -223,20 +225,28 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
       const uint32_t kt = ring + s * C::kStageBytes + slice_at;
       const uint32_t vt = kt + C::kTileBytes;
 
-      // Rows past the request's last hold anything (a pool's old rows, or
-      // what the stage held before): their weight is 0, but 0 * NaN is not,
-      // so their V rows are cleared.
       const int slice0 = t * kRows + slice * 16;
-      const bool partial = slice0 + 16 > rows;
-      if (partial) {
-        const int first_bad = max(rows - slice0, 0);
+      const bool tail = slice0 + 16 > it.len;  // tree rows, or rows past the last
+      if (tail) {
+        // Rows past the request's last hold anything (a pool's old rows, or
+        // what the stage held before): their weight is 0, but 0 * NaN is not,
+        // so their V rows are cleared, and infinities and NaN of tree rows too.
+        const int first = max(it.len - slice0, 0), past = min(max(rows - slice0, 0), 16);
         uint8_t* vslice = smem + s * C::kStageBytes + C::kTileBytes + slice_at;
-        for (int idx = lane; idx < (16 - first_bad) * C::kBoxes * 8; idx += 32) {
-          const int row = first_bad + idx / (C::kBoxes * 8);
-          const int rem = idx % (C::kBoxes * 8);
-          *reinterpret_cast<uint4*>(vslice + (rem >> 3) * box_bytes + sw128_off(row, rem & 7)) =
-              make_uint4(0u, 0u, 0u, 0u);
-        }
+        auto chunk = [&](int from, int i) {  // 16 bytes i of the rows from `from` on
+          const int row = from + i / (C::kBoxes * 8), rem = i % (C::kBoxes * 8);
+          return reinterpret_cast<uint4*>(vslice + (rem >> 3) * box_bytes + sw128_off(row, rem & 7));
+        };
+        for (int i = lane; i < (16 - past) * C::kBoxes * 8; i += 32)
+          *chunk(past, i) = make_uint4(0u, 0u, 0u, 0u);
+        if (it.n > 1)
+          for (int i = lane; i < (past - first) * C::kBoxes * 8; i += 32) {
+            uint4 u = *chunk(first, i);
+            if (clear_special<T>(u)) {
+              *chunk(first, i) = u;
+              s_special = 1;
+            }
+          }
         __syncwarp();
       }
 
@@ -251,7 +261,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(sc[nt], a, qf[nt][ks]);
       }
-      if (slice0 + 16 > it.len) {
+      if (tail) {
         // tree rows: visible to a query row whose node has them as ancestor
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -307,7 +317,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
         for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(o[mt][nt], a, pb[nt]);
       }
       // the generic-proxy zeros come before the next TMA write of the stage
-      if (partial) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (tail) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[s]);
     }
@@ -394,13 +404,25 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
         }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32));
+    const bool special = s_special != 0;
+    if (special) {
+      asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32));
+      if (threadIdx.x == 0) s_special = 0;
+    }
     const int live = min(RB, R - it.blk * RB);
+    // adds what was taken out of the V rows to n elements of row r from column d on
+    auto put_back = [&](int r, int d, int n, auto* dst) {
+      const uint32_t* a = s_anc[(it.blk * RB + r) / bt.group];
+      add_special(bt, vc, page_stride, it.b, it.kvh, it.len, max(it.t0 * kRows - it.len, 0),
+                  min(it.t1 * kRows - it.len, it.n), make_uint4(a[0], a[1], a[2], a[3]), dst, D, d, n);
+    };
     if (slot >= 0) {
       float* po = part_o + static_cast<size_t>(slot) * RB * D;
       for (int i = threadIdx.x; i < live * (D / 4); i += kConsumers * 32) {
         const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
         *reinterpret_cast<float4*>(po + r * D + d) =
             *reinterpret_cast<const float4*>(fin + r * kPad + d);
+        if (special) put_back(r, d, 4, po + r * D + d);
       }
       if (threadIdx.x < 2 * live) part_ml[static_cast<size_t>(slot) * RB * 2 + threadIdx.x] = fml[threadIdx.x];
     } else {
@@ -415,6 +437,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
         u.z = MmaOp<T>::pack(x[4], x[5]);
         u.w = MmaOp<T>::pack(x[6], x[7]);
         *reinterpret_cast<uint4*>(out + row * D + d) = u;
+        if (special) put_back(r, d, 8, out + row * D + d);
         if (lse && d == 0)
           lse[row] = fml[r * 2 + 1] > 0.f ? (fml[r * 2] + log2f(fml[r * 2 + 1])) * kLn2 : -INFINITY;
       }
@@ -462,6 +485,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
   __shared__ int s_par[kMaxNodes];
   __shared__ uint32_t s_anc[kMaxNodes][kWords];
   __shared__ float s_m[kF32Rows], s_l[kF32Rows], s_alpha[kF32Rows];
+  __shared__ int s_special;  // the item's tree rows held infinities or NaN
   pdl_wait();
   float* ks = fsm;
   float* vs = ks + C::kK;
@@ -527,6 +551,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
       s_m[tid] = -INFINITY;
       s_l[tid] = 0.f;
     }
+    if (tid == 0) s_special = 0;
     __syncthreads();
     ancestor_masks(s_par, bt.parents == nullptr, it.n, s_anc, tid, kF32Threads, it.b);
 
@@ -611,6 +636,18 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
       }
       asm volatile("cp.async.wait_group 1;" ::: "memory");  // V(t)
       __syncthreads();
+      if (it.n > 1 && (t + 1) * TILE > it.len) {
+        const int first = max(it.len - t * TILE, 0), past = min(rows - t * TILE, TILE);
+        for (int i = tid; i < (past - first) * (D / 4); i += kF32Threads) {
+          uint4* at = reinterpret_cast<uint4*>(vs + first * D) + i;
+          uint4 u = *at;
+          if (clear_special<float>(u)) {
+            *at = u;
+            s_special = 1;
+          }
+        }
+        __syncthreads();
+      }
 #pragma unroll
       for (int r = 0; r < kORows; ++r) {
         const float al = s_alpha[or0 + r];
@@ -643,6 +680,13 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     const int live = min(kF32Rows, R - it.blk * kF32Rows);
     const int slot = part_slot(it, blockIdx.x);
+    const bool special = s_special != 0;
+    // adds what was taken out of the V rows to column d of row rr
+    auto put_back = [&](int rr, int d, float* dst) {
+      const uint32_t* a = s_anc[(it.blk * kF32Rows + rr) / bt.group];
+      add_special(bt, vc, page_stride, it.b, it.kvh, it.len, max(it.t0 * TILE - it.len, 0),
+                  min(it.t1 * TILE - it.len, it.n), make_uint4(a[0], a[1], a[2], a[3]), dst, D, d, 1);
+    };
 #pragma unroll
     for (int r = 0; r < kORows; ++r) {
       const int rr = or0 + r;
@@ -651,7 +695,10 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
       if (slot >= 0) {
         float* po = part_o + (static_cast<size_t>(slot) * kF32Rows + rr) * D;
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) po[oc + c * kF32Threads] = o[r][c];
+        for (int c = 0; c < kCols; ++c) {
+          po[oc + c * kF32Threads] = o[r][c];
+          if (special) put_back(rr, oc + c * kF32Threads, po + oc + c * kF32Threads);
+        }
         if (oc == 0) {
           part_ml[(static_cast<size_t>(slot) * kF32Rows + rr) * 2] = s_m[rr];
           part_ml[(static_cast<size_t>(slot) * kF32Rows + rr) * 2 + 1] = l;
@@ -661,7 +708,10 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(
         const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + it.kvh * bt.group + (gr - node * bt.group);
         const float f = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) out[row * D + oc + c * kF32Threads] = o[r][c] * f;
+        for (int c = 0; c < kCols; ++c) {
+          out[row * D + oc + c * kF32Threads] = o[r][c] * f;
+          if (special) put_back(rr, oc + c * kF32Threads, out + row * D + oc + c * kF32Threads);
+        }
         if (lse && oc == 0) lse[row] = l > 0.f ? (s_m[rr] + log2f(l)) * kLn2 : -INFINITY;
       }
     }
@@ -910,8 +960,9 @@ int tree_mma(const TreeArgs& a) {
   if (rc == B2A_OK) rc = tree_map(&tv, a, a.v, piece, D / 64);
   if (rc) return rc;
   e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kMmaThreads), smem, a.st, tk, tv, a.bt,
-                       static_cast<const T*>(a.q), a.q_stride, static_cast<T*>(a.out), a.lse,
-                       a.part_o, a.part_ml, piece, a.sscale);
+                       static_cast<const T*>(a.q), a.q_stride, static_cast<const T*>(a.v),
+                       a.page_stride, static_cast<T*>(a.out), a.lse, a.part_o, a.part_ml, piece,
+                       a.sscale);
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "tree_decode launch");
   return tree_merge<T, D>(a);
 }
@@ -941,7 +992,7 @@ int tree_wide(const TreeArgs& a) {
                              3, const_cast<void*>(a.q), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kWideThreads), C::kSmem, a.st, tq, tk, tv, a.bt,
-                       static_cast<T*>(a.out), a.lse, a.part_o, a.part_ml, piece, a.sscale);
+                       static_cast<const T*>(a.v), a.page_stride, static_cast<T*>(a.out), a.lse, a.part_o, a.part_ml, piece, a.sscale);
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "tree_wide launch");
   return tree_merge<T, D>(a);
 }

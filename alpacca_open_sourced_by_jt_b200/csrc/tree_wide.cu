@@ -63,6 +63,7 @@ struct WideShared {
   uint64_t bar_sf[kWideGroups], bar_pf[kWideGroups], bar_pv[2], bar_m[kWideGroups][4];
   Start start;
   uint32_t tmem;
+  int special;  // the item's tree rows held infinities or NaN
   float x[kWideGroups][kWideM];  // maxima, at an item's end sums, between the warpgroups
 };
 
@@ -89,8 +90,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Batch bt,
-    T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o,
-    float* __restrict__ part_ml, int piece_rows, float sscale) {
+    const T* __restrict__ vc, long long page_stride, T* __restrict__ out, float* __restrict__ lse,
+    float* __restrict__ part_o, float* __restrict__ part_ml, int piece_rows, float sscale) {
   using C = WideCfg<D>;
   constexpr int BN = C::kBN;
   constexpr int kSlots = C::kSlots;
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
     mbar_init(&sh.bar_pv[0], 1);
     mbar_init(&sh.bar_pv[1], 1);
     fence_mbar_init();
+    sh.special = 0;
   }
   tc_fence_before();
   __syncthreads();
@@ -454,9 +456,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
         } else if (lane == 0) {
           mbar_arrive(&sh.bar_m[w][quarter]);  // keeps the barrier's count of tiles
         }
-        if ((t + 1) * BN > rows) {
+        const int first = max(it.len - t * BN, 0), past = min(rows - t * BN, BN);  // tree rows
+        if (past < BN || (it.n > 1 && first < past)) {
           // V rows past the request's last hold anything: their weight is 0,
-          // but 0 * NaN is not, so they are cleared before the product
+          // but 0 * NaN is not, so they are cleared before the product, and the
+          // infinities and NaN of the tree's rows with them
           // (the slot's use before this one has to be over: its PV is, by S's
           // buffer, unless the ring is shorter than the S buffers)
           if (kSlots / 2 < C::kS && jj >= kSlots / 2) {
@@ -467,13 +471,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
           vround ^= (vslot / kSlots) & 1;
           vslot %= kSlots;
           if (wait(&bar_full[vslot], vround, 0x3D000)) {
-            const int bad = max(rows - t * BN, 0);
             uint8_t* vt = smem + C::kRing + vslot * C::kTileKV;
-            for (int i = r; i < (BN - bad) * (D / 8); i += 128) {
-              const int row = bad + i / (D / 8), c16 = i % (D / 8);
-              *reinterpret_cast<uint4*>(vt + (c16 >> 3) * C::kBoxKV + sw128_off(row, c16 & 7)) =
-                  make_uint4(0u, 0u, 0u, 0u);
-            }
+            auto chunk = [&](int from, int i) {  // 16 bytes i of the rows from `from` on
+              const int row = from + i / (D / 8), c16 = i % (D / 8);
+              return reinterpret_cast<uint4*>(vt + (c16 >> 3) * C::kBoxKV + sw128_off(row, c16 & 7));
+            };
+            for (int i = r; i < (BN - past) * (D / 8); i += 128)
+              *chunk(past, i) = make_uint4(0u, 0u, 0u, 0u);
+            if (it.n > 1)
+              for (int i = r; i < (past - first) * (D / 8); i += 128) {
+                uint4 u = *chunk(first, i);
+                if (clear_special<T>(u)) {
+                  *chunk(first, i) = u;
+                  sh.special = 1;
+                }
+              }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
         }
@@ -485,6 +497,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
       meet();  // the last tile's maximum is the one that O is relative to
       const float M = sh.x[(n - 1) % kWideGroups][r];
       const float mref = (M == -INFINITY) ? 0.f : M;
+      const bool special = sh.special != 0;
       meet();
       sh.x[w][r] = (m == -INFINITY) ? 0.f : l * fast_exp2(m - mref);
       meet();
@@ -522,6 +535,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
             }
           }
         }
+        if (special && good) {
+          const uint4 sees = make_uint4(anc[0], anc[1], anc[2], anc[3]);
+          const int lo = max(it.t0 * BN - it.len, 0), hi = min(it.t1 * BN - it.len, it.n);
+          for (int col = w * 32; col < D; col += 32 * kWideGroups) {
+            if (slot >= 0)
+              add_special(bt, vc, page_stride, it.b, it.kvh, it.len, lo, hi, sees, po + col, D, col, 32);
+            else
+              add_special(bt, vc, page_stride, it.b, it.kvh, it.len, lo, hi, sees, out + row * D + col,
+                          D, col, 32);
+          }
+        }
         if (good && w == 0) {
           if (slot >= 0) {
             float* ml = part_ml + (static_cast<size_t>(slot) * bt.rows_per_block + r) * 2;
@@ -540,6 +564,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tree_wide_kernel(
         kround ^= 1;
       }
       tc_fence_before();
+      if (special && threadIdx.x == 128) sh.special = 0;  // (all have read it: meet() above)
       meet();  // the exchanged numbers and O are read
       if (lane == 0) mbar_arrive(&sh.bar_oe);
     }

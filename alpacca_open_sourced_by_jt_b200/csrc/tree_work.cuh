@@ -17,6 +17,8 @@
 // for one that goes on past its range.
 #pragma once
 
+#include <type_traits>
+
 #include "b2a_common.cuh"
 
 namespace b2a {
@@ -24,6 +26,7 @@ namespace tree {
 
 constexpr int kMaxNodes = B2A_TREE_MAX_NODES;  // nodes of one request's tree
 constexpr int kWords = kMaxNodes / 32;         // words of an ancestor mask
+static_assert(kWords == 4, "add_special takes a mask as four words");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -292,6 +295,54 @@ __device__ __forceinline__ int checked_page(const Batch& bt, int b, int pg) {
   if (pg >= 0 && pg < bt.n_pages) return pg;
   set_dev_error(B2A_ERR_POSITION, b);
   return bt.n_pages;
+}
+
+// Infinities and NaN in the V rows of nodes.  A hidden row has weight 0 in the
+// product P.V, but 0 * inf is NaN: where a request has several nodes, the kernels
+// take such elements out of a tile's tree rows (clear_special), and an item that
+// had some adds them at its end to the rows whose node sees them (add_special), as
+// the sum over the visible rows alone has them.
+
+// Clears the infinities and NaN among 16 bytes of T; true if there were any.
+template <typename T>
+__device__ __forceinline__ bool clear_special(uint4& u) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t keep = 0xffffffffu;
+    if constexpr (sizeof(T) == 4) {
+      if ((w[i] & 0x7f800000u) == 0x7f800000u) keep = 0u;
+    } else {
+      constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+      if ((w[i] & kExp) == kExp) keep &= 0xffff0000u;
+      if ((w[i] >> 16 & kExp) == kExp) keep &= 0x0000ffffu;
+    }
+    any |= keep != 0xffffffffu;
+    w[i] &= keep;
+  }
+  return any;
+}
+
+// Adds the infinities and NaN in columns d0 .. d0 + nd - 1 of a node's V rows to
+// dst (a row of out, or of a part): tree rows [lo, hi) among the bits of anc.
+template <typename T, typename TO>
+__device__ __noinline__ void add_special(const Batch& bt, const T* v, long long page_stride, int b,
+                                         int kvh, int len, int lo, int hi, uint4 anc, TO* dst,
+                                         int D, int d0, int nd) {
+  for (int j = lo; j < hi; ++j) {
+    const uint32_t word = j < 32 ? anc.x : j < 64 ? anc.y : j < 96 ? anc.z : anc.w;
+    if (!((word >> (j & 31)) & 1u)) continue;
+    const int row = len + j;
+    const int pg = checked_page(bt, b, table_entry(bt, b, row));
+    if (pg >= bt.n_pages) continue;
+    const int in_page = bt.table ? row & ((1 << bt.page_shift) - 1) : row;
+    const T* src = v + pg * page_stride + (static_cast<long long>(in_page) * bt.KV + kvh) * D + d0;
+    for (int e = 0; e < nd; ++e) {
+      const float x = ld_elem(src + e);
+      if (!(fabsf(x) < INFINITY)) st_elem(dst + e, ld_elem(dst + e) + x);
+    }
+  }
 }
 
 // Part slot of an item in CTA c's range, or -1 if the item is whole in it.

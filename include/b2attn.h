@@ -573,7 +573,8 @@ int b2a_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
  *   lse_out   f32 [n_tok][H] or NULL
  *   max_len   host bound on lens[b] + nodes (<= table_width * page_rows, or
  *             page_rows without a table); paged caches: page_rows >= 16
- * Padding rows of out, and the rows of a request that is left out, become 0
+ * What a node does not see does not reach its row, infinities and NaN
+ * included.  Padding rows of out, and the rows of a request that is left out, become 0
  * (lse -inf).  16-bit types: tensor cores, f32
  * scores, sums and accumulators, the weights rounded to the type for the
  * product with V.  F32: f32 products and sums.  Short contexts (max_len up to

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import paged_ref as ref
-from tests.paged_ref import TDT
+from tests.paged_ref import TDT, UNIT
 
 pytestmark = pytest.mark.gpu
 
@@ -133,6 +133,47 @@ def test_attention_rows_of_requests_left_out_are_zero(cuda_dev, dt, D, H, KV, n,
     for rows in (slice(odd[5], odd[6]), slice(odd[B - 1], B * n + 7)):
         assert (out[rows] == 0).all() and torch.isneginf(lse[rows]).all()
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dt,D,H,KV,nodes", [("bf16", 64, 4, 2, [6, 3]), ("f16", 128, 8, 1, [2, 1]),
+                                             ("bf16", 128, 8, 2, [4, 9]), ("f16", 256, 4, 2, [4, 3]),
+                                             ("bf16", 256, 16, 1, [40, 7]), ("f16", 64, 16, 2, [33, 128]),
+                                             ("bf16", 128, 16, 2, [128, 70]), ("f32", 64, 8, 2, [7, 128]),
+                                             ("f32", 256, 4, 4, [9, 2])])
+@pytest.mark.parametrize("lens,page", [([45, 0], 16), ([500, 127], 0), ([4990, 3000], 32)])
+def test_attention_hidden_infinities_and_nan_stay_hidden(cuda_dev, dt, D, H, KV, nodes, lens, page):
+    """A branch whose K or V rows overflowed: the nodes that do not see it are what
+    they were, those that do have the infinities and NaN of the sum over their rows."""
+    from tests.test_paged_gpu import Setup
+    s = Setup(cuda_dev, dt, D, H, KV, lens, nodes, page, seed=D + nodes[0])
+    clean = s.run()
+
+    def put(pool, host, b, node, cols, value):
+        row = lens[b] + node
+        at = (int(s.table[b, row // page]), row % page) if page else (b, row)
+        pool[at[0], at[1], KV - 1, cols] = value
+        host[b][row, KV - 1, cols] = value
+
+    inf, nan = float("inf"), float("nan")
+    for b, n in enumerate(nodes):
+        put(s.v, s.vh, b, n - 1, 3, inf)
+        put(s.v, s.vh, b, n - 1, D - 1, nan)
+        put(s.v, s.vh, b, n // 2, 3, -inf)
+        put(s.v, s.vh, b, n // 2, slice(8, 24), inf)
+        if n > 3:
+            put(s.k, s.kh, b, 2, slice(0, D), nan)
+            put(s.v, s.vh, b, 2, slice(0, D), nan)
+    out = s.run().double().cpu().numpy()
+    u = UNIT[dt] if dt != "f32" else 0.0
+    with np.errstate(all="ignore"):
+        o, _, w = ref.attention(s.q.double().cpu().numpy(), s.kh, s.vh, s.lens, s.cu, s.parents, D ** -0.5)
+        close = np.abs(out - o) <= u * (np.abs(o) + w) + 2e-4 * w + 1e-7
+    fine = np.isfinite(o)
+    assert 0 < fine.sum() < fine.size and close[fine].all()
+    assert np.array_equal(out[~fine], o[~fine], equal_nan=True)
+    # rows that see none of it, as before to the bit
+    same = np.isfinite(o).all(axis=-1)
+    assert np.array_equal(out[same], clean.double().cpu().numpy()[same])
 
 
 # ---------------------------------------------------------------------------
