@@ -739,12 +739,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
   // the item that holds the range's last tile
   int b = s.b, n, len;
   long long off = s.off + s.left - 1;  // the range's last tile, counted in request b
-  request(bt, b, n, len);
+  request(bt, b, n, len, s.left_out);
   long long u = units_of(bt, n, len);
   while (off >= u) {
     off -= u;
     if (++b >= bt.B) return;
-    request(bt, b, n, len);
+    request(bt, b, n, len, s.left_out);
     u = units_of(bt, n, len);
   }
   const int tiles = (len + n + bt.tile - 1) / bt.tile;

@@ -62,14 +62,17 @@ struct Batch {
 // Nodes and cache rows of request b; false for a request that is left out (no
 // nodes and no rows): its numbers are out of bounds (recorded), or its last row
 // has no page, -1 in the table, where the plan could not serve it (no error).
-__device__ __forceinline__ bool request(const Batch& bt, int b, int& n, int& len) {
+// Where it is known that no request is left out (Start), `check` false spares
+// the look-up in the table.
+__device__ __forceinline__ bool request(const Batch& bt, int b, int& n, int& len,
+                                        bool check = true) {
   const int c0 = bt.cu[b], c1 = bt.cu[b + 1];
   len = bt.lens[b];
   n = c1 - c0;
   if (n < 0 || n > bt.max_nodes || c0 < 0 || c1 > bt.n_tok || len < 0 ||
       len > bt.max_len - n) {
     set_dev_error(B2A_ERR_POSITION, b);
-  } else if (n == 0 || !bt.table ||
+  } else if (!check || n == 0 || !bt.table ||
              __ldg(bt.table + b * bt.table_stride + ((len + n - 1) >> bt.page_shift)) != -1) {
     return true;
   }
@@ -126,7 +129,7 @@ __device__ __forceinline__ Start locate(const Batch& bt, int team) {
   long long run = 0;
   for (int b0 = 0; b0 < bt.B; b0 += 32) {
     int n = 0, len = 0;
-    if (b0 + lane < bt.B) request(bt, b0 + lane, n, len);
+    if (b0 + lane < bt.B) request(bt, b0 + lane, n, len, s.left_out);
     const long long u = units_of(bt, n, len);
     long long inc = u;
 #pragma unroll
@@ -177,11 +180,13 @@ __device__ __forceinline__ int team_of(const Batch& bt, int c) {
 struct Walker {
   long long off, left;
   int b, n, len;
+  bool check;
   __device__ __forceinline__ void start(const Batch& bt, const Start& s) {
     off = s.off;
     left = s.left;
     b = s.b;
-    if (left > 0) request(bt, b, n, len);
+    check = s.left_out;
+    if (left > 0) request(bt, b, n, len, check);
   }
   __device__ __forceinline__ bool next(const Batch& bt, Item& it) {
     while (left > 0) {
@@ -189,7 +194,7 @@ struct Walker {
       if (off >= u) {
         off -= u;
         if (++b >= bt.B) return false;
-        request(bt, b, n, len);
+        request(bt, b, n, len, check);
         continue;
       }
       it.b = b;
