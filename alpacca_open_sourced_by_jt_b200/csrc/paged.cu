@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_pairs(const __grid_co
 // Accepted path and row moves (b2a_tree_commit)
 // ---------------------------------------------------------------------------
 // From the root, the path goes on to the first child whose token is the
-// node's pick.  A request that the plan did not serve (its last row has no page)
+// node's pick (-1, nothing to pick, ends it).  A request that the plan did not serve (its last row has no page)
 // has no path.  Warp 0 of every CTA walks it (each step is one ballot over
 // the request's nodes), then each thread moves one 16-byte column of the
 // path's rows, in path order: the row at depth d comes from node path[d] >= d,
@@ -514,7 +514,8 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __gri
 #pragma unroll
         for (int w = 0; w < kMaxNodes / 32; ++w) {
           const int j = w * 32 + lane;
-          const unsigned hit = __ballot_sync(0xffffffffu, par[w] == cur && j > cur && tok[w] == last);
+          const unsigned hit =
+              __ballot_sync(0xffffffffu, last >= 0 && par[w] == cur && j > cur && tok[w] == last);
           if (nxt < 0 && hit) nxt = w * 32 + __ffs(hit) - 1;
         }
         if (nxt < 0) break;

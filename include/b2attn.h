@@ -626,7 +626,8 @@ int b2a_constrain_logits(const void* logits, long long row_stride, int in_dtype,
 
 /* The accepted path of each tree, and its K/V rows moved into place.  The
  * path begins at node 0 and goes from a node to its first child whose token
- * is the node's pick.
+ * is the node's pick; a pick of -1 (nothing could be picked) ends it, whatever
+ * stands for a token in nodes behind.
  *   picks, tokens  int32 [n_tok]: the model's token after each node, the
  *                  node's own token (NULL if n_tok is 0)
  *   k_cache, v_cache  n_layers caches layer_stride elements apart (dtype for

@@ -201,6 +201,25 @@ def test_logits_rows_of_requests_left_out_have_no_pick(cuda_dev, cu, left_out):
 
 
 # ---------------------------------------------------------------------------
+# commit
+# ---------------------------------------------------------------------------
+
+def test_commit_ends_where_nothing_could_be_picked(cuda_dev):
+    """A node whose whole row is masked has pick -1: a filler token of -1 behind it is
+    not accepted."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, paged
+    k = torch.randn((4, 16, 2, 64), device=cuda_dev)
+    v, k0 = k.clone(), k.clone()
+    tokens, parents, cu = i32([5, 7, -1, 9, -1], cuda_dev), i32([-1, 0, 1, -1, 0], cuda_dev), i32([0, 3, 5], cuda_dev)
+    c = paged.tree_commit(i32([7, -1, -1, -1, 3], cuda_dev), tokens, parents, cu, i32([0, 4], cuda_dev), k, v,
+                          table=i32([[0, 1], [2, 3]], cuda_dev), max_nodes=3)
+    assert c.accepted.tolist() == [2, 1] and c.next_token.tolist() == [-1, -1]
+    assert c.path.tolist() == [[0, 1, -1], [0, -1, -1]] and c.lens.tolist() == [2, 5]
+    assert torch.equal(k, k0)
+    _lib.raise_device_error()
+
+
+# ---------------------------------------------------------------------------
 # steps of a serving loop
 # ---------------------------------------------------------------------------
 
