@@ -211,7 +211,11 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
       const int row = len + i, pg = row >> p.page_shift;
       const int page = pg < held ? p.table[b * p.table_stride + pg]
                                  : p.ring[(static_cast<long long>(head) + lo + pg - held) % p.ring_size];
-      sl[e] = (page << p.page_shift) + (row & ((1 << p.page_shift) - 1));
+      if (page < 0 || page > (INT_MAX >> p.page_shift)) {
+        set_dev_error(B2A_ERR_POSITION, b);  // no page: its slot would be another's
+      } else {
+        sl[e] = (page << p.page_shift) + (row & ((1 << p.page_shift) - 1));
+      }
     }
   }
   if (p.whole && first + 3 < p.max_tokens) {

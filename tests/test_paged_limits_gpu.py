@@ -75,6 +75,27 @@ def test_page_plan_ended_request_takes_no_pages(cuda_dev):
     assert p.slots[:13].tolist() == [table[1, r // 16].item() * 16 + r % 16 for r in range(20, 33)]
 
 
+@pytest.mark.parametrize("where", ["table", "ring"])
+@pytest.mark.parametrize("page", [-1, 1 << 28, 2 ** 31 - 1])
+def test_page_plan_records_pages_that_are_none(cuda_dev, where, page):
+    """A number in the table or the ring that no pool has: recorded, and no slot (a
+    shifted one would name a row of another page)."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, paged
+    t, r = [[6, 7], [3, 4]], [0, 1, 2, 5]
+    if where == "table":
+        t[0][1] = page
+    else:
+        r[0] = page
+    p = paged.page_plan(i32([30, 20], cuda_dev), i32([5, 2], cuda_dev), i32([2, 2], cuda_dev),
+                        i32([x + [0] for x in t], cuda_dev), i32(r, cuda_dev), i32([0, 4], cuda_dev),
+                        page_rows=16, max_tokens=7)
+    assert _lib.device_error(clear=True)[0] == _lib.ERR_POSITION
+    first = -1 if where == "table" else 7 * 16 + 14
+    last = -1 if where == "ring" else 0
+    assert p.slots.tolist() == [first, first if first < 0 else first + 1] + [
+        last if last < 0 else last + i for i in range(3)] + [4 * 16 + 4, 4 * 16 + 5]
+
+
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
