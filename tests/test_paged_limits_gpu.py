@@ -197,6 +197,57 @@ def test_attention_hidden_infinities_and_nan_stay_hidden(cuda_dev, dt, D, H, KV,
     assert np.array_equal(out[same], clean.double().cpu().numpy()[same])
 
 
+@pytest.mark.parametrize("dt,D,H,KV,lens,nodes", [
+    ("bf16", 64, 32, 2, [3000, 2000, 4100], [128, 100, 128]),  # 16 blocks a head: two rounds of 8
+    ("f16", 128, 32, 4, [1500, 3000, 2100, 40, 900], [128, 1, 2, 1, 1]),  # one far above the average
+    ("f32", 64, 16, 2, [1100, 2500], [40, 64])])
+def test_attention_cut_items_of_many_row_blocks(cuda_dev, dt, D, H, KV, lens, nodes):
+    from tests.test_paged_gpu import Setup
+    s = Setup(cuda_dev, dt, D, H, KV, lens, nodes, 64, seed=sum(nodes))
+    lse = torch.empty((s.cu[-1], H), device=cuda_dev)
+    out = s.run(lse=lse)
+    s.check(out, lse)
+    assert torch.equal(out, s.run())
+
+
+def test_offsets_past_32_bits(cuda_dev):
+    """A pool of more than 2^31 elements: append, attention of many rows and commit at
+    rows whose offsets pass 32 bits."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, device, paged
+    KV, D, page, H, pages, ln, n = 8, 256, 128, 16, 8256, 240, 70
+    k = torch.zeros((pages, page, KV, D), dtype=torch.bfloat16, device=cuda_dev)
+    v = torch.zeros_like(k)
+    mine = [pages - 1, 2, pages - 2]
+    g = torch.Generator("cuda").manual_seed(7)
+    qkv = torch.randn((ln + n, H + 2 * KV, D), device=cuda_dev, generator=g)
+    rows = np.arange(ln + n)
+    slots = np.array(mine)[rows // page] * page + rows % page
+    tree = ref.random_tree(n, np.random.default_rng(4))
+    pos = list(range(ln)) + [ln + len(ref.chain_of(tree, i)) - 1 for i in range(n)]
+    cos, sin = device.rope_tables(512, D, 10000.0, device=cuda_dev)
+    q = paged.rope_append(qkv[:, :H], qkv[:, H:H + KV], qkv[:, H + KV:], i32(pos, cuda_dev), i32(slots, cuda_dev),
+                          cos, sin, k_pool=k, v_pool=v)
+    small_k = torch.zeros((3, page, KV, D), dtype=torch.bfloat16, device=cuda_dev)
+    small_v = torch.zeros_like(small_k)
+    q2 = paged.rope_append(qkv[:, :H], qkv[:, H:H + KV], qkv[:, H + KV:], i32(pos, cuda_dev), i32(rows, cuda_dev),
+                           cos, sin, k_pool=small_k, v_pool=small_v)
+    assert torch.equal(q, q2) and torch.equal(k[mine], small_k) and torch.equal(v[mine], small_v)
+    assert k.view(-1, KV * D)[:, 0].count_nonzero() == (small_k.view(-1, KV * D)[:, 0] != 0).sum()
+    args = (i32([ln], cuda_dev), i32([0, n], cuda_dev), i32(tree, cuda_dev))
+    out = paged.tree_decode(q[ln:], k, v, *args, table=i32([mine], cuda_dev), max_nodes=n)
+    kh, vh = ([x.reshape(-1, KV, D)[:ln + n].double().cpu().numpy()] for x in (small_k, small_v))
+    o, _, w = ref.attention(q[ln:].double().cpu().numpy(), kh, vh, [ln], [0, n], tree, 1 / 16)
+    assert (np.abs(out.double().cpu().numpy() - o) <= UNIT["bf16"] * (np.abs(o) + w) + 2e-4 * w).all()
+    tokens = list(range(n))
+    picks = [max([j for j in range(n) if tree[j] == i], default=-1) for i in range(n)]
+    for kp, vp, t in ((k, v, mine), (small_k, small_v, [0, 1, 2])):
+        c = paged.tree_commit(i32(picks, cuda_dev), i32(tokens, cuda_dev), i32(tree, cuda_dev), args[1], args[0],
+                              kp, vp, table=i32([t], cuda_dev), max_nodes=n)
+        assert c.accepted.item() > 5 and c.path[0, c.accepted.item() - 1].item() > c.accepted.item()
+    assert torch.equal(k[mine], small_k) and torch.equal(v[mine], small_v)
+    _lib.raise_device_error()
+
+
 # ---------------------------------------------------------------------------
 # logits
 # ---------------------------------------------------------------------------
@@ -370,3 +421,57 @@ def test_step_without_nodes(cuda_dev, paged_cache):
     assert c.lens.tolist() == [20, 0, 32] and (c.path == -1).all()
     assert torch.equal(k, k0) and torch.equal(v, v0)
     _lib.raise_device_error()
+
+
+@pytest.mark.parametrize("page,n_pages,seed", [(16, 14, 0), (16, 24, 1), (64, 8, 2)])
+def test_pages_over_many_steps(cuda_dev, page, n_pages, seed):
+    """Requests that come, grow by trees, find no pages and end, over forty steps on a
+    ring that runs short: the device's numbers are those of the definition, and no
+    page is held twice or lost."""
+    from alpacca_open_sourced_by_jt_b200 import _lib, paged
+    rng = np.random.default_rng(seed)
+    B, wide = 9, 12
+    table, ring = np.full((B, wide), -1, np.int64), np.arange(n_pages)
+    state, lens, held = [0, n_pages], [0] * B, [0] * B
+    t, r, st = i32(table, cuda_dev), i32(ring, cuda_dev), i32(state, cuda_dev)
+    ln, hd = i32(lens, cuda_dev), i32(held, cuda_dev)
+    k = torch.zeros((n_pages, page, 1, 64), dtype=torch.bfloat16, device=cuda_dev)
+    v = torch.zeros_like(k)
+    unserved = 0
+    for _ in range(40):
+        add = [int(rng.integers(1, 40)) if rng.random() < 0.7 else 0 for _ in range(B)]
+        for b in range(B):
+            if held[b] and rng.random() < 0.1:
+                add[b] = -1
+            elif lens[b] + max(add[b], 0) > wide * page:
+                add[b] = 0
+        nodes = [max(a, 0) for a in add]
+        trees = [ref.random_tree(m, rng) for m in nodes]
+        par = sum(trees, []) + [-1] * 3
+        n = sum(nodes)
+        want = ref.plan(lens, add, held, table, ring, state, page, n + 3, par)
+        plan = paged.page_plan(ln, i32(add, cuda_dev), hd, t, r, st, page_rows=page, max_tokens=n + 3,
+                               parents=i32(par, cuda_dev))
+        tokens, picks = rng.integers(0, 3, n + 3), rng.integers(0, 3, n + 3)
+        paths = ref.accept(picks.tolist(), tokens.tolist(), par, want["cu"])
+        c = paged.tree_commit(i32(picks, cuda_dev), i32(tokens, cuda_dev), i32(par, cuda_dev), plan.cu, ln, k, v,
+                              table=t, max_nodes=128)
+        _lib.raise_device_error()
+        served = [m == 0 or want["slot"][want["cu"][b]] >= 0 for b, m in enumerate(nodes)]
+        unserved += served.count(False)
+        assert plan.slots.tolist() == want["slot"] and plan.held.tolist() == want["held"]
+        assert plan.ring_state.tolist() == want["state"]
+        assert c.accepted.tolist() == [len(p) if ok else 0 for (p, _), ok in zip(paths, served)]
+        assert c.next_token.tolist() == [x if ok else -1 for (_, x), ok in zip(paths, served)]
+        lens = [a + (len(p) if ok else 0) for a, (p, _), ok in zip(lens, paths, served)]
+        assert c.lens.tolist() == lens
+        table, ring, state, held = want["table"], want["ring"], want["state"], want["held"]
+        ln, hd, st = c.lens, plan.held, plan.ring_state
+        for b in range(B):
+            if add[b] == -1:
+                lens[b] = 0
+                ln[b] = 0
+            assert t[b, :held[b]].tolist() == table[b, :held[b]].tolist()
+        free = [int(ring[(state[0] + i) % n_pages]) for i in range(state[1])]
+        assert sorted(free + [int(x) for b in range(B) for x in table[b, :held[b]]]) == list(range(n_pages))
+    assert unserved > 5
