@@ -22,8 +22,8 @@ constexpr int kMaxNodes = B2A_TREE_MAX_NODES;
 // thread per 4 tokens for the slot map.  Pages taken come from the ring's
 // head and pages given back go to its tail: the two regions do not meet
 // while free and held pages together fit the ring, so CTAs need no order.
-// Latency-bound: 64 requests with 513 tree nodes 7.5 us, 251 requests with 511K
-// tokens 9.9 us (6.4 MB).
+// Latency-bound: 64 requests with 513 tree nodes 7.7 us, 251 requests with 511K
+// tokens 10.4 us (6.4 MB).
 constexpr int kPlanThreads = 256;
 constexpr int kPlanTokens = kPlanThreads * 4;  // tokens of a CTA
 
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
 //   rope_paged_rows   rows in 16-byte aligned groups of 8 elements.  A thread
 //     keeps its 4 pairs' cosines and sines and goes over heads with them; the
 //     loads of kHeads heads are in flight at once, before the position is known.
-//     8 CTAs per SM go over the tokens (8191 tokens, 32/8 heads x 64, f16: 27.8 us;
+//     8 CTAs per SM go over the tokens (8191 tokens, 32/8 heads x 64, f16: 27.7 us;
 //     a CTA per token 29.7; one pair per thread and step 83).
 //   rope_paged_pairs  anything else (odd head or rotation widths, unaligned
 //     strides): one pair per thread and step.
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_pairs(const __grid_co
 // the request's nodes), then each thread moves one 16-byte column of the
 // path's rows, in path order: the row at depth d comes from node path[d] >= d,
 // so no row is overwritten before it was read.  Latency-bound: 16 layers, one
-// request 3.8 us.
+// request 4.1 us.
 constexpr int kCommitThreads = 256;
 
 struct Commit {

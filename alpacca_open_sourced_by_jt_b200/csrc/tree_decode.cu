@@ -40,10 +40,13 @@ namespace tree {
 // P is rounded to the cache's type for the second product (its error, one
 // part in 2^8 or 2^11 of each weight, is what the output's own rounding
 // makes); scores, maxima, sums and accumulators are f32.  Q is not
-// pre-scaled: the scale goes onto the f32 scores.  Measured, 16 x 32760 rows,
-// bf16, 32/8 heads x 128, pages of 64: 4 rows 345 to 355 us (6.1 TB/s; the decode
-// kernel on one block per sequence 342 to 350); x 64: 223 us, where the warps'
-// chain of a tile, not HBM, sets the time.
+// pre-scaled: the scale goes onto the f32 scores.  Measured, 16 x 32768 rows,
+// 32/8 heads, 4 rows: bf16 x 128, pages of 64: 327 to 341 us (6.3 to 6.6 TB/s),
+// one block per sequence 337; the decode kernel (decode.cu) takes 305 for the same
+// rows on the same GPU (7.0 TB/s), and why this one is a tenth behind has not been
+// found.  f16 x 64, pages of 64: 199 us (5.4 TB/s), pages of 16 220; the decode
+// kernel 168 to 221 with its split of 2048 to 8192 rows.  There the warps' chain of a
+// tile, not HBM, sets the time.
 constexpr int kRows = 64;
 constexpr int kConsumers = 8;
 constexpr int kProducers = 4;
@@ -455,7 +458,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(
 // rows x kTile/32 keys (32 FMAs per 6 shared 16-byte reads, which the pipes do
 // in about the same time), a warp the softmax of 2 rows, a thread the output
 // column(s) of its rows.  3 requests of 77 to 2049 rows, 1 to 12 nodes, 32/8
-// heads x 128: 65 us (88 with half the threads).
+// heads x 128: 63 to 64 us (floor 7.3: the FMAs; with half the threads 88).
 constexpr int kF32Threads = 256;
 constexpr int kF32Rows = 16;
 
@@ -865,12 +868,12 @@ cudaError_t allow_smem(K kern, int smem, std::atomic<unsigned long long>& done) 
 }
 
 // Which kernel, by type and by the most rows a KV head can have.  16 x 32K rows,
-// bf16, pages of 64, tree_mma against tree_wide, us: D = 64, 4 rows 223 / 243, 16
-// rows 244 / 244; D = 128, 4 rows 355 / 356, 16 rows 346 / 358; D = 256, 8 rows
-// 202 / 210 (16 rows do not fit tree_mma's registers: 295 / 213).  From 17 rows on
-// tree_mma would read shared memory once more per 16 rows: 32 rows of D = 128
-// took 445 / 365.  In short contexts tree_wide's set-up shows too: one request of
-// 64 rows 7.0 / 9.7, 16 of 1024 24 / 37.
+// 8 KV heads, bf16, pages of 64, tree_mma against tree_wide, us: D = 64, 4 rows
+// 199 / 224, 16 rows 219 / 226; D = 128, 4 rows 330 / 335, 16 rows 324 / 342; D =
+// 256, 8 rows 640 / 700 (16 rows do not fit tree_mma's registers).  From 17 rows on
+// tree_mma would read the cache once more per 16 rows: 32 rows of D = 128 took 623
+// / 346.  In short contexts tree_wide's set-up shows too: one request of 64 rows
+// 8.3 / 12.9, 16 of 1024 14.7 / 22.
 enum TreeKernel { kTreeF32, kTreeMma, kTreeWide };
 
 TreeKernel tree_kernel(int dtype, int rows, int D) {
@@ -891,10 +894,14 @@ int tree_tile(TreeKernel k, int D) {
 // Whole items per CTA, one launch without parts to join, or items cut evenly
 // over the CTAs.  Cutting costs some 12 us (division of the work by tiles, the
 // parts, the second kernel).  Whole against cut, 32/8 heads x 64, f16, pages of
-// 16, us: 1 request of 512 rows 9.3 / 12.2, of 1024 12.1 / 12.6, of 2048 18.8 /
-// 13.2; 4 of 1024 12.4 / 15.8, of 4000 32 / 21; 16 of 1024 12.6 / 24.6, of 4000
-// 35 / 43; 64 of 200 to 2047 55 / 76, of 4000 122 / 127.  So: short contexts, and
-// middling ones where the items alone nearly fill the SMs.
+// 16, one node, us: 1 request of 512 rows 9.5 / 13.4, of 1024 12.7 / 13.6, of 2048
+// 19.5 / 14.1; 4 of 1024 12.9 / 17.6, of 4000 32 / 22; 16 of 1024 13.5 / 26.5, of
+// 4000 35.5 / 45; 64 of 200 to 2047 55 / 80, of 4000 123 / 128.  tree_wide, bf16 x
+// 128, 8 nodes: 1 of 1000 15.6 / 19.3, 16 of 1000 17.5 / 35.4, of 4000 49 / 77.  So:
+// short contexts, and middling ones where the items alone nearly fill the SMs.
+// Where the rule is behind: requests that do not divide by the teams (19 of 4000
+// rows 63 / 52: two rounds of items for ten teams of 18) and few short f32 requests
+// (1 of 1000 rows 95 / 25, 16 of 1000 97 / 106: one item's tiles in series).
 bool tree_always_whole(int max_len) { return max_len <= 1024; }
 bool tree_by_item(int max_len, int B, int KV) {
   return tree_always_whole(max_len) ||
@@ -1118,9 +1125,9 @@ int b2a_tree_decode(const void* q, long long q_tok_stride, const void* k_cache,
   // Side by side in a team: the KV heads, or, where a request has several
   // blocks of query rows, those (as many as the average request has, or as the
   // largest where that is not much more; a request with more goes round again).
-  // 16 x 32K rows, bf16, 32/8 heads x 128, 128 nodes (4 blocks): 1465 us with the
-  // heads side by side (every block reads K and V from HBM again), 1170 with the
-  // blocks.
+  // 16 x 32K rows, bf16, 32/8 heads x 128, 128 nodes (4 blocks), before
+  // tree_wide's third softmax warpgroup: 1465 us with the heads side by side (every
+  // block reads K and V from HBM again), 1170 with the blocks.
   const long long avg_rows = static_cast<long long>(n_tok) * group / B;
   long long blks = (avg_rows + rb / 2) / rb;
   const int most = max_rows_blocks(rows, rb);

@@ -24,10 +24,10 @@
 // 512 threads: warps 0 and 2 TMA producers (a box per page piece and 64
 // columns, or one per tile where a page holds it), warp 1 TMEM owner and MMA
 // issuer, warps 4-15 softmax (TMEM lane quarter = warp % 4).
-// Measured, 16 x 32760 rows, bf16, 32/8 heads x 128, pages of 128: 32 rows 365 us
-// (5.9 TB/s, HBM), 128 rows 383, 512 rows 1037 to 1051 (1050 TFLOP/s, 0.64 of the
-// measured burst: the softmax chain and the issue of 16 MMAs a tile); pages of 16:
-// 461, 478, 1668, the boxes' issue.
+// Measured, 16 x 32760 rows, bf16, 32/8 heads x 128, pages of 128: 32 rows 343 us
+// (6.3 TB/s, HBM), 128 rows 363, 512 rows 1046 to 1080 (1020 to 1050 TFLOP/s, 0.62
+// to 0.64 of the measured burst: the softmax chain and the issue of 16 MMAs a
+// tile); pages of 16: 466, 472 to 493, 1662 to 1679, the boxes' issue.
 // TMEM: S0 .. S2 (BN columns each), O (D columns).
 
 #include <limits.h>

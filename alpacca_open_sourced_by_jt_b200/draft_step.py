@@ -112,8 +112,9 @@ class DraftStep:
     def prefill(self, prompts):
         """Append prompts (a list of ids per request, empty: none) to the
         requests; returns each request's pick after its last token (-1: no
-        prompt) as a list.  Where pages run out between chunks, the chunks before
-        are in the cache (`lens` says how far each request came)."""
+        prompt) as a list.  Where pages run out between two chunks of
+        paged.MAX_NODES, those before are in the cache (`lens` says how far each
+        request came)."""
         self._check(prompts)
         last = [-1] * self.B
         done = [0] * self.B

@@ -538,7 +538,8 @@ int b2a_q8_dequant(const void* codes, long long ldq, const void* scales, long lo
  * up to and including its own are there (or it wants none) and its rows fit
  * max_pages; else it keeps what it holds, its tokens' slots are -1 and so are
  * the table entries of the pages it wanted, by which b2a_tree_decode and
- * b2a_tree_commit leave it out of the step. */
+ * b2a_tree_commit leave it out of the step (one that does not fit max_pages is
+ * past their max_len, and recorded there). */
 int b2a_page_plan(const int* lens_dev, const int* add_dev, const int* parents_dev,
                   const int* held_dev, int* held_out_dev, int* table_dev, long long table_stride,
                   int* ring_dev, int ring_size, const int* ring_state_dev,
