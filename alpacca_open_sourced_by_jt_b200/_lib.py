@@ -137,6 +137,31 @@ SIGNATURES = [
                                 c_longlong, c_int, c_void_p, c_void_p, c_int, c_longlong, c_int,
                                 c_int, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("b2a_norm_rope_append_paged", c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p,
+                                           c_longlong, c_int, c_void_p, c_void_p, c_void_p,
+                                           c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
+                                           c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                           c_longlong, c_int, c_void_p, c_int, c_int, c_int, c_int,
+                                           c_int, c_int, c_void_p]),
+    ("b2a_rope_append_q4", c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong,
+                                   c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
+                                   c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                                   c_int, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                   c_int, c_int, c_void_p]),
+    ("b2a_q4_rows", c_int, [c_void_p, c_int, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int,
+                            c_int, c_int, c_int, c_void_p]),
+    ("b2a_tree_decode_q4_workspace_bytes", c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    ("b2a_tree_decode_q4", c_int, [c_void_p, c_longlong, c_void_p, c_int, c_int, c_longlong,
+                                   c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int, c_int,
+                                   c_int, c_int, c_int, c_int, c_float, c_int, c_void_p]),
+    ("b2a_tree_commit_q4", c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_longlong, c_int, c_void_p, c_int, c_longlong, c_int, c_int,
+                                   c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("b2a_verify_picks", c_int, [c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                 c_int, c_int, c_int, c_void_p]),
 ]
 
 _lib = None

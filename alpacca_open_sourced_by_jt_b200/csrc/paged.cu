@@ -483,6 +483,60 @@ struct Commit {
   int *path, *accepted, *next, *lens_out;
 };
 
+// Warp-collective: the path of request b into s_path, its number of nodes returned,
+// its cached rows in len.  The CTAs of blockIdx.x 0 write it down.
+__device__ __forceinline__ int accepted_path(const Commit& c, int b, int* s_path, int& len) {
+  const int lane = threadIdx.x & 31;
+  const int c0 = c.cu[b], n = c.cu[b + 1] - c0;
+  len = c.lens[b];
+  const bool bad = n < 0 || n > c.max_nodes || c0 < 0 || c0 + n > c.n_tok || len < 0 ||
+                   len > c.max_len - n;
+  const bool served = !bad && n > 0 &&
+                      (c.page_shift < 0 ||
+                       c.table[b * c.table_stride + ((len + n - 1) >> c.page_shift)] != -1);
+  int par[kMaxNodes / 32], tok[kMaxNodes / 32], pick[kMaxNodes / 32];
+#pragma unroll
+  for (int w = 0; w < kMaxNodes / 32; ++w) {
+    const int j = w * 32 + lane;
+    const bool in = served && j < n;
+    par[w] = in ? (c.parents ? c.parents[c0 + j] : j - 1) : -2;
+    tok[w] = in ? c.tokens[c0 + j] : 0;
+    pick[w] = in ? c.picks[c0 + j] : 0;
+  }
+  int len_path = 0, cur = 0, last = -1;
+  if (served) {
+    while (true) {
+      if (lane == 0) s_path[len_path] = cur;
+      ++len_path;
+#pragma unroll
+      for (int w = 0; w < kMaxNodes / 32; ++w)
+        if (w == cur >> 5) last = __shfl_sync(0xffffffffu, pick[w], cur & 31);
+      int nxt = -1;
+#pragma unroll
+      for (int w = 0; w < kMaxNodes / 32; ++w) {
+        const int j = w * 32 + lane;
+        const unsigned hit =
+            __ballot_sync(0xffffffffu, last >= 0 && par[w] == cur && j > cur && tok[w] == last);
+        if (nxt < 0 && hit) nxt = w * 32 + __ffs(hit) - 1;
+      }
+      if (nxt < 0) break;
+      cur = nxt;
+    }
+  }
+  __syncwarp();
+  if (blockIdx.x == 0) {
+    for (int d = lane; d < c.max_nodes; d += 32)
+      c.path[static_cast<size_t>(b) * c.max_nodes + d] = d < len_path ? s_path[d] : -1;
+    if (lane == 0) {
+      c.accepted[b] = len_path;
+      c.next[b] = last;
+      c.lens_out[b] = len + len_path;
+      if (bad) set_dev_error(B2A_ERR_POSITION, b);
+    }
+  }
+  return len_path;
+}
+
 __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __grid_constant__ Commit c) {
   pdl_wait();
   __shared__ int s_path[kMaxNodes];
@@ -490,53 +544,9 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __gri
   __shared__ int s_n;
   const int b = blockIdx.y;
   const int lane = threadIdx.x & 31;
-  const int c0 = c.cu[b], n = c.cu[b + 1] - c0, len = c.lens[b];
-  const bool bad = n < 0 || n > c.max_nodes || c0 < 0 || c0 + n > c.n_tok || len < 0 ||
-                   len > c.max_len - n;
-  const bool served = !bad && n > 0 &&
-                      (c.page_shift < 0 ||
-                       c.table[b * c.table_stride + ((len + n - 1) >> c.page_shift)] != -1);
   if (threadIdx.x < 32) {
-    int par[kMaxNodes / 32], tok[kMaxNodes / 32], pick[kMaxNodes / 32];
-#pragma unroll
-    for (int w = 0; w < kMaxNodes / 32; ++w) {
-      const int j = w * 32 + lane;
-      const bool in = served && j < n;
-      par[w] = in ? (c.parents ? c.parents[c0 + j] : j - 1) : -2;
-      tok[w] = in ? c.tokens[c0 + j] : 0;
-      pick[w] = in ? c.picks[c0 + j] : 0;
-    }
-    int len_path = 0, cur = 0, last = -1;
-    if (served) {
-      while (true) {
-        if (lane == 0) s_path[len_path] = cur;
-        ++len_path;
-#pragma unroll
-        for (int w = 0; w < kMaxNodes / 32; ++w)
-          if (w == cur >> 5) last = __shfl_sync(0xffffffffu, pick[w], cur & 31);
-        int nxt = -1;
-#pragma unroll
-        for (int w = 0; w < kMaxNodes / 32; ++w) {
-          const int j = w * 32 + lane;
-          const unsigned hit =
-              __ballot_sync(0xffffffffu, last >= 0 && par[w] == cur && j > cur && tok[w] == last);
-          if (nxt < 0 && hit) nxt = w * 32 + __ffs(hit) - 1;
-        }
-        if (nxt < 0) break;
-        cur = nxt;
-      }
-    }
-    __syncwarp();
-    if (blockIdx.x == 0) {
-      for (int d = lane; d < c.max_nodes; d += 32)
-        c.path[static_cast<size_t>(b) * c.max_nodes + d] = d < len_path ? s_path[d] : -1;
-      if (lane == 0) {
-        c.accepted[b] = len_path;
-        c.next[b] = last;
-        c.lens_out[b] = len + len_path;
-        if (bad) set_dev_error(B2A_ERR_POSITION, b);
-      }
-    }
+    int len;
+    const int len_path = accepted_path(c, b, s_path, len);
     for (int d = lane; d < len_path; d += 32) {
       const int from = len + s_path[d], to = len + d;
       long long src = -1, dst = -1;

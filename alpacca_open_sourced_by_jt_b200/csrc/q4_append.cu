@@ -1,0 +1,525 @@
+// RMSNorm of the heads of q and k, RoPE and append into a paged cache in one
+// pass (b2a_norm_rope_append_paged, b2a_rope_append_q4), rows of a 4-bit pool
+// read back (b2a_q4_rows) and the commit of a draft tree in it
+// (b2a_tree_commit_q4).
+//
+// Per head of q and k:  y = x * s * w,  s = 1 / sqrt(sum x^2 / D + eps), then the
+// rotation.  The sum is taken in 64 bits and rounded once, with eps, to 32: the
+// factor then does not depend on the order of the sum, nor do the codes of
+// values next to a border.  Products and sums are rounded one by one, as
+// paged.cu does.
+//
+// Bound by reading the projections and writing q and the pool.  A thread takes 8
+// consecutive dims of a head (one word of codes), D / 8 lanes a head; neox pairs
+// meet by shuffles.  kHeads heads of a thread are loaded before the first is
+// used, and before the position is known; the cosines and sines of a token serve
+// all of a thread's heads.
+
+#include "q4.cuh"
+
+namespace b2a {
+namespace q4 {
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  long long q_stride, k_stride, v_stride;
+  const float *bq, *bk, *bv, *wq, *wk, *cos_tab, *sin_tab;
+  const int *pos, *slots;
+  void *k_pool, *v_pool, *q_out;  // k_pool: the 4-bit pool, or K rows (and v_pool V rows)
+  long long page_stride;          // elements; 4-bit pools: bytes
+  long long n_slots;
+  double inv_d;  // 1 / D (a power of two: the product is the quotient)
+  float eps;
+  int tab_rows, page_shift, H, KV, D, n_rot, neox, n_tok;
+};
+
+// What a block stands for: the scale of 32 values whose largest (by magnitude;
+// the negative one of two) has key, as value_key gives it.
+__device__ __forceinline__ uint32_t value_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u << 1 | u >> 31;
+}
+__device__ __forceinline__ __half block_scale(uint32_t key) {
+  if ((key >> 1) > 0x7f800000u) return __ushort_as_half(0x7fff);  // NaN
+  const float m = __uint_as_float(key >> 1 | key << 31);
+  // 8 significant bits; values above 8 x 8160 saturate, so that d * (code - 8)
+  // stays inside f16
+  const float d = __bfloat162float(__float2bfloat16_rn(m * -0.125f));
+  const uint16_t h = __half_as_ushort(__float2half_rn(fminf(fmaxf(d, -8160.f), 8160.f)));
+  return __ushort_as_half((h & 0x7fff) ? h : 0);
+}
+__device__ __forceinline__ uint32_t code_of(float x, float d) {
+  if (d == 0.f) return 8u;
+  const int c = __float2int_rd(__fadd_rn(__fdiv_rn(x, d), 8.5f));
+  return static_cast<uint32_t>(min(max(c, 0), 15));
+}
+
+constexpr int kThreads = 256;
+constexpr int kHeads = 3;  // heads of a thread with their loads in flight
+
+// Q4: the 4-bit pool; otherwise pools of TK.
+template <typename TS, typename TK, typename TQ, bool Q4>
+__global__ void __launch_bounds__(kThreads) norm_append_kernel(const __grid_constant__ AppendArgs a) {
+  pdl_wait();
+  const int D = a.D, L = D >> 3;  // a head's dims and lanes: 8, 16 or 32
+  const int u = threadIdx.x % L, at_once = blockDim.x / L;
+  const int lane = threadIdx.x & 31;
+  const int half = a.n_rot >> 1;
+  const int all = a.H + 2 * a.KV;
+  const int step = at_once * gridDim.y;
+  // the rotation of the thread's dims: norm style 4 pairs of its own, neox 8 dims
+  // whose partners are half further on or back
+  const bool turned = 8 * u < a.n_rot;
+  const bool low = 8 * u < half;
+  const int partner = a.neox && turned ? (low ? lane + half / 8 : lane - half / 8) : lane;
+  for (int i = blockIdx.x; i < a.n_tok; i += gridDim.x) {
+    float c[8], s[8];
+    int p = -1, in_page = 0;
+    long long page = 0;
+    bool stored = false, known = false, ok = true;
+    for (int hb = blockIdx.y * at_once; hb < all && ok; hb += kHeads * step) {
+      float x[kHeads][8];
+#pragma unroll
+      for (int e = 0; e < kHeads; ++e) {
+        const int h = hb + static_cast<int>(threadIdx.x) / L + e * step;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) x[e][d] = 0.f;
+        if (h >= all) continue;
+        const TS* src = h < a.H ? static_cast<const TS*>(a.q) + i * a.q_stride + h * D
+                      : h < a.H + a.KV ? static_cast<const TS*>(a.k) + i * a.k_stride + (h - a.H) * D
+                                       : static_cast<const TS*>(a.v) + i * a.v_stride + (h - a.H - a.KV) * D;
+        paged::load8(src + 8 * u, x[e]);
+      }
+      if (!known) {
+        known = true;
+        p = a.pos[i];
+        const int slot = a.slots[i];
+        if (p < 0 || p >= a.tab_rows || slot >= a.n_slots) {
+          if (threadIdx.x == 0 && blockIdx.y == 0) set_dev_error(B2A_ERR_POSITION, i);
+          ok = false;
+          break;
+        }
+        stored = slot >= 0;
+        page = slot >> a.page_shift;
+        in_page = slot & ((1 << a.page_shift) - 1);
+        if (turned) {
+          const size_t row = static_cast<size_t>(p) * half;
+          if (a.neox) {
+            const int at = low ? 8 * u : 8 * u - half;
+            paged::load8(a.cos_tab + row + at, c);
+            paged::load8(a.sin_tab + row + at, s);
+          } else {
+            paged::load4(a.cos_tab + row + 4 * u, c);
+            paged::load4(a.sin_tab + row + 4 * u, s);
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kHeads; ++e) {
+        const int h0 = hb + (static_cast<int>(threadIdx.x) - lane) / L + e * step;  // the warp's first head
+        if (h0 >= all) continue;
+        const int h = hb + static_cast<int>(threadIdx.x) / L + e * step;
+        const bool is_q = h < a.H, is_v = h >= a.H + a.KV;
+        const int hh = is_q ? h : (is_v ? h - a.H - a.KV : h - a.H);
+        const float* bias = is_q ? a.bq : (is_v ? a.bv : a.bk);
+        if (bias && h < all) {
+          float b[8];
+          paged::load8(bias + hh * D + 8 * u, b);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) x[e][d] = __fadd_rn(x[e][d], b[d]);
+        }
+        const float* w = is_q ? a.wq : a.wk;
+        const bool normed = w != nullptr && !is_v;
+        if (__any_sync(0xffffffffu, normed)) {
+          double ss = 0.0;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) ss = fma(static_cast<double>(x[e][d]), static_cast<double>(x[e][d]), ss);
+          for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (normed) {
+            const float mean = static_cast<float>(ss * a.inv_d + static_cast<double>(a.eps));
+            const float f = __frcp_rn(__fsqrt_rn(mean));
+            float g[8];
+            paged::load8(w + 8 * u, g);
+#pragma unroll
+            for (int d = 0; d < 8; ++d) x[e][d] = __fmul_rn(__fmul_rn(x[e][d], f), g[d]);
+          }
+        }
+        if (a.neox) {
+          if (__any_sync(0xffffffffu, !is_v)) {
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+              const float other = __shfl_sync(0xffffffffu, x[e][d], partner);
+              if (turned && !is_v)
+                x[e][d] = low ? __fsub_rn(__fmul_rn(x[e][d], c[d]), __fmul_rn(other, s[d]))
+                              : __fadd_rn(__fmul_rn(other, s[d]), __fmul_rn(x[e][d], c[d]));
+            }
+          }
+        } else if (turned && !is_v) {
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const float x0 = x[e][2 * d], x1 = x[e][2 * d + 1];
+            x[e][2 * d] = __fsub_rn(__fmul_rn(x0, c[d]), __fmul_rn(x1, s[d]));
+            x[e][2 * d + 1] = __fadd_rn(__fmul_rn(x0, s[d]), __fmul_rn(x1, c[d]));
+          }
+        }
+        if (is_q)
+          paged::store8(static_cast<TQ*>(a.q_out) + (static_cast<size_t>(i) * a.H + h) * D + 8 * u, x[e]);
+        if constexpr (Q4) {
+          if (!stored || !__any_sync(0xffffffffu, !is_q && h < all)) continue;
+          uint32_t key = 0;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) key = max(key, value_key(x[e][d]));
+          key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
+          key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
+          if (is_q || h >= all) continue;
+          const __half d16 = block_scale(key);
+          const float d = __half2float(d16);
+          uint32_t word = 0;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) word |= code_of(x[e][n], d) << ((n >> 1) * 4 + (n & 1) * 16);
+          unsigned char* g = static_cast<unsigned char*>(a.k_pool) + page * a.page_stride +
+                             (static_cast<long long>(hh) * ((1 << a.page_shift) >> 4) + (in_page >> 4)) * granule_bytes(D);
+          const int r = in_page & 15;
+          *reinterpret_cast<uint32_t*>(g + (is_v ? v_word(D, r, u) : k_word(D, r, u))) = word;
+          if ((u & 3) == 0)
+            *reinterpret_cast<__half*>(g + (is_v ? v_scale(D, r, u >> 2) : k_scale(D, r, u >> 2))) = d16;
+        } else {
+          if (is_q || h >= all || !stored) continue;
+          TK* row = static_cast<TK*>(is_v ? a.v_pool : a.k_pool) + page * a.page_stride +
+                    (static_cast<long long>(in_page) * a.KV + hh) * D;
+          paged::store8(row + 8 * u, x[e]);
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows of a 4-bit pool, as values
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kThreads) q4_rows_kernel(const Pool pool, const int* __restrict__ slots,
+                                                           T* __restrict__ k, T* __restrict__ v,
+                                                           int n_tok, int KV, int D) {
+  pdl_wait();
+  const int words = D / 8;
+  const long long total = static_cast<long long>(n_tok) * KV * words;
+  const long long n_slots = static_cast<long long>(pool.n_pages) << pool.page_shift;
+  for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * kThreads) {
+    const int u = static_cast<int>(i % words);
+    const long long th = i / words;
+    const int h = static_cast<int>(th % KV), tok = static_cast<int>(th / KV);
+    const int slot = slots[tok];
+    float x[8], y[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) x[d] = y[d] = 0.f;
+    if (slot >= n_slots) {
+      if (h == 0 && u == 0) set_dev_error(B2A_ERR_POSITION, tok);
+    } else if (slot >= 0) {
+      const int in_page = slot & ((1 << pool.page_shift) - 1), r = in_page & 15;
+      const unsigned char* g = granule(pool, D, slot >> pool.page_shift, h, in_page);
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(g + k_word(D, r, u));
+      const uint32_t vw = *reinterpret_cast<const uint32_t*>(g + v_word(D, r, u));
+      const float dk = __half2float(*reinterpret_cast<const __half*>(g + k_scale(D, r, u >> 2)));
+      const float dv = __half2float(*reinterpret_cast<const __half*>(g + v_scale(D, r, u >> 2)));
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const int sh = (d >> 1) * 4 + (d & 1) * 16;
+        x[d] = dk * static_cast<float>(static_cast<int>(kw >> sh & 15u) - 8);
+        y[d] = dv * static_cast<float>(static_cast<int>(vw >> sh & 15u) - 8);
+      }
+    }
+    paged::store8(k + i * 8, x);
+    paged::store8(v + i * 8, y);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The accepted path's rows moved into place (paged.cu has the path)
+// ---------------------------------------------------------------------------
+// A thread moves one word of K and V of a head of a layer for all rows of the
+// path, in path order, and the scales of a block; no row is overwritten before it
+// was read, since the row at depth d comes from node path[d] >= d.
+__global__ void __launch_bounds__(paged::kCommitThreads) tree_commit_q4_kernel(
+    const __grid_constant__ paged::Commit c, const __grid_constant__ Pool pool, int KV, int D) {
+  pdl_wait();
+  __shared__ int s_path[paged::kMaxNodes];
+  __shared__ long long s_from[paged::kMaxNodes], s_to[paged::kMaxNodes];  // page, row in it
+  __shared__ int s_n;
+  const int b = blockIdx.y, lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    int len = 0;
+    const int m = paged::accepted_path(c, b, s_path, len);
+    for (int d = lane; d < m; d += 32) {
+      const int from = len + s_path[d], to = len + d;
+      long long src = -1, dst = -1;
+      if (from != to) {
+        if (c.page_shift < 0) {
+          src = static_cast<long long>(b) << 32 | from;
+          dst = static_cast<long long>(b) << 32 | to;
+        } else {
+          const int pf = c.table[b * c.table_stride + (from >> c.page_shift)];
+          const int pt = c.table[b * c.table_stride + (to >> c.page_shift)];
+          const int mask = (1 << c.page_shift) - 1;
+          if (pf < 0 || pf >= c.n_pages || pt < 0 || pt >= c.n_pages) {
+            set_dev_error(B2A_ERR_POSITION, b);
+          } else {
+            src = static_cast<long long>(pf) << 32 | (from & mask);
+            dst = static_cast<long long>(pt) << 32 | (to & mask);
+          }
+        }
+      }
+      s_from[d] = src;
+      s_to[d] = dst;
+    }
+    if (lane == 0) s_n = m;
+  }
+  __syncthreads();
+  const int m = s_n, words = D / 8;
+  const long long cols = static_cast<long long>(c.n_layers) * KV * words;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < cols;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const int u = static_cast<int>(i % words);
+    const long long lh = i / words;
+    const int h = static_cast<int>(lh % KV);
+    const long long layer = lh / KV * c.layer_bytes;
+    for (int d = 0; d < m; ++d) {
+      if (s_from[d] < 0) continue;
+      const int rf = static_cast<int>(s_from[d] & 0x7fffffff), rt = static_cast<int>(s_to[d] & 0x7fffffff);
+      const unsigned char* f = granule(pool, D, s_from[d] >> 32, h, rf) + layer;
+      unsigned char* t = granule(pool, D, s_to[d] >> 32, h, rt) + layer;
+      const int a = rf & 15, z = rt & 15;
+      *reinterpret_cast<uint32_t*>(t + k_word(D, z, u)) = *reinterpret_cast<const uint32_t*>(f + k_word(D, a, u));
+      *reinterpret_cast<uint32_t*>(t + v_word(D, z, u)) = *reinterpret_cast<const uint32_t*>(f + v_word(D, a, u));
+      if (u < D / 32) {
+        *reinterpret_cast<uint16_t*>(t + k_scale(D, z, u)) = *reinterpret_cast<const uint16_t*>(f + k_scale(D, a, u));
+        *reinterpret_cast<uint16_t*>(t + v_scale(D, z, u)) = *reinterpret_cast<const uint16_t*>(f + v_scale(D, a, u));
+      }
+    }
+  }
+}
+
+}  // namespace q4
+}  // namespace b2a
+
+// ===========================================================================
+// Host side
+// ===========================================================================
+namespace {
+
+namespace Q4 = b2a::q4;
+
+// What b2a_norm_rope_append_paged and b2a_rope_append_q4 ask of their common
+// arguments.
+int norm_append_check(const char* who, const Q4::AppendArgs& a, int in_dtype, int q_out_dtype,
+                      int n_pages, int page_rows, int style) {
+  if (!a.q || !a.k || !a.v || !a.cos_tab || !a.sin_tab || !a.pos || !a.slots || !a.k_pool || !a.v_pool ||
+      !a.q_out)
+    return fail(B2A_ERR_ARG, "%s: null pointer argument", who);
+  if (a.n_tok < 0 || a.H <= 0 || a.KV <= 0 || a.tab_rows <= 0 || n_pages <= 0)
+    return fail(B2A_ERR_ARG, "%s: sizes must be positive (n_tok=%d H=%d KV=%d)", who, a.n_tok, a.H, a.KV);
+  if (a.D != 64 && a.D != 128 && a.D != 256)
+    return fail(B2A_ERR_UNSUPPORTED, "%s: head_dim %d (64/128/256)", who, a.D);
+  if (style != B2A_ROPE_NORM && style != B2A_ROPE_NEOX) return fail(B2A_ERR_ARG, "%s: style %d", who, style);
+  if (a.n_rot < 0 || a.n_rot > a.D || a.n_rot % (style == B2A_ROPE_NEOX ? 16 : 8) != 0)
+    return fail(B2A_ERR_SHAPE, "%s: n_rot %d (a multiple of %d, at most D=%d)", who, a.n_rot,
+                style == B2A_ROPE_NEOX ? 16 : 8, a.D);
+  const int es = b2a_host::elem_size(in_dtype), qs = b2a_host::elem_size(q_out_dtype);
+  if (es == 0 || qs == 0) return fail(B2A_ERR_DTYPE, "%s: dtypes %d, %d", who, in_dtype, q_out_dtype);
+  if (!power_of_two(page_rows))
+    return fail(B2A_ERR_SHAPE, "%s: page_rows %d is not a power of two", who, page_rows);
+  if ((a.wq || a.wk) && !(a.eps >= 0.f && isfinite(a.eps)))
+    return fail(B2A_ERR_ARG, "%s: eps must not be negative", who);
+  if (a.q_stride < static_cast<long long>(a.H) * a.D || a.k_stride < static_cast<long long>(a.KV) * a.D ||
+      a.v_stride < static_cast<long long>(a.KV) * a.D)
+    return fail(B2A_ERR_SHAPE, "%s: token strides overlap the rows", who);
+  const void* ptrs[] = {a.q, a.k, a.v, a.q_out, a.k_pool, a.v_pool, a.cos_tab, a.sin_tab, a.bq, a.bk, a.bv, a.wq, a.wk};
+  bool ok = (a.q_stride * es) % 16 == 0 && (a.k_stride * es) % 16 == 0 && (a.v_stride * es) % 16 == 0;
+  for (const void* p : ptrs) ok = ok && b2a_host::aligned16(p);
+  if (!ok) return fail(B2A_ERR_ALIGN, "%s: rows, tables, weights and pools must be 16-byte aligned", who);
+  return B2A_OK;
+}
+
+template <typename TS, typename TK, typename TQ, bool kQ4>
+cudaError_t norm_append_launch(const Q4::AppendArgs& a, cudaStream_t st) {
+  // as many threads as give each kHeads heads; few tokens: a token's heads over
+  // more CTAs, until there are a few per SM
+  const int all = a.H + 2 * a.KV, lanes = a.D / 8;
+  int threads = ((all + Q4::kHeads - 1) / Q4::kHeads * lanes + 31) / 32 * 32;
+  if (threads > Q4::kThreads) threads = Q4::kThreads;
+  int gy = (all + threads / lanes - 1) / (threads / lanes);
+  const int enough = (4 * b2a_host::sm_count() + a.n_tok - 1) / a.n_tok;
+  if (gy > enough) gy = enough;
+  const int resident = 8 * b2a_host::sm_count();
+  return b2a_host::launch(Q4::norm_append_kernel<TS, TK, TQ, kQ4>,
+                          dim3(a.n_tok < resident ? a.n_tok : resident, gy), dim3(threads), 0, st, a);
+}
+
+// A 4-bit pool's checks and its description.
+int q4_pool_check(const char* who, const void* pool, int n_pages, int page_rows, long long& page_bytes,
+                  int KV, int D, bool paged_cache) {
+  if (!pool) return fail(B2A_ERR_ARG, "%s: null pointer argument", who);
+  if (n_pages <= 0 || page_rows <= 0 || KV <= 0)
+    return fail(B2A_ERR_ARG, "%s: sizes must be positive (n_pages=%d page_rows=%d KV=%d)", who, n_pages, page_rows, KV);
+  if (D != 64 && D != 128 && D != 256)
+    return fail(B2A_ERR_UNSUPPORTED, "%s: head_dim %d (64/128/256)", who, D);
+  if (page_rows % 16 != 0 || (paged_cache && !power_of_two(page_rows)))
+    return fail(B2A_ERR_SHAPE, "%s: page_rows %d must be a %s from 16 up", who, page_rows,
+                paged_cache ? "power of two" : "multiple of 16");
+  const long long dense = static_cast<long long>(KV) * (page_rows / 16) * Q4::granule_bytes(D);
+  if (dense / KV > INT_MAX) return fail(B2A_ERR_UNSUPPORTED, "%s: page_rows %d", who, page_rows);
+  if (page_bytes == 0) page_bytes = dense;
+  if (page_bytes < dense)
+    return fail(B2A_ERR_SHAPE, "%s: page_bytes %lld < %lld", who, page_bytes, dense);
+  if (!b2a_host::aligned16(pool) || page_bytes % 16 != 0)
+    return fail(B2A_ERR_ALIGN, "%s: the pool and its pages must be 16-byte aligned", who);
+  return B2A_OK;
+}
+
+Q4::Pool q4_pool_of(const void* pool, int n_pages, int page_rows, long long page_bytes, int D, bool paged_cache) {
+  return Q4::Pool{static_cast<unsigned char*>(const_cast<void*>(pool)), page_bytes,
+                  paged_cache ? log2_of(page_rows) : -1, page_rows / 16 * Q4::granule_bytes(D), n_pages};
+}
+
+}  // namespace
+
+extern "C" {
+
+int b2a_norm_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
+                               long long k_tok_stride, const void* v, long long v_tok_stride,
+                               int in_dtype, const float* bq, const float* bk, const float* bv,
+                               const float* wq, const float* wk, float eps, const float* cos_tab,
+                               const float* sin_tab, int tab_rows, const int* pos_dev,
+                               const int* slot_dev, void* k_pool, void* v_pool, int n_pages,
+                               int page_rows, long long page_stride, int kv_dtype, void* q_out,
+                               int n_tok, int H, int KV, int D, int n_rot, int style, void* stream) {
+  Q4::AppendArgs a = {q, k, v, q_tok_stride, k_tok_stride, v_tok_stride, bq, bk, bv, wq, wk, cos_tab, sin_tab,
+                      pos_dev, slot_dev, k_pool, v_pool, q_out, page_stride,
+                      static_cast<long long>(n_pages) * page_rows, D > 0 ? 1.0 / D : 0.0, eps, tab_rows,
+                      log2_of(page_rows), H, KV, D, n_rot, style == B2A_ROPE_NEOX ? 1 : 0, n_tok};
+  const int rc = norm_append_check("norm_rope_append_paged", a, in_dtype, kv_dtype, n_pages, page_rows, style);
+  if (rc) return rc;
+  const long long page_elems = static_cast<long long>(page_rows) * KV * D;
+  if (a.page_stride == 0) a.page_stride = page_elems;
+  if (a.page_stride < page_elems)
+    return fail(B2A_ERR_SHAPE, "norm_rope_append_paged: page_stride %lld < page_rows*KV*D %lld", page_stride, page_elems);
+  if (a.page_stride * b2a_host::elem_size(kv_dtype) % 16 != 0)
+    return fail(B2A_ERR_ALIGN, "norm_rope_append_paged: pages must be 16-byte aligned");
+  if (n_tok == 0) return B2A_OK;
+  const cudaError_t e = with_type(in_dtype, [&](auto* ts) {
+    return with_type(kv_dtype, [&](auto* tk) {
+      using TS = typename std::remove_pointer<decltype(ts)>::type;
+      using TK = typename std::remove_pointer<decltype(tk)>::type;
+      return norm_append_launch<TS, TK, TK, false>(a, static_cast<cudaStream_t>(stream));
+    });
+  });
+  return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "norm_rope_append_paged launch");
+}
+
+int b2a_rope_append_q4(const void* q, long long q_tok_stride, const void* k, long long k_tok_stride,
+                       const void* v, long long v_tok_stride, int in_dtype, const float* bq,
+                       const float* bk, const float* bv, const float* wq, const float* wk, float eps,
+                       const float* cos_tab, const float* sin_tab, int tab_rows, const int* pos_dev,
+                       const int* slot_dev, void* pool, int n_pages, int page_rows,
+                       long long page_bytes, void* q_out, int q_out_dtype, int n_tok, int H, int KV,
+                       int D, int n_rot, int style, void* stream) {
+  Q4::AppendArgs a = {q, k, v, q_tok_stride, k_tok_stride, v_tok_stride, bq, bk, bv, wq, wk, cos_tab, sin_tab,
+                      pos_dev, slot_dev, pool, pool, q_out, 0,
+                      static_cast<long long>(n_pages) * page_rows, D > 0 ? 1.0 / D : 0.0, eps, tab_rows,
+                      log2_of(page_rows), H, KV, D, n_rot, style == B2A_ROPE_NEOX ? 1 : 0, n_tok};
+  int rc = norm_append_check("rope_append_q4", a, in_dtype, q_out_dtype, n_pages, page_rows, style);
+  if (rc == B2A_OK) rc = q4_pool_check("rope_append_q4", pool, n_pages, page_rows, page_bytes, KV, D, true);
+  if (rc) return rc;
+  if (q_out_dtype == B2A_F32) return fail(B2A_ERR_DTYPE, "rope_append_q4: q_out must be f16 or bf16");
+  a.page_stride = page_bytes;
+  if (n_tok == 0) return B2A_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = with_type(in_dtype, [&](auto* ts) {
+    using TS = typename std::remove_pointer<decltype(ts)>::type;
+    if (q_out_dtype == B2A_F16) return norm_append_launch<TS, float, __half, true>(a, st);
+    return norm_append_launch<TS, float, __nv_bfloat16, true>(a, st);
+  });
+  return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "rope_append_q4 launch");
+}
+
+int b2a_q4_rows(const void* pool, int n_pages, int page_rows, long long page_bytes, const int* slot_dev,
+                void* k_out, void* v_out, int out_dtype, int n_tok, int KV, int D, void* stream) {
+  const int rc = q4_pool_check("q4_rows", pool, n_pages, page_rows, page_bytes, KV, D, true);
+  if (rc) return rc;
+  if (!slot_dev || !k_out || !v_out) return fail(B2A_ERR_ARG, "q4_rows: null pointer argument");
+  if (n_tok < 0) return fail(B2A_ERR_ARG, "q4_rows: n_tok %d", n_tok);
+  if (b2a_host::elem_size(out_dtype) == 0) return fail(B2A_ERR_DTYPE, "q4_rows: dtype %d", out_dtype);
+  if (!b2a_host::aligned16(k_out) || !b2a_host::aligned16(v_out))
+    return fail(B2A_ERR_ALIGN, "q4_rows: outputs must be 16-byte aligned");
+  if (n_tok == 0) return B2A_OK;
+  const Q4::Pool p = q4_pool_of(pool, n_pages, page_rows, page_bytes, D, true);
+  const long long ctas = (static_cast<long long>(n_tok) * KV * (D / 8) + Q4::kThreads - 1) / Q4::kThreads;
+  const int most = 8 * b2a_host::sm_count();
+  const cudaError_t e = with_type(out_dtype, [&](auto* t) {
+    using T = typename std::remove_pointer<decltype(t)>::type;
+    return b2a_host::launch(Q4::q4_rows_kernel<T>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)),
+                            dim3(Q4::kThreads), 0, static_cast<cudaStream_t>(stream), p, slot_dev,
+                            static_cast<T*>(k_out), static_cast<T*>(v_out), n_tok, KV, D);
+  });
+  return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "q4_rows launch");
+}
+
+int b2a_tree_commit_q4(const int* picks_dev, const int* tokens_dev, const int* parents_dev,
+                       const int* cu_dev, const int* lens_dev, const int* table_dev,
+                       long long table_stride, int table_width, void* pool, int n_layers,
+                       long long layer_bytes, int n_pages, int page_rows, long long page_bytes, int KV,
+                       int D, int B, int n_tok, int max_nodes, int max_len, int* path_dev,
+                       int* accepted_dev, int* next_dev, int* lens_out_dev, void* stream) {
+  if ((n_tok > 0 && (!picks_dev || !tokens_dev)) || !cu_dev || !lens_dev || !path_dev || !accepted_dev ||
+      !next_dev || !lens_out_dev)
+    return fail(B2A_ERR_ARG, "tree_commit_q4: null pointer argument");
+  if (n_layers <= 0 || B <= 0 || n_tok < 0 || max_len <= 0)
+    return fail(B2A_ERR_ARG, "tree_commit_q4: sizes must be positive");
+  if (max_nodes <= 0 || max_nodes > B2A_TREE_MAX_NODES)
+    return fail(B2A_ERR_ARG, "tree_commit_q4: max_nodes %d (1..%d)", max_nodes, B2A_TREE_MAX_NODES);
+  if (B > 65535) return fail(B2A_ERR_UNSUPPORTED, "tree_commit_q4: %d requests > 65535", B);
+  if (lens_out_dev == lens_dev)
+    return fail(B2A_ERR_ARG, "tree_commit_q4: lens_out needs a buffer of its own");
+  const int rc = q4_pool_check("tree_commit_q4", pool, n_pages, page_rows, page_bytes, KV, D, table_dev != nullptr);
+  if (rc) return rc;
+  const long long dense = static_cast<long long>(KV) * (page_rows / 16) * Q4::granule_bytes(D);
+  if (n_layers > 1 && (layer_bytes < page_bytes * (n_pages - 1) + dense || layer_bytes % 16 != 0))
+    return fail(B2A_ERR_SHAPE, "tree_commit_q4: layers overlap or are not 16-byte aligned");
+  if (table_dev) {
+    if (table_width <= 0 || table_stride < table_width ||
+        static_cast<long long>(table_width) * page_rows < max_len)
+      return fail(B2A_ERR_SHAPE, "tree_commit_q4: a table row of %d pages (stride %lld) does not hold max_len %d rows",
+                  table_width, table_stride, max_len);
+  } else if (n_pages < B || page_rows < max_len) {
+    return fail(B2A_ERR_SHAPE, "tree_commit_q4: %d blocks of %d rows for %d sequences of up to %d",
+                n_pages, page_rows, B, max_len);
+  }
+  const Q4::Pool p = q4_pool_of(pool, n_pages, page_rows, page_bytes, D, table_dev != nullptr);
+  PG::Commit c = {};
+  c.picks = picks_dev;
+  c.tokens = tokens_dev;
+  c.parents = parents_dev;
+  c.cu = cu_dev;
+  c.lens = lens_dev;
+  c.table = table_dev;
+  c.table_stride = table_stride;
+  c.layer_bytes = n_layers > 1 ? layer_bytes : 0;
+  c.n_layers = n_layers;
+  c.n_pages = n_pages;
+  c.page_shift = p.page_shift;
+  c.max_len = max_len;
+  c.n_tok = n_tok;
+  c.max_nodes = max_nodes;
+  c.path = path_dev;
+  c.accepted = accepted_dev;
+  c.next = next_dev;
+  c.lens_out = lens_out_dev;
+  const long long cols = static_cast<long long>(n_layers) * KV * (D / 8);
+  const long long gx = (cols + PG::kCommitThreads - 1) / PG::kCommitThreads;
+  const cudaError_t e = b2a_host::launch(Q4::tree_commit_q4_kernel, dim3(static_cast<unsigned>(gx < 64 ? gx : 64), B),
+                                         dim3(PG::kCommitThreads), 0, static_cast<cudaStream_t>(stream), c, p, KV, D);
+  return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "tree_commit_q4 launch");
+}
+
+}  // extern "C"

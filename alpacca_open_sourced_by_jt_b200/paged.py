@@ -10,6 +10,11 @@ A step of a serving loop:
     logits, picks = constrain_logits(logits, plan.cu, parents, tokens, ...)
     done  = tree_commit(picks, tokens, parents, plan.cu, lens, k_pools, v_pools, table=table, ...)
 
+With a cache of 4 bits (`q4_pool`, 0.28 of a 16-bit cache's bytes) the layers call
+rope_append_q4 and tree_decode_q4, and the step ends in tree_commit_q4.  Where
+tokens are sampled, verify_picks takes the place of constrain_logits' greedy
+picks.
+
 Pools are (n_pages, page_rows, KV, D) tensors and `table` (B, max_pages) int32
 names each request's pages; page_rows is a power of two.  The step's tokens
 (nodes) of all requests lie behind one another: request b owns rows cu[b] ..
@@ -170,19 +175,23 @@ def page_plan(lens: torch.Tensor, add: torch.Tensor, held: torch.Tensor, table: 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
                 slots: torch.Tensor, cos_tab: torch.Tensor, sin_tab: torch.Tensor, *, k_pool,
                 v_pool, n_rot: int | None = None, style: str = "norm", q_out=None, bq=None,
-                bk=None, bv=None, stream=None) -> torch.Tensor:
+                bk=None, bv=None, q_norm=None, k_norm=None, eps: float = 1e-6,
+                stream=None) -> torch.Tensor:
     """Fused bias + RoPE + append into a paged cache (b2a_rope_append_paged).
 
     q (n, H, D), k, v (n, KV, D) of one type (f32, f16 or bf16), contiguous per
     token (views into one packed projection are fine); positions, slots (n,)
     int32 as page_plan writes them: the rotary position and the pool row are
-    apart, a negative slot stores nothing.  Returns q_out (n, H, D), in the
-    pools' type unless given."""
+    apart, a negative slot stores nothing.  q_norm, k_norm (D,) f32: RMSNorm of
+    each head of q and k, with these weights and eps, before the rotation
+    (b2a_norm_rope_append_paged: head_dim 64, 128 or 256, rows 16-byte aligned,
+    q_out in the pools' type).  Returns q_out (n, H, D), in the pools' type unless
+    given."""
     if stream is not None:
         with _on(stream):
             return rope_append(q, k, v, positions, slots, cos_tab, sin_tab, k_pool=k_pool,
                                v_pool=v_pool, n_rot=n_rot, style=style, q_out=q_out, bq=bq, bk=bk,
-                               bv=bv)
+                               bv=bv, q_norm=q_norm, k_norm=k_norm, eps=eps)
     (P, R, KV, D), pstride = _pool(k_pool, v_pool)
     dt, qs, ks, vs = q.dtype, q.stride(), k.stride(), v.stride()
     n, H, Dq = q.shape
@@ -203,7 +212,20 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
         q_out = k_pool.new_empty((n, H, D))
     elif not q_out.is_cuda or not q_out.is_contiguous() or q_out.numel() != n * H * D:
         _bad("q_out must be a contiguous CUDA tensor (n, H, D)")
+    normed = q_norm is not None or k_norm is not None
+    if normed and q_out.dtype is not k_pool.dtype:
+        _bad("with norms q_out must be in the pools' type")
     if n == 0:  # (an empty tensor has no address)
+        return q_out
+    if normed:
+        _lib.check(_lib.load().b2a_norm_rope_append_paged(
+            q.data_ptr(), qs[0] if n > 1 else H * D, k.data_ptr(), ks[0] if n > 1 else KV * D,
+            v.data_ptr(), vs[0] if n > 1 else KV * D, _code(dt), _f32("bq", bq, H * D),
+            _f32("bk", bk, KV * D), _f32("bv", bv, KV * D), _f32("q_norm", q_norm, D),
+            _f32("k_norm", k_norm, D), eps, cos, sin, rows, positions.data_ptr(), slots.data_ptr(),
+            k_pool.data_ptr(), v_pool.data_ptr(), P, R, pstride[0] if P > 1 else R * KV * D,
+            _code(k_pool.dtype), q_out.data_ptr(), n, H, KV, D, n_rot, device._STYLE[style],
+            _stream(q)))
         return q_out
     _lib.check(_lib.load().b2a_rope_append_paged(
         q.data_ptr(), qs[0] if n > 1 else H * D, k.data_ptr(), ks[0] if n > 1 else KV * D,
@@ -417,4 +439,232 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
         strides[-4] if P > 1 else R * KV * D, KV, D, _code(k_pool.dtype), B, n, max_nodes, max_len,
         path.data_ptr(), accepted.data_ptr(), nxt.data_ptr(), lens_out.data_ptr(),
         _stream(lens)))
+    return out
+
+
+# ---- the 4-bit cache ---------------------------------------------------------
+
+def q4_pool(n_pages: int, page_rows: int, n_kv: int, head_dim: int, *, layers: int | None = None,
+            device) -> torch.Tensor:
+    """An empty 4-bit pool for K and V: uint8 (n_pages, KV, page_rows / 16, 18 D),
+    with `layers` (L, ...).  A granule (the last axis) holds 16 rows of one head,
+    as b2attn.h lays them out."""
+    if page_rows <= 0 or page_rows % 16 or head_dim not in (64, 128, 256):
+        _bad("a 4-bit pool has pages of a multiple of 16 rows and head_dim 64, 128 or 256")
+    shape = (n_pages, n_kv, page_rows // 16, 18 * head_dim)
+    return torch.zeros(shape if layers is None else (layers,) + shape, dtype=torch.uint8, device=device)
+
+
+def _q4(pool: torch.Tensor, dims: int = 4):
+    """(pages, page_rows, KV, D, bytes between pages) of a 4-bit pool."""
+    shape, stride = pool.shape, pool.stride()
+    if pool.dtype is not torch.uint8 or not pool.is_cuda or len(shape) != dims:
+        _bad("a 4-bit pool is a CUDA uint8 tensor (n_pages, KV, page_rows / 16, 18 * D)")
+    P, KV, G, width = shape[-4:]
+    if width % 18 or stride[-1] != 1 or (G > 1 and stride[-2] != width) or (
+            KV > 1 and stride[-3] != G * width):
+        _bad("each page of a 4-bit pool must be contiguous, 18 * D bytes per 16 rows of a head")
+    return P, 16 * G, KV, width // 18, (stride[-4] if P > 1 else KV * G * width)
+
+
+def rope_append_q4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                   slots: torch.Tensor, cos_tab: torch.Tensor, sin_tab: torch.Tensor, *, pool,
+                   n_rot: int | None = None, style: str = "norm", q_out=None, bq=None, bk=None,
+                   bv=None, q_norm=None, k_norm=None, eps: float = 1e-6,
+                   stream=None) -> torch.Tensor:
+    """Fused bias + RMSNorm of each head + RoPE + append into a 4-bit paged cache
+    (b2a_rope_append_q4).
+
+    As rope_append, with pool from q4_pool; q_norm / k_norm None: no norm.
+    Returns q_out (n, H, D), f16 or bf16: q's type unless given, f16 for f32."""
+    if stream is not None:
+        with _on(stream):
+            return rope_append_q4(q, k, v, positions, slots, cos_tab, sin_tab, pool=pool, n_rot=n_rot,
+                                  style=style, q_out=q_out, bq=bq, bk=bk, bv=bv, q_norm=q_norm,
+                                  k_norm=k_norm, eps=eps)
+    P, R, KV, D, page_bytes = _q4(pool)
+    dt, qs, ks, vs = q.dtype, q.stride(), k.stride(), v.stride()
+    n, H, Dq = q.shape
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and k.dtype is dt and v.dtype is dt and
+            Dq == D and k.shape == (n, KV, D) and v.shape == (n, KV, D)):
+        _bad("q (n, H, D), k and v (n, KV, D): CUDA tensors of one type, as the pool's rows")
+    if qs[2] != 1 or qs[1] != D or ks[2] != 1 or ks[1] != D or vs[2] != 1 or vs[1] != D:
+        _bad("q, k and v rows must be contiguous per token")
+    _i32("positions", positions, n)
+    _i32("slots", slots, n)
+    rows, half = cos_tab.shape
+    if n_rot is None:
+        n_rot = 2 * half
+    if half * 2 != n_rot:
+        _bad("cos/sin tables f32 (rows, n_rot/2)")
+    cos, sin = _f32("cos_tab", cos_tab, rows * half), _f32("sin_tab", sin_tab, rows * half)
+    if q_out is None:
+        q_out = torch.empty((n, H, D), dtype=torch.float16 if dt is torch.float32 else dt, device=q.device)
+    elif not q_out.is_cuda or not q_out.is_contiguous() or q_out.numel() != n * H * D:
+        _bad("q_out must be a contiguous CUDA tensor (n, H, D)")
+    if n == 0:
+        return q_out
+    _lib.check(_lib.load().b2a_rope_append_q4(
+        q.data_ptr(), qs[0] if n > 1 else H * D, k.data_ptr(), ks[0] if n > 1 else KV * D,
+        v.data_ptr(), vs[0] if n > 1 else KV * D, _code(dt), _f32("bq", bq, H * D),
+        _f32("bk", bk, KV * D), _f32("bv", bv, KV * D), _f32("q_norm", q_norm, D),
+        _f32("k_norm", k_norm, D), eps, cos, sin, rows, positions.data_ptr(), slots.data_ptr(),
+        pool.data_ptr(), P, R, page_bytes, q_out.data_ptr(), _code(q_out.dtype), n, H, KV, D, n_rot,
+        device._STYLE[style], _stream(q)))
+    return q_out
+
+
+def q4_rows(pool: torch.Tensor, slots: torch.Tensor, *, dtype: torch.dtype = torch.float32,
+            stream=None):
+    """The K and V rows (n, KV, D) that slots (n,) int32 of a 4-bit pool stand for,
+    in dtype (b2a_q4_rows); zeros for negative slots."""
+    if stream is not None:
+        with _on(stream):
+            return q4_rows(pool, slots, dtype=dtype)
+    P, R, KV, D, page_bytes = _q4(pool)
+    n = slots.numel()
+    _i32("slots", slots)
+    out = torch.empty((2, n, KV, D), dtype=dtype, device=pool.device)
+    if n:
+        _lib.check(_lib.load().b2a_q4_rows(
+            pool.data_ptr(), P, R, page_bytes, slots.data_ptr(), out.data_ptr(), out[1].data_ptr(),
+            _code(dtype), n, KV, D, _stream(pool)))
+    return out[0], out[1]
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_q4_bytes(device_index, max_nodes, n_head, n_kv, head_dim, max_len) -> int:
+    return _lib.load().b2a_tree_decode_q4_workspace_bytes(max_nodes, n_head, n_kv, head_dim, max_len)
+
+
+def tree_decode_q4_workspace(max_nodes: int, n_head: int, n_kv: int, head_dim: int, max_len: int,
+                             dev) -> torch.Tensor:
+    """Allocate (via torch) a workspace big enough for b2a_tree_decode_q4."""
+    n = _lib.load().b2a_tree_decode_q4_workspace_bytes(max_nodes, n_head, n_kv, head_dim, max_len)
+    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=dev)
+
+
+def tree_decode_q4(q: torch.Tensor, pool: torch.Tensor, lens: torch.Tensor, cu: torch.Tensor,
+                   parents: torch.Tensor | None, *, table=None, max_nodes: int,
+                   max_len: int | None = None, scale: float | None = None, out=None, lse=None,
+                   workspace=None, stream=None) -> torch.Tensor:
+    """Attention of drafted tokens over a 4-bit cache (b2a_tree_decode_q4).
+
+    q (n, H, D) f16 or bf16; pool as q4_pool makes it, with table (B, max_pages),
+    or, with table None, one page per sequence (n_ctx rows, a multiple of 16).
+    All else as tree_decode.  Returns out (n, H, D) in q's type."""
+    if stream is not None:
+        with _on(stream):
+            return tree_decode_q4(q, pool, lens, cu, parents, table=table, max_nodes=max_nodes,
+                                  max_len=max_len, scale=scale, out=out, lse=lse, workspace=workspace)
+    P, R, KV, D, page_bytes = _q4(pool)
+    dt, qs = q.dtype, q.stride()
+    n, H, Dq = q.shape
+    if not q.is_cuda or qs[2] != 1 or qs[1] != D or Dq != D:
+        _bad("q must be a CUDA tensor (n, H, D), contiguous per token, as the pool's rows")
+    B = lens.numel()
+    _i32("lens", lens)
+    _i32("cu", cu, B + 1)
+    pptr = _i32_rows("parents", parents, n)
+    tptr, tstride, width = _table(table, B)
+    if max_len is None:
+        max_len = width * R if table is not None else R
+    if out is None:
+        out = q.new_empty((n, H, D))
+    elif not out.is_cuda or not out.is_contiguous() or out.shape != (n, H, D) or out.dtype is not dt:
+        _bad("out must be a contiguous CUDA tensor (n, H, D) in q's type")
+    if n == 0:
+        return out
+    if workspace is None:
+        ws_bytes = _tree_q4_bytes(q.device.index, max_nodes, H, KV, D, max_len)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    else:
+        ws_bytes = workspace.numel() * workspace.element_size()
+    _lib.check(_lib.load().b2a_tree_decode_q4(
+        q.data_ptr(), qs[0] if n > 1 else H * D, pool.data_ptr(), P, R, page_bytes, tptr, tstride,
+        width, lens.data_ptr(), cu.data_ptr(), pptr, out.data_ptr(), _f32("lse", lse, n * H),
+        None if workspace is None else workspace.data_ptr(), ws_bytes, B, n, max_nodes, H, KV, D,
+        _code(dt), 1.0 / math.sqrt(D) if scale is None else scale, max_len, _stream(q)))
+    return out
+
+
+def tree_commit_q4(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor | None,
+                   cu: torch.Tensor, lens: torch.Tensor, pool: torch.Tensor, *, table=None,
+                   max_nodes: int, max_len: int | None = None, out: Commit | None = None,
+                   stream=None) -> Commit:
+    """tree_commit in a 4-bit pool (b2a_tree_commit_q4): (L, n_pages, KV, page_rows /
+    16, 18 D) for all layers at once, or one layer's 4-D pool."""
+    if stream is not None:
+        with _on(stream):
+            return tree_commit_q4(picks, tokens, parents, cu, lens, pool, table=table,
+                                  max_nodes=max_nodes, max_len=max_len, out=out)
+    dims = pool.dim()
+    P, R, KV, D, page_bytes = _q4(pool, 5 if dims == 5 else 4)
+    L = pool.shape[0] if dims == 5 else 1
+    B, n = lens.numel(), tokens.numel()
+    _i32("lens", lens)
+    _i32("cu", cu, B + 1)
+    tptr, tstride, width = _table(table, B)
+    if max_len is None:
+        max_len = width * R if table is not None else R
+    if out is None:
+        path, accepted, nxt, lens_out = torch.empty(
+            B * (max_nodes + 3), dtype=torch.int32,
+            device=lens.device).split_with_sizes((B * max_nodes, B, B, B))
+        out = Commit(path.view(B, max_nodes), accepted, nxt, lens_out)
+    else:
+        path, accepted, nxt, lens_out = out
+        _i32("out.path", path, B * max_nodes)
+        for name, t in (("accepted", accepted), ("next_token", nxt), ("lens", lens_out)):
+            _i32("out." + name, t, B)
+    _lib.check(_lib.load().b2a_tree_commit_q4(
+        _i32_rows("picks", picks, n), _i32_rows("tokens", tokens, n),
+        _i32_rows("parents", parents, n), cu.data_ptr(), lens.data_ptr(), tptr, tstride, width,
+        pool.data_ptr(), L, pool.stride(0) if L > 1 else 0, P, R, page_bytes, KV, D, B, n, max_nodes,
+        max_len, path.data_ptr(), accepted.data_ptr(), nxt.data_ptr(), lens_out.data_ptr(),
+        _stream(lens)))
+    return out
+
+
+# ---- sampled verification ----------------------------------------------------
+
+def verify_picks(logits: torch.Tensor, cu: torch.Tensor, parents: torch.Tensor | None,
+                 tokens: torch.Tensor, uniforms: torch.Tensor, draws: torch.Tensor, *,
+                 max_nodes: int, temperature=None, draft=None, out=None, stream=None) -> torch.Tensor:
+    """Which drafted tokens stand, by sampling from the model's probabilities with
+    given random numbers (b2a_verify_picks); the picks are tree_commit's.
+
+    logits (n, V) f32, f16 or bf16, unit stride along V (constrain_logits' output:
+    penalties and masks apply); uniforms (n,) f32 in [0, 1), a node's own; draws
+    (B,) f32 in [0, 1) for the token behind the accepted path; temperature (B,) f32
+    (None: 1; 0: greedy).  draft (n, V) f32: row i holds the probabilities from
+    which node i's children were drawn, independently; None: the drafts are
+    certain (an n-gram table's, a search's).  Returns picks (n,) int32: the next
+    token after each node of the accepted path, -1 elsewhere."""
+    if stream is not None:
+        with _on(stream):
+            return verify_picks(logits, cu, parents, tokens, uniforms, draws, max_nodes=max_nodes,
+                                temperature=temperature, draft=draft, out=out)
+    n, V = logits.shape
+    ls = logits.stride()
+    if not logits.is_cuda or ls[1] != 1:
+        _bad("logits must be a CUDA tensor (n, V), unit stride along V")
+    B = cu.numel() - 1
+    _i32("cu", cu)
+    dptr, dstride = None, 0
+    if draft is not None:
+        if draft.dtype is not torch.float32 or not draft.is_cuda or draft.shape != (n, V) or draft.stride(1) != 1:
+            _bad("draft must be a CUDA f32 tensor (n, V), unit stride along V")
+        dptr, dstride = draft.data_ptr(), (draft.stride(0) if n > 1 else V)
+    if out is None:
+        out = torch.empty(n, dtype=torch.int32, device=logits.device)
+    else:
+        _i32("out", out, n)
+    if n == 0:
+        return out
+    _lib.check(_lib.load().b2a_verify_picks(
+        logits.data_ptr(), ls[0] if n > 1 else V, _code(logits.dtype), dptr, dstride, cu.data_ptr(),
+        _i32_rows("parents", parents, n), _i32_rows("tokens", tokens, n), _f32("uniforms", uniforms, n),
+        _f32("draws", draws, B), _f32("temperature", temperature, B), out.data_ptr(), B, n, max_nodes,
+        V, _stream(logits)))
     return out

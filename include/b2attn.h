@@ -648,6 +648,115 @@ int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* pare
                     int max_nodes, int max_len, int* path_dev, int* accepted_dev, int* next_dev,
                     int* lens_out_dev, void* stream);
 
+/* ---- normed heads, the 4-bit paged cache, sampled verification -------------
+ *
+ * No reference counterpart (it serves one sequence from f32 rows; of its model
+ * families, alpaccaroo/model.py:30-38, qwen3 and gemma3 norm their heads).  The
+ * step of the section above with a cache of 4 bits:
+ *   b2a_page_plan          as above
+ *   per layer: b2a_rope_append_q4, b2a_tree_decode_q4
+ *   b2a_constrain_logits, then b2a_verify_picks where tokens are sampled
+ *   b2a_tree_commit_q4     takes either's picks
+ *
+ * A 4-bit block is 32 consecutive values of a row: with m the value of largest
+ * magnitude (of two, the negative one) and
+ *   d    = m / -8 rounded to 8 significant bits, within +-8160, kept as f16
+ *   code = floor(x / d + 8.5) within 0 .. 15
+ * it stands for d * (code - 8), which f16 holds exactly, half a step |d| / 2 from x
+ * (up to a whole one at the end of the range without the code 16).  Values beyond 65280 saturate; a block with a NaN has d = NaN
+ * and stands for NaN.
+ *
+ * A 4-bit pool is [n_pages][KV][page_rows / 16] granules of 18 D bytes (K and V
+ * of 16 rows of one head), pages page_bytes apart (0: dense), a multiple of 16;
+ * D is 64, 128 or 256, page_rows a power of two from 16 up (without a table: a
+ * multiple of 16).  A granule: 8 D bytes of K codes, 8 D of V codes, D of K
+ * scales, D of V scales.  Codes are in 32-bit words of 8 consecutive dims, dim
+ * 2i in bits 4i .. 4i + 3, dim 2i + 1 in bits 4i + 16 .. 4i + 19.  K words
+ * [ceil(D / 128)][16 rows][4 words of a block][min(4, D / 32) blocks]; V words
+ * [D / 8][16 rows]; scales f16 [16 rows][D / 32].  Tables, slots, trees, requests
+ * that are left out and numbers out of bounds are as in the section above. */
+
+/* b2a_rope_append_paged with RMSNorm of each head of q and k in front:
+ *   x = x (+ bias);  s = 1 / sqrt(f32(sum x^2 / D + eps)), the sum in 64 bits;
+ *   x = (x * s) * w;  then the rotation
+ *   wq, wk    f32 [D] the norms' weights, or NULL: no norm of q, of k
+ * q_out is of kv_dtype.  D 64, 128 or 256; n_rot a multiple of 8 (norm style)
+ * or 16 (neox); all rows, tables, weights and pools 16-byte aligned. */
+int b2a_norm_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
+                               long long k_tok_stride, const void* v, long long v_tok_stride,
+                               int in_dtype, const float* bq, const float* bk, const float* bv,
+                               const float* wq, const float* wk, float eps, const float* cos_tab,
+                               const float* sin_tab, int tab_rows, const int* pos_dev,
+                               const int* slot_dev, void* k_pool, void* v_pool, int n_pages,
+                               int page_rows, long long page_stride, int kv_dtype, void* q_out,
+                               int n_tok, int H, int KV, int D, int n_rot, int style, void* stream);
+
+/* The same into a 4-bit pool; q_out is F16 or BF16. */
+int b2a_rope_append_q4(const void* q, long long q_tok_stride, const void* k, long long k_tok_stride,
+                       const void* v, long long v_tok_stride, int in_dtype, const float* bq,
+                       const float* bk, const float* bv, const float* wq, const float* wk, float eps,
+                       const float* cos_tab, const float* sin_tab, int tab_rows, const int* pos_dev,
+                       const int* slot_dev, void* pool, int n_pages, int page_rows,
+                       long long page_bytes, void* q_out, int q_out_dtype, int n_tok, int H, int KV,
+                       int D, int n_rot, int style, void* stream);
+
+/* Rows of a 4-bit pool as values: k_out, v_out [n_tok][KV][D] of out_dtype get the
+ * rows of the slots (zeros for a negative slot; one past the pool records
+ * B2A_ERR_POSITION and gives zeros). */
+int b2a_q4_rows(const void* pool, int n_pages, int page_rows, long long page_bytes, const int* slot_dev,
+                void* k_out, void* v_out, int out_dtype, int n_tok, int KV, int D, void* stream);
+
+/* b2a_tree_decode over a 4-bit pool: q and out of dtype F16 or BF16.  f32 scores
+ * (q is scaled by a power of two to f16, exact but for elements 2^28 times smaller
+ * than their row's largest), sums and accumulators; weights times V scales are
+ * rounded to f16 for the product with V's codes. */
+size_t b2a_tree_decode_q4_workspace_bytes(int max_nodes, int H, int KV, int D, int max_len);
+int b2a_tree_decode_q4(const void* q, long long q_tok_stride, const void* pool, int n_pages,
+                       int page_rows, long long page_bytes, const int* table_dev,
+                       long long table_stride, int table_width, const int* lens_dev,
+                       const int* cu_dev, const int* parents_dev, void* out, float* lse_out,
+                       void* workspace, size_t workspace_bytes, int B, int n_tok, int max_nodes, int H,
+                       int KV, int D, int dtype, float scale, int max_len, void* stream);
+
+/* b2a_tree_commit in 4-bit pools, n_layers of them layer_bytes apart. */
+int b2a_tree_commit_q4(const int* picks_dev, const int* tokens_dev, const int* parents_dev,
+                       const int* cu_dev, const int* lens_dev, const int* table_dev,
+                       long long table_stride, int table_width, void* pool, int n_layers,
+                       long long layer_bytes, int n_pages, int page_rows, long long page_bytes, int KV,
+                       int D, int B, int n_tok, int max_nodes, int max_len, int* path_dev,
+                       int* accepted_dev, int* next_dev, int* lens_out_dev, void* stream);
+
+/* Which drafted tokens stand by sampling, from given random numbers: picks for
+ * b2a_tree_commit.  At a node, beginning with node 0, the weights of the next
+ * token are r = exp((x - max x) / T), x the node's logits row.  Its children are
+ * looked at in order; one with token v and number u is accepted if
+ *   u q(v) < r(v) / sum r
+ * (q its parent's row of draft, or 1 without draft); one that is not:  r(v) = 0,
+ * or with draft r = max(r / sum r - q, 0) and r(v) = 0.  An accepted child is the
+ * next node and its token the node's pick.  Where none is, the path ends and the
+ * pick is the lowest v with r(0) + .. + r(v) > draw * sum r.  The picks are then
+ * distributed as the model's own tokens, if without draft the drafts do not
+ * depend on the random numbers, and with draft each child was drawn
+ * independently from its parent's row.
+ *   logits     [n_rows][V] F32, F16 or BF16, rows row_stride apart; -inf and NaN
+ *              have weight 0
+ *   draft      f32 [n_rows][V] probabilities, draft_row_stride apart, or NULL
+ *   tokens     int32 [n_rows] the nodes' tokens; one outside [0, V) is passed over
+ *   uniforms   f32 [n_rows] in [0, 1): a node's own (node 0's is not used)
+ *   draws      f32 [B] in [0, 1)
+ *   temperature  f32 [B] or NULL (1).  Not above 0, or a largest logit of
+ *              +inf: the largest logit's lowest v has all the weight
+ * picks of nodes off the path, of padding rows and of requests left out (numbers
+ * out of bounds) are -1, and where a row has no weight at all.  Where a residual
+ * has none left (draft rows that do not sum to 1) the largest logit's v is
+ * taken.  Decisions: exponentials in 32 bits (relative error 2^-21), sums in 64;
+ * the draw and residuals in 64. */
+int b2a_verify_picks(const void* logits, long long row_stride, int dtype, const float* draft,
+                     long long draft_row_stride, const int* cu_dev, const int* parents_dev,
+                     const int* tokens_dev, const float* uniforms_dev, const float* draws_dev,
+                     const float* temperature_dev, int* picks_dev, int B, int n_rows, int max_nodes,
+                     int V, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
