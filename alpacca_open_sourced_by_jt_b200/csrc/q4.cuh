@@ -28,8 +28,8 @@ __host__ __device__ constexpr int granule_bytes(int D) { return 18 * D; }
 // Byte offsets inside a granule: the word of dims 8u .. 8u + 7 of row r, the
 // scale of block b.
 __device__ __forceinline__ int k_word(int D, int r, int u) {
-  const int nb = D >= 128 ? 4 : D / 32;
-  return (u >> 2) / nb * (256 * nb) + r * (16 * nb) + (u & 3) * (4 * nb) + (u >> 2) % nb * 4;
+  const int lg = D >= 128 ? 2 : 1, b = u >> 2;  // 4 or 2 blocks in a plane
+  return ((b >> lg) << (8 + lg)) + (r << (4 + lg)) + ((u & 3) << (2 + lg)) + (b & ((1 << lg) - 1)) * 4;
 }
 __device__ __forceinline__ int v_word(int D, int r, int u) { return 8 * D + u * 64 + r * 4; }
 __device__ __forceinline__ int k_scale(int D, int r, int b) { return 16 * D + (r * (D / 32) + b) * 2; }

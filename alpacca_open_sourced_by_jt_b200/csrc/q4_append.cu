@@ -9,11 +9,12 @@
 // values next to a border.  Products and sums are rounded one by one, as
 // paged.cu does.
 //
-// Bound by reading the projections and writing q and the pool.  A thread takes 8
-// consecutive dims of a head (one word of codes), D / 8 lanes a head; neox pairs
-// meet by shuffles.  kHeads heads of a thread are loaded before the first is
-// used, and before the position is known; the cosines and sines of a token serve
-// all of a thread's heads.
+// Bound by reading the projections and writing q and the pool, and nearly as much by
+// its instructions.  A thread takes eight pairs of a head, which it rotates by itself:
+// 16 consecutive dims, or for neox rows 8 and the 8 that are half the rotation further
+// on, so two words of codes; D / 16 lanes a head (with 8 dims a thread the sum, the
+// root and the addresses of a head weigh twice as much: 72 us for 8191 tokens, 32/8
+// heads x 128, bf16).  The cosines and sines of a token serve all of a thread's heads.
 
 #include "q4.cuh"
 
@@ -49,146 +50,179 @@ __device__ __forceinline__ __half block_scale(uint32_t key) {
   return __ushort_as_half((h & 0x7fff) ? h : 0);
 }
 __device__ __forceinline__ uint32_t code_of(float x, float d) {
-  if (d == 0.f) return 8u;
   const int c = __float2int_rd(__fadd_rn(__fdiv_rn(x, d), 8.5f));
-  return static_cast<uint32_t>(min(max(c, 0), 15));
+  return d == 0.f ? 8u : static_cast<uint32_t>(min(max(c, 0), 15));
+}
+// The word of 8 consecutive dims.
+__device__ __forceinline__ uint32_t codes8(const float* x, float d) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) w |= code_of(x[n], d) << ((n >> 1) * 4 + (n & 1) * 16);
+  return w;
+}
+__device__ __forceinline__ uint32_t largest8(const float* x) {
+  uint32_t k = 0;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) k = max(k, value_key(x[n]));
+  return k;
 }
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 3;  // heads of a thread with their loads in flight
+constexpr int kResident = 4;  // CTAs per SM of norm_append_kernel
 
-// Q4: the 4-bit pool; otherwise pools of TK.
-template <typename TS, typename TK, typename TQ, bool Q4>
-__global__ void __launch_bounds__(kThreads) norm_append_kernel(const __grid_constant__ AppendArgs a) {
+// 8 elements as loaded.
+template <typename TS>
+struct Raw {
+  uint4 w[sizeof(TS) / 2];
+  __device__ __forceinline__ void load(const TS* p) {
+    w[0] = reinterpret_cast<const uint4*>(p)[0];
+    if constexpr (sizeof(TS) == 4) w[1] = reinterpret_cast<const uint4*>(p)[1];
+  }
+  __device__ __forceinline__ void floats(float* x) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = ld_elem(reinterpret_cast<const TS*>(w) + e);
+  }
+};
+
+// Q4: the 4-bit pool; otherwise pools of TK.  A thread goes over the heads that it has
+// of a token and over tokens; while it works on a row the next one comes.
+template <typename TS, typename TK, typename TQ, bool Q4, bool kNeox>
+__global__ void __launch_bounds__(kThreads, kResident) norm_append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
-  const int D = a.D, L = D >> 3;  // a head's dims and lanes: 8, 16 or 32
-  const int u = threadIdx.x % L, at_once = blockDim.x / L;
-  const int lane = threadIdx.x & 31;
-  const int half = a.n_rot >> 1;
-  const int all = a.H + 2 * a.KV;
-  const int step = at_once * gridDim.y;
-  // the rotation of the thread's dims: norm style 4 pairs of its own, neox 8 dims
-  // whose partners are half further on or back
-  const bool turned = 8 * u < a.n_rot;
-  const bool low = 8 * u < half;
-  const int partner = a.neox && turned ? (low ? lane + half / 8 : lane - half / 8) : lane;
+  const int D = a.D, L = D >> 4;  // a head's dims and lanes: 4, 8 or 16
+  const int u = threadIdx.x & (L - 1);
+  const int half = a.n_rot >> 1, all = a.H + 2 * a.KV;
+  const bool turned = 16 * u < a.n_rot;  // the thread's pairs rotate
+  // the thread's dims: 8 from lo on and 8 from hi on (V rows: 16 from 16 u on)
+  const int lo = kNeox && turned ? 8 * u : 16 * u, hi = kNeox && turned ? half + 8 * u : 16 * u + 8;
+  const int h0 = (blockIdx.y * blockDim.x + threadIdx.x) / L, step = gridDim.y * blockDim.x / L;
+  // (the same for all lanes: a warp's lanes leave the loop over heads together)
+  const int warp_h0 = (blockIdx.y * blockDim.x + (threadIdx.x & ~31u)) / L;
+  auto fetch = [&](int i, int h, Raw<TS>* r) {
+    if (h >= all) return;
+    const TS* at;
+    if (h < a.H) at = static_cast<const TS*>(a.q) + i * a.q_stride + h * D;
+    else if (h < a.H + a.KV) at = static_cast<const TS*>(a.k) + i * a.k_stride + (h - a.H) * D;
+    else at = static_cast<const TS*>(a.v) + i * a.v_stride + (h - a.H - a.KV) * D;
+    const bool is_v = h >= a.H + a.KV;
+    r[0].load(at + (is_v ? 16 * u : lo));
+    r[1].load(at + (is_v ? 16 * u + 8 : hi));
+  };
+  Raw<TS> raw[2];
+  int p = -1, now = -1;
+  if (static_cast<int>(blockIdx.x) < a.n_tok) {
+    fetch(blockIdx.x, h0, raw);
+    p = a.pos[blockIdx.x];
+    now = a.slots[blockIdx.x];
+  }
   for (int i = blockIdx.x; i < a.n_tok; i += gridDim.x) {
+    const int next = i + gridDim.x;
+    const bool ok = p >= 0 && p < a.tab_rows && now < a.n_slots;
+    if (!ok && threadIdx.x == 0 && blockIdx.y == 0) set_dev_error(B2A_ERR_POSITION, i);
     float c[8], s[8];
-    int p = -1, in_page = 0;
-    long long page = 0;
-    bool stored = false, known = false, ok = true;
-    for (int hb = blockIdx.y * at_once; hb < all && ok; hb += kHeads * step) {
-      float x[kHeads][8];
+    if (ok && turned) {
+      const size_t row = static_cast<size_t>(p) * half + 8 * u;
+      paged::load8(a.cos_tab + row, c);
+      paged::load8(a.sin_tab + row, s);
+    }
+    const bool kept = now >= 0;
+    const long long page = (now >> a.page_shift) * a.page_stride;
+    const int in_page = now & ((1 << a.page_shift) - 1);
+    if (next < a.n_tok) {
+      p = a.pos[next];
+      now = a.slots[next];
+    }
+#pragma unroll 1
+    for (int h = h0, wh = warp_h0; wh < all; h += step, wh += step) {
+      float x[16];
+      raw[0].floats(x);
+      raw[1].floats(x + 8);
+      if (wh + step < all) fetch(i, h + step, raw);
+      else if (next < a.n_tok) fetch(next, h0, raw);
+      if (!ok) continue;
+      const bool none = h >= all, is_q = h < a.H, is_v = h >= a.H + a.KV;
+      const int hh = is_q ? h : (is_v ? h - a.H - a.KV : h - a.H);
+      const bool split = kNeox && turned && !is_v;
+      const int la = is_v ? 16 * u : lo, ha = is_v ? 16 * u + 8 : hi;
+      const float* bias = is_q ? a.bq : (is_v ? a.bv : a.bk);
+      if (bias && !none) {
+        float b[16];
+        paged::load8(bias + hh * D + la, b);
+        paged::load8(bias + hh * D + ha, b + 8);
 #pragma unroll
-      for (int e = 0; e < kHeads; ++e) {
-        const int h = hb + static_cast<int>(threadIdx.x) / L + e * step;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) x[e][d] = 0.f;
-        if (h >= all) continue;
-        const TS* src = h < a.H ? static_cast<const TS*>(a.q) + i * a.q_stride + h * D
-                      : h < a.H + a.KV ? static_cast<const TS*>(a.k) + i * a.k_stride + (h - a.H) * D
-                                       : static_cast<const TS*>(a.v) + i * a.v_stride + (h - a.H - a.KV) * D;
-        paged::load8(src + 8 * u, x[e]);
+        for (int d = 0; d < 16; ++d) x[d] = __fadd_rn(x[d], b[d]);
       }
-      if (!known) {
-        known = true;
-        p = a.pos[i];
-        const int slot = a.slots[i];
-        if (p < 0 || p >= a.tab_rows || slot >= a.n_slots) {
-          if (threadIdx.x == 0 && blockIdx.y == 0) set_dev_error(B2A_ERR_POSITION, i);
-          ok = false;
-          break;
+      const float* w = is_q ? a.wq : (is_v ? nullptr : a.wk);
+      if (__any_sync(0xffffffffu, w != nullptr)) {
+        double s0 = 0.0, s1 = 0.0;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          s0 = fma(static_cast<double>(x[d]), static_cast<double>(x[d]), s0);
+          s1 = fma(static_cast<double>(x[d + 8]), static_cast<double>(x[d + 8]), s1);
         }
-        stored = slot >= 0;
-        page = slot >> a.page_shift;
-        in_page = slot & ((1 << a.page_shift) - 1);
-        if (turned) {
-          const size_t row = static_cast<size_t>(p) * half;
-          if (a.neox) {
-            const int at = low ? 8 * u : 8 * u - half;
-            paged::load8(a.cos_tab + row + at, c);
-            paged::load8(a.sin_tab + row + at, s);
-          } else {
-            paged::load4(a.cos_tab + row + 4 * u, c);
-            paged::load4(a.sin_tab + row + 4 * u, s);
-          }
+        s0 += s1;
+        s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
+        s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
+        if (L > 4) s0 += __shfl_xor_sync(0xffffffffu, s0, 4);
+        if (L > 8) s0 += __shfl_xor_sync(0xffffffffu, s0, 8);
+        const float f = __frcp_rn(__fsqrt_rn(static_cast<float>(s0 * a.inv_d + static_cast<double>(a.eps))));
+        if (w != nullptr) {
+          float g[8];
+          paged::load8(w + lo, g);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) x[d] = __fmul_rn(__fmul_rn(x[d], f), g[d]);
+          paged::load8(w + hi, g);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) x[d + 8] = __fmul_rn(__fmul_rn(x[d + 8], f), g[d]);
         }
       }
+      if (turned && !is_v) {
 #pragma unroll
-      for (int e = 0; e < kHeads; ++e) {
-        const int h0 = hb + (static_cast<int>(threadIdx.x) - lane) / L + e * step;  // the warp's first head
-        if (h0 >= all) continue;
-        const int h = hb + static_cast<int>(threadIdx.x) / L + e * step;
-        const bool is_q = h < a.H, is_v = h >= a.H + a.KV;
-        const int hh = is_q ? h : (is_v ? h - a.H - a.KV : h - a.H);
-        const float* bias = is_q ? a.bq : (is_v ? a.bv : a.bk);
-        if (bias && h < all) {
-          float b[8];
-          paged::load8(bias + hh * D + 8 * u, b);
-#pragma unroll
-          for (int d = 0; d < 8; ++d) x[e][d] = __fadd_rn(x[e][d], b[d]);
+        for (int d = 0; d < 8; ++d) {
+          float& x0 = kNeox ? x[d] : x[2 * d];
+          float& x1 = kNeox ? x[d + 8] : x[2 * d + 1];
+          const float y0 = __fsub_rn(__fmul_rn(x0, c[d]), __fmul_rn(x1, s[d]));
+          x1 = __fadd_rn(__fmul_rn(x0, s[d]), __fmul_rn(x1, c[d]));
+          x0 = y0;
         }
-        const float* w = is_q ? a.wq : a.wk;
-        const bool normed = w != nullptr && !is_v;
-        if (__any_sync(0xffffffffu, normed)) {
-          double ss = 0.0;
-#pragma unroll
-          for (int d = 0; d < 8; ++d) ss = fma(static_cast<double>(x[e][d]), static_cast<double>(x[e][d]), ss);
-          for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          if (normed) {
-            const float mean = static_cast<float>(ss * a.inv_d + static_cast<double>(a.eps));
-            const float f = __frcp_rn(__fsqrt_rn(mean));
-            float g[8];
-            paged::load8(w + 8 * u, g);
-#pragma unroll
-            for (int d = 0; d < 8; ++d) x[e][d] = __fmul_rn(__fmul_rn(x[e][d], f), g[d]);
-          }
+      }
+      if (is_q) {
+        TQ* to = static_cast<TQ*>(a.q_out) + (static_cast<size_t>(i) * a.H + h) * D;
+        paged::store8(to + la, x);
+        paged::store8(to + ha, x + 8);
+      }
+      if (!kept) continue;
+      if constexpr (Q4) {
+        if (__all_sync(0xffffffffu, is_q || none)) continue;
+        // the largest of the block: 2 lanes hold 16 consecutive dims each; split, 4 lanes
+        // hold 8 each of two blocks
+        uint32_t ka = largest8(x), kb = largest8(x + 8);
+        if (!split) ka = kb = max(ka, kb);
+        ka = max(ka, __shfl_xor_sync(0xffffffffu, ka, 1));
+        kb = max(kb, __shfl_xor_sync(0xffffffffu, kb, 1));
+        const uint32_t oa = __shfl_xor_sync(0xffffffffu, ka, 2), ob = __shfl_xor_sync(0xffffffffu, kb, 2);
+        if (split) {
+          ka = max(ka, oa);
+          kb = max(kb, ob);
         }
-        if (a.neox) {
-          if (__any_sync(0xffffffffu, !is_v)) {
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-              const float other = __shfl_sync(0xffffffffu, x[e][d], partner);
-              if (turned && !is_v)
-                x[e][d] = low ? __fsub_rn(__fmul_rn(x[e][d], c[d]), __fmul_rn(other, s[d]))
-                              : __fadd_rn(__fmul_rn(other, s[d]), __fmul_rn(x[e][d], c[d]));
-            }
-          }
-        } else if (turned && !is_v) {
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const float x0 = x[e][2 * d], x1 = x[e][2 * d + 1];
-            x[e][2 * d] = __fsub_rn(__fmul_rn(x0, c[d]), __fmul_rn(x1, s[d]));
-            x[e][2 * d + 1] = __fadd_rn(__fmul_rn(x0, s[d]), __fmul_rn(x1, c[d]));
-          }
-        }
-        if (is_q)
-          paged::store8(static_cast<TQ*>(a.q_out) + (static_cast<size_t>(i) * a.H + h) * D + 8 * u, x[e]);
-        if constexpr (Q4) {
-          if (!stored || !__any_sync(0xffffffffu, !is_q && h < all)) continue;
-          uint32_t key = 0;
-#pragma unroll
-          for (int d = 0; d < 8; ++d) key = max(key, value_key(x[e][d]));
-          key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
-          key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
-          if (is_q || h >= all) continue;
-          const __half d16 = block_scale(key);
-          const float d = __half2float(d16);
-          uint32_t word = 0;
-#pragma unroll
-          for (int n = 0; n < 8; ++n) word |= code_of(x[e][n], d) << ((n >> 1) * 4 + (n & 1) * 16);
-          unsigned char* g = static_cast<unsigned char*>(a.k_pool) + page * a.page_stride +
-                             (static_cast<long long>(hh) * ((1 << a.page_shift) >> 4) + (in_page >> 4)) * granule_bytes(D);
-          const int r = in_page & 15;
-          *reinterpret_cast<uint32_t*>(g + (is_v ? v_word(D, r, u) : k_word(D, r, u))) = word;
-          if ((u & 3) == 0)
-            *reinterpret_cast<__half*>(g + (is_v ? v_scale(D, r, u >> 2) : k_scale(D, r, u >> 2))) = d16;
-        } else {
-          if (is_q || h >= all || !stored) continue;
-          TK* row = static_cast<TK*>(is_v ? a.v_pool : a.k_pool) + page * a.page_stride +
-                    (static_cast<long long>(in_page) * a.KV + hh) * D;
-          paged::store8(row + 8 * u, x[e]);
-        }
+        if (is_q || none) continue;
+        const __half da = block_scale(ka), db = block_scale(kb);
+        unsigned char* g = static_cast<unsigned char*>(a.k_pool) + page +
+                           (static_cast<long long>(hh) * ((1 << a.page_shift) >> 4) + (in_page >> 4)) * granule_bytes(D);
+        const int r = in_page & 15, ua = la >> 3, ub = ha >> 3;
+        *reinterpret_cast<uint32_t*>(g + (is_v ? v_word(D, r, ua) : k_word(D, r, ua))) = codes8(x, __half2float(da));
+        *reinterpret_cast<uint32_t*>(g + (is_v ? v_word(D, r, ub) : k_word(D, r, ub))) = codes8(x + 8, __half2float(db));
+        // (the lane with a block's first word writes its scale)
+        if ((ua & 3) == 0)
+          *reinterpret_cast<__half*>(g + (is_v ? v_scale(D, r, ua >> 2) : k_scale(D, r, ua >> 2))) = da;
+        if ((ub & 3) == 0)
+          *reinterpret_cast<__half*>(g + (is_v ? v_scale(D, r, ub >> 2) : k_scale(D, r, ub >> 2))) = db;
+      } else {
+        if (is_q || none) continue;
+        TK* row = static_cast<TK*>(is_v ? a.v_pool : a.k_pool) + page +
+                  (static_cast<long long>(in_page) * a.KV + hh) * D;
+        paged::store8(row + la, x);
+        paged::store8(row + ha, x + 8);
       }
     }
   }
@@ -322,9 +356,8 @@ int norm_append_check(const char* who, const Q4::AppendArgs& a, int in_dtype, in
   if (a.D != 64 && a.D != 128 && a.D != 256)
     return fail(B2A_ERR_UNSUPPORTED, "%s: head_dim %d (64/128/256)", who, a.D);
   if (style != B2A_ROPE_NORM && style != B2A_ROPE_NEOX) return fail(B2A_ERR_ARG, "%s: style %d", who, style);
-  if (a.n_rot < 0 || a.n_rot > a.D || a.n_rot % (style == B2A_ROPE_NEOX ? 16 : 8) != 0)
-    return fail(B2A_ERR_SHAPE, "%s: n_rot %d (a multiple of %d, at most D=%d)", who, a.n_rot,
-                style == B2A_ROPE_NEOX ? 16 : 8, a.D);
+  if (a.n_rot < 0 || a.n_rot > a.D || a.n_rot % 16 != 0)
+    return fail(B2A_ERR_SHAPE, "%s: n_rot %d (a multiple of 16, at most D=%d)", who, a.n_rot, a.D);
   const int es = b2a_host::elem_size(in_dtype), qs = b2a_host::elem_size(q_out_dtype);
   if (es == 0 || qs == 0) return fail(B2A_ERR_DTYPE, "%s: dtypes %d, %d", who, in_dtype, q_out_dtype);
   if (!power_of_two(page_rows))
@@ -343,17 +376,17 @@ int norm_append_check(const char* who, const Q4::AppendArgs& a, int in_dtype, in
 
 template <typename TS, typename TK, typename TQ, bool kQ4>
 cudaError_t norm_append_launch(const Q4::AppendArgs& a, cudaStream_t st) {
-  // as many threads as give each kHeads heads; few tokens: a token's heads over
-  // more CTAs, until there are a few per SM
-  const int all = a.H + 2 * a.KV, lanes = a.D / 8;
-  int threads = ((all + Q4::kHeads - 1) / Q4::kHeads * lanes + 31) / 32 * 32;
-  if (threads > Q4::kThreads) threads = Q4::kThreads;
-  int gy = (all + threads / lanes - 1) / (threads / lanes);
-  const int enough = (4 * b2a_host::sm_count() + a.n_tok - 1) / a.n_tok;
+  // A CTA per token, going over its heads; few tokens: a token's heads over more CTAs,
+  // until there are a few per SM.
+  const int all = a.H + 2 * a.KV, lanes = a.D / 16, at_once = Q4::kThreads / lanes;
+  int gy = (all + at_once - 1) / at_once;
+  const int enough = (Q4::kResident * b2a_host::sm_count() + a.n_tok - 1) / a.n_tok;
   if (gy > enough) gy = enough;
-  const int resident = 8 * b2a_host::sm_count();
-  return b2a_host::launch(Q4::norm_append_kernel<TS, TK, TQ, kQ4>,
-                          dim3(a.n_tok < resident ? a.n_tok : resident, gy), dim3(threads), 0, st, a);
+  const int resident = Q4::kResident * b2a_host::sm_count();
+  const dim3 grid(a.n_tok < resident ? a.n_tok : resident, gy);
+  const dim3 block(all <= at_once ? (all * lanes + 31) / 32 * 32 : Q4::kThreads);
+  if (a.neox) return b2a_host::launch(Q4::norm_append_kernel<TS, TK, TQ, kQ4, true>, grid, block, 0, st, a);
+  return b2a_host::launch(Q4::norm_append_kernel<TS, TK, TQ, kQ4, false>, grid, block, 0, st, a);
 }
 
 // A 4-bit pool's checks and its description.
@@ -368,7 +401,7 @@ int q4_pool_check(const char* who, const void* pool, int n_pages, int page_rows,
     return fail(B2A_ERR_SHAPE, "%s: page_rows %d must be a %s from 16 up", who, page_rows,
                 paged_cache ? "power of two" : "multiple of 16");
   const long long dense = static_cast<long long>(KV) * (page_rows / 16) * Q4::granule_bytes(D);
-  if (dense / KV > INT_MAX) return fail(B2A_ERR_UNSUPPORTED, "%s: page_rows %d", who, page_rows);
+  if (dense > INT_MAX) return fail(B2A_ERR_UNSUPPORTED, "%s: pages of %lld bytes", who, dense);
   if (page_bytes == 0) page_bytes = dense;
   if (page_bytes < dense)
     return fail(B2A_ERR_SHAPE, "%s: page_bytes %lld < %lld", who, page_bytes, dense);
@@ -431,6 +464,8 @@ int b2a_rope_append_q4(const void* q, long long q_tok_stride, const void* k, lon
   int rc = norm_append_check("rope_append_q4", a, in_dtype, q_out_dtype, n_pages, page_rows, style);
   if (rc == B2A_OK) rc = q4_pool_check("rope_append_q4", pool, n_pages, page_rows, page_bytes, KV, D, true);
   if (rc) return rc;
+  if (style == B2A_ROPE_NEOX && n_rot % 64 != 0)
+    return fail(B2A_ERR_SHAPE, "rope_append_q4: neox n_rot %d is not a multiple of 64", n_rot);
   if (q_out_dtype == B2A_F32) return fail(B2A_ERR_DTYPE, "rope_append_q4: q_out must be f16 or bf16");
   a.page_stride = page_bytes;
   if (n_tok == 0) return B2A_OK;

@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       if (in_ring == 0) bring();  // (its segment is the products', so it is there)
       if (!arrived(&sh.full[warp][stage], phase, 0x3F000 | warp)) return;
       const uint8_t* base = ring + stage * C::kStage;
-      const int row0 = st * kQ4Keys;
+      int row0 = st * kQ4Keys;
       const bool tail = row0 + kQ4Keys > it.len;
       const uint32_t no_page = (bad >> (2 * stage)) & 3u;
       if (tail && !have_anc) {
@@ -409,27 +409,26 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
         }
       }
 
-      // ---- scores ------------------------------------------------------------------
-      float s[2][NT][4];  // [granule][query row][key 4t + i]
-#pragma unroll
-      for (int gr = 0; gr < 2; ++gr) {
-        const uint8_t* gb = base + gr * C::kGranule;
+      // (a granule at a time: both at once need more registers than 14 warps have)
+#pragma unroll 1
+      for (int gr = 0; gr < 2; ++gr, base += C::kGranule, row0 += 16) {
+        // ---- scores ----------------------------------------------------------------
         uint32_t dk[NB * 2];  // [key][block] f16
 #pragma unroll
         for (int i = 0; i < NB / 2; ++i) {
-          const uint4 u = *reinterpret_cast<const uint4*>(gb + 16 * D + t * (8 * NB) + i * 16);
+          const uint4 u = *reinterpret_cast<const uint4*>(base + 16 * D + t * (8 * NB) + i * 16);
           dk[4 * i] = u.x; dk[4 * i + 1] = u.y; dk[4 * i + 2] = u.z; dk[4 * i + 3] = u.w;
         }
-        float2 sc[NT][2];
+        float2 s[NT][2];  // of keys 4t, 4t + 1 | 4t + 2, 4t + 3
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = make_float2(0.f, 0.f);
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = make_float2(0.f, 0.f);
         constexpr int NBP = NB < 4 ? NB : 4;
 #pragma unroll
         for (int pl = 0; pl < NB / NBP; ++pl) {
           uint32_t kw[2][NBP];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint8_t* at = gb + pl * (256 * NBP) + k_at + h * (32 * NBP);
+            const uint8_t* at = base + pl * (256 * NBP) + k_at + h * (32 * NBP);
             if constexpr (NBP == 4) {
               const uint4 u = *reinterpret_cast<const uint4*>(at);
               kw[h][0] = u.x; kw[h][1] = u.y; kw[h][2] = u.z; kw[h][3] = u.w;
@@ -454,36 +453,25 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
               const float2 d = make_float2(__half2float(hk[0]), __half2float(hk[NB]));
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                sc[nt][h] = fma2(d, make_float2(qc[b][nt], qc[b][nt]), sc[nt][h]);
-                sc[nt][h] = fma2(d, make_float2(acc[2 * nt], acc[2 * nt + 1]), sc[nt][h]);
-                if constexpr (NT == 1) sc[nt][h] = fma2(d, make_float2(odd[2], odd[3]), sc[nt][h]);
+                s[nt][h] = fma2(d, make_float2(qc[b][nt], qc[b][nt]), s[nt][h]);
+                s[nt][h] = fma2(d, make_float2(acc[2 * nt], acc[2 * nt + 1]), s[nt][h]);
+                if constexpr (NT == 1) s[nt][h] = fma2(d, make_float2(odd[2], odd[3]), s[nt][h]);
               }
             }
           }
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            s[gr][nt][2 * h] = sc[nt][h].x;
-            s[gr][nt][2 * h + 1] = sc[nt][h].y;
-          }
-      }
-      // ---- softmax ------------------------------------------------------------------
-      uint32_t dv[2][NB * 2];  // [granule][key][block] f16
-      __half2 top = __float2half2_rn(0.f);
-#pragma unroll
-      for (int gr = 0; gr < 2; ++gr) {
+        // ---- softmax ----------------------------------------------------------------
+        uint32_t dv[NB * 2];  // [key][block] f16
 #pragma unroll
         for (int i = 0; i < NB / 2; ++i) {
-          const uint4 u = *reinterpret_cast<const uint4*>(base + gr * C::kGranule + 17 * D + t * (8 * NB) + i * 16);
-          dv[gr][4 * i] = u.x; dv[gr][4 * i + 1] = u.y; dv[gr][4 * i + 2] = u.z; dv[gr][4 * i + 3] = u.w;
+          const uint4 u = *reinterpret_cast<const uint4*>(base + 17 * D + t * (8 * NB) + i * 16);
+          dv[4 * i] = u.x; dv[4 * i + 1] = u.y; dv[4 * i + 2] = u.z; dv[4 * i + 3] = u.w;
         }
         if (tail || no_page) {
           // keys that are not there, or that only some rows see, may hold anything
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int j = row0 + gr * 16 + 4 * t + i - it.len;
+            const int j = row0 + 4 * t + i - it.len;
             bool any = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -496,102 +484,92 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
                 see = (word >> (j & 31)) & 1u;
               }
               if ((no_page >> gr) & 1u) see = false;
-              if (!see) s[gr][nt][i] = -INFINITY;
+              float& x = i & 1 ? s[nt][i >> 1].y : s[nt][i >> 1].x;
+              if (!see) x = -INFINITY;
               any |= see;
             }
             if (!any)
 #pragma unroll
-              for (int b = 0; b < NB / 2; ++b) dv[gr][i * (NB / 2) + b] = 0u;
+              for (int b = 0; b < NB / 2; ++b) dv[i * (NB / 2) + b] = 0u;
           }
         }
+        __half2 top = __float2half2_rn(0.f);
 #pragma unroll
         for (int i = 0; i < NB * 2; ++i)
-          top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&dv[gr][i])));
-      }
-      // A power of two (its exponent) that is at least the largest |d_v| of the lane's
-      // keys: with whole exponents the weight of a row's only key is exact.
-      const uint32_t top_bits = *reinterpret_cast<const uint32_t*>(&top);
-      const uint32_t top16 = max(top_bits & 0x7fffu, top_bits >> 16 & 0x7fffu);
-      const float far = static_cast<float>(min(static_cast<int>(top16 >> 10), 30) - 14);
-      if (__any_sync(0xffffffffu, top16 > 0x7c00u)) {
-        // A NaN scale of a key that is seen: its block's outputs become NaN at the item's
-        // end; here it counts as zero.
-#pragma unroll
-        for (int gr = 0; gr < 2; ++gr)
+          top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&dv[i])));
+        // A power of two (its exponent) that is at least the largest |d_v| of the lane's
+        // keys: with whole exponents the weight of a row's only key is exact.
+        const uint32_t top_bits = *reinterpret_cast<const uint32_t*>(&top);
+        const uint32_t top16 = max(top_bits & 0x7fffu, top_bits >> 16 & 0x7fffu);
+        const float far = static_cast<float>(min(static_cast<int>(top16 >> 10), 30) - 14);
+        if (__any_sync(0xffffffffu, top16 > 0x7c00u)) {
+          // A NaN scale of a key that is seen: its block's outputs become NaN at the
+          // item's end; here it counts as zero.
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-              uint32_t& u = dv[gr][i * (NB / 2) + (b >> 1)];
+              uint32_t& u = dv[i * (NB / 2) + (b >> 1)];
               const uint32_t half = b & 1 ? u >> 16 : u & 0xffffu;
               if ((half & 0x7fffu) <= 0x7c00u) continue;
               u &= b & 1 ? 0x0000ffffu : 0xffff0000u;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                if (s[gr][nt][i] != -INFINITY) spoilt[nt] |= 1u << b;
+                if ((i & 1 ? s[nt][i >> 1].y : s[nt][i >> 1].x) != -INFINITY) spoilt[nt] |= 1u << b;
             }
-      }
-      bool grow = false;
-      float mx[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float x = s[0][nt][0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) x = fmaxf(x, s[i >> 2][nt][i & 3]);
-        x = fmaf(x, sscale[nt], far);
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        mx[nt] = x;
-        grow |= x > m[nt] + 8.f;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
+        }
+        bool grow = false;
+        float mx[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float now = fmaxf(m[nt], mx[nt]);
-          const float alpha = now == -INFINITY ? 0.f : fast_exp2(m[nt] - now);
-          m[nt] = now;
-          l[nt] *= alpha;
-          const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
-#pragma unroll
-          for (int i = 0; i < 2 * NB; ++i) {
-            o[i][nt][0] *= a0;
-            o[i][nt][1] *= a1;
-            o[i][nt][2] *= a0;
-            o[i][nt][3] *= a1;
-          }
-          ws[nt][0] *= a0;
-          ws[nt][1] *= a1;
+          float x = fmaxf(fmaxf(s[nt][0].x, s[nt][0].y), fmaxf(s[nt][1].x, s[nt][1].y));
+          x = fmaf(x, sscale[nt], far);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          mx[nt] = x;
+          grow |= x > m[nt] + 8.f;
         }
-      }
-      float2 p[2][NT][2];
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float mref = m[nt] == -INFINITY ? 0.f : m[nt];
+          for (int nt = 0; nt < NT; ++nt) {
+            const float now = fmaxf(m[nt], mx[nt]);
+            const float alpha = now == -INFINITY ? 0.f : fast_exp2(m[nt] - now);
+            m[nt] = now;
+            l[nt] *= alpha;
+            const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
 #pragma unroll
-        for (int gr = 0; gr < 2; ++gr) {
+            for (int i = 0; i < 2 * NB; ++i) {
+              o[i][nt][0] *= a0;
+              o[i][nt][1] *= a1;
+              o[i][nt][2] *= a0;
+              o[i][nt][3] *= a1;
+            }
+            ws[nt][0] *= a0;
+            ws[nt][1] *= a1;
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float mref = m[nt] == -INFINITY ? 0.f : m[nt];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 x = fma2(make_float2(s[gr][nt][2 * h], s[gr][nt][2 * h + 1]),
-                                  make_float2(sscale[nt], sscale[nt]), make_float2(-mref, -mref));
-            p[gr][nt][h] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            const float2 x = fma2(s[nt][h], make_float2(sscale[nt], sscale[nt]), make_float2(-mref, -mref));
+            s[nt][h] = make_float2(fast_exp2(x.x), fast_exp2(x.y));  // the weights, unscaled
           }
-          l[nt] += (p[gr][nt][0].x + p[gr][nt][0].y) + (p[gr][nt][1].x + p[gr][nt][1].y);
+          l[nt] += (s[nt][0].x + s[nt][0].y) + (s[nt][1].x + s[nt][1].y);
         }
-      }
-      // ---- output -------------------------------------------------------------------
-#pragma unroll
-      for (int gr = 0; gr < 2; ++gr) {
-        const uint8_t* vb = base + gr * C::kGranule + 8 * D + (g & 3) * 64 + t * 16;
+        // ---- output -----------------------------------------------------------------
+        const uint8_t* vb = base + 8 * D + (g & 3) * 64 + t * 16;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           uint32_t w[NT][2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const __half* hv = reinterpret_cast<const __half*>(dv[gr]) + 2 * h * NB + b;
+            const __half* hv = reinterpret_cast<const __half*>(dv) + 2 * h * NB + b;
             const float2 d = make_float2(__half2float(hv[0]), __half2float(hv[NB]));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const float2 x = mul2(p[gr][nt][h], d);
+              const float2 x = mul2(s[nt][h], d);
               w[nt][h] = MmaOp<__half>::pack(x.x, x.y);
             }
           }

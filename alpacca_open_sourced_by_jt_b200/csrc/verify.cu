@@ -24,8 +24,6 @@
 namespace b2a {
 namespace verify {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
 constexpr int kMaxNodes = B2A_TREE_MAX_NODES;
 
@@ -38,8 +36,27 @@ struct Args {
   const float *uniforms, *draws, *temperature;
   int* picks;
   int B, n_tok, max_nodes, V;
-  int slice, warp_slice;  // tokens of a CTA and of a warp of it
+  int all_nodes;  // a cluster per node (verify_path_kernel follows) rather than per request
+  int slice, warp_slice, warp_groups;  // tokens of a CTA, of a warp of it, that in groups of 128
 };
+
+// e^y for y <= 0 in 64 bits (relative error about 10^-13): y log2(e) = n + i / 16 + f
+// with |f| <= 1 / 32, a table of 2^(i / 16) and the series of 2^f up to f^5.
+constexpr int kTable = 16;
+__device__ __forceinline__ double exp_below(double y16, const double* table) {  // of y log2(e) x 16
+  if (!(y16 > -16.0 * 1000.0)) return 0.0;
+  constexpr double kRound = 6755399441055744.0;  // 1.5 x 2^52: the sum's low bits are the whole part
+  const double t = y16 + kRound;
+  const int n = __double2loint(t);
+  const double f = (y16 - (t - kRound)) * 0.043321698784996582;  // ln(2) / 16
+  double p = fma(f, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(f, p, 1.0 / 6.0);
+  p = fma(f, p, 0.5);
+  p = fma(f, p, 1.0);
+  p = fma(f, p, 1.0);
+  p *= table[n & (kTable - 1)];
+  return __hiloint2double(__double2hiint(p) + (n >> 4) * (1 << 20), __double2loint(p));
+}
 
 struct Exchange {
   double sum;
@@ -50,11 +67,16 @@ struct Exchange {
 template <typename T>
 __device__ __forceinline__ float at(const T* row, int v) { return ld_elem(row + v); }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ Args a) {
+// kDraft: drafts have a row.
+template <typename T, int kThreads, bool kDraft>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const __grid_constant__ Args a) {
   namespace cg = cooperative_groups;
+  constexpr int kWarps = kThreads / 32;
   cg::cluster_group cluster = cg::this_cluster();
-  extern __shared__ uint32_t gone[];  // bit v of the CTA's slice: rejected at this node
+  extern __shared__ __align__(16) double s_group[];  // sums of the warps' groups of 128 tokens
+  uint32_t* gone = reinterpret_cast<uint32_t*>(s_group + kWarps * a.warp_groups);  // bit v of the CTA's
+                                                                  // slice: rejected at this node
+  __shared__ double s_table[kTable];
   __shared__ Exchange s_ex[2];
   __shared__ double s_warp[kWarps];
   __shared__ float s_top[kWarps], s_part[kWarps];
@@ -62,14 +84,33 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
   __shared__ int s_par[kMaxNodes], s_tok[kMaxNodes], s_pick[kMaxNodes];
   __shared__ float s_u[kMaxNodes];
   __shared__ int s_rej[kMaxNodes];      // tokens rejected at this node
-  __shared__ double s_mass[kMaxNodes];  // sums of the residuals after each
+  __shared__ double s_mass[kMaxNodes], s_per[kMaxNodes];  // sums of the residuals after each, 1 / them
   pdl_wait();
   const int ranks = static_cast<int>(cluster.num_blocks());
-  const int rank = static_cast<int>(cluster.block_rank()), b = blockIdx.x / ranks;
+  const int rank = static_cast<int>(cluster.block_rank());
+  int b = blockIdx.x / ranks, first = 0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (a.all_nodes) {
+    // the request of node row b: the last that begins at or before it
+    const int node = b;
+    int lo = 0, hi = a.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.cu[mid] <= node) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    first = node - a.cu[b];
+    // padding, or numbers that are out of bounds (verify_path_kernel records them)
+    if (first < 0 || node >= a.cu[b + 1] || a.cu[b + 1] - a.cu[b] > a.max_nodes || a.cu[b] < 0 ||
+        a.cu[b + 1] > a.n_tok) {
+      if (rank == 0 && tid == 0) a.picks[node] = -1;
+      return;  // the whole cluster
+    }
+  }
   const int c0 = a.cu[b], c1 = a.cu[b + 1], n = c1 - c0;
   const bool bad = n < 0 || n > a.max_nodes || c0 < 0 || c1 > a.n_tok;
-  if (rank == 0) {
+  if (rank == 0 && !a.all_nodes) {
     // rows behind the last node, and of a request that is left out, have no pick
     const int last = max(a.cu[a.B], 0);
     for (int i = last + b * kThreads + tid; i < a.n_tok; i += a.B * kThreads) a.picks[i] = -1;
@@ -81,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
   if (bad || n == 0) return;  // the whole cluster
   for (int i = tid; i < n; i += kThreads) {
     const int p = a.parents ? a.parents[c0 + i] : i - 1;
-    if (rank == 0 && p != -1 && (p < 0 || p >= i)) set_dev_error(B2A_ERR_POSITION, b);
+    if (rank == 0 && first == 0 && p != -1 && (p < 0 || p >= i)) set_dev_error(B2A_ERR_POSITION, b);
     s_par[i] = p >= 0 && p < i ? p : -1;
     s_tok[i] = a.tokens[c0 + i];
     s_u[i] = a.uniforms[c0 + i];
@@ -89,10 +130,12 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
   }
   const int v0 = min(rank * a.slice, a.V), v1 = min(v0 + a.slice, a.V);
   for (int i = tid; i < (a.slice + 31) / 32; i += kThreads) gone[i] = 0u;
+  if (tid < kTable) s_table[tid] = exp2(tid * (1.0 / kTable));
   __syncthreads();
   const float heat = a.temperature ? a.temperature[b] : 1.f;
   const bool greedy = !(heat > 0.f);
   const double cold = greedy ? 0.0 : 1.0 / static_cast<double>(heat);
+  const double cold16 = fmin(cold * 1.4426950408889634 * kTable, 1e300);
   const float cold2 = static_cast<float>(fmin(cold * 1.4426950408889634, 1e30));
   int buf = 0;
 
@@ -100,16 +143,17 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
   auto exchange_sum = [&](double mine) {
     if (tid == 0) s_ex[buf].sum = mine;
     cluster.sync();
-    double sum = 0.0;
-    for (int r = 0; r < ranks; ++r) sum += cluster.map_shared_rank(&s_ex[buf], r)->sum;
+    double sum = lane < ranks ? cluster.map_shared_rank(&s_ex[buf], lane)->sum : 0.0;
+#pragma unroll
+    for (int o = kCluster / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     buf ^= 1;
-    return sum;
+    return __shfl_sync(0xffffffffu, sum, 0);
   };
 
-  int cur = 0;
+  int cur = first;
   while (true) {
     const T* row = static_cast<const T*>(a.logits) + (c0 + cur) * a.stride;
-    const float* qrow = a.draft ? a.draft + (c0 + cur) * a.draft_stride : nullptr;
+    const float* qrow = kDraft ? a.draft + (c0 + cur) * a.draft_stride : nullptr;
     // ---- the row's largest logit, its place, the sum of exponentials -----------------
     float top = -INFINITY, part = 0.f;
     int place = a.V;
@@ -128,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
         }
         if (top > -INFINITY) {
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) part += x[e] > -INFINITY ? fast_exp2((x[e] - top) * cold2) : 0.f;
+          for (int e = 0; e < kVec; ++e) part += fast_exp2((x[e] - top) * cold2);
         }
       };
       if (reinterpret_cast<uintptr_t>(row) % 16 == 0) {  // (slices are whole groups)
@@ -146,13 +190,14 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
             if (i >= groups) continue;
             float x[kVec];
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) x[e] = ld_elem(reinterpret_cast<const T*>(&u[k]) + e);
+            for (int e = 0; e < kVec; ++e)  // (a NaN has weight 0)
+              x[e] = fmaxf(ld_elem(reinterpret_cast<const T*>(&u[k]) + e), -INFINITY);
             take(x, v0 + i * kVec);
           }
         }
         for (int v = v0 + groups * kVec + tid; v < v1; v += kThreads) {
           float x[kVec];
-          x[0] = at(row, v);
+          x[0] = fmaxf(at(row, v), -INFINITY);
 #pragma unroll
           for (int e = 1; e < kVec; ++e) x[e] = -INFINITY;
           take(x, v);
@@ -161,7 +206,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
         for (int v = v0 + tid; v < v1; v += kThreads * kVec) {
           float x[kVec];
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) x[e] = v + e * kThreads < v1 ? at(row, v + e * kThreads) : -INFINITY;
+          for (int e = 0; e < kVec; ++e)
+            x[e] = v + e * kThreads < v1 ? fmaxf(at(row, v + e * kThreads), -INFINITY) : -INFINITY;
           float m = x[0];
 #pragma unroll
           for (int e = 1; e < kVec; ++e) m = fmaxf(m, x[e]);
@@ -174,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
           }
           if (top > -INFINITY) {
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) part += x[e] > -INFINITY ? fast_exp2((x[e] - top) * cold2) : 0.f;
+            for (int e = 0; e < kVec; ++e) part += fast_exp2((x[e] - top) * cold2);
           }
         }
       }
@@ -201,19 +247,33 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
       s_at[warp] = place;
     }
     __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < kWarps; ++w) join(s_top[w], s_part[w], s_at[w]);
-      s_ex[buf].top = top;
-      s_ex[buf].part = part;
-      s_ex[buf].at = place;
+    auto join_lanes = [&](int most) {  // of the first `most` lanes, a power of two
+      for (int o = most / 2; o > 0; o >>= 1) {
+        const float t2 = __shfl_xor_sync(0xffffffffu, top, o), p2 = __shfl_xor_sync(0xffffffffu, part, o);
+        join(t2, p2, __shfl_xor_sync(0xffffffffu, place, o));
+      }
+    };
+    if (warp == 0) {
+      top = lane < kWarps ? s_top[lane] : -INFINITY;
+      part = lane < kWarps ? s_part[lane] : 0.f;
+      place = lane < kWarps ? s_at[lane] : a.V;
+      join_lanes(32);
+      if (lane == 0) {
+        s_ex[buf].top = top;
+        s_ex[buf].part = part;
+        s_ex[buf].at = place;
+      }
     }
     cluster.sync();
-    top = -INFINITY;
-    part = 0.f;
-    place = a.V;
-    for (int r = 0; r < ranks; ++r) {
-      const Exchange* e = cluster.map_shared_rank(&s_ex[buf], r);
-      join(e->top, e->part, e->at);
+    {
+      const Exchange* e = cluster.map_shared_rank(&s_ex[buf], lane < ranks ? lane : 0);
+      top = lane < ranks ? e->top : -INFINITY;
+      part = lane < ranks ? e->part : 0.f;
+      place = lane < ranks ? e->at : a.V;
+      join_lanes(kCluster);
+      top = __shfl_sync(0xffffffffu, top, 0);
+      part = __shfl_sync(0xffffffffu, part, 0);
+      place = __shfl_sync(0xffffffffu, place, 0);
     }
     buf ^= 1;
     if (!(top > -INFINITY)) {  // nothing can be picked
@@ -226,43 +286,58 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     int rejected = 0, next = -1;
     double total = part;  // sum of r (certain drafts); drafts with a row: r is relative to it
     auto weight = [&](float x) {  // e^((x - M) / T)
-      return x > -INFINITY ? exp((static_cast<double>(x) - M) * cold) : 0.0;
+      return x > -INFINITY ? exp_below((static_cast<double>(x) - M) * cold16, s_table) : 0.0;
     };
     // r(v) after k rejections of drafts with a row, from e^((x - M) / T)
+    double per_total = 1.0 / total;
     auto residual = [&](double e, float q, int k) {
-      double r = e / total;
-      for (int i = 0; i < k; ++i) r = fmax((i ? r / s_mass[i - 1] : r) - static_cast<double>(q), 0.0);
+      double r = e * per_total;
+      for (int i = 0; i < k; ++i) r = fmax((i ? r * s_per[i - 1] : r) - static_cast<double>(q), 0.0);
       return r;
     };
-    // Sum over the row of what is left after k rejections (the rejected tokens
-    // themselves apart); the warps' shares stay in s_warp, the CTA's in s_ex
-    // (the other buffer, until the next exchange but one).
-    auto mass = [&](int k) {
-      double sum = 0.0;
-      const int lo = v0 + warp * a.warp_slice, hi = min(lo + a.warp_slice, v1);
-      for (int v = lo + lane; v < hi; v += 128) {
-        float x[4], q[4];
+    const bool whole = reinterpret_cast<uintptr_t>(row) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(qrow) % 16 == 0;  // (slices are whole groups)
+    // What is left of 4 consecutive tokens after k rejections (the rejected themselves
+    // apart).
+    auto left4 = [&](int v, int k, double* r) {
+      float x[4], q[4] = {0.f, 0.f, 0.f, 0.f};
+      if (whole && v + 4 <= v1) {
+        paged::load4(row + v, x);
+        if (kDraft && k) paged::load4(qrow + v, q);
+      } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int w = v + 32 * e;
-          x[e] = w < hi ? at(row, w) : -INFINITY;
-          q[e] = k && w < hi ? __ldg(qrow + w) : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int w = v + 32 * e - v0;
-          if (v + 32 * e >= hi || (gone[w >> 5] >> (w & 31) & 1u)) continue;
-          const double y = weight(x[e]);
-          sum += k ? residual(y, q[e], k) : y;
+          x[e] = v + e < v1 ? at(row, v + e) : -INFINITY;
+          if (kDraft && k && v + e < v1) q[e] = qrow[v + e];
         }
       }
+      const uint32_t marks = gone[(v - v0) >> 5] >> ((v - v0) & 31);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      __syncthreads();  // s_warp and the marks of rejected tokens
+      for (int e = 0; e < 4; ++e) {
+        const double y = weight(x[e]);
+        r[e] = (marks >> e & 1u) ? 0.0 : (kDraft && k ? residual(y, q[e], k) : y);
+      }
+    };
+    // The sum of it over the row; those of the warps' groups stay in s_group, the warps'
+    // in s_warp, the CTA's in s_ex (the other buffer).
+    auto mass = [&](int k) {
+      double sum = 0.0;
+      const int lo = v0 + warp * a.warp_slice;
+      for (int i = 0; i < a.warp_groups && lo + 128 * i < v1; ++i) {
+        double r[4];
+        left4(lo + 128 * i + 4 * lane, k, r);
+        double s = (r[0] + r[1]) + (r[2] + r[3]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) s_group[warp * a.warp_groups + i] = s;
+        sum += s;
+      }
+      __syncthreads();  // (s_warp has been read)
       if (lane == 0) s_warp[warp] = sum;
       __syncthreads();
-      double mine = 0.0;
-      for (int w = 0; w < kWarps; ++w) mine += s_warp[w];
+      double mine = lane < kWarps ? s_warp[lane] : 0.0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
       return exchange_sum(mine);
     };
     bool exact = false;  // total is the 64-bit sum of all weights
@@ -292,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
       again = __any_sync(0xffffffffu, again);
       const double u = s_u[c];
       const double e = weight(at(row, v));
-      if (!qrow) {
+      if constexpr (!kDraft) {
         if (again) continue;
         if (u * total < e) {
           next = c;
@@ -315,18 +390,26 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
       }
       ++rejected;
       __syncthreads();
-      if (qrow) {
+      if constexpr (kDraft) {
         if (!exact) {
           // (the weights' own sum counts the rejected token too)
           const double rest = mass(0);
           double lost = weight(at(row, s_rej[0]));
           total = rest + lost;
+          per_total = 1.0 / total;
           exact = true;
         }
         const double left = mass(rejected);
-        if (tid == 0) s_mass[rejected - 1] = left;
+        if (tid == 0) {
+          s_mass[rejected - 1] = left;
+          s_per[rejected - 1] = left > 0.0 ? 1.0 / left : 0.0;
+        }
         __syncthreads();
       }
+    }
+    if (next >= 0 && a.all_nodes) {
+      if (rank == 0 && tid == 0) a.picks[c0 + cur] = s_tok[next];
+      break;
     }
     if (next >= 0) {
       if (rank == 0 && tid == 0) s_pick[cur] = s_tok[next];
@@ -342,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     // ---- nothing drafted follows: the draw --------------------------------------------
     int drawn = place;  // the largest, -1 for nothing
     if (!sure) {
-      const int k = qrow ? rejected : 0;
+      const int k = kDraft ? rejected : 0;
       const double left = k ? s_mass[k - 1] : mass(0);
       const Exchange* ex = &s_ex[buf ^ 1];
       if (left > 0.0) {
@@ -371,43 +454,105 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
             wb += s_warp[w];
           }
           if (ww == warp) {
-            const int lo = v0 + warp * a.warp_slice, hi = min(lo + a.warp_slice, v1);
-            double run = ww_before;
-            int found = -1, last = -1;
-            for (int v = lo; v < hi && found < 0; v += 32) {
-              const int w = v + lane;
-              double r = 0.0;
-              if (w < hi && !(gone[(w - v0) >> 5] >> ((w - v0) & 31) & 1u)) {
-                r = weight(at(row, w));
-                if (k) r = residual(r, __ldg(qrow + w), k);
+            // the group of 128 tokens, then the token; of the last bits that sums
+            // in another order differ by, the last token with a weight makes up
+            const int lo = v0 + warp * a.warp_slice;
+            double run = ww_before, group_before = ww_before;
+            int group = 0;
+            bool passed = false;
+            for (int i = 0; i < a.warp_groups && lo + 128 * i < v1 && !passed; ++i) {
+              const double s = s_group[warp * a.warp_groups + i];
+              if (s > 0.0) {
+                group = i;
+                group_before = run;
+                passed = run + s > goal;
               }
-              double inc = r;
-#pragma unroll
-              for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
-              }
-              const unsigned pass = __ballot_sync(0xffffffffu, r > 0.0 && run + inc > goal);
-              const unsigned some = __ballot_sync(0xffffffffu, r > 0.0);
-              if (some) last = v + 31 - __clz(some);
-              if (pass) found = v + __ffs(pass) - 1;
-              run += __shfl_sync(0xffffffffu, inc, 31);
+              run += s;
             }
-            // (the sums above and this one differ in their last bits)
-            if (lane == 0) a.picks[c0 + cur] = found >= 0 ? found : last;
+            const int v = lo + 128 * group + 4 * lane;
+            double r[4];
+            left4(v, k, r);
+            double inc = (r[0] + r[1]) + (r[2] + r[3]);
+            const double mine = inc;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const double y = __shfl_up_sync(0xffffffffu, inc, o);
+              if (lane >= o) inc += y;
+            }
+            double cum = group_before + (inc - mine);
+            int found = -1, last = -1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              cum += r[e];
+              if (r[e] > 0.0) {
+                last = v + e;
+                if (found < 0 && cum > goal) found = v + e;
+              }
+            }
+            const unsigned pass = __ballot_sync(0xffffffffu, found >= 0);
+            const unsigned some = __ballot_sync(0xffffffffu, last >= 0);
+            const int pick = pass ? __shfl_sync(0xffffffffu, found, __ffs(pass) - 1)
+                                  : __shfl_sync(0xffffffffu, last, some ? 31 - __clz(some) : 0);
+            if (lane == 0) a.picks[c0 + cur] = pick;
           }
         }
       }
     }
     if (rank == 0) {
       __syncthreads();
-      for (int i = tid; i < n; i += kThreads)
-        if (i != cur) a.picks[c0 + i] = s_pick[i];
+      if (!a.all_nodes)
+        for (int i = tid; i < n; i += kThreads)
+          if (i != cur) a.picks[c0 + i] = s_pick[i];
       if (tid == 0 && drawn > -2) a.picks[c0 + cur] = drawn;
     }
     break;
   }
   cluster.sync();  // no CTA leaves while others read its shared memory
+}
+
+// Behind a cluster per node: the picks of nodes off the path become -1.  The child
+// that was accepted is the first whose token is the pick (a token that a sibling
+// had is never accepted again, and the draw leaves out the children's tokens).  A warp
+// per request.
+constexpr int kPathWarps = 4;
+__global__ void __launch_bounds__(kPathWarps * 32) verify_path_kernel(const __grid_constant__ Args a) {
+  pdl_wait();
+  const int b = blockIdx.x * kPathWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (b >= a.B) return;
+  const int c0 = a.cu[b], n = a.cu[b + 1] - c0;
+  if (n < 0 || n > a.max_nodes || c0 < 0 || c0 + n > a.n_tok) {
+    if (lane == 0) set_dev_error(B2A_ERR_POSITION, b);
+    return;
+  }
+  int par[kMaxNodes / 32], tok[kMaxNodes / 32], pick[kMaxNodes / 32];
+  bool on[kMaxNodes / 32];
+#pragma unroll
+  for (int w = 0; w < kMaxNodes / 32; ++w) {
+    const int j = w * 32 + lane;
+    par[w] = j < n ? (a.parents ? a.parents[c0 + j] : j - 1) : -2;
+    tok[w] = j < n ? a.tokens[c0 + j] : -1;
+    pick[w] = j < n ? a.picks[c0 + j] : -1;
+    on[w] = false;
+  }
+  int cur = n > 0 ? 0 : -1;
+  while (cur >= 0) {
+    int want = -1;
+#pragma unroll
+    for (int w = 0; w < kMaxNodes / 32; ++w) {
+      if (w == cur >> 5) want = __shfl_sync(0xffffffffu, pick[w], cur & 31);
+      if (w * 32 + lane == cur) on[w] = true;
+    }
+    int next = -1;
+#pragma unroll
+    for (int w = 0; w < kMaxNodes / 32; ++w) {
+      const unsigned hit = __ballot_sync(0xffffffffu, want >= 0 && par[w] == cur && w * 32 + lane > cur && tok[w] == want);
+      if (next < 0 && hit) next = w * 32 + __ffs(hit) - 1;
+    }
+    cur = next;
+  }
+#pragma unroll
+  for (int w = 0; w < kMaxNodes / 32; ++w)
+    if (w * 32 + lane < n && !on[w]) a.picks[c0 + w * 32 + lane] = -1;
 }
 
 }  // namespace verify
@@ -420,12 +565,17 @@ namespace {
 
 namespace VF = b2a::verify;
 
-template <typename T>
-cudaError_t verify_launch(const VF::Args& a, cudaStream_t st) {
+template <typename T, int kThreads>
+cudaError_t verify_launch(VF::Args a, cudaStream_t st) {
+  // whole groups of 128 tokens for each warp
+  constexpr int kWarps = kThreads / 32;
+  a.warp_groups = (a.V + VF::kCluster * kWarps * 128 - 1) / (VF::kCluster * kWarps * 128);
+  a.warp_slice = a.warp_groups * 128;
+  a.slice = a.warp_slice * kWarps;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.B * VF::kCluster);
-  cfg.blockDim = dim3(VF::kThreads);
-  cfg.dynamicSmemBytes = (a.slice + 31) / 32 * 4;
+  cfg.gridDim = dim3((a.all_nodes ? a.n_tok : a.B) * VF::kCluster);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kWarps * a.warp_groups * sizeof(double) + (a.slice + 31) / 32 * 4;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -436,7 +586,12 @@ cudaError_t verify_launch(const VF::Args& a, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (b2a_host::launch_flags() & B2A_LAUNCH_PDL) ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, VF::verify_kernel<T>, a);
+  cudaError_t e = a.draft ? cudaLaunchKernelEx(&cfg, VF::verify_kernel<T, kThreads, true>, a)
+                          : cudaLaunchKernelEx(&cfg, VF::verify_kernel<T, kThreads, false>, a);
+  if (e == cudaSuccess && a.all_nodes)
+    e = launch_second(VF::verify_path_kernel, dim3((a.B + VF::kPathWarps - 1) / VF::kPathWarps),
+                      dim3(VF::kPathWarps * 32), 0, st, a);
+  return e;
 }
 
 }  // namespace
@@ -459,18 +614,21 @@ int b2a_verify_picks(const void* logits, long long row_stride, int dtype, const 
   if (row_stride < V || (draft && draft_row_stride < V))
     return fail(B2A_ERR_SHAPE, "verify_picks: row strides %lld, %lld < V=%d", row_stride, draft_row_stride, V);
   if (V > 2000000) return fail(B2A_ERR_UNSUPPORTED, "verify_picks: V %d > 2000000", V);
-  if (B > INT_MAX / VF::kCluster) return fail(B2A_ERR_UNSUPPORTED, "verify_picks: %d requests", B);
+  if (B > INT_MAX / VF::kCluster || n_rows > INT_MAX / VF::kCluster) return fail(B2A_ERR_UNSUPPORTED, "verify_picks: %d requests", B);
   if (reinterpret_cast<uintptr_t>(logits) % es || reinterpret_cast<uintptr_t>(draft) % 4)
     return fail(B2A_ERR_ALIGN, "verify_picks: rows must be aligned to their elements");
   if (n_rows == 0) return B2A_OK;
   VF::Args a = {logits, row_stride, draft, draft_row_stride, cu_dev, parents_dev, tokens_dev, uniforms_dev,
-                draws_dev, temperature_dev, picks_dev, B, n_rows, max_nodes, V, 0, 0};
-  // whole 32-token groups for each warp
-  a.warp_slice = (V + VF::kCluster * VF::kWarps * 32 - 1) / (VF::kCluster * VF::kWarps * 32) * 32;
-  a.slice = a.warp_slice * VF::kWarps;
+                draws_dev, temperature_dev, picks_dev, B, n_rows, max_nodes, V, 0, 0, 0, 0};
+  // Few rows: a cluster for each, all at once, rather than node after node of a path.
+  a.all_nodes = n_rows > B && static_cast<long long>(n_rows) * VF::kCluster <= 4 * b2a_host::sm_count();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(dtype, [&](auto* t) {
-    return verify_launch<typename std::remove_pointer<decltype(t)>::type>(a, st);
+    using T = typename std::remove_pointer<decltype(t)>::type;
+    // Wider CTAs where all clusters are resident with them (2 of 512 threads an SM, 4 of
+    // 256): 24 requests with drafts' rows 141 us with 256 threads, 94 with 512.
+    const long long ctas = static_cast<long long>(a.all_nodes ? n_rows : B) * VF::kCluster;
+    return ctas <= 2 * b2a_host::sm_count() ? verify_launch<T, 512>(a, st) : verify_launch<T, 256>(a, st);
   });
   return e == cudaSuccess ? B2A_OK : b2a_host::cuda_fail(e, "verify_picks launch");
 }

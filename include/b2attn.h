@@ -680,8 +680,7 @@ int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* pare
  *   x = x (+ bias);  s = 1 / sqrt(f32(sum x^2 / D + eps)), the sum in 64 bits;
  *   x = (x * s) * w;  then the rotation
  *   wq, wk    f32 [D] the norms' weights, or NULL: no norm of q, of k
- * q_out is of kv_dtype.  D 64, 128 or 256; n_rot a multiple of 8 (norm style)
- * or 16 (neox); all rows, tables, weights and pools 16-byte aligned. */
+ * q_out is of kv_dtype.  D 64, 128 or 256; n_rot a multiple of 16; all rows, tables, weights and pools 16-byte aligned. */
 int b2a_norm_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
                                long long k_tok_stride, const void* v, long long v_tok_stride,
                                int in_dtype, const float* bq, const float* bk, const float* bv,
@@ -691,7 +690,8 @@ int b2a_norm_rope_append_paged(const void* q, long long q_tok_stride, const void
                                int page_rows, long long page_stride, int kv_dtype, void* q_out,
                                int n_tok, int H, int KV, int D, int n_rot, int style, void* stream);
 
-/* The same into a 4-bit pool; q_out is F16 or BF16. */
+/* The same into a 4-bit pool; q_out is F16 or BF16, n_rot of neox rows a multiple
+ * of 64 (a block of 32 values is then of one half of the rotation). */
 int b2a_rope_append_q4(const void* q, long long q_tok_stride, const void* k, long long k_tok_stride,
                        const void* v, long long v_tok_stride, int in_dtype, const float* bq,
                        const float* bk, const float* bv, const float* wq, const float* wk, float eps,
