@@ -58,6 +58,8 @@ struct Q4Seg {
 
 template <int W, int S>
 struct alignas(128) Q4Shared {  // (the rings stand behind it)
+  static constexpr int kTileSteps = 1;             // steps of a tile of the work division
+  static constexpr bool kItems = false;            // the items go by a queue of their own, too
   uint64_t full[W][S];                             // a warp's stages
   uint64_t seg_full[kQ4Queue], seg_empty[kQ4Queue];
   uint64_t handed, joined, read;                   // at an item's end
@@ -118,11 +120,12 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 }
 
 // The planning warp.  Requests are looked at 32 at a time, one by each lane.
-template <int W, int S>
-__device__ __forceinline__ void q4_plan(const Batch& bt, Q4Shared<W, S>& sh, int lane) {
+template <int W, typename Shared>
+__device__ __forceinline__ void q4_plan(const Batch& bt, Shared& sh, int lane) {
+  constexpr int TS = Shared::kTileSteps;
   const Start start = locate(bt, team_of(bt, blockIdx.x));
   long long off = start.off, left = start.left;
-  int b = start.b, base = -32, slot = 0;
+  int b = start.b, base = -32, slot = 0, items = 0;
   uint32_t round = 0;
   int n32 = 0, len32 = 0, node32 = 0;  // of request base + lane
   const bool split = bt.table && bt.page_shift == 4;
@@ -152,7 +155,7 @@ __device__ __forceinline__ void q4_plan(const Batch& bt, Q4Shared<W, S>& sh, int
     it.n = __shfl_sync(0xffffffffu, n32, b - base);
     it.len = __shfl_sync(0xffffffffu, len32, b - base);
     it.node0 = __shfl_sync(0xffffffffu, node32, b - base);
-    it.tiles = (it.len + it.n + kQ4Keys - 1) / kQ4Keys;
+    it.tiles = (it.len + it.n + TS * kQ4Keys - 1) / (TS * kQ4Keys);
     const long long u = units_of(bt, it.n, it.len);
     if (off >= u) {
       off -= u;
@@ -172,19 +175,31 @@ __device__ __forceinline__ void q4_plan(const Batch& bt, Q4Shared<W, S>& sh, int
     left -= take;
     if (!member_item(bt, blockIdx.x, idx, blocks_of(bt, it.n), it.kvh, it.blk)) continue;
     const int rows = it.len + it.n;
-    for (int t0 = it.t0; t0 < it.t1; t0 += kQ4Rounds * W) {
+    if constexpr (Shared::kItems) {
+      const int place = items % kQ4Queue;
+      if (items >= kQ4Queue && !__all_sync(0xffffffffu, mbar_wait(&sh.item_empty[place], (items / kQ4Queue - 1) & 1, 0x3F210)))
+        return;
+      if (lane == 0) {
+        sh.item[place] = it;
+        sh.item_end[place] = 0;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.item_full[place]);
+      ++items;
+    }
+    for (int t0 = it.t0 * TS; t0 < it.t1 * TS; t0 += kQ4Rounds * W) {
       if (!room()) return;
       Q4Seg<W>& seg = sh.seg[slot];
-      const int t1 = min(t0 + kQ4Rounds * W, it.t1);
+      const int t1 = min(t0 + kQ4Rounds * W, it.t1 * TS);
       bool gone = false;
 #pragma unroll 4
       for (int i = lane; i < t1 - t0; i += 32) {
         const int row = (t0 + i) * kQ4Keys;
-        const bool two = row + 16 < rows;
-        const int e0 = table_entry(bt, it.b, row);
+        const bool one = row < rows, two = row + 16 < rows;  // (a tile's last steps may hold nothing)
+        const int e0 = one ? table_entry(bt, it.b, row) : 0;
         const int e1 = split && two ? table_entry(bt, it.b, row + 16) : e0;
         const int p0 = checked_page(bt, it.b, e0), p1 = checked_page(bt, it.b, e1);
-        seg.pages[0][i] = p0 < bt.n_pages ? p0 : -1;
+        seg.pages[0][i] = one && p0 < bt.n_pages ? p0 : -1;
         seg.pages[1][i] = two && p1 < bt.n_pages ? p1 : -1;
         gone |= p0 >= bt.n_pages || p1 >= bt.n_pages;
       }
@@ -193,12 +208,20 @@ __device__ __forceinline__ void q4_plan(const Batch& bt, Q4Shared<W, S>& sh, int
         seg.it = it;
         seg.t0 = t0;
         seg.t1 = t1;
-        seg.last = t1 == it.t1;
+        seg.last = t1 == it.t1 * TS;
         seg.end = 0;
         seg.gone = gone;
       }
       hand_on();
     }
+  }
+  if constexpr (Shared::kItems) {
+    const int place = items % kQ4Queue;
+    if (items >= kQ4Queue && !__all_sync(0xffffffffu, mbar_wait(&sh.item_empty[place], (items / kQ4Queue - 1) & 1, 0x3F210)))
+      return;
+    if (lane == 0) sh.item_end[place] = start.left_out ? 2 : 1;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.item_full[place]);
   }
   if (!room()) return;
   if (lane == 0) sh.seg[slot].end = start.left_out ? 2 : 1;
@@ -231,7 +254,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == W) {
-    q4_plan(bt, sh, lane);
+    q4_plan<W>(bt, sh, lane);
     return;
   }
   const int g = lane >> 2, t = lane & 3;
@@ -732,132 +755,3 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
 
 }  // namespace tree
 }  // namespace b2a
-
-// ===========================================================================
-// Host side
-// ===========================================================================
-namespace {
-
-// Query rows of an item.
-int tree_q4_rows(int rows, int D) { return rows <= 8 || D > 128 ? 8 : 16; }
-
-template <typename T, int D, int NT>
-int tree_q4_launch(const TreeArgs& a, const Q4::Pool& pool) {
-  auto kern = TR::tree_q4_kernel<T, D, NT>;
-  using C = TR::Q4Cfg<D, NT>;
-  static std::atomic<unsigned long long> done{0};
-  cudaError_t e = allow_smem(kern, C::kSmem, done);
-  if (e != cudaSuccess) return b2a_host::cuda_fail(e, "cudaFuncSetAttribute(tree_decode_q4)");
-  e = b2a_host::launch(kern, dim3(a.grid), dim3(C::kThreads), C::kSmem, a.st, a.bt, pool,
-                       static_cast<const T*>(a.q), a.q_stride, static_cast<T*>(a.out), a.lse, a.part_o,
-                       a.part_ml, a.sscale);
-  if (e != cudaSuccess) return b2a_host::cuda_fail(e, "tree_decode_q4 launch");
-  return tree_merge<T, D>(a);
-}
-
-template <typename T, int D>
-int tree_q4_dispatch(const TreeArgs& a, const Q4::Pool& pool) {
-  if constexpr (D <= 128) {
-    if (a.bt.rows_per_block == 16) return tree_q4_launch<T, D, 2>(a, pool);
-  }
-  return tree_q4_launch<T, D, 1>(a, pool);
-}
-
-template <typename T>
-int tree_q4_type(const TreeArgs& a, const Q4::Pool& pool) {
-  if (a.D == 64) return tree_q4_dispatch<T, 64>(a, pool);
-  if (a.D == 128) return tree_q4_dispatch<T, 128>(a, pool);
-  return tree_q4_dispatch<T, 256>(a, pool);
-}
-
-}  // namespace
-
-extern "C" {
-
-size_t b2a_tree_decode_q4_workspace_bytes(int max_nodes, int H, int KV, int D, int max_len) {
-  if (max_nodes <= 0 || H <= 0 || KV <= 0 || D <= 0 || H % KV != 0) return 0;
-  if (tree_always_whole(max_len)) return 0;
-  const int rb = tree_q4_rows(max_nodes * (H / KV), D);
-  return tree_part_o_bytes(D, KV, rb) + static_cast<size_t>(2) * tree_ctas(KV) * rb * 2 * sizeof(float);
-}
-
-int b2a_tree_decode_q4(const void* q, long long q_tok_stride, const void* pool, int n_pages,
-                       int page_rows, long long page_bytes, const int* table_dev,
-                       long long table_stride, int table_width, const int* lens_dev,
-                       const int* cu_dev, const int* parents_dev, void* out, float* lse_out,
-                       void* workspace, size_t workspace_bytes, int B, int n_tok, int max_nodes, int H,
-                       int KV, int D, int dtype, float scale, int max_len, void* stream) {
-  if (!q || !lens_dev || !cu_dev || !out) return fail(B2A_ERR_ARG, "tree_decode_q4: null pointer argument");
-  if (B <= 0 || n_tok < 0 || H <= 0 || max_len <= 0)
-    return fail(B2A_ERR_ARG, "tree_decode_q4: sizes must be positive (B=%d n_tok=%d H=%d max_len=%d)", B, n_tok, H, max_len);
-  if (max_nodes <= 0 || max_nodes > B2A_TREE_MAX_NODES)
-    return fail(B2A_ERR_ARG, "tree_decode_q4: max_nodes %d (1..%d)", max_nodes, B2A_TREE_MAX_NODES);
-  const int rc = q4_pool_check("tree_decode_q4", pool, n_pages, page_rows, page_bytes, KV, D, table_dev != nullptr);
-  if (rc) return rc;
-  if (H % KV != 0) return fail(B2A_ERR_SHAPE, "tree_decode_q4: H=%d is not a multiple of KV=%d", H, KV);
-  if (dtype != B2A_F16 && dtype != B2A_BF16) return fail(B2A_ERR_DTYPE, "tree_decode_q4: dtype %d", dtype);
-  if (!(scale > 0.f) || !isfinite(scale)) return fail(B2A_ERR_ARG, "tree_decode_q4: scale must be positive");
-  if (table_dev) {
-    if (table_width <= 0 || table_stride < table_width ||
-        static_cast<long long>(table_width) * page_rows < max_len)
-      return fail(B2A_ERR_SHAPE, "tree_decode_q4: a table row of %d pages (stride %lld) does not hold max_len %d rows",
-                  table_width, table_stride, max_len);
-  } else if (n_pages < B || page_rows < max_len) {
-    return fail(B2A_ERR_SHAPE, "tree_decode_q4: %d blocks of %d rows for %d sequences of up to %d",
-                n_pages, page_rows, B, max_len);
-  }
-  if (q_tok_stride == 0) q_tok_stride = static_cast<long long>(H) * D;
-  if (q_tok_stride < static_cast<long long>(H) * D)
-    return fail(B2A_ERR_SHAPE, "tree_decode_q4: q_tok_stride %lld < H*D", q_tok_stride);
-  if (!b2a_host::aligned16(q) || !b2a_host::aligned16(out) || !b2a_host::aligned16(workspace) ||
-      (q_tok_stride * 2) % 16 != 0)
-    return fail(B2A_ERR_ALIGN, "tree_decode_q4: q, its stride, out and workspace must be 16-byte aligned");
-  if (n_tok == 0) return B2A_OK;
-  const int group = H / KV;
-  if (group > 128) return fail(B2A_ERR_UNSUPPORTED, "tree_decode_q4: group %d", group);
-
-  TreeArgs a = {};
-  const int rows = max_nodes * group;
-  const int rb = tree_q4_rows(rows, D);
-  a.bt = TR::Batch{lens_dev, cu_dev, parents_dev, table_dev, table_stride, B, n_tok, max_nodes, max_len,
-                   n_pages, table_dev ? log2_of(page_rows) : 0, H, KV, group, rb, TR::kQ4Keys, 0, 1, 1, 1, 1};
-  // Side by side in a team: the KV heads, or, where a request has several blocks of
-  // query rows, those (b2a_tree_decode's rule)
-  const long long avg_rows = static_cast<long long>(n_tok) * group / B;
-  long long blks = (avg_rows + rb / 2) / rb;
-  const int most = max_rows_blocks(rows, rb);
-  if (blks > most || 4 * blks >= 3 * most) blks = most;
-  if (blks > kTreeBlocks) blks = (blks + (blks + kTreeBlocks - 1) / kTreeBlocks - 1) / ((blks + kTreeBlocks - 1) / kTreeBlocks);
-  a.bt.m_blks = blks > 1 ? static_cast<int>(blks) : 1;
-  a.bt.m_heads = a.bt.m_blks > 1 ? 1 : KV;
-  const int members = a.bt.m_heads * a.bt.m_blks;
-  const long long max_tiles = (max_len + TR::kQ4Keys - 1) / TR::kQ4Keys;
-  const long long items = static_cast<long long>(B) * (KV / a.bt.m_heads) * ((most + a.bt.m_blks - 1) / a.bt.m_blks);
-  a.bt.by_item = tree_by_item(max_len, B, KV) ? 1 : 0;
-  a.bt.min_units = a.bt.by_item ? 1 : 8;
-  const long long units = (items * (a.bt.by_item ? 1 : max_tiles) + a.bt.min_units - 1) / a.bt.min_units;
-  const int teams = b2a_host::sm_count() > members ? b2a_host::sm_count() / members : 1;
-  a.bt.teams = static_cast<int>(units < teams ? units : teams);
-  a.grid = a.bt.teams * members;
-  a.merge = !a.bt.by_item;
-  if (a.merge) {
-    const size_t need = b2a_tree_decode_q4_workspace_bytes(max_nodes, H, KV, D, max_len);
-    if (!workspace || workspace_bytes < need)
-      return fail(B2A_ERR_WORKSPACE, "tree_decode_q4: workspace %zu bytes < %zu needed", workspace_bytes, need);
-  }
-  a.q = q;
-  a.q_stride = q_tok_stride;
-  a.out = out;
-  a.lse = lse_out;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + tree_part_o_bytes(D, KV, rb)) : nullptr;
-  a.D = D;
-  a.dtype = dtype;
-  a.sscale = scale * TR::kLog2e;
-  a.st = static_cast<cudaStream_t>(stream);
-  const Q4::Pool p = q4_pool_of(pool, n_pages, page_rows, page_bytes, D, table_dev != nullptr);
-  if (dtype == B2A_BF16) return tree_q4_type<__nv_bfloat16>(a, p);
-  return tree_q4_type<__half>(a, p);
-}
-
-}  // extern "C"
