@@ -53,6 +53,7 @@ struct Q4Seg {
   int last;      // the item ends with it
   int end;       // nothing follows (1, with requests left out 2)
   int gone;      // some granule has no page
+  int g0;        // number of step t0 among all of the CTA's
   int pages[2][kQ4Rounds * W];  // of a step's two granules, -1: none
 };
 
@@ -125,7 +126,7 @@ __device__ __forceinline__ void q4_plan(const Batch& bt, Shared& sh, int lane) {
   constexpr int TS = Shared::kTileSteps;
   const Start start = locate(bt, team_of(bt, blockIdx.x));
   long long off = start.off, left = start.left;
-  int b = start.b, base = -32, slot = 0, items = 0;
+  int b = start.b, base = -32, slot = 0, items = 0, steps = 0;
   uint32_t round = 0;
   int n32 = 0, len32 = 0, node32 = 0;  // of request base + lane
   const bool split = bt.table && bt.page_shift == 4;
@@ -211,7 +212,9 @@ __device__ __forceinline__ void q4_plan(const Batch& bt, Shared& sh, int lane) {
         seg.last = t1 == it.t1 * TS;
         seg.end = 0;
         seg.gone = gone;
+        seg.g0 = steps;
       }
+      steps += t1 - t0;
       hand_on();
     }
   }

@@ -10,9 +10,9 @@
 // are those of the cache's own values; q is scaled by a power of two to f16 as in
 // tree_q4.cu, the weights are rounded to f16.
 //
-// 512 threads: warps 0-7 softmax (two warpgroups, tiles in turn, an S buffer each),
-// 8-13 converters (each brings its own steps, as tree_q4_kernel's warps do), 14 plans,
-// 15 owns TMEM and issues the MMAs.
+// 576 threads: warps 0-7 softmax (two warpgroups, tiles in turn, an S buffer each),
+// 8-15 converters (each brings its own steps, as tree_q4_kernel's warps do), 16 plans,
+// 17 owns TMEM and issues the MMAs.
 // TMEM: S0, S1 (128 columns each), O (D), Q (D / 2).
 
 #include <limits.h>
@@ -24,9 +24,10 @@
 namespace b2a {
 namespace tree {
 
-constexpr int kQWThreads = 512;
 constexpr int kQWGroups = 2;     // softmax warpgroups
-constexpr int kQWConvert = 6;    // converting warps
+constexpr int kQWConvert = 8;    // converting warps
+constexpr int kQWPlan = 8 + kQWConvert, kQWIssue = kQWPlan + 1;  // the planning and the issuing warp
+constexpr int kQWThreads = (kQWIssue + 1) * 32;
 constexpr int kQWKeys = 128;     // keys per tile
 constexpr int kQWSlots = 2;      // K tiles, and V tiles, in shared memory
 
@@ -41,7 +42,7 @@ struct alignas(128) QWShared {
   uint64_t q_full, last;                               // an item's Q, its last PV
   uint64_t s_full[kQWGroups], p_full[kQWGroups], pv[2], bar_m[kQWGroups][4];
   uint32_t tmem;
-  int special[4];  // an item's tree rows held NaN (converters are at most 3 items ahead)
+  int special[8];  // an item's tree rows held NaN (converters are less than 8 items ahead)
   int item_end[kQ4Queue];
   Item item[kQ4Queue];
   Q4Seg<kQWConvert> seg[kQ4Queue];
@@ -61,6 +62,9 @@ struct QWCfg {
   static constexpr int kSmem = kTiles + kQWConvert * kStages * kStage + static_cast<int>(sizeof(Shared));
   static_assert(kStages >= 2 && kSmem <= 227 * 1024, "ring");
   static_assert(kQ4Rounds * kQWConvert % Shared::kTileSteps == 0, "segments hold whole tiles");
+  // A converter takes every kQWConvert-th of all steps, so at least one of the tiles in
+  // the slots: further apart, it could not tell the phase of a slot by its parity.
+  static_assert(kQWConvert <= kQWSlots * Shared::kTileSteps, "converters");
 };
 
 // Does a tree row j in [lo, hi) that the node sees have a NaN scale in V's block?
@@ -111,12 +115,12 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 15) {
+  if (warp == kQWIssue) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&sh.tmem)),
                  "r"(prefill::kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  } else if (warp == 14 && lane == 0) {
+  } else if (warp == kQWPlan && lane == 0) {
     for (int w = 0; w < W; ++w)
       for (int s = 0; s < C::kStages; ++s) mbar_init(&sh.full[w][s], 1);
     for (int i = 0; i < kQ4Queue; ++i) {
@@ -141,7 +145,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     mbar_init(&sh.pv[0], 1);
     mbar_init(&sh.pv[1], 1);
     fence_mbar_init();
-    for (int i = 0; i < 4; ++i) sh.special[i] = 0;
+    for (int i = 0; i < 8; ++i) sh.special[i] = 0;
   }
   tc_fence_before();
   __syncthreads();
@@ -153,10 +157,10 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, where)) != 0;
   };
 
-  if (warp == 14) {
+  if (warp == kQWPlan) {
     // ------------------------------ the plan --------------------------------
     q4_plan<W>(bt, sh, lane);
-  } else if (warp == 15) {
+  } else if (warp == kQWIssue) {
     // ------------------------------ MMA issuer -----------------------------
     // (the whole warp walks, one elected lane issues: tree_wide.cu says why)
     constexpr uint32_t idesc_qk = make_idesc<__half>(128, BN, false, false);
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
         const Q4Seg<W>& seg = sh.seg[f_seg % kQ4Queue];
         f_end = seg.end != 0;
         if (f_end) return;
-        f_step = seg.t0 + cw;
+        f_step = seg.t0 + (cw + W - seg.g0 % W) % W;
         f_t1 = seg.t1;
         ++f_seg;
       }
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       if (++f_stage == C::kStages) f_stage = 0;
     };
     uint32_t stage = 0, phase = 0;
-    uint32_t before = 0, f_items = 0;  // tiles of the items before this one, their number
+    uint32_t f_items = 0;  // items done
     bool ok = true;
     for (uint32_t c_seg = 0; ok; ++c_seg) {
       if (!arrived(&sh.seg_full[c_seg % kQ4Queue], (c_seg / kQ4Queue) & 1, 0x3F870)) break;
@@ -284,10 +288,9 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       }
       const int rows = seg.it.len + seg.it.n, len = seg.it.len;
       const bool tree = seg.it.n > 1;
-      const int first = seg.it.t0 * TS;  // the item's first step
-      for (int st = seg.t0 + cw; st < seg.t1; st += W) {
+      for (int st = seg.t0 + (cw + W - seg.g0 % W) % W; st < seg.t1; st += W) {
         if (in_ring == 0) bring();
-        const uint32_t tile = before + (st - first) / TS;
+        const uint32_t tile = (seg.g0 + st - seg.t0) / TS;
         const uint32_t slot = tile % kQWSlots, round = tile / kQWSlots;
         const int gone = (seg.pages[0][st - seg.t0] < 0 ? 1 : 0) | (seg.pages[1][st - seg.t0] < 0 ? 2 : 0);
         if (!arrived(&sh.full[cw][stage], phase, 0x3F880)) {
@@ -310,11 +313,11 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
             // a NaN that some rows do not see: taken out here, put back at the item's end
             if ((dv[i] & 0x7fffu) > 0x7c00u) {
               dv[i] &= 0xffff0000u;
-              sh.special[f_items & 3] = 1;
+              sh.special[f_items & 7] = 1;
             }
             if ((dv[i] & 0x7fff0000u) > 0x7c000000u) {
               dv[i] &= 0x0000ffffu;
-              sh.special[f_items & 3] = 1;
+              sh.special[f_items & 7] = 1;
             }
           }
         }
@@ -385,10 +388,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
         }
       }
       if (!ok) break;
-      if (seg.last) {
-        before += seg.it.t1 - seg.it.t0;
-        ++f_items;
-      }
+      f_items += seg.last;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.seg_empty[c_seg % kQ4Queue]);
     }
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       meet();
       const float L = sh.x[0][r] + sh.x[1][r];
       wait(&sh.last, items & 1, 0x3F8F0);
-      const uint32_t which = items & 3;
+      const uint32_t which = items & 7;
       ++items;
       tc_fence_after();
       const bool special = sh.special[which] != 0;  // (all of the item's tiles are converted)
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
   // ------------------------------ teardown -----------------------------------
   tc_fence_before();
   __syncthreads();
-  if (warp == 15) {
+  if (warp == kQWIssue) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(prefill::kTmemCols));
