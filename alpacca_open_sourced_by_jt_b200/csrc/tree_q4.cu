@@ -64,6 +64,7 @@ struct alignas(128) Q4Shared {  // (the rings stand behind it)
   uint64_t full[W][S];                             // a warp's stages
   uint64_t seg_full[kQ4Queue], seg_empty[kQ4Queue];
   uint64_t handed, joined, read;                   // at an item's end
+  uint4 sees[W][16];                               // the nodes that a warp's rows see
   Q4Seg<W> seg[kQ4Queue];
 };
 
@@ -72,10 +73,10 @@ struct Q4Cfg {
   static constexpr int NB = D / 32;
   static constexpr int kGranule = q4::granule_bytes(D);
   static constexpr int kStage = 2 * kGranule;
-  static constexpr int kWarps = NT == 1 && D <= 128 ? 14 : 8;
+  static constexpr int kWarps = NT == 1 && D <= 128 ? 15 : 7;
   static constexpr int RB = 8 * NT;
   static constexpr int kPad = D + 4;
-  static constexpr int kMerge = kWarps / 2 * RB * (kPad + 2) * 4;  // half the warps' rows, maxima and sums
+  static constexpr int kMerge = (kWarps + 1) / 2 * RB * (kPad + 2) * 4;  // half the warps' rows, maxima and sums
   static constexpr int kFit = (227 * 1024 - static_cast<int>(sizeof(Q4Shared<kWarps, 6>)) - kMerge) / (kWarps * kStage);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   using Shared = Q4Shared<kWarps, kStages>;
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
     long long q_stride, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o,
     float* __restrict__ part_ml, float scale_log2) {
   using C = Q4Cfg<D, NT>;
-  constexpr int NB = C::NB, W = C::kWarps, RB = C::RB;
+  constexpr int NB = C::NB, W = C::kWarps, RB = C::RB, H = (W + 1) / 2;  // H: the lower half of the warps
   extern __shared__ __align__(128) uint8_t q4_smem[];
   typename C::Shared& sh = *reinterpret_cast<typename C::Shared*>(q4_smem);
   pdl_wait();
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       mbar_init(&sh.seg_empty[i], W);
     }
     mbar_init(&sh.handed, W / 2);
-    mbar_init(&sh.joined, W / 2);
+    mbar_init(&sh.joined, (W + 1) / 2);
     mbar_init(&sh.read, W);
   }
   fence_mbar_init();
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = q4_smem + sizeof(typename C::Shared) + warp * C::kStages * C::kStage;
   float* merge = reinterpret_cast<float*>(q4_smem + sizeof(typename C::Shared) + W * C::kStages * C::kStage);
-  float* merge_ml = merge + W / 2 * RB * C::kPad;
+  float* merge_ml = merge + H * RB * C::kPad;
   // A whole warp's wait, with one answer for all lanes.  After one that ran out the
   // warp leaves; the others' waits for it run out too.
   auto arrived = [](uint64_t* bar, uint32_t parity, int where) {
@@ -312,7 +313,6 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
     if (++f_stage == C::kStages) f_stage = 0;
   };
 
-  Item it;
   uint32_t stage = 0, phase = 0, items = 0;
   int end = 0;
   // the lane's K words of keys 2j, 2j + 1 of each four (their partners two rows on)
@@ -324,9 +324,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
   uint32_t qa[NB][NT][4];
   float qc[NB][NT];       // -8 sum q of a block
   float sscale[NT];
-  int node[NT];
   float o[2 * NB][NT][4], ws[NT][4], m[NT], l[NT];
-  uint32_t anc[NT][kWords];
   uint32_t spoilt[NT];    // blocks with a NaN scale that the row sees
   bool have_anc = false;
   for (uint32_t c_seg = 0;; ++c_seg) {
@@ -339,7 +337,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       bring();
       if (in_ring == before) break;
     }
-    it = seg.it;
+    const Item& it = seg.it;
     const int R = it.n * bt.group, row_lo = it.blk * RB;
     if (seg.t0 == it.t0) {
       // ---- the item's rows of q, scaled, and -8 sum q of each block -----------------
@@ -347,9 +345,9 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       for (int nt = 0; nt < NT; ++nt) {
         const int r = row_lo + nt * 8 + g;
         const bool valid = r < R;
-        node[nt] = valid ? r / bt.group : 0;
-        const int head = it.kvh * bt.group + (valid ? r - node[nt] * bt.group : 0);
-        const T* qr = q + (it.node0 + node[nt]) * q_stride + head * D + 8 * t;
+        const int node = valid ? r / bt.group : 0;
+        const int head = it.kvh * bt.group + (valid ? r - node * bt.group : 0);
+        const T* qr = q + (it.node0 + node) * q_stride + head * D + 8 * t;
         float x[NB][8];
         float big = 0.f;
 #pragma unroll
@@ -409,21 +407,22 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       const bool tail = row0 + kQ4Keys > it.len;
       const uint32_t no_page = (bad >> (2 * stage)) & 3u;
       if (tail && !have_anc) {
-        // the nodes that the lane's rows see
+        // the nodes that the rows see: a lane per row
         have_anc = true;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        if (lane < RB) {
+          const int node = min((row_lo + lane) / bt.group, it.n - 1);
+          uint32_t anc[kWords];
 #pragma unroll
           for (int w = 0; w < kWords; ++w) {
-            const int k = node[nt] + 1 - w * 32;
-            anc[nt][w] = bt.parents ? 0u : k >= 32 ? 0xffffffffu : (k > 0 ? (1u << k) - 1u : 0u);
+            const int k = node + 1 - w * 32;
+            anc[w] = bt.parents ? 0u : k >= 32 ? 0xffffffffu : (k > 0 ? (1u << k) - 1u : 0u);
           }
           if (bt.parents) {
-            int at = node[nt];
+            int at = node;
             while (true) {
 #pragma unroll
               for (int w = 0; w < kWords; ++w)
-                if ((at >> 5) == w) anc[nt][w] |= 1u << (at & 31);
+                if ((at >> 5) == w) anc[w] |= 1u << (at & 31);
               const int up = __ldg(bt.parents + it.node0 + at);
               if (up < 0 || up >= at) {
                 if (up != -1) set_dev_error(B2A_ERR_POSITION, it.b);
@@ -432,10 +431,12 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
               at = up;
             }
           }
+          sh.sees[warp][lane] = make_uint4(anc[0], anc[1], anc[2], anc[3]);
         }
+        __syncwarp();
       }
 
-      // (a granule at a time: both at once need more registers than 14 warps have)
+      // (a granule at a time: both at once need more registers than 15 warps have)
 #pragma unroll 1
       for (int gr = 0; gr < 2; ++gr, base += C::kGranule, row0 += 16) {
         // ---- scores ----------------------------------------------------------------
@@ -502,13 +503,8 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               bool see = j < 0;
-              if (j >= 0 && j < it.n && row_lo + nt * 8 + g < R) {
-                uint32_t word = anc[nt][0];
-#pragma unroll
-                for (int w = 1; w < kWords; ++w)
-                  if ((j >> 5) == w) word = anc[nt][w];
-                see = (word >> (j & 31)) & 1u;
-              }
+              if (j >= 0 && j < it.n && row_lo + nt * 8 + g < R)
+                see = reinterpret_cast<const uint32_t*>(&sh.sees[warp][nt * 8 + g])[j >> 5] >> (j & 31) & 1u;
               if ((no_page >> gr) & 1u) see = false;
               float& x = i & 1 ? s[nt][i >> 1].y : s[nt][i >> 1].x;
               if (!see) x = -INFINITY;
@@ -628,8 +624,6 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       if (lane == 0) mbar_arrive(&sh.seg_empty[c_seg % kQ4Queue]);
       continue;
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.seg_empty[c_seg % kQ4Queue]);
 
     // ---------------- join the warps ---------------------------------------------------
     // the upper half hands its rows to the lower, whose rows are then added up
@@ -660,7 +654,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
         }
       }
     }
-    const int half = warp % (W / 2);
+    const int half = warp % H;
     float* mine = merge + half * RB * C::kPad + 2 * t * C::kPad + 8 * (g & 3) + (g >> 2);
     float* mine_ml = merge_ml + half * RB * 2;
     auto put = [&]() {
@@ -682,14 +676,14 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
     };
     // (the item before has been read)
     if (items > 0 && !arrived(&sh.read, (items - 1) & 1, 0x3F300)) return;
-    if (warp >= W / 2) {
+    if (warp >= H) {
       put();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.handed);
     } else {
       if (!arrived(&sh.handed, items & 1, 0x3F400)) return;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT && warp + H < W; ++nt) {
         const float m2 = mine_ml[(nt * 8 + g) * 2], l2 = mine_ml[(nt * 8 + g) * 2 + 1];
         const float now = fmaxf(m[nt], m2), mref = now == -INFINITY ? 0.f : now;
         const float a = fast_exp2(m[nt] - mref), c = fast_exp2(m2 - mref);
@@ -720,13 +714,13 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       const int r = i / (D / 8), d = (i - r * (D / 8)) * 8;
       float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < W / 2; ++w) M = fmaxf(M, merge_ml[(w * RB + r) * 2]);
+      for (int w = 0; w < H; ++w) M = fmaxf(M, merge_ml[(w * RB + r) * 2]);
       const float mref = M == -INFINITY ? 0.f : M;
       float L = 0.f, x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = 0.f;
 #pragma unroll 4
-      for (int w = 0; w < W / 2; ++w) {
+      for (int w = 0; w < H; ++w) {
         const float f = fast_exp2(merge_ml[(w * RB + r) * 2] - mref);
         L += merge_ml[(w * RB + r) * 2 + 1] * f;
         const float4 y0 = *reinterpret_cast<const float4*>(merge + (w * RB + r) * C::kPad + d);
@@ -751,7 +745,10 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.read);
+    if (lane == 0) {
+      mbar_arrive(&sh.read);
+      mbar_arrive(&sh.seg_empty[c_seg % kQ4Queue]);
+    }
   }
   zero_unwritten<T, D>(bt, end == 2, out, lse, warp, W);
 }

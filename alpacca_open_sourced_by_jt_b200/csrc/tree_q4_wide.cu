@@ -47,6 +47,7 @@ struct alignas(128) QWShared {
   Item item[kQ4Queue];
   Q4Seg<kQWConvert> seg[kQ4Queue];
   float x[kQWGroups][128];  // maxima, at an item's end sums, between the warpgroups
+  float o[128][33];         // rows of O, where several lanes share a query row
 };
 
 template <int D>
@@ -101,7 +102,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     const __grid_constant__ Batch bt, const __grid_constant__ q4::Pool pool, const T* __restrict__ q,
     long long q_stride, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o,
-    float* __restrict__ part_ml, float scale_log2) {
+    float* __restrict__ part_ml, float scale_log2, int rep_shift) {
   using C = QWCfg<D>;
   constexpr int BN = kQWKeys, TS = C::Shared::kTileSteps, W = kQWConvert, NB = D / 32;
   constexpr uint32_t kOCol = kQWGroups * BN, kQCol = kOCol + D;
@@ -400,6 +401,9 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     const uint32_t tl = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t ts = tl + w * BN;
     const int before_w = 1 - w;                    // whose tile comes before
+    const int lanes_of = 128 >> rep_shift;         // query rows of a block
+    const int rr = r & (lanes_of - 1);             // the lane's query row
+    const int width = BN >> rep_shift, c0 = (r >> (7 - rep_shift)) * width;  // its keys of a tile
     uint32_t own = 0, theirs = 0;  // tiles this warpgroup and that one have done
     uint32_t pvbase = 0, items = 0;
     int end = 0;
@@ -421,10 +425,10 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       const int n = it.t1 - it.t0;
       const int row0 = it.blk * bt.rows_per_block;
       const int live = min(bt.rows_per_block, it.n * bt.group - row0);
-      const bool busy = quarter * 32 < live;  // this warp holds query rows
-      const bool good = r < live;
-      const int node = good ? (row0 + r) / bt.group : 0;
-      const int head = it.kvh * bt.group + (good ? row0 + r - node * bt.group : 0);
+      const bool busy = (rr & ~31) < live;  // this warp holds query rows
+      const bool good = rr < live;
+      const int node = good ? (row0 + rr) / bt.group : 0;
+      const int head = it.kvh * bt.group + (good ? row0 + rr - node * bt.group : 0);
       // ---- the row of q, scaled to f16, into TMEM: half of it by each warpgroup -----------
       float sscale;
       {
@@ -504,9 +508,9 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
         tc_fence_after();
         if (busy && alive) {
           float mxa = -INFINITY, mxb = -INFINITY;
+          float s[32];  // (the last 32 of the lane's keys, which are all of them for 4 lanes a row)
 #pragma unroll 1
-          for (int c = 0; c < BN; c += 32) {
-            float s[32];
+          for (int c = c0; c < c0 + width; c += 32) {
             tc_ld32(ts + c, s);
             tc_wait_ld();
             if (tail) hide(s, tree0 + c);
@@ -535,11 +539,12 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
           m = now;
           float suma = 0.f, sumb = 0.f;
 #pragma unroll 1
-          for (int c = 0; c < BN; c += 32) {
-            float s[32];
-            tc_ld32(ts + c, s);
-            tc_wait_ld();
-            if (tail) hide(s, tree0 + c);
+          for (int c = c0; c < c0 + width; c += 32) {
+            if (width > 32) {
+              tc_ld32(ts + c, s);
+              tc_wait_ld();
+              if (tail) hide(s, tree0 + c);
+            }
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -549,6 +554,15 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
               pk[e] = Pack2<__half>::run(p0, p1);
             }
             tc_st16(ts + (c >> 1), pk);
+          }
+          if (rep_shift) {
+            // the tile's other keys are other lanes': weight 0 here
+            uint32_t zero[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) zero[e] = 0u;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 32)
+              if (c < c0 || c >= c0 + width) tc_st16(ts + (c >> 1), zero);
           }
           tc_wait_st();
           l += suma + sumb;
@@ -594,10 +608,11 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       const int slot = part_slot(it, blockIdx.x);
       const size_t row = static_cast<size_t>(it.node0 + node) * bt.H + head;
       const float f = L > 0.f ? 1.f / L : 0.f;
+      const int lo = max(it.t0 * BN - it.len, 0), hi = min(it.t1 * BN - it.len, it.n);
+      const uint4 sees = make_uint4(anc[0], anc[1], anc[2], anc[3]);
       float* po = part_o + (static_cast<size_t>(max(slot, 0)) * bt.rows_per_block + r) * D;
-      if (busy && !dead) {
+      if (rep_shift == 0 && busy && !dead) {
         // the warpgroups write the columns in turn, 32 (a block) at a time
-        const int lo = max(it.t0 * BN - it.len, 0), hi = min(it.t1 * BN - it.len, it.n);
 #pragma unroll 1
         for (int col = w * 32; col < D; col += 32 * kQWGroups) {
           float o[32];
@@ -605,7 +620,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
           tc_wait_ld();
           if (good) {
             if (special && q4_special(bt, pool, D, it.b, it.kvh, it.len, lo, hi,
-                                      make_uint4(anc[0], anc[1], anc[2], anc[3]), col / 32)) {
+                                      sees, col / 32)) {
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(0x7fffffffu);
             }
@@ -628,6 +643,58 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
             ml[1] = L;
           } else if (lse) {
             lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+          }
+        }
+      }
+      if (rep_shift) {
+        // Several lanes share a query row, each with its own keys' sums relative to its own
+        // maximum: they meet in shared memory, 32 columns at a time.
+        meet();  // (L has been read)
+        if (w == 0) {
+          sh.x[0][r] = M;
+          sh.x[1][r] = L;
+        }
+        meet();
+        if (w == 0 && !dead) {
+          float top = -INFINITY, sum = 0.f;
+          for (int i = rr; i < 128; i += lanes_of) top = fmaxf(top, sh.x[0][i]);
+          const float tref = top == -INFINITY ? 0.f : top;
+          for (int i = rr; i < 128; i += lanes_of) sum = fmaf(sh.x[1][i], fast_exp2(sh.x[0][i] - tref), sum);
+          const float mine = M == -INFINITY ? 0.f : fast_exp2(M - tref) * (slot >= 0 ? 1.f : (sum > 0.f ? 1.f / sum : 0.f));
+#pragma unroll 1
+          for (int col = 0; col < D; col += 32) {
+            float o[32];
+            tc_ld32(tl + kOCol + col, o);
+            tc_wait_ld();
+            const bool gone = special && good && q4_special(bt, pool, D, it.b, it.kvh, it.len, lo, hi, sees, col / 32);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sh.o[r][e] = gone ? __uint_as_float(0x7fffffffu) : o[e] * mine;
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+            for (int i = threadIdx.x; i < live * 4; i += 128) {
+              const int qr = i >> 2, at = (i & 3) * 8;
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = 0.f;
+              for (int j = qr; j < 128; j += lanes_of) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] += sh.o[j][at + e];
+              }
+              const int nd = (row0 + qr) / bt.group;
+              if (slot >= 0)
+                paged::store8(part_o + (static_cast<size_t>(slot) * bt.rows_per_block + qr) * D + col + at, x);
+              else
+                paged::store8(out + (static_cast<size_t>(it.node0 + nd) * bt.H + it.kvh * bt.group + row0 + qr - nd * bt.group) * D + col + at, x);
+            }
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+          }
+          if (good && r < lanes_of) {
+            if (slot >= 0) {
+              float* ml = part_ml + (static_cast<size_t>(slot) * bt.rows_per_block + rr) * 2;
+              ml[0] = top;
+              ml[1] = sum;
+            } else if (lse) {
+              lse[row] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+            }
           }
         }
       }
@@ -658,8 +725,10 @@ namespace {
 
 // Which kernel, by the most rows a KV head can have, and the rows of an item.
 bool tree_q4_is_wide(int rows, int D) { return rows > 16 && D <= 128; }
+// (the wide kernel: as many lanes of 128 to a row as the most rows leave)
+int tree_q4_rep(int rows) { return rows <= 32 ? 2 : rows <= 64 ? 1 : 0; }
 int tree_q4_rows(int rows, int D, int group) {
-  if (tree_q4_is_wide(rows, D)) return 128 / group * group;
+  if (tree_q4_is_wide(rows, D)) return (128 >> tree_q4_rep(rows)) / group * group;
   return rows <= 8 || D > 128 ? 8 : 16;
 }
 
@@ -686,7 +755,7 @@ int tree_q4_wide_launch(const TreeArgs& a, const Q4::Pool& pool) {
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "cudaFuncSetAttribute(tree_decode_q4)");
   e = b2a_host::launch(kern, dim3(a.grid), dim3(TR::kQWThreads), C::kSmem, a.st, a.bt, pool,
                        static_cast<const T*>(a.q), a.q_stride, static_cast<T*>(a.out), a.lse, a.part_o,
-                       a.part_ml, a.sscale);
+                       a.part_ml, a.sscale, tree_q4_rep(a.bt.rows_per_block));
   if (e != cudaSuccess) return b2a_host::cuda_fail(e, "tree_decode_q4 wide launch");
   return tree_merge<T, D>(a);
 }
