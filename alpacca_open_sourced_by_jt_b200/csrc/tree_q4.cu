@@ -59,7 +59,7 @@ struct Q4Seg {
 
 template <int W, int S>
 struct alignas(128) Q4Shared {  // (the rings stand behind it)
-  static constexpr int kTileSteps = 1;             // steps of a tile of the work division
+  static constexpr int kStepKeys = kQ4Keys, kTileSteps = 1;  // a step's keys, a tile's steps
   static constexpr bool kItems = false;            // the items go by a queue of their own, too
   uint64_t full[W][S];                             // a warp's stages
   uint64_t seg_full[kQ4Queue], seg_empty[kQ4Queue];
@@ -124,7 +124,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // The planning warp.  Requests are looked at 32 at a time, one by each lane.
 template <int W, typename Shared>
 __device__ __forceinline__ void q4_plan(const Batch& bt, Shared& sh, int lane) {
-  constexpr int TS = Shared::kTileSteps;
+  constexpr int TS = Shared::kTileSteps, SK = Shared::kStepKeys;
   const Start start = locate(bt, team_of(bt, blockIdx.x));
   long long off = start.off, left = start.left;
   int b = start.b, base = -32, slot = 0, items = 0, steps = 0;
@@ -157,7 +157,7 @@ __device__ __forceinline__ void q4_plan(const Batch& bt, Shared& sh, int lane) {
     it.n = __shfl_sync(0xffffffffu, n32, b - base);
     it.len = __shfl_sync(0xffffffffu, len32, b - base);
     it.node0 = __shfl_sync(0xffffffffu, node32, b - base);
-    it.tiles = (it.len + it.n + TS * kQ4Keys - 1) / (TS * kQ4Keys);
+    it.tiles = (it.len + it.n + TS * SK - 1) / (TS * SK);
     const long long u = units_of(bt, it.n, it.len);
     if (off >= u) {
       off -= u;
@@ -196,8 +196,8 @@ __device__ __forceinline__ void q4_plan(const Batch& bt, Shared& sh, int lane) {
       bool gone = false;
 #pragma unroll 4
       for (int i = lane; i < t1 - t0; i += 32) {
-        const int row = (t0 + i) * kQ4Keys;
-        const bool one = row < rows, two = row + 16 < rows;  // (a tile's last steps may hold nothing)
+        const int row = (t0 + i) * SK;
+        const bool one = row < rows, two = SK > 16 && row + 16 < rows;  // (a tile's last steps may hold nothing)
         const int e0 = one ? table_entry(bt, it.b, row) : 0;
         const int e1 = split && two ? table_entry(bt, it.b, row + 16) : e0;
         const int p0 = checked_page(bt, it.b, e0), p1 = checked_page(bt, it.b, e1);

@@ -3,19 +3,20 @@
 //
 // A block of up to 128 rows is the M of tcgen05.mma; S = Q.K^T and O += P.V accumulate
 // in TMEM, P goes over S's columns and Q stays in TMEM too, so that shared memory
-// carries only the tiles.  Converting warps turn each step of 32 keys (a granule of
-// q4.cuh is 16) into rows of the K and V tiles, 128-byte swizzled as the MMAs read
+// carries only the tiles.  Converting warps turn each granule of 16 keys into rows of the K and V tiles, 128-byte swizzled as the MMAs read
 // them: a code at bits 6 to 9 of 0x4c00 is the f16 16 + code, and (16 + code) d - 24 d,
 // one fused operation, is d * (code - 8) exactly (24 d has 10 bits).  So both products
 // are those of the cache's own values; q is scaled by a power of two to f16 as in
 // tree_q4.cu, the weights are rounded to f16.
 //
-// 576 threads: warps 0-7 softmax (two warpgroups, tiles in turn, an S buffer each),
-// 8-15 converters (each brings its own steps, as tree_q4_kernel's warps do), 16 plans,
-// 17 owns TMEM and issues the MMAs.
+// 896 threads: warps 0-7 softmax (two warpgroups, tiles in turn, an S buffer each),
+// 8-23 converters (each brings its own steps, as tree_q4_kernel's warps do, here of 16
+// keys), 24 plans, 25 owns TMEM and issues the MMAs.
 // TMEM: S0, S1 (128 columns each), O (D), Q (D / 2).
 
 #include <limits.h>
+
+#include <type_traits>
 
 #include "b2a_common.cuh"
 #include "q4.cuh"
@@ -25,15 +26,18 @@ namespace b2a {
 namespace tree {
 
 constexpr int kQWGroups = 2;     // softmax warpgroups
-constexpr int kQWConvert = 8;    // converting warps
+constexpr int kQWConvert = 16;   // converting warps
 constexpr int kQWPlan = 8 + kQWConvert, kQWIssue = kQWPlan + 1;  // the planning and the issuing warp
-constexpr int kQWThreads = (kQWIssue + 1) * 32;
+constexpr int kQWThreads = (kQWIssue + 3) * 32;  // whole warpgroups
+// Registers: 896 x 72 at launch; softmax 104, converters 56, the last four warps 72.
+constexpr int kQWSoftmaxRegs = 104, kQWConvertRegs = 56;
+static_assert(256 * kQWSoftmaxRegs + kQWConvert * 32 * kQWConvertRegs + 128 * 72 <= kQWThreads * 72, "registers");
 constexpr int kQWKeys = 128;     // keys per tile
 constexpr int kQWSlots = 2;      // K tiles, and V tiles, in shared memory
 
 template <int S>
 struct alignas(128) QWShared {
-  static constexpr int kTileSteps = kQWKeys / kQ4Keys;
+  static constexpr int kStepKeys = 16, kTileSteps = kQWKeys / 16;  // a step is a granule
   static constexpr bool kItems = true;
   uint64_t full[kQWConvert][S];                        // a converter's stages
   uint64_t seg_full[kQ4Queue], seg_empty[kQ4Queue];    // planner -> converters
@@ -53,7 +57,7 @@ struct alignas(128) QWShared {
 template <int D>
 struct QWCfg {
   static constexpr int kGranule = q4::granule_bytes(D);
-  static constexpr int kStage = 2 * kGranule;
+  static constexpr int kStage = kGranule;
   static constexpr int kBox = kQWKeys * 128;        // 128 rows x 64 columns
   static constexpr int kTile = (D / 64) * kBox;     // one K or V tile
   static constexpr int kTiles = 2 * kQWSlots * kTile;
@@ -86,13 +90,14 @@ __device__ __noinline__ bool q4_special(const Batch& bt, const q4::Pool& pool, i
 }
 
 // 8 values of a word: code places 0 to 3 give dims (0, 1), (2, 3), (4, 5), (6, 7).
-__device__ __forceinline__ uint4 q4_values(uint32_t w, __half2 d, __half2 d24, bool large) {
+template <bool kLarge>  // 24 d is past f16
+__device__ __forceinline__ uint4 q4_values(uint32_t w, __half2 d, __half2 d24) {
   uint32_t x[4] = {((w << 6) & 0x03c003c0u) | 0x4c004c00u, ((w << 2) & 0x03c003c0u) | 0x4c004c00u,
                    ((w >> 2) & 0x03c003c0u) | 0x4c004c00u, ((w >> 6) & 0x03c003c0u) | 0x4c004c00u};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2 c = *reinterpret_cast<const __half2*>(&x[i]);
-    const __half2 y = large ? __hmul2(__hsub2(c, __float2half2_rn(24.f)), d) : __hfma2(c, d, d24);
+    const __half2 y = kLarge ? __hmul2(__hsub2(c, __float2half2_rn(24.f)), d) : __hfma2(c, d, d24);
     x[i] = *reinterpret_cast<const uint32_t*>(&y);
   }
   return make_uint4(x[0], x[1], x[2], x[3]);
@@ -238,11 +243,11 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       }
       ++items;
     }
-  } else if (warp >= 8) {
+  } else if (warp >= 8 && warp < kQWPlan) {
     // ------------------------------ converters -------------------------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQWConvertRegs));
     const int cw = warp - 8;
     uint8_t* ring = qw_smem + C::kTiles + cw * C::kStages * C::kStage;
-    const bool split = bt.table && bt.page_shift == 4;  // a step's granules lie in two pages
     const int page_mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
     uint32_t f_seg = 0, f_stage = 0, in_ring = 0;
     int f_step = 0, f_t1 = 0;
@@ -260,16 +265,13 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       }
       const Q4Seg<W>& seg = sh.seg[(f_seg - 1) % kQ4Queue];
       const int i = f_step - seg.t0;
-      const int p0 = seg.pages[0][i], p1 = seg.pages[1][i];
+      const int page = seg.pages[0][i];
       if (lane == 0) {
         uint64_t* bar = &sh.full[cw][f_stage];
-        uint8_t* dst = ring + f_stage * C::kStage;
-        const int row = (f_step * kQ4Keys) & page_mask, row1 = (f_step * kQ4Keys + 16) & page_mask;
-        mbar_arrive_expect_tx(bar, ((p0 >= 0 ? 1 : 0) + (p1 >= 0 ? 1 : 0)) * C::kGranule);
-        if (p0 >= 0)
-          bulk_load(dst, q4::granule(pool, D, p0, seg.it.kvh, row), p1 >= 0 && !split ? 2 * C::kGranule : C::kGranule, bar);
-        if (p1 >= 0 && split)
-          bulk_load(dst + C::kGranule, q4::granule(pool, D, p1, seg.it.kvh, row1), C::kGranule, bar);
+        mbar_arrive_expect_tx(bar, page >= 0 ? C::kGranule : 0);
+        if (page >= 0)
+          bulk_load(ring + f_stage * C::kStage, q4::granule(pool, D, page, seg.it.kvh, (f_step * 16) & page_mask),
+                    C::kGranule, bar);
       }
       f_step += W;
       ++in_ring;
@@ -293,45 +295,85 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
         if (in_ring == 0) bring();
         const uint32_t tile = (seg.g0 + st - seg.t0) / TS;
         const uint32_t slot = tile % kQWSlots, round = tile / kQWSlots;
-        const int gone = (seg.pages[0][st - seg.t0] < 0 ? 1 : 0) | (seg.pages[1][st - seg.t0] < 0 ? 2 : 0);
+        const bool gone = seg.pages[0][st - seg.t0] < 0;
         if (!arrived(&sh.full[cw][stage], phase, 0x3F880)) {
           ok = false;
           break;
         }
-        const int gr = lane >> 4, r = lane & 15;
-        const uint8_t* g = ring + stage * C::kStage + gr * C::kGranule;
-        const int key = (st % TS) * kQ4Keys + lane;  // row of the tile
-        const int at = st * kQ4Keys + lane;          // row of the cache
-        const bool none = at >= rows || ((gone >> gr) & 1);
+        const int part = lane >> 4, r = lane & 15;   // two lanes to a row
+        const uint8_t* g = ring + stage * C::kStage;
+        const int at = st * 16 + r;                  // row of the cache
+        const bool none = at >= rows || gone;
+        // the row in a tile, swizzled: chunk c is at `swz` with c & 7 in bits 4 to 6 flipped
+        const uint32_t key = (st % TS) * 16 + r, swz = key * 128 + ((key & 7) << 4);
         // scales of K and V, [block] f16; of rows that are not there 0
         uint32_t dk[NB / 2], dv[NB / 2];
 #pragma unroll
         for (int i = 0; i < NB / 2; ++i) {
           dk[i] = *reinterpret_cast<const uint32_t*>(g + 16 * D + r * (2 * NB) + i * 4);
           dv[i] = *reinterpret_cast<const uint32_t*>(g + 17 * D + r * (2 * NB) + i * 4);
-          if (none) dk[i] = dv[i] = 0u;
-          if (tree && at >= len) {
-            // a NaN that some rows do not see: taken out here, put back at the item's end
-            if ((dv[i] & 0x7fffu) > 0x7c00u) {
-              dv[i] &= 0xffff0000u;
-              sh.special[f_items & 7] = 1;
-            }
-            if ((dv[i] & 0x7fff0000u) > 0x7c000000u) {
-              dv[i] &= 0x0000ffffu;
-              sh.special[f_items & 7] = 1;
+        }
+        if (st * 16 + 16 > len || gone) {  // rows of the tree, or past the last
+#pragma unroll
+          for (int i = 0; i < NB / 2; ++i) {
+            if (none) dk[i] = dv[i] = 0u;
+            if (tree && at >= len) {
+              // a NaN that some rows do not see: taken out here, put back at the item's end
+              if ((dv[i] & 0x7fffu) > 0x7c00u) {
+                dv[i] &= 0xffff0000u;
+                sh.special[f_items & 7] = 1;
+              }
+              if ((dv[i] & 0x7fff0000u) > 0x7c000000u) {
+                dv[i] &= 0x0000ffffu;
+                sh.special[f_items & 7] = 1;
+              }
             }
           }
         }
-        bool large = false;  // 24 d is past f16
+        __half2 most = __float2half2_rn(0.f);
 #pragma unroll
-        for (int i = 0; i < NB / 2; ++i)
-          large |= (dk[i] & 0x7fffu) > 0x6800u || (dk[i] >> 16 & 0x7fffu) > 0x6800u ||
-                   (dv[i] & 0x7fffu) > 0x6800u || (dv[i] >> 16 & 0x7fffu) > 0x6800u;
-        large = __any_sync(0xffffffffu, large);
+        for (int i = 0; i < NB / 2; ++i) {
+          most = __hmax2(most, __habs2(*reinterpret_cast<const __half2*>(&dk[i])));
+          most = __hmax2(most, __habs2(*reinterpret_cast<const __half2*>(&dv[i])));
+        }
+        const bool large = __any_sync(0xffffffffu, !__hble2(most, __float2half2_rn(2048.f)));
         const __half2 m24 = __float2half2_rn(-24.f);
         auto scale_of = [](const uint32_t* d, int b) {
           const uint32_t u = __byte_perm(d[b >> 1], 0u, b & 1 ? 0x3232u : 0x1010u);
           return *reinterpret_cast<const __half2*>(&u);
+        };
+        auto convert_k = [&](uint8_t* kt, auto is_large) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int t = 2 * part + ((j + (r >> 1)) & 1);  // (rows begin at different words: fewer bank conflicts)
+            uint32_t w[4];
+            if constexpr (NB >= 4) {
+              const uint4 u = *reinterpret_cast<const uint4*>(g + r * 64 + t * 16);
+              w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(g + r * 32 + t * 8);
+              w[0] = u.x; w[1] = u.y;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const __half2 d = scale_of(dk, b);  // (chunk 4 b + t of the row)
+              *reinterpret_cast<uint4*>(kt + (b >> 1) * C::kBox + ((swz ^ (t << 4)) ^ ((b & 1) << 6))) =
+                  q4_values<decltype(is_large)::value>(w[b], d, __hmul2(d, m24));
+            }
+          }
+        };
+        auto convert_v = [&](uint8_t* vt, auto is_large) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const __half2 d = scale_of(dv, b), d24 = __hmul2(d, m24);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int t = 2 * j + part;
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(g + 8 * D + (4 * b + t) * 64 + r * 4);
+              *reinterpret_cast<uint4*>(vt + (b >> 1) * C::kBox + ((swz ^ (t << 4)) ^ ((b & 1) << 6))) =
+                  q4_values<decltype(is_large)::value>(w, d, d24);
+            }
+          }
         };
         // ---- K ----
         if (round > 0 && !arrived(&sh.k_empty[slot], (round & 1) ^ 1, 0x3F890)) {
@@ -339,25 +381,8 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
           break;
         }
         uint8_t* kt = qw_smem + slot * C::kTile;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int t = (j + (r >> 1)) & 3;  // (lanes begin at different words: no bank conflicts)
-          uint32_t w[4];
-          if constexpr (NB >= 4) {
-            const uint4 u = *reinterpret_cast<const uint4*>(g + r * 64 + t * 16);
-            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-          } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(g + r * 32 + t * 8);
-            w[0] = u.x; w[1] = u.y;
-          }
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            const __half2 d = scale_of(dk, b);
-            const int c = 4 * b + t;  // 16-byte chunk of the row
-            *reinterpret_cast<uint4*>(kt + (b >> 1) * C::kBox + sw128_off(key, c & 7)) =
-                q4_values(w[b], d, __hmul2(d, m24), large);
-          }
-        }
+        if (large) convert_k(kt, std::true_type());
+        else convert_k(kt, std::false_type());
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full[slot]);
@@ -367,16 +392,8 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
           break;
         }
         uint8_t* vt = qw_smem + (kQWSlots + slot) * C::kTile;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const __half2 d = scale_of(dv, b), d24 = __hmul2(d, m24);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int c = 4 * b + t;
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(g + 8 * D + c * 64 + r * 4);
-            *reinterpret_cast<uint4*>(vt + (b >> 1) * C::kBox + sw128_off(key, c & 7)) = q4_values(w, d, d24, large);
-          }
-        }
+        if (large) convert_v(vt, std::true_type());
+        else convert_v(vt, std::false_type());
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.v_full[slot]);
@@ -393,8 +410,9 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.seg_empty[c_seg % kQ4Queue]);
     }
-  } else {
+  } else if (warp < 8) {
     // ------------------------------ softmax ----------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kQWSoftmaxRegs));
     const int w = warp >> 2;                       // warpgroup: tiles jj % 2 == w, S buffer w
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;             // row of the block == TMEM lane
