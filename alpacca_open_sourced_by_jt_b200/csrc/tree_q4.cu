@@ -515,15 +515,15 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
               for (int b = 0; b < NB / 2; ++b) dv[i * (NB / 2) + b] = 0u;
           }
         }
-        __half2 top = __float2half2_rn(0.f);
+        auto top_scale = [&]() {  // the largest |d_v| of the lane's keys, a NaN before all
+          __half2 top = __float2half2_rn(0.f);
 #pragma unroll
-        for (int i = 0; i < NB * 2; ++i)
-          top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&dv[i])));
-        // A power of two (its exponent) that is at least the largest |d_v| of the lane's
-        // keys: with whole exponents the weight of a row's only key is exact.
-        const uint32_t top_bits = *reinterpret_cast<const uint32_t*>(&top);
-        const uint32_t top16 = max(top_bits & 0x7fffu, top_bits >> 16 & 0x7fffu);
-        const float far = static_cast<float>(min(static_cast<int>(top16 >> 10), 30) - 14);
+          for (int i = 0; i < NB * 2; ++i)
+            top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&dv[i])));
+          const uint32_t bits = *reinterpret_cast<const uint32_t*>(&top);
+          return max(bits & 0x7fffu, bits >> 16 & 0x7fffu);
+        };
+        uint32_t top16 = top_scale();
         if (__any_sync(0xffffffffu, top16 > 0x7c00u)) {
           // A NaN scale of a key that is seen: its block's outputs become NaN at the
           // item's end; here it counts as zero.
@@ -539,7 +539,11 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
               for (int nt = 0; nt < NT; ++nt)
                 if ((i & 1 ? s[nt][i >> 1].y : s[nt][i >> 1].x) != -INFINITY) spoilt[nt] |= 1u << b;
             }
+          top16 = top_scale();
         }
+        // A power of two (its exponent) that is at least the largest |d_v| of the lane's
+        // keys: with whole exponents the weight of a row's only key is exact.
+        const float far = static_cast<float>(min(static_cast<int>(top16 >> 10), 30) - 14);
         bool grow = false;
         float mx[NT];
 #pragma unroll
