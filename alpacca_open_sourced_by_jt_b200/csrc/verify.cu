@@ -19,6 +19,8 @@
 
 #include <cooperative_groups.h>
 
+#include <cfloat>
+
 #include "b2a_common.cuh"
 
 namespace b2a {
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
   for (int i = tid; i < (a.slice + 31) / 32; i += kThreads) gone[i] = 0u;
   if (tid < kTable) s_table[tid] = exp2(tid * (1.0 / kTable));
   __syncthreads();
-  const float heat = a.temperature ? a.temperature[b] : 1.f;
+  const float heat = a.temperature ? (a.temperature[b] > FLT_MAX ? FLT_MAX : a.temperature[b]) : 1.f;
   const bool greedy = !(heat > 0.f);
   const double cold = greedy ? 0.0 : 1.0 / static_cast<double>(heat);
   const double cold16 = fmin(cold * 1.4426950408889634 * kTable, 1e300);
@@ -340,71 +342,104 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
       for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
       return exchange_sum(mine);
     };
-    bool exact = false;  // total is the 64-bit sum of all weights
+    bool exact = false;  // total is the 64-bit sum of all weights (certain drafts: of those left)
+    double left = 0.0;   // what the draw takes from
     int child = cur;
-    while (place >= 0) {
-      // the next child
-      int c = kMaxNodes;
+    while (true) {
+      int ask = -1;  // rejections behind which a sum is needed before the next child
+      while (place >= 0) {
+        // the next child
+        int c = kMaxNodes;
+#pragma unroll
+        for (int w = 0; w < kMaxNodes / 32; ++w) {
+          const int j = w * 32 + lane;
+          const unsigned hit = __ballot_sync(0xffffffffu, j > child && j < n && s_par[j] == cur);
+          if (c == kMaxNodes && hit) c = w * 32 + __ffs(hit) - 1;
+        }
+        if (c == kMaxNodes) break;
+        child = c;
+        const int v = s_tok[c];
+        if (v < 0 || v >= a.V) continue;
+        if (sure) {
+          if (v == place) {
+            next = c;
+            break;
+          }
+          continue;
+        }
+        bool again = false;
+        for (int i = lane; i < rejected; i += 32) again |= s_rej[i] == v;
+        again = __any_sync(0xffffffffu, again);
+        const double u = s_u[c];
+        const double e = weight(at(row, v));
+        if constexpr (!kDraft) {
+          if (again) continue;
+          if (u * total < e) {
+            next = c;
+            break;
+          }
+          total -= e;
+        } else {
+          const float q = __ldg(qrow + v);
+          const double r = again ? 0.0 : residual(e, q, rejected);
+          if (u * static_cast<double>(q) * (rejected ? s_mass[rejected - 1] : 1.0) < r) {
+            next = c;
+            break;
+          }
+        }
+        __syncthreads();  // all have read s_rej
+        if (tid == 0) {
+          s_rej[rejected] = v;
+          const int w = v - v0;
+          if (v >= v0 && v < v1) gone[w >> 5] |= 1u << (w & 31);
+        }
+        ++rejected;
+        __syncthreads();
+        if (kDraft) {
+          ask = exact ? rejected : 0;
+          break;
+        }
+        // (where little is left of the 32-bit sum, the rest is summed up by itself)
+        if (!exact && total < 0.0625 * part) {
+          ask = 0;
+          break;
+        }
+      }
+      if (next >= 0 || sure) break;
+      if (kDraft && ask < 0 && rejected) {
+        left = s_mass[rejected - 1];
+        break;
+      }
+      double sum;
+      while (true) {
+        sum = mass(max(ask, 0));
+        if (!kDraft || ask != 0) break;
+        total = sum + weight(at(row, s_rej[0]));  // (the weights' own sum counts the rejected token too)
+        per_total = 1.0 / total;
+        ask = rejected;
+      }
+      exact = true;
+      if (ask < 0) {
+        left = sum;
+        break;
+      }
+      if constexpr (kDraft) {
+        if (tid == 0) {
+          s_mass[rejected - 1] = sum;
+          s_per[rejected - 1] = sum > 0.0 ? 1.0 / sum : 0.0;
+        }
+        __syncthreads();
+      } else {
+        total = sum;
+      }
+    }
+    if (next < 0 && !sure && !(left > 0.0)) {
+      // the largest is taken, and the path goes on to a child that has it as its token
 #pragma unroll
       for (int w = 0; w < kMaxNodes / 32; ++w) {
         const int j = w * 32 + lane;
-        const unsigned hit = __ballot_sync(0xffffffffu, j > child && j < n && s_par[j] == cur);
-        if (c == kMaxNodes && hit) c = w * 32 + __ffs(hit) - 1;
-      }
-      if (c == kMaxNodes) break;
-      child = c;
-      const int v = s_tok[c];
-      if (v < 0 || v >= a.V) continue;
-      if (sure) {
-        if (v == place) {
-          next = c;
-          break;
-        }
-        continue;
-      }
-      bool again = false;
-      for (int i = lane; i < rejected; i += 32) again |= s_rej[i] == v;
-      again = __any_sync(0xffffffffu, again);
-      const double u = s_u[c];
-      const double e = weight(at(row, v));
-      if constexpr (!kDraft) {
-        if (again) continue;
-        if (u * total < e) {
-          next = c;
-          break;
-        }
-        total -= e;
-      } else {
-        const float q = __ldg(qrow + v);
-        const double r = again ? 0.0 : residual(e, q, rejected);
-        if (u * static_cast<double>(q) * (rejected ? s_mass[rejected - 1] : 1.0) < r) {
-          next = c;
-          break;
-        }
-      }
-      __syncthreads();  // all have read s_rej
-      if (tid == 0) {
-        s_rej[rejected] = v;
-        const int w = v - v0;
-        if (v >= v0 && v < v1) gone[w >> 5] |= 1u << (w & 31);
-      }
-      ++rejected;
-      __syncthreads();
-      if constexpr (kDraft) {
-        if (!exact) {
-          // (the weights' own sum counts the rejected token too)
-          const double rest = mass(0);
-          double lost = weight(at(row, s_rej[0]));
-          total = rest + lost;
-          per_total = 1.0 / total;
-          exact = true;
-        }
-        const double left = mass(rejected);
-        if (tid == 0) {
-          s_mass[rejected - 1] = left;
-          s_per[rejected - 1] = left > 0.0 ? 1.0 / left : 0.0;
-        }
-        __syncthreads();
+        const unsigned hit = __ballot_sync(0xffffffffu, j > cur && j < n && s_par[j] == cur && s_tok[j] == place);
+        if (next < 0 && hit) next = w * 32 + __ffs(hit) - 1;
       }
     }
     if (next >= 0 && a.all_nodes) {
@@ -426,7 +461,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
     int drawn = place;  // the largest, -1 for nothing
     if (!sure) {
       const int k = kDraft ? rejected : 0;
-      const double left = k ? s_mass[k - 1] : mass(0);
       const Exchange* ex = &s_ex[buf ^ 1];
       if (left > 0.0) {
         const double goal = static_cast<double>(a.draws[b]) * left;
