@@ -170,7 +170,15 @@ class LlamaQ8:
     """Weights of a llama-architecture model with Q8_0 matrices, on the device."""
 
     def __init__(self, *, n_embd, n_head, n_kv, head_dim, n_ff, n_vocab, rms_eps, rope_base,
-                 layers, tok_embd: Q8Matrix, out_norm, output: Q8Matrix, dev):
+                 layers, tok_embd: Q8Matrix, out_norm, output: Q8Matrix, dev,
+                 rope_style: str = "norm"):
+        if rope_style not in device._STYLE:
+            raise _lib.B2AShapeError(_lib.ERR_ARG, f"rope style {rope_style!r}")
+        self.rope_style = rope_style
+        # normed heads (qwen3 class): weights of both or of neither in every layer
+        self.normed_heads = bool(layers) and "q_norm" in layers[0]
+        if any(("q_norm" in ly) != self.normed_heads or ("k_norm" in ly) != self.normed_heads for ly in layers):
+            raise _lib.B2AShapeError(_lib.ERR_ARG, "q_norm and k_norm in every layer or in none")
         self.E, self.H, self.KV, self.D, self.F, self.V = (int(n_embd), int(n_head), int(n_kv),
                                                           int(head_dim), int(n_ff), int(n_vocab))
         self.eps, self.rope_base = float(rms_eps), float(rope_base)
@@ -181,8 +189,10 @@ class LlamaQ8:
     @classmethod
     def from_spec(cls, spec: dict, dev) -> "LlamaQ8":
         """spec: hp values, per-layer dicts of Q8_0 bytes (wq, wk, wv, wo,
-        w_gate, w_up, w_down) and f32 norms (attn_norm, ffn_norm), tok_embd,
-        out_norm and output, as a GGUF loader would hand them over."""
+        w_gate, w_up, w_down) and f32 norms (attn_norm, ffn_norm and, of models
+        that norm their heads, q_norm and k_norm of head_dim), tok_embd, out_norm
+        and output, rope_style ("norm" unless given), as a GGUF loader would hand
+        them over."""
         E, H, KV, D, F, V = (spec["n_embd"], spec["n_head"], spec["n_kv"], spec["head_dim"],
                              spec["n_ff"], spec["n_vocab"])
         q8 = lambda data, rows, cols: Q8Matrix.from_q8_0(data, rows, cols, dev)  # noqa: E731
@@ -196,10 +206,17 @@ class LlamaQ8:
                 wo=q8(ly["wo"], E, H * D),
                 wgu=Q8Matrix.interleave(q8(ly["w_gate"], F, E), q8(ly["w_up"], F, E)),
                 w_down=q8(ly["w_down"], E, F)))
+            for name in ("q_norm", "k_norm"):
+                if name in ly:
+                    w = torch.as_tensor(ly[name], dtype=torch.float32).to(dev).contiguous()
+                    if w.shape != (D,):
+                        raise _lib.B2AShapeError(_lib.ERR_SHAPE, f"{name} must have head_dim={D} weights")
+                    layers[-1][name] = w
         return cls(n_embd=E, n_head=H, n_kv=KV, head_dim=D, n_ff=F, n_vocab=V,
                    rms_eps=spec["rms_eps"], rope_base=spec["rope_base"], layers=layers,
                    tok_embd=q8(spec["tok_embd"], V, E), out_norm=spec["out_norm"],
-                   output=q8(spec["output"], V, E), dev=dev)
+                   output=q8(spec["output"], V, E), dev=dev,
+                   rope_style=spec.get("rope_style", "norm"))
 
     @classmethod
     def random(cls, *, n_layer, n_embd, n_head, n_kv, head_dim, n_ff, n_vocab, rms_eps,
@@ -244,6 +261,9 @@ class DecodeChain:
     def __init__(self, model: LlamaQ8, n_ctx: int, kv_dtype: torch.dtype = torch.float16):
         _lib.load()
         m = model
+        if m.normed_heads or m.rope_style != "norm":
+            raise _lib.B2AShapeError(_lib.ERR_UNSUPPORTED,
+                                     "the token chain runs models without normed heads, RoPE of norm style")
         dev = m.device
         self.m, self.n_ctx = m, int(n_ctx)
         self.k_cache = [torch.zeros((1, n_ctx, m.KV, m.D), dtype=kv_dtype, device=dev)

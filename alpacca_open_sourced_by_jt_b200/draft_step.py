@@ -14,12 +14,15 @@ the model itself would have picked:
     qkv  = h . Wqkv^T    b2a_gemm, f32 rows
     RoPE, K/V rows to their slots, q to 16 bits   b2a_rope_append_paged
     att  = the nodes over the cache               b2a_tree_decode
+      (models that norm their heads: b2a_norm_rope_append_paged; a cache of 4
+      bits: b2a_rope_append_q4, b2a_tree_decode_q4)
     x   += att . Wo^T    b2a_gemm, in place
     act  = SwiGLU(RMSNorm(x) . Wgu^T)             b2a_gemm
     x   += act . Wdown^T b2a_gemm, in place
   logits = RMSNorm(x) . Woutput^T                 b2a_gemm_q8
   penalties, biases, masks, picks                 b2a_constrain_logits
-  accepted paths, K/V rows into place             b2a_tree_commit
+  where tokens are sampled, which drafts stand    b2a_verify_picks
+  accepted paths, K/V rows into place             b2a_tree_commit, b2a_tree_commit_q4
 
 Prompts go through the same layers in chunks, as chains.  Where the drafts
 come from is the caller's (an n-gram table, a small model)."""
@@ -34,21 +37,29 @@ from .prefill_chain import ChunkPrefill, _dequant
 
 class DraftStep:
     """`requests` slots over a pool of n_pages pages of page_rows rows per
-    layer (f16 or bf16), at most max_len rows a request (prompts and trees that
-    pass it are refused)."""
+    layer, at most max_len rows a request (prompts and trees that pass it are
+    refused).  dtype (f16 or bf16) is the 16-bit operands'; kv_bits 16: the
+    cache's too, 4: the cache holds blocks of 32 values with a scale
+    (paged.q4_pool)."""
 
     def __init__(self, model: LlamaQ8, requests: int, n_pages: int, *, page_rows: int = 64,
-                 max_len: int = 4096, dtype: torch.dtype = torch.float16):
+                 max_len: int = 4096, dtype: torch.dtype = torch.float16, kv_bits: int = 16):
         _lib.load()
         if dtype not in (torch.float16, torch.bfloat16):
             raise _lib.B2AShapeError(_lib.ERR_DTYPE, "the paged cache must be f16 or bf16")
+        if kv_bits not in (4, 16):
+            raise _lib.B2AShapeError(_lib.ERR_ARG, f"kv_bits {kv_bits} (4 or 16)")
         if model.F % 128:
             raise _lib.B2AShapeError(_lib.ERR_SHAPE, "16-bit GEMMs need n_ff % 128 == 0")
         m, dev = model, model.device
         self.m, self.dt, self.B, self.page_rows, self.max_len = m, dtype, requests, page_rows, max_len
         i32 = dict(dtype=torch.int32, device=dev)
-        self.k_pool = torch.zeros((len(m.layers), n_pages, page_rows, m.KV, m.D), dtype=dtype, device=dev)
-        self.v_pool = torch.zeros_like(self.k_pool)
+        self.pool = self.k_pool = self.v_pool = None
+        if kv_bits == 4:
+            self.pool = paged.q4_pool(n_pages, page_rows, m.KV, m.D, layers=len(m.layers), device=dev)
+        else:
+            self.k_pool = torch.zeros((len(m.layers), n_pages, page_rows, m.KV, m.D), dtype=dtype, device=dev)
+            self.v_pool = torch.zeros_like(self.k_pool)
         self.table = torch.zeros((requests, -(-max_len // page_rows)), **i32)
         self.ring = torch.arange(n_pages, **i32)
         self.ring_state = torch.tensor([0, n_pages], **i32)
@@ -98,11 +109,18 @@ class DraftStep:
         nodes = max(add)
         for li, (ly, w) in enumerate(zip(m.layers, self.w)):
             qkv = device.gemm(self._norm(x, ly["attn_norm"]), w["qkv"]).view(n, m.H + 2 * m.KV, m.D)
-            kp, vp = self.k_pool[li], self.v_pool[li]
-            q = paged.rope_append(qkv[:, :m.H], qkv[:, m.H:m.H + m.KV], qkv[:, m.H + m.KV:],
-                                  plan.positions, plan.slots, self.cos, self.sin, k_pool=kp, v_pool=vp)
-            att = paged.tree_decode(q, kp, vp, self.lens, plan.cu, parents, table=self.table,
-                                    max_nodes=nodes, max_len=self.max_len)
+            rows = (qkv[:, :m.H], qkv[:, m.H:m.H + m.KV], qkv[:, m.H + m.KV:], plan.positions,
+                    plan.slots, self.cos, self.sin)
+            turn = dict(style=m.rope_style, q_norm=ly.get("q_norm"), k_norm=ly.get("k_norm"), eps=m.eps)
+            tree = dict(table=self.table, max_nodes=nodes, max_len=self.max_len)
+            if self.pool is not None:
+                q = paged.rope_append_q4(*rows, pool=self.pool[li], **turn,
+                                         q_out=torch.empty((n, m.H, m.D), dtype=self.dt, device=m.device))
+                att = paged.tree_decode_q4(q, self.pool[li], self.lens, plan.cu, parents, **tree)
+            else:
+                kp, vp = self.k_pool[li], self.v_pool[li]
+                q = paged.rope_append(*rows, k_pool=kp, v_pool=vp, **turn)
+                att = paged.tree_decode(q, kp, vp, self.lens, plan.cu, parents, **tree)
             device.gemm(att.view(n, m.H * m.D), w["wo"], out=x, c_in=x)
             act = torch.empty((n, m.F), dtype=self.dt, device=m.device)
             device.gemm(self._norm(x, ly["ffn_norm"]), w["gu"], out=act, epilogue=device.GEMM_SWIGLU)
@@ -134,12 +152,17 @@ class DraftStep:
                     last[b] = picks[at - 1]
         return last
 
-    def verify(self, trees, **limits):
+    def verify(self, trees, *, uniforms=None, draws=None, temperature=None, draft=None, **limits):
         """One step.  trees: per request (tokens, parents) with the request's
         last token (not yet in the cache) as node 0, or None.  limits: the
         history, penalty, bias and mask arguments of paged.constrain_logits.
+        Greedy unless draws (requests,) f32 and uniforms f32 of all nodes are
+        given: then tokens are sampled with these numbers from [0, 1), with
+        temperature and the drafts' own rows as paged.verify_picks takes them.
         Returns per request the tokens that are new: the accepted drafts and the
         model's own next token (None without a tree)."""
+        if (uniforms is None) != (draws is None) or (draws is None and (temperature is not None or draft is not None)):
+            raise _lib.B2AShapeError(_lib.ERR_ARG, "sampling needs uniforms and draws")
         self._check([() if t is None else t[0] for t in trees])
         for b, t in enumerate(trees):
             if t is None:
@@ -154,14 +177,28 @@ class DraftStep:
         add = [0 if t is None else len(t[0]) for t in trees]
         flat = [x for t in trees if t is not None for x in t[0]]
         par = [x for t in trees if t is not None for x in t[1]]
+        if draws is not None:  # (refused before the step takes pages)
+            for name, t, n in (("uniforms", uniforms, len(flat)), ("draws", draws, self.B),
+                               ("temperature", temperature, self.B)):
+                paged._f32(name, t, n)
+            if draft is not None and (draft.dtype is not torch.float32 or not draft.is_cuda or
+                                      draft.shape != (len(flat), self.m.V) or draft.stride(1) != 1):
+                raise _lib.B2AShapeError(_lib.ERR_SHAPE, "draft must be a CUDA f32 tensor, a row per node")
         dev = self.m.device
         tokens = torch.tensor(flat, dtype=torch.int32, device=dev)
         parents = torch.tensor(par, dtype=torch.int32, device=dev)
         logits, plan = self._forward(add, tokens, parents)
         self.logits, self.picks = paged.constrain_logits(
             logits, plan.cu, parents, tokens, max_nodes=max(add), out=logits, **limits)
-        c = paged.tree_commit(self.picks, tokens, parents, plan.cu, self.lens, self.k_pool,
-                              self.v_pool, table=self.table, max_nodes=max(add), max_len=self.max_len)
+        if draws is not None:
+            self.picks = paged.verify_picks(self.logits, plan.cu, parents, tokens, uniforms, draws,
+                                            max_nodes=max(add), temperature=temperature, draft=draft)
+        commit = dict(table=self.table, max_nodes=max(add), max_len=self.max_len)
+        if self.pool is not None:
+            c = paged.tree_commit_q4(self.picks, tokens, parents, plan.cu, self.lens, self.pool, **commit)
+        else:
+            c = paged.tree_commit(self.picks, tokens, parents, plan.cu, self.lens, self.k_pool,
+                                  self.v_pool, **commit)
         self.lens = c.lens
         path, accepted, nxt = c.path.tolist(), c.accepted.tolist(), c.next_token.tolist()
         self._rows = [r + a for r, a in zip(self._rows, accepted)]
