@@ -16,6 +16,8 @@
 // root and the addresses of a head weigh twice as much: 72 us for 8191 tokens, 32/8
 // heads x 128, bf16).  The cosines and sines of a token serve all of a thread's heads.
 
+#include <cfloat>
+
 #include "q4.cuh"
 
 namespace b2a {
@@ -49,16 +51,28 @@ __device__ __forceinline__ __half block_scale(uint32_t key) {
   const uint16_t h = __half_as_ushort(__float2half_rn(fminf(fmaxf(d, -8160.f), 8160.f)));
   return __ushort_as_half((h & 0x7fff) ? h : 0);
 }
-__device__ __forceinline__ uint32_t code_of(float x, float d) {
-  const int c = __float2int_rd(__fadd_rn(__fdiv_rn(x, d), 8.5f));
-  return d == 0.f ? 8u : static_cast<uint32_t>(min(max(c, 0), 15));
-}
-// The word of 8 consecutive dims.
+// The codes of 8 consecutive dims, a word:  floor(x / d + 8.5), the quotient rounded to
+// nearest.  It is corrected once from x times the rounded reciprocal (P. Markstein, IBM J.
+// Res. Dev. 34, 1990): q + (x - q d) / d with an exact remainder, off by 2^-47 of itself
+// before its rounding.  No quotient lies as near to a border of the rounding: with the 8
+// significant bits of d, a border times d differs from x by 2^-33 of it at least (equal they
+// cannot be: the product of an odd number of 25 bits has more than the 24 of x).
 __device__ __forceinline__ uint32_t codes8(const float* x, float d) {
+  const float r = __frcp_rn(d);
+  const bool far = fabsf(d) == 8160.f;  // (saturated: an infinity has no remainder)
+  const float2 r2 = make_float2(r, r), nd = make_float2(-d, -d);
   uint32_t w = 0;
 #pragma unroll
-  for (int n = 0; n < 8; ++n) w |= code_of(x[n], d) << ((n >> 1) * 4 + (n & 1) * 16);
-  return w;
+  for (int n = 0; n < 4; ++n) {
+    float2 y = make_float2(x[2 * n], x[2 * n + 1]);
+    if (far) y = make_float2(fminf(fmaxf(y.x, -FLT_MAX), FLT_MAX), fminf(fmaxf(y.y, -FLT_MAX), FLT_MAX));
+    const float2 q = mul2(y, r2);
+    const float2 t = fma2(fma2(fma2(q, nd, y), r2, q), make_float2(1.f, 1.f), make_float2(8.5f, 8.5f));
+    // 2^23 + the whole part: its low bits
+    w += __float_as_uint(__fadd_rd(fminf(fmaxf(t.x, 0.f), 15.f), 8388608.f)) << (4 * n);
+    w += __float_as_uint(__fadd_rd(fminf(fmaxf(t.y, 0.f), 15.f), 8388608.f)) << (4 * n + 16);
+  }
+  return d == 0.f ? 0x88888888u : w - (0x4b000000u + (0x4b000000u << 4));
 }
 __device__ __forceinline__ uint32_t largest8(const float* x) {
   uint32_t k = 0;
@@ -68,7 +82,7 @@ __device__ __forceinline__ uint32_t largest8(const float* x) {
 }
 
 constexpr int kThreads = 256;
-constexpr int kResident = 4;  // CTAs per SM of norm_append_kernel
+constexpr int kAppendThreads = 384, kResident = 2;  // most threads, CTAs per SM of norm_append_kernel
 
 // 8 elements as loaded.
 template <typename TS>
@@ -84,76 +98,73 @@ struct Raw {
   }
 };
 
-// Q4: the 4-bit pool; otherwise pools of TK.  A thread goes over the heads that it has
-// of a token and over tokens; while it works on a row the next one comes.
+// Q4: the 4-bit pool; otherwise pools of TK.  A thread keeps its head and goes over tokens;
+// while it works on a row the next one comes.
 template <typename TS, typename TK, typename TQ, bool Q4, bool kNeox>
-__global__ void __launch_bounds__(kThreads, kResident) norm_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, kResident) norm_append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
   const int D = a.D, L = D >> 4;  // a head's dims and lanes: 4, 8 or 16
   const int u = threadIdx.x & (L - 1);
-  const int half = a.n_rot >> 1, all = a.H + 2 * a.KV;
-  const bool turned = 16 * u < a.n_rot;  // the thread's pairs rotate
-  // the thread's dims: 8 from lo on and 8 from hi on (V rows: 16 from 16 u on)
-  const int lo = kNeox && turned ? 8 * u : 16 * u, hi = kNeox && turned ? half + 8 * u : 16 * u + 8;
-  const int h0 = (blockIdx.y * blockDim.x + threadIdx.x) / L, step = gridDim.y * blockDim.x / L;
+  const int half = a.n_rot >> 1, all = a.H + 2 * a.KV, step = gridDim.y * blockDim.x / L;
+  int h = (blockIdx.y * blockDim.x + threadIdx.x) / L;
   // (the same for all lanes: a warp's lanes leave the loop over heads together)
-  const int warp_h0 = (blockIdx.y * blockDim.x + (threadIdx.x & ~31u)) / L;
-  auto fetch = [&](int i, int h, Raw<TS>* r) {
-    if (h >= all) return;
-    const TS* at;
-    if (h < a.H) at = static_cast<const TS*>(a.q) + i * a.q_stride + h * D;
-    else if (h < a.H + a.KV) at = static_cast<const TS*>(a.k) + i * a.k_stride + (h - a.H) * D;
-    else at = static_cast<const TS*>(a.v) + i * a.v_stride + (h - a.H - a.KV) * D;
-    const bool is_v = h >= a.H + a.KV;
-    r[0].load(at + (is_v ? 16 * u : lo));
-    r[1].load(at + (is_v ? 16 * u + 8 : hi));
-  };
-  Raw<TS> raw[2];
-  int p = -1, now = -1;
-  if (static_cast<int>(blockIdx.x) < a.n_tok) {
-    fetch(blockIdx.x, h0, raw);
-    p = a.pos[blockIdx.x];
-    now = a.slots[blockIdx.x];
-  }
-  for (int i = blockIdx.x; i < a.n_tok; i += gridDim.x) {
-    const int next = i + gridDim.x;
-    const bool ok = p >= 0 && p < a.tab_rows && now < a.n_slots;
-    if (!ok && threadIdx.x == 0 && blockIdx.y == 0) set_dev_error(B2A_ERR_POSITION, i);
+  for (int wh = (blockIdx.y * blockDim.x + (threadIdx.x & ~31u)) / L; wh < all; wh += step, h += step) {
+    const bool none = h >= all, is_q = h < a.H, is_v = h >= a.H + a.KV;
+    const int hh = is_q ? h : (is_v ? h - a.H - a.KV : h - a.H);
+    // the thread's dims: 8 from lo on and 8 from hi on; its pairs rotate
+    const bool turned = 16 * u < a.n_rot && !is_v, split = kNeox && turned;
+    const int lo = split ? 8 * u : 16 * u, hi = split ? half + 8 * u : 16 * u + 8;
+    const TS* src = static_cast<const TS*>(is_q ? a.q : (is_v ? a.v : a.k)) + hh * D;
+    const long long stride = is_q ? a.q_stride : (is_v ? a.v_stride : a.k_stride);
+    const float* bias = none ? nullptr : (is_q ? a.bq : (is_v ? a.bv : a.bk));
+    const float* w = none || is_v ? nullptr : (is_q ? a.wq : a.wk);
+    const bool normed = __any_sync(0xffffffffu, w != nullptr);
+    Raw<TS> raw[2];
     float c[8], s[8];
-    if (ok && turned) {
-      const size_t row = static_cast<size_t>(p) * half + 8 * u;
-      paged::load8(a.cos_tab + row, c);
-      paged::load8(a.sin_tab + row, s);
+    int p = -1, now = -1;
+    auto fetch = [&](int i) {
+      if (none) return;
+      raw[0].load(src + i * stride + lo);
+      raw[1].load(src + i * stride + hi);
+    };
+    auto fetch_turn = [&]() {  // of the token at p
+      if (turned && p >= 0 && p < a.tab_rows) {
+        const size_t row = static_cast<size_t>(p) * half + 8 * u;
+        paged::load8(a.cos_tab + row, c);
+        paged::load8(a.sin_tab + row, s);
+      }
+    };
+    if (static_cast<int>(blockIdx.x) < a.n_tok) {
+      fetch(blockIdx.x);
+      p = a.pos[blockIdx.x];
+      now = a.slots[blockIdx.x];
+      fetch_turn();
     }
-    const bool kept = now >= 0;
-    const long long page = (now >> a.page_shift) * a.page_stride;
-    const int in_page = now & ((1 << a.page_shift) - 1);
-    if (next < a.n_tok) {
-      p = a.pos[next];
-      now = a.slots[next];
-    }
-#pragma unroll 1
-    for (int h = h0, wh = warp_h0; wh < all; h += step, wh += step) {
+    for (int i = blockIdx.x; i < a.n_tok; i += gridDim.x) {
+      const int next = i + gridDim.x;
+      const bool ok = p >= 0 && p < a.tab_rows && now < a.n_slots;
+      if (!ok && h == 0 && u == 0) set_dev_error(B2A_ERR_POSITION, i);
+      const int slot = now;
       float x[16];
       raw[0].floats(x);
       raw[1].floats(x + 8);
-      if (wh + step < all) fetch(i, h + step, raw);
-      else if (next < a.n_tok) fetch(next, h0, raw);
-      if (!ok) continue;
-      const bool none = h >= all, is_q = h < a.H, is_v = h >= a.H + a.KV;
-      const int hh = is_q ? h : (is_v ? h - a.H - a.KV : h - a.H);
-      const bool split = kNeox && turned && !is_v;
-      const int la = is_v ? 16 * u : lo, ha = is_v ? 16 * u + 8 : hi;
-      const float* bias = is_q ? a.bq : (is_v ? a.bv : a.bk);
-      if (bias && !none) {
+      if (next < a.n_tok) {
+        fetch(next);
+        p = a.pos[next];
+        now = a.slots[next];
+      }
+      if (!ok) {
+        fetch_turn();
+        continue;
+      }
+      if (bias) {
         float b[16];
-        paged::load8(bias + hh * D + la, b);
-        paged::load8(bias + hh * D + ha, b + 8);
+        paged::load8(bias + hh * D + lo, b);
+        paged::load8(bias + hh * D + hi, b + 8);
 #pragma unroll
         for (int d = 0; d < 16; ++d) x[d] = __fadd_rn(x[d], b[d]);
       }
-      const float* w = is_q ? a.wq : (is_v ? nullptr : a.wk);
-      if (__any_sync(0xffffffffu, w != nullptr)) {
+      if (normed) {
         double s0 = 0.0, s1 = 0.0;
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
@@ -167,31 +178,54 @@ __global__ void __launch_bounds__(kThreads, kResident) norm_append_kernel(const 
         if (L > 8) s0 += __shfl_xor_sync(0xffffffffu, s0, 8);
         const float f = __frcp_rn(__fsqrt_rn(static_cast<float>(s0 * a.inv_d + static_cast<double>(a.eps))));
         if (w != nullptr) {
-          float g[8];
-          paged::load8(w + lo, g);
+          const float2 f2 = make_float2(f, f);
 #pragma unroll
-          for (int d = 0; d < 8; ++d) x[d] = __fmul_rn(__fmul_rn(x[d], f), g[d]);
-          paged::load8(w + hi, g);
+          for (int part = 0; part < 2; ++part) {
+            float g[8];
+            paged::load8(w + (part ? hi : lo), g);
 #pragma unroll
-          for (int d = 0; d < 8; ++d) x[d + 8] = __fmul_rn(__fmul_rn(x[d + 8], f), g[d]);
+            for (int n = 0; n < 8; n += 2) {
+              float* y = x + 8 * part + n;
+              const float2 z = mul2(mul2(make_float2(y[0], y[1]), f2), make_float2(g[n], g[n + 1]));
+              y[0] = z.x;
+              y[1] = z.y;
+            }
+          }
         }
       }
-      if (turned && !is_v) {
+      if (turned) {
+        if constexpr (kNeox) {
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          float& x0 = kNeox ? x[d] : x[2 * d];
-          float& x1 = kNeox ? x[d + 8] : x[2 * d + 1];
-          const float y0 = __fsub_rn(__fmul_rn(x0, c[d]), __fmul_rn(x1, s[d]));
-          x1 = __fadd_rn(__fmul_rn(x0, s[d]), __fmul_rn(x1, c[d]));
-          x0 = y0;
+          for (int n = 0; n < 8; n += 2) {
+            const float2 x0 = make_float2(x[n], x[n + 1]), x1 = make_float2(x[n + 8], x[n + 9]);
+            const float2 c2 = make_float2(c[n], c[n + 1]), s2 = make_float2(s[n], s[n + 1]);
+            const float2 y0 = fma2(mul2(x1, s2), make_float2(-1.f, -1.f), mul2(x0, c2));
+            const float2 y1 = fma2(mul2(x0, s2), make_float2(1.f, 1.f), mul2(x1, c2));
+            x[n] = y0.x;
+            x[n + 1] = y0.y;
+            x[n + 8] = y1.x;
+            x[n + 9] = y1.y;
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const float2 y = fma2(mul2(make_float2(x[2 * n + 1], x[2 * n]), make_float2(s[n], s[n])),
+                                  make_float2(-1.f, 1.f),
+                                  mul2(make_float2(x[2 * n], x[2 * n + 1]), make_float2(c[n], c[n])));
+            x[2 * n] = y.x;
+            x[2 * n + 1] = y.y;
+          }
         }
       }
+      fetch_turn();
       if (is_q) {
         TQ* to = static_cast<TQ*>(a.q_out) + (static_cast<size_t>(i) * a.H + h) * D;
-        paged::store8(to + la, x);
-        paged::store8(to + ha, x + 8);
+        paged::store8(to + lo, x);
+        paged::store8(to + hi, x + 8);
       }
-      if (!kept) continue;
+      if (slot < 0) continue;
+      const long long page = (slot >> a.page_shift) * a.page_stride;
+      const int in_page = slot & ((1 << a.page_shift) - 1);
       if constexpr (Q4) {
         if (__all_sync(0xffffffffu, is_q || none)) continue;
         // the largest of the block: 2 lanes hold 16 consecutive dims each; split, 4 lanes
@@ -209,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, kResident) norm_append_kernel(const 
         const __half da = block_scale(ka), db = block_scale(kb);
         unsigned char* g = static_cast<unsigned char*>(a.k_pool) + page +
                            (static_cast<long long>(hh) * ((1 << a.page_shift) >> 4) + (in_page >> 4)) * granule_bytes(D);
-        const int r = in_page & 15, ua = la >> 3, ub = ha >> 3;
+        const int r = in_page & 15, ua = lo >> 3, ub = hi >> 3;
         *reinterpret_cast<uint32_t*>(g + (is_v ? v_word(D, r, ua) : k_word(D, r, ua))) = codes8(x, __half2float(da));
         *reinterpret_cast<uint32_t*>(g + (is_v ? v_word(D, r, ub) : k_word(D, r, ub))) = codes8(x + 8, __half2float(db));
         // (the lane with a block's first word writes its scale)
@@ -221,8 +255,8 @@ __global__ void __launch_bounds__(kThreads, kResident) norm_append_kernel(const 
         if (is_q || none) continue;
         TK* row = static_cast<TK*>(is_v ? a.v_pool : a.k_pool) + page +
                   (static_cast<long long>(in_page) * a.KV + hh) * D;
-        paged::store8(row + la, x);
-        paged::store8(row + ha, x + 8);
+        paged::store8(row + lo, x);
+        paged::store8(row + hi, x + 8);
       }
     }
   }
@@ -231,41 +265,44 @@ __global__ void __launch_bounds__(kThreads, kResident) norm_append_kernel(const 
 // ---------------------------------------------------------------------------
 // Rows of a 4-bit pool, as values
 // ---------------------------------------------------------------------------
+// A warp takes a block of 32 dims of one head of 8 tokens, a word a lane: 8 rows side by
+// side fill the sectors of V words, 4 words those of K words and of the outputs.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) q4_rows_kernel(const Pool pool, const int* __restrict__ slots,
                                                            T* __restrict__ k, T* __restrict__ v,
                                                            int n_tok, int KV, int D) {
   pdl_wait();
-  const int words = D / 8;
-  const long long total = static_cast<long long>(n_tok) * KV * words;
   const long long n_slots = static_cast<long long>(pool.n_pages) << pool.page_shift;
-  for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * kThreads) {
-    const int u = static_cast<int>(i % words);
-    const long long th = i / words;
-    const int h = static_cast<int>(th % KV), tok = static_cast<int>(th / KV);
+  const int lane = threadIdx.x & 31, blocks = D >> 5;
+  for (long long tok = blockIdx.x * 8LL + (lane >> 2); tok - (lane >> 2) < n_tok; tok += gridDim.x * 8LL) {
+    if (tok >= n_tok) continue;
     const int slot = slots[tok];
-    float x[8], y[8];
+    if (slot >= n_slots && threadIdx.x < 32 && (lane & 3) == 0) set_dev_error(B2A_ERR_POSITION, static_cast<int>(tok));
+    const bool held = slot >= 0 && slot < n_slots;
+    const int in_page = slot & ((1 << pool.page_shift) - 1), r = in_page & 15;
+    for (int j = threadIdx.x >> 5; j < KV * blocks; j += kThreads / 32) {
+      const int h = j / blocks, b = j - h * blocks, u = 4 * b + (lane & 3);
+      float x[8], y[8];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) x[d] = y[d] = 0.f;
-    if (slot >= n_slots) {
-      if (h == 0 && u == 0) set_dev_error(B2A_ERR_POSITION, tok);
-    } else if (slot >= 0) {
-      const int in_page = slot & ((1 << pool.page_shift) - 1), r = in_page & 15;
-      const unsigned char* g = granule(pool, D, slot >> pool.page_shift, h, in_page);
-      const uint32_t kw = *reinterpret_cast<const uint32_t*>(g + k_word(D, r, u));
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(g + v_word(D, r, u));
-      const float dk = __half2float(*reinterpret_cast<const __half*>(g + k_scale(D, r, u >> 2)));
-      const float dv = __half2float(*reinterpret_cast<const __half*>(g + v_scale(D, r, u >> 2)));
+      for (int d = 0; d < 8; ++d) x[d] = y[d] = 0.f;
+      if (held) {
+        const unsigned char* g = granule(pool, D, slot >> pool.page_shift, h, in_page);
+        const uint32_t kw = *reinterpret_cast<const uint32_t*>(g + k_word(D, r, u));
+        const uint32_t vw = *reinterpret_cast<const uint32_t*>(g + v_word(D, r, u));
+        const float dk = __half2float(*reinterpret_cast<const __half*>(g + k_scale(D, r, b)));
+        const float dv = __half2float(*reinterpret_cast<const __half*>(g + v_scale(D, r, b)));
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const int sh = (d >> 1) * 4 + (d & 1) * 16;
-        x[d] = dk * static_cast<float>(static_cast<int>(kw >> sh & 15u) - 8);
-        y[d] = dv * static_cast<float>(static_cast<int>(vw >> sh & 15u) - 8);
+        for (int d = 0; d < 8; ++d) {
+          const int sh = (d >> 1) * 4 + (d & 1) * 16;
+          // (2^23 + code less 2^23 + 8)
+          x[d] = dk * (__uint_as_float(0x4b000000u | (kw >> sh & 15u)) - 8388616.f);
+          y[d] = dv * (__uint_as_float(0x4b000000u | (vw >> sh & 15u)) - 8388616.f);
+        }
       }
+      const size_t at = (static_cast<size_t>(tok) * KV + h) * D + 8 * u;
+      paged::store8(k + at, x);
+      paged::store8(v + at, y);
     }
-    paged::store8(k + i * 8, x);
-    paged::store8(v + i * 8, y);
   }
 }
 
@@ -376,15 +413,16 @@ int norm_append_check(const char* who, const Q4::AppendArgs& a, int in_dtype, in
 
 template <typename TS, typename TK, typename TQ, bool kQ4>
 cudaError_t norm_append_launch(const Q4::AppendArgs& a, cudaStream_t st) {
-  // A CTA per token, going over its heads; few tokens: a token's heads over more CTAs,
-  // until there are a few per SM.
-  const int all = a.H + 2 * a.KV, lanes = a.D / 16, at_once = Q4::kThreads / lanes;
-  int gy = (all + at_once - 1) / at_once;
-  const int enough = (Q4::kResident * b2a_host::sm_count() + a.n_tok - 1) / a.n_tok;
-  if (gy > enough) gy = enough;
-  const int resident = Q4::kResident * b2a_host::sm_count();
-  const dim3 grid(a.n_tok < resident ? a.n_tok : resident, gy);
-  const dim3 block(all <= at_once ? (all * lanes + 31) / 32 * 32 : Q4::kThreads);
+  // A CTA per token, its threads dealt evenly to rounds over the heads; few tokens: a
+  // token's rounds over more CTAs, until there are a few per SM.
+  const int all = a.H + 2 * a.KV, lanes = a.D / 16;
+  int rounds = (all * lanes + Q4::kAppendThreads - 1) / Q4::kAppendThreads;
+  const int threads = ((all + rounds - 1) / rounds * lanes + 31) / 32 * 32;
+  const int at_once = threads / lanes;
+  rounds = (all + at_once - 1) / at_once;
+  const int resident = Q4::kResident * (Q4::kAppendThreads / threads) * b2a_host::sm_count();
+  const int enough = (resident + a.n_tok - 1) / a.n_tok;
+  const dim3 grid(a.n_tok < resident ? a.n_tok : resident, rounds < enough ? rounds : enough), block(threads);
   if (a.neox) return b2a_host::launch(Q4::norm_append_kernel<TS, TK, TQ, kQ4, true>, grid, block, 0, st, a);
   return b2a_host::launch(Q4::norm_append_kernel<TS, TK, TQ, kQ4, false>, grid, block, 0, st, a);
 }
@@ -489,11 +527,11 @@ int b2a_q4_rows(const void* pool, int n_pages, int page_rows, long long page_byt
     return fail(B2A_ERR_ALIGN, "q4_rows: outputs must be 16-byte aligned");
   if (n_tok == 0) return B2A_OK;
   const Q4::Pool p = q4_pool_of(pool, n_pages, page_rows, page_bytes, D, true);
-  const long long ctas = (static_cast<long long>(n_tok) * KV * (D / 8) + Q4::kThreads - 1) / Q4::kThreads;
+  const int ctas = n_tok / 8 + (n_tok % 8 != 0);
   const int most = 8 * b2a_host::sm_count();
   const cudaError_t e = with_type(out_dtype, [&](auto* t) {
     using T = typename std::remove_pointer<decltype(t)>::type;
-    return b2a_host::launch(Q4::q4_rows_kernel<T>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)),
+    return b2a_host::launch(Q4::q4_rows_kernel<T>, dim3(ctas < most ? ctas : most),
                             dim3(Q4::kThreads), 0, static_cast<cudaStream_t>(stream), p, slot_dev,
                             static_cast<T*>(k_out), static_cast<T*>(v_out), n_tok, KV, D);
   });
