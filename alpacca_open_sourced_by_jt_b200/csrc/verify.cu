@@ -42,22 +42,22 @@ struct Args {
   int slice, warp_slice, warp_groups;  // tokens of a CTA, of a warp of it, that in groups of 128
 };
 
-// e^y for y <= 0 in 64 bits (relative error about 10^-13): y log2(e) = n + i / 16 + f
-// with |f| <= 1 / 32, a table of 2^(i / 16) and the series of 2^f up to f^5.
-constexpr int kTable = 16;
-__device__ __forceinline__ double exp_below(double y16, const double* table) {  // of y log2(e) x 16
-  if (!(y16 > -16.0 * 1000.0)) return 0.0;
+// e^y in 64 bits (relative error about 10^-13) from y log2(e) x kTable between about -kTable
+// x 1000 and 0:  n + f with n whole, a table of 2^(i / kTable) and the series of 2^(f /
+// kTable), |f| <= 1/2, up to f^4.
+constexpr int kTable = 64;
+__device__ __forceinline__ double exp_below(double y, const double* table) {
   constexpr double kRound = 6755399441055744.0;  // 1.5 x 2^52: the sum's low bits are the whole part
-  const double t = y16 + kRound;
+  constexpr double c = 0.6931471805599453 / kTable;
+  const double t = y + kRound;
   const int n = __double2loint(t);
-  const double f = (y16 - (t - kRound)) * 0.043321698784996582;  // ln(2) / 16
-  double p = fma(f, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(f, p, 1.0 / 6.0);
-  p = fma(f, p, 0.5);
-  p = fma(f, p, 1.0);
+  const double f = y - (t - kRound);
+  double p = fma(f, c * c * c * c / 24.0, c * c * c / 6.0);
+  p = fma(f, p, c * c / 2.0);
+  p = fma(f, p, c);
   p = fma(f, p, 1.0);
   p *= table[n & (kTable - 1)];
-  return __hiloint2double(__double2hiint(p) + (n >> 4) * (1 << 20), __double2loint(p));
+  return __hiloint2double(__double2hiint(p) + (n & ~(kTable - 1)) * ((1 << 20) / kTable), __double2loint(p));
 }
 
 struct Exchange {
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
   const float heat = a.temperature ? (a.temperature[b] > FLT_MAX ? FLT_MAX : a.temperature[b]) : 1.f;
   const bool greedy = !(heat > 0.f);
   const double cold = greedy ? 0.0 : 1.0 / static_cast<double>(heat);
-  const double cold16 = fmin(cold * 1.4426950408889634 * kTable, 1e300);
+  const double cold_t = fmin(cold * 1.4426950408889634 * kTable, 1e300);
   const float cold2 = static_cast<float>(fmin(cold * 1.4426950408889634, 1e30));
   int buf = 0;
 
@@ -227,39 +227,30 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
         }
       }
     }
-    // the lowest place of the largest, the sum relative to it
-    auto join = [&](float t2, float p2, int i2) {
-      if (t2 > top) {
-        part = p2 + (top > -INFINITY ? part * fast_exp2((top - t2) * cold2) : 0.f);
-        top = t2;
-        place = i2;
-      } else {
-        part += t2 > -INFINITY ? p2 * fast_exp2((t2 - top) * cold2) : 0.f;
-        if (t2 == top) place = min(place, i2);
-      }
-    };
+    // The lowest place of the largest, the sum relative to it: of a warp's lanes.
+    auto join = [&]() {
+      const uint32_t u = __float_as_uint(top);  // (in the order of the floats)
+      const uint32_t key = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+      const uint32_t most = __reduce_max_sync(0xffffffffu, key);
+      const float all = __uint_as_float((most & 0x80000000u) ? most ^ 0x80000000u : ~most);
+      place = __reduce_min_sync(0xffffffffu, top == all ? place : a.V);
+      part = top > -INFINITY ? part * fast_exp2((top - all) * cold2) : 0.f;
+      top = all;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float t2 = __shfl_xor_sync(0xffffffffu, top, o), p2 = __shfl_xor_sync(0xffffffffu, part, o);
-      join(t2, p2, __shfl_xor_sync(0xffffffffu, place, o));
-    }
+      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    };
+    join();
     if (lane == 0) {
       s_top[warp] = top;
       s_part[warp] = part;
       s_at[warp] = place;
     }
     __syncthreads();
-    auto join_lanes = [&](int most) {  // of the first `most` lanes, a power of two
-      for (int o = most / 2; o > 0; o >>= 1) {
-        const float t2 = __shfl_xor_sync(0xffffffffu, top, o), p2 = __shfl_xor_sync(0xffffffffu, part, o);
-        join(t2, p2, __shfl_xor_sync(0xffffffffu, place, o));
-      }
-    };
     if (warp == 0) {
       top = lane < kWarps ? s_top[lane] : -INFINITY;
       part = lane < kWarps ? s_part[lane] : 0.f;
       place = lane < kWarps ? s_at[lane] : a.V;
-      join_lanes(32);
+      join();
       if (lane == 0) {
         s_ex[buf].top = top;
         s_ex[buf].part = part;
@@ -272,10 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
       top = lane < ranks ? e->top : -INFINITY;
       part = lane < ranks ? e->part : 0.f;
       place = lane < ranks ? e->at : a.V;
-      join_lanes(kCluster);
-      top = __shfl_sync(0xffffffffu, top, 0);
-      part = __shfl_sync(0xffffffffu, part, 0);
-      place = __shfl_sync(0xffffffffu, place, 0);
+      join();
     }
     buf ^= 1;
     if (!(top > -INFINITY)) {  // nothing can be picked
@@ -287,22 +275,29 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
     // ---- the children in order ----------------------------------------------------------
     int rejected = 0, next = -1;
     double total = part;  // sum of r (certain drafts); drafts with a row: r is relative to it
+    // (weights below e^-690 are 0; comparing with the logit that has it, a NaN is 0 too)
+    const float least = fmaxf(fmaf(-690.f, heat, top), -FLT_MAX);
     auto weight = [&](float x) {  // e^((x - M) / T)
-      return x > -INFINITY ? exp_below((static_cast<double>(x) - M) * cold16, s_table) : 0.0;
+      const double e = exp_below((static_cast<double>(fmaxf(x, least)) - M) * cold_t, s_table);
+      return x >= least ? e : 0.0;
     };
     // r(v) after k rejections of drafts with a row, from e^((x - M) / T)
     double per_total = 1.0 / total;
     auto residual = [&](double e, float q, int k) {
-      double r = e * per_total;
-      for (int i = 0; i < k; ++i) r = fmax((i ? r * s_per[i - 1] : r) - static_cast<double>(q), 0.0);
-      return r;
+      const double p = q;
+      double r = fma(e, per_total, -p);
+      for (int i = 1; i <= k; ++i) {
+        r = r > 0.0 ? r : 0.0;
+        if (i < k) r = fma(r, s_per[i - 1], -p);
+      }
+      return k ? r : e * per_total;
     };
     const bool whole = reinterpret_cast<uintptr_t>(row) % 16 == 0 &&
                        reinterpret_cast<uintptr_t>(qrow) % 16 == 0;  // (slices are whole groups)
-    // What is left of 4 consecutive tokens after k rejections (the rejected themselves
-    // apart).
-    auto left4 = [&](int v, int k, double* r) {
-      float x[4], q[4] = {0.f, 0.f, 0.f, 0.f};
+    // 4 consecutive tokens' logits and draft probabilities; what is left of them after k
+    // rejections (the rejected themselves apart).  The tokens go through each step side by
+    // side: a chain of 64-bit operations is long.
+    auto load4 = [&](int v, int k, float* x, float* q) {
       if (whole && v + 4 <= v1) {
         paged::load4(row + v, x);
         if (kDraft && k) paged::load4(qrow + v, q);
@@ -310,24 +305,44 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[e] = v + e < v1 ? at(row, v + e) : -INFINITY;
-          if (kDraft && k && v + e < v1) q[e] = qrow[v + e];
+          q[e] = kDraft && k && v + e < v1 ? qrow[v + e] : 0.f;
         }
       }
-      const uint32_t marks = gone[(v - v0) >> 5] >> ((v - v0) & 31);
+    };
+    auto left4 = [&](int v, int k, const float* x, const float* q, double* r) {
+      const uint32_t marks = v < v1 ? gone[(v - v0) >> 5] >> ((v - v0) & 31) : 0u;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const double y = weight(x[e]);
-        r[e] = (marks >> e & 1u) ? 0.0 : (kDraft && k ? residual(y, q[e], k) : y);
+      for (int e = 0; e < 4; ++e) r[e] = weight(x[e]);
+      if (kDraft && k) {
+        double per = per_total;
+        for (int i = 0; i < k; ++i) {
+          if (i) per = s_per[i - 1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const double y = fma(r[e], per, -static_cast<double>(q[e]));
+            r[e] = y > 0.0 ? y : 0.0;
+          }
+        }
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = (marks >> e & 1u) ? 0.0 : r[e];
     };
     // The sum of it over the row; those of the warps' groups stay in s_group, the warps'
     // in s_warp, the CTA's in s_ex (the other buffer).
     auto mass = [&](int k) {
       double sum = 0.0;
       const int lo = v0 + warp * a.warp_slice;
+      float x[4], q[4], x_next[4], q_next[4];
+      load4(lo + 4 * lane, k, x_next, q_next);
       for (int i = 0; i < a.warp_groups && lo + 128 * i < v1; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = x_next[e];
+          q[e] = q_next[e];
+        }
+        if (i + 1 < a.warp_groups) load4(lo + 128 * (i + 1) + 4 * lane, k, x_next, q_next);
         double r[4];
-        left4(lo + 128 * i + 4 * lane, k, r);
+        left4(lo + 128 * i + 4 * lane, k, x, q, r);
         double s = (r[0] + r[1]) + (r[2] + r[3]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -504,8 +519,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
               run += s;
             }
             const int v = lo + 128 * group + 4 * lane;
+            float x[4], q[4];
             double r[4];
-            left4(v, k, r);
+            load4(v, k, x, q);
+            left4(v, k, x, q, r);
             double inc = (r[0] + r[1]) + (r[2] + r[3]);
             const double mine = inc;
 #pragma unroll
