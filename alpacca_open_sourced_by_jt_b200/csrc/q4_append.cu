@@ -199,21 +199,19 @@ __global__ void __launch_bounds__(kAppendThreads, kResident) norm_append_kernel(
           for (int n = 0; n < 8; n += 2) {
             const float2 x0 = make_float2(x[n], x[n + 1]), x1 = make_float2(x[n + 8], x[n + 9]);
             const float2 c2 = make_float2(c[n], c[n + 1]), s2 = make_float2(s[n], s[n + 1]);
-            const float2 y0 = fma2(mul2(x1, s2), make_float2(-1.f, -1.f), mul2(x0, c2));
-            const float2 y1 = fma2(mul2(x0, s2), make_float2(1.f, 1.f), mul2(x1, c2));
-            x[n] = y0.x;
-            x[n + 1] = y0.y;
-            x[n + 8] = y1.x;
-            x[n + 9] = y1.y;
+            const float2 p0 = mul2(x0, c2), p1 = mul2(x1, s2), p2 = mul2(x0, s2), p3 = mul2(x1, c2);
+            x[n] = __fsub_rn(p0.x, p1.x);
+            x[n + 1] = __fsub_rn(p0.y, p1.y);
+            x[n + 8] = __fadd_rn(p2.x, p3.x);
+            x[n + 9] = __fadd_rn(p2.y, p3.y);
           }
         } else {
 #pragma unroll
           for (int n = 0; n < 8; ++n) {
-            const float2 y = fma2(mul2(make_float2(x[2 * n + 1], x[2 * n]), make_float2(s[n], s[n])),
-                                  make_float2(-1.f, 1.f),
-                                  mul2(make_float2(x[2 * n], x[2 * n + 1]), make_float2(c[n], c[n])));
-            x[2 * n] = y.x;
-            x[2 * n + 1] = y.y;
+            const float2 p = mul2(make_float2(x[2 * n], x[2 * n + 1]), make_float2(c[n], c[n]));
+            const float2 r = mul2(make_float2(x[2 * n + 1], x[2 * n]), make_float2(s[n], s[n]));
+            x[2 * n] = __fsub_rn(p.x, r.x);
+            x[2 * n + 1] = __fadd_rn(r.y, p.y);
           }
         }
       }
