@@ -25,11 +25,10 @@
 // second product (no transposition), and a lane's four keys of a granule are rows
 // 4t .. 4t + 3, side by side in the pool.
 //
-// One persistent CTA per SM.  One warp plans: it walks the CTA's items and looks up
-// their pages, segment by segment, into a queue in shared memory.  The others take
-// the steps (32 keys) of a segment in turn.  Each brings its own steps, one bulk
-// copy or two where pages have 16 rows, through a ring of its own, so they meet only
-// at an item's end.
+// One persistent CTA per SM.  One warp feeds the others: it walks the CTA's items, looks
+// up their pages and brings the steps (32 keys) in by bulk copies, one a step or two where
+// pages have 16 rows, a step a lane.  The others take the steps in turn, each through a
+// ring of its own, so they meet only at an item's end.
 #include <limits.h>
 #include <math.h>
 
@@ -42,30 +41,24 @@ namespace tree {
 
 constexpr int kQ4Keys = 32;  // keys of a step (and of a tile of the work division)
 
-// What the planning warp hands on: steps t0 .. t1 - 1 of an item and their pages.
-constexpr int kQ4Rounds = 8;  // steps of a warp in a segment
 constexpr int kQ4Queue = 4;
 
-template <int W>
-struct Q4Seg {
+// What the feeding warp hands on.
+struct Q4Item {
   Item it;
-  int t0, t1;
-  int last;      // the item ends with it
-  int end;       // nothing follows (1, with requests left out 2)
-  int gone;      // some granule has no page
-  int g0;        // number of step t0 among all of the CTA's
-  int pages[2][kQ4Rounds * W];  // of a step's two granules, -1: none
+  int g0;   // number of its first step among all of the CTA's
+  int end;  // nothing follows (1, with requests left out 2)
 };
 
 template <int W, int S>
 struct alignas(128) Q4Shared {  // (the rings stand behind it)
   static constexpr int kStepKeys = kQ4Keys, kTileSteps = 1;  // a step's keys, a tile's steps
-  static constexpr bool kItems = false;            // the items go by a queue of their own, too
-  uint64_t full[W][S];                             // a warp's stages
-  uint64_t seg_full[kQ4Queue], seg_empty[kQ4Queue];
+  uint64_t full[W][S], empty[W][S];                // a warp's stages
+  uint64_t item_full[kQ4Queue], item_empty[kQ4Queue];
   uint64_t handed, joined, read;                   // at an item's end
   uint4 sees[W][16];                               // the nodes that a warp's rows see
-  Q4Seg<W> seg[kQ4Queue];
+  Q4Item item[kQ4Queue];
+  uint8_t gone[W][S];                              // bit i: granule i of the step has no page
 };
 
 template <int D, int NT>
@@ -104,115 +97,110 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0
         "f"(c[3]));
 }
 
-// The planning warp.  Requests are looked at 32 at a time, one by each lane.
-template <int W, typename Shared>
-__device__ __forceinline__ void q4_plan(const Batch& bt, Shared& sh, int lane) {
+// The walk over a CTA's items by a whole warp.  Requests are looked at 32 at a time, one by
+// each lane.
+struct Q4Walk {
+  long long off, left;
+  int b, base, n32, len32, node32;  // of request base + lane
+  bool left_out;
+  __device__ __forceinline__ explicit Q4Walk(const Start& start)
+      : off(start.off), left(start.left), b(start.b), base(-32), n32(0), len32(0), node32(0),
+        left_out(start.left_out) {}
+  // (as Walker::next)
+  __device__ __forceinline__ bool next(const Batch& bt, int lane, int tile_keys, Item& it) {
+    while (left > 0 && b < bt.B) {
+      if (b - base >= 32) {
+        base = b & ~31;
+        n32 = len32 = node32 = 0;
+        if (base + lane < bt.B) {
+          request(bt, base + lane, n32, len32, left_out);
+          node32 = bt.cu[base + lane];
+        }
+      }
+      it.b = b;
+      it.n = __shfl_sync(0xffffffffu, n32, b - base);
+      it.len = __shfl_sync(0xffffffffu, len32, b - base);
+      it.node0 = __shfl_sync(0xffffffffu, node32, b - base);
+      it.tiles = (it.len + it.n + tile_keys - 1) / tile_keys;
+      const long long u = units_of(bt, it.n, it.len);
+      if (off >= u) {
+        off -= u;
+        ++b;
+        continue;
+      }
+      const int per = bt.by_item ? 1 : it.tiles;
+      const int idx = (off >> 31) == 0 ? static_cast<int>(static_cast<uint32_t>(off) / static_cast<uint32_t>(per))
+                                       : static_cast<int>(off / per);
+      const int at = static_cast<int>(off - static_cast<long long>(idx) * per);
+      int take = per - at;
+      if (take > left) take = static_cast<int>(left);
+      it.t0 = bt.by_item ? 0 : at;
+      it.t1 = bt.by_item ? it.tiles : at + take;
+      off += take;
+      left -= take;
+      if (member_item(bt, blockIdx.x, idx, blocks_of(bt, it.n), it.kvh, it.blk)) return true;
+    }
+    return false;
+  }
+};
+
+// The feeding warp: items to the queue, and each step's granules to the ring of the warp
+// that takes it, a step a lane.  Step number g goes to warp g % W; the slots of a batch of
+// steps are all different, so no lane waits for a copy that another is to make.
+template <int W, int S, int D, typename Shared>
+__device__ __forceinline__ void q4_feed(const Batch& bt, const q4::Pool& pool, Shared& sh, uint8_t* rings, int lane) {
   constexpr int TS = Shared::kTileSteps, SK = Shared::kStepKeys;
+  constexpr int kBatch = W * S < 32 ? W * S : 32, kGranule = q4::granule_bytes(D);
   const Start start = locate(bt, team_of(bt, blockIdx.x));
-  long long off = start.off, left = start.left;
-  int b = start.b, base = -32, slot = 0, items = 0, steps = 0;
-  uint32_t round = 0;
-  int n32 = 0, len32 = 0, node32 = 0;  // of request base + lane
-  const bool split = bt.table && bt.page_shift == 4;
-  auto room = [&]() {  // a free place in the queue
-    return round == 0 ||
-           __all_sync(0xffffffffu, mbar_wait(&sh.seg_empty[slot], (round & 1) ^ 1, 0x3F200)) != 0;
+  Q4Walk walk(start);
+  uint32_t items = 0;
+  int g = 0;
+  const bool split = bt.table && bt.page_shift == 4;  // a step's granules lie in two pages
+  const int page_mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
+  auto hand_on = [&](const Item& it, int end) {
+    const int place = items % kQ4Queue;
+    if (items >= kQ4Queue &&
+        !__all_sync(0xffffffffu, mbar_wait(&sh.item_empty[place], (items / kQ4Queue - 1) & 1, 0x3F210)))
+      return false;
+    if (lane == 0) {
+      sh.item[place] = Q4Item{it, g, end};
+      mbar_arrive(&sh.item_full[place]);
+    }
+    ++items;
+    return true;
   };
-  auto hand_on = [&]() {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.seg_full[slot]);
-    if (++slot == kQ4Queue) {
-      slot = 0;
-      ++round;
-    }
-  };
-  while (left > 0 && b < bt.B) {
-    if (b - base >= 32) {
-      base = b & ~31;
-      n32 = len32 = node32 = 0;
-      if (base + lane < bt.B) {
-        request(bt, base + lane, n32, len32, start.left_out);
-        node32 = bt.cu[base + lane];
-      }
-    }
-    Item it;
-    it.b = b;
-    it.n = __shfl_sync(0xffffffffu, n32, b - base);
-    it.len = __shfl_sync(0xffffffffu, len32, b - base);
-    it.node0 = __shfl_sync(0xffffffffu, node32, b - base);
-    it.tiles = (it.len + it.n + TS * SK - 1) / (TS * SK);
-    const long long u = units_of(bt, it.n, it.len);
-    if (off >= u) {
-      off -= u;
-      ++b;
-      continue;
-    }
-    // (as Walker::next)
-    const int per = bt.by_item ? 1 : it.tiles;
-    const int idx = (off >> 31) == 0 ? static_cast<int>(static_cast<uint32_t>(off) / static_cast<uint32_t>(per))
-                                     : static_cast<int>(off / per);
-    const int at = static_cast<int>(off - static_cast<long long>(idx) * per);
-    int take = per - at;
-    if (take > left) take = static_cast<int>(left);
-    it.t0 = bt.by_item ? 0 : at;
-    it.t1 = bt.by_item ? it.tiles : at + take;
-    off += take;
-    left -= take;
-    if (!member_item(bt, blockIdx.x, idx, blocks_of(bt, it.n), it.kvh, it.blk)) continue;
-    const int rows = it.len + it.n;
-    if constexpr (Shared::kItems) {
-      const int place = items % kQ4Queue;
-      if (items >= kQ4Queue && !__all_sync(0xffffffffu, mbar_wait(&sh.item_empty[place], (items / kQ4Queue - 1) & 1, 0x3F210)))
-        return;
-      if (lane == 0) {
-        sh.item[place] = it;
-        sh.item_end[place] = 0;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.item_full[place]);
-      ++items;
-    }
-    for (int t0 = it.t0 * TS; t0 < it.t1 * TS; t0 += kQ4Rounds * W) {
-      if (!room()) return;
-      Q4Seg<W>& seg = sh.seg[slot];
-      const int t1 = min(t0 + kQ4Rounds * W, it.t1 * TS);
-      bool gone = false;
-#pragma unroll 4
-      for (int i = lane; i < t1 - t0; i += 32) {
-        const int row = (t0 + i) * SK;
+  Item it = {};
+  while (walk.next(bt, lane, TS * SK, it)) {
+    if (!hand_on(it, 0)) return;
+    const int rows = it.len + it.n, steps = (it.t1 - it.t0) * TS;
+    for (int i0 = 0; i0 < steps; i0 += kBatch) {
+      const int i = i0 + lane;
+      bool ok = true;
+      if (lane < kBatch && i < steps) {
+        const int row = (it.t0 * TS + i) * SK;
         const bool one = row < rows, two = SK > 16 && row + 16 < rows;  // (a tile's last steps may hold nothing)
         const int e0 = one ? table_entry(bt, it.b, row) : 0;
         const int e1 = split && two ? table_entry(bt, it.b, row + 16) : e0;
         const int p0 = checked_page(bt, it.b, e0), p1 = checked_page(bt, it.b, e1);
-        seg.pages[0][i] = one && p0 < bt.n_pages ? p0 : -1;
-        seg.pages[1][i] = two && p1 < bt.n_pages ? p1 : -1;
-        gone |= p0 >= bt.n_pages || p1 >= bt.n_pages;
+        const bool has0 = one && p0 < bt.n_pages, has1 = two && p1 < bt.n_pages;
+        const uint32_t turn = static_cast<uint32_t>(g + i), w = turn % W, use = turn / W, s = use % S;
+        if (use >= S) ok = mbar_wait(&sh.empty[w][s], (use / S - 1) & 1, 0x3F200) != 0;
+        if (ok) {
+          sh.gone[w][s] = (has0 ? 0 : 1) | (two && !has1 ? 2 : 0);
+          uint64_t* bar = &sh.full[w][s];
+          uint8_t* dst = rings + (w * S + s) * (SK / 16 * kGranule);
+          mbar_arrive_expect_tx(bar, (has0 + has1) * kGranule);
+          if (has0)
+            bulk_load(dst, q4::granule(pool, D, p0, it.kvh, row & page_mask), has1 && !split ? 2 * kGranule : kGranule, bar);
+          if (has1 && split)
+            bulk_load(dst + kGranule, q4::granule(pool, D, p1, it.kvh, (row + 16) & page_mask), kGranule, bar);
+        }
       }
-      gone = __any_sync(0xffffffffu, gone);
-      if (lane == 0) {
-        seg.it = it;
-        seg.t0 = t0;
-        seg.t1 = t1;
-        seg.last = t1 == it.t1 * TS;
-        seg.end = 0;
-        seg.gone = gone;
-        seg.g0 = steps;
-      }
-      steps += t1 - t0;
-      hand_on();
+      if (!__all_sync(0xffffffffu, ok)) return;
     }
+    g += steps;
   }
-  if constexpr (Shared::kItems) {
-    const int place = items % kQ4Queue;
-    if (items >= kQ4Queue && !__all_sync(0xffffffffu, mbar_wait(&sh.item_empty[place], (items / kQ4Queue - 1) & 1, 0x3F210)))
-      return;
-    if (lane == 0) sh.item_end[place] = start.left_out ? 2 : 1;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.item_full[place]);
-  }
-  if (!room()) return;
-  if (lane == 0) sh.seg[slot].end = start.left_out ? 2 : 1;
-  hand_on();
+  hand_on(it, start.left_out ? 2 : 1);
 }
 
 template <typename T, int D, int NT>
@@ -227,11 +215,14 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < W) {
-    for (int s = 0; s < C::kStages; ++s) mbar_init(&sh.full[threadIdx.x][s], 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&sh.full[threadIdx.x][s], 1);
+      mbar_init(&sh.empty[threadIdx.x][s], 1);
+    }
   } else if (threadIdx.x == W * 32) {
     for (int i = 0; i < kQ4Queue; ++i) {
-      mbar_init(&sh.seg_full[i], 1);
-      mbar_init(&sh.seg_empty[i], W);
+      mbar_init(&sh.item_full[i], 1);
+      mbar_init(&sh.item_empty[i], W);
     }
     mbar_init(&sh.handed, W / 2);
     mbar_init(&sh.joined, (W + 1) / 2);
@@ -241,7 +232,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == W) {
-    q4_plan<W>(bt, sh, lane);
+    q4_feed<W, C::kStages, D>(bt, pool, sh, q4_smem + sizeof(typename C::Shared), lane);
     return;
   }
   const int g = lane >> 2, t = lane & 3;
@@ -252,48 +243,6 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
   // warp leaves; the others' waits for it run out too.
   auto arrived = [](uint64_t* bar, uint32_t parity, int where) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, where)) != 0;
-  };
-
-  // ---- this warp's copies, ahead of its products -----------------------------------------
-  uint32_t f_seg = 0;       // segments taken by the copies
-  int f_step = 0, f_t1 = 0; // the next step, the segment's end (none taken: equal)
-  uint32_t f_stage = 0, in_ring = 0;
-  uint32_t bad = 0;         // bit 2 s + i: granule i of stage s has no page
-  bool f_end = false;
-  const bool split = bt.table && bt.page_shift == 4;  // a step's granules lie in two pages
-  const int page_mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
-  // Brings the warp's next step if the plan is that far.
-  auto bring = [&]() {
-    while (f_step >= f_t1) {
-      if (f_end || !mbar_test(&sh.seg_full[f_seg % kQ4Queue], (f_seg / kQ4Queue) & 1)) return;
-      const Q4Seg<W>& seg = sh.seg[f_seg % kQ4Queue];
-      f_end = seg.end != 0;
-      if (f_end) return;
-      f_step = seg.t0 + warp;
-      f_t1 = seg.t1;
-      ++f_seg;
-    }
-    const Q4Seg<W>& seg = sh.seg[(f_seg - 1) % kQ4Queue];
-    const int i = f_step - seg.t0;
-    const int p0 = seg.pages[0][i], p1 = seg.pages[1][i];
-    if (seg.gone) {
-      bad = (bad & ~(3u << (2 * f_stage))) | ((p0 < 0 ? 1u : 0u) | (p1 < 0 ? 2u : 0u)) << (2 * f_stage);
-    } else {
-      bad &= ~(3u << (2 * f_stage));
-    }
-    if (lane == 0) {
-      uint64_t* bar = &sh.full[warp][f_stage];
-      uint8_t* dst = ring + f_stage * C::kStage;
-      const int row = (f_step * kQ4Keys) & page_mask, row1 = (f_step * kQ4Keys + 16) & page_mask;
-      mbar_arrive_expect_tx(bar, ((p0 >= 0 ? 1 : 0) + (p1 >= 0 ? 1 : 0)) * C::kGranule);
-      const unsigned char* src = q4::granule(pool, D, p0, seg.it.kvh, row);
-      if (p0 >= 0) bulk_load(dst, src, p1 >= 0 && !split ? 2 * C::kGranule : C::kGranule, bar);
-      if (p1 >= 0 && split)
-        bulk_load(dst + C::kGranule, q4::granule(pool, D, p1, seg.it.kvh, row1), C::kGranule, bar);
-    }
-    f_step += W;
-    ++in_ring;
-    if (++f_stage == C::kStages) f_stage = 0;
   };
 
   uint32_t stage = 0, phase = 0, items = 0;
@@ -310,19 +259,14 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
   float o[2 * NB][NT][4], ws[NT][4], m[NT], l[NT];
   uint32_t spoilt[NT];    // blocks with a NaN scale that the row sees
   bool have_anc = false;
-  for (uint32_t c_seg = 0;; ++c_seg) {
-    if (!arrived(&sh.seg_full[c_seg % kQ4Queue], (c_seg / kQ4Queue) & 1, 0x3F100)) return;
-    const Q4Seg<W>& seg = sh.seg[c_seg % kQ4Queue];
-    end = seg.end;
+  while (true) {
+    if (!arrived(&sh.item_full[items % kQ4Queue], (items / kQ4Queue) & 1, 0x3F100)) return;
+    const Q4Item& entry = sh.item[items % kQ4Queue];
+    end = entry.end;
     if (end) break;
-    while (in_ring < C::kStages) {
-      const uint32_t before = in_ring;
-      bring();
-      if (in_ring == before) break;
-    }
-    const Item& it = seg.it;
-    const int R = it.n * bt.group, row_lo = it.blk * RB;
-    if (seg.t0 == it.t0) {
+    const Item& it = entry.it;
+    const int R = it.n * bt.group, row_lo = it.blk * RB, steps = it.t1 - it.t0;
+    {
       // ---- the item's rows of q, scaled, and -8 sum q of each block -----------------
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -382,13 +326,13 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       have_anc = false;
     }
 
-    for (int st = seg.t0 + warp; st < seg.t1; st += W) {
-      if (in_ring == 0) bring();  // (its segment is the products', so it is there)
+    int i_step = warp - entry.g0 % W;
+    for (i_step += i_step < 0 ? W : 0; i_step < steps; i_step += W) {
       if (!arrived(&sh.full[warp][stage], phase, 0x3F000 | warp)) return;
       const uint8_t* base = ring + stage * C::kStage;
-      int row0 = st * kQ4Keys;
+      int row0 = (it.t0 + i_step) * kQ4Keys;
       const bool tail = row0 + kQ4Keys > it.len;
-      const uint32_t no_page = (bad >> (2 * stage)) & 3u;
+      const uint32_t no_page = sh.gone[warp][stage];
       if (tail && !have_anc) {
         // the nodes that the rows see: a lane per row
         have_anc = true;
@@ -597,21 +541,14 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           }
         }
       }
-      // the stage is read: a next step
+      // the stage is read
       __syncwarp();
-      --in_ring;
-      bring();
+      if (lane == 0) mbar_arrive(&sh.empty[warp][stage]);
       if (++stage == C::kStages) {
         stage = 0;
         phase ^= 1;
       }
     }
-    if (!seg.last) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.seg_empty[c_seg % kQ4Queue]);
-      continue;
-    }
-
     // ---------------- join the warps ---------------------------------------------------
     // the upper half hands its rows to the lower, whose rows are then added up
 #pragma unroll
@@ -693,7 +630,6 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       if (lane == 0) mbar_arrive(&sh.joined);
     }
     if (!arrived(&sh.joined, items & 1, 0x3F500)) return;
-    ++items;
     const int slot = part_slot(it, blockIdx.x);
     const int live = min(RB, R - row_lo);
     // warps that had no step have m = -inf and l = 0
@@ -734,8 +670,9 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
     __syncwarp();
     if (lane == 0) {
       mbar_arrive(&sh.read);
-      mbar_arrive(&sh.seg_empty[c_seg % kQ4Queue]);
+      mbar_arrive(&sh.item_empty[items % kQ4Queue]);
     }
+    ++items;
   }
   zero_unwritten<T, D>(bt, end == 2, out, lse, warp, W);
 }

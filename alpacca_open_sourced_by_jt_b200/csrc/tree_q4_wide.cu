@@ -3,15 +3,15 @@
 //
 // A block of up to 128 rows is the M of tcgen05.mma; S = Q.K^T and O += P.V accumulate
 // in TMEM, P goes over S's columns and Q stays in TMEM too, so that shared memory
-// carries only the tiles.  Converting warps turn each granule of 16 keys into rows of the K and V tiles, 128-byte swizzled as the MMAs read
-// them: a code at bits 6 to 9 of 0x4c00 is the f16 16 + code, and (16 + code) d - 24 d,
-// one fused operation, is d * (code - 8) exactly (24 d has 10 bits).  So both products
-// are those of the cache's own values; q is scaled by a power of two to f16 as in
-// tree_q4.cu, the weights are rounded to f16.
+// carries only the tiles.  Converting warps turn each granule of 16 keys into rows of the
+// K and V tiles, 128-byte swizzled as the MMAs read them: a code at bits 6 to 9 of 0x4c00
+// is the f16 16 + code, and (16 + code) d - 24 d, one fused operation, is d * (code - 8)
+// exactly (24 d has 10 bits).  So both products are those of the cache's own values; q is
+// scaled by a power of two to f16 as in tree_q4.cu, the weights are rounded to f16.
 //
 // 896 threads: warps 0-7 softmax (two warpgroups, tiles in turn, an S buffer each),
-// 8-23 converters (each brings its own steps, as tree_q4_kernel's warps do, here of 16
-// keys), 24 plans, 25 owns TMEM and issues the MMAs.
+// 8-23 converters, 24 feeds them (as tree_q4_kernel's warps are fed, here by steps of 16
+// keys), 25 owns TMEM and issues the MMAs.
 // TMEM: S0, S1 (128 columns each), O (D), Q (D / 2).
 
 #include <limits.h>
@@ -38,18 +38,15 @@ constexpr int kQWSlots = 2;      // K tiles, and V tiles, in shared memory
 template <int S>
 struct alignas(128) QWShared {
   static constexpr int kStepKeys = 16, kTileSteps = kQWKeys / 16;  // a step is a granule
-  static constexpr bool kItems = true;
-  uint64_t full[kQWConvert][S];                        // a converter's stages
-  uint64_t seg_full[kQ4Queue], seg_empty[kQ4Queue];    // planner -> converters
-  uint64_t item_full[kQ4Queue], item_empty[kQ4Queue];  // planner -> issuer, softmax
+  uint64_t full[kQWConvert][S], empty[kQWConvert][S];  // a converter's stages
+  uint64_t item_full[kQ4Queue], item_empty[kQ4Queue];  // feeding warp -> all others
   uint64_t k_full[kQWSlots], k_empty[kQWSlots], v_full[kQWSlots], v_empty[kQWSlots];
   uint64_t q_full, last;                               // an item's Q, its last PV
   uint64_t s_full[kQWGroups], p_full[kQWGroups], pv[2], bar_m[kQWGroups][4];
   uint32_t tmem;
   int special[8];  // an item's tree rows held NaN (converters are less than 8 items ahead)
-  int item_end[kQ4Queue];
-  Item item[kQ4Queue];
-  Q4Seg<kQWConvert> seg[kQ4Queue];
+  Q4Item item[kQ4Queue];
+  uint8_t gone[kQWConvert][S];  // a step without a page or without rows
   float x[kQWGroups][128];  // maxima, at an item's end sums, between the warpgroups
   float o[128][33];         // rows of O, where several lanes share a query row
 };
@@ -66,7 +63,6 @@ struct QWCfg {
   using Shared = QWShared<kStages>;
   static constexpr int kSmem = kTiles + kQWConvert * kStages * kStage + static_cast<int>(sizeof(Shared));
   static_assert(kStages >= 2 && kSmem <= 227 * 1024, "ring");
-  static_assert(kQ4Rounds * kQWConvert % Shared::kTileSteps == 0, "segments hold whole tiles");
   // A converter takes every kQWConvert-th of all steps, so at least one of the tiles in
   // the slots: further apart, it could not tell the phase of a slot by its parity.
   static_assert(kQWConvert <= kQWSlots * Shared::kTileSteps, "converters");
@@ -128,12 +124,13 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   } else if (warp == kQWPlan && lane == 0) {
     for (int w = 0; w < W; ++w)
-      for (int s = 0; s < C::kStages; ++s) mbar_init(&sh.full[w][s], 1);
+      for (int s = 0; s < C::kStages; ++s) {
+        mbar_init(&sh.full[w][s], 1);
+        mbar_init(&sh.empty[w][s], 1);
+      }
     for (int i = 0; i < kQ4Queue; ++i) {
-      mbar_init(&sh.seg_full[i], 1);
-      mbar_init(&sh.seg_empty[i], W);
       mbar_init(&sh.item_full[i], 1);
-      mbar_init(&sh.item_empty[i], 1 + 4 * kQWGroups);
+      mbar_init(&sh.item_empty[i], 1 + 4 * kQWGroups + W);
     }
     for (int i = 0; i < kQWSlots; ++i) {
       mbar_init(&sh.k_full[i], TS);
@@ -164,8 +161,8 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
   };
 
   if (warp == kQWPlan) {
-    // ------------------------------ the plan --------------------------------
-    q4_plan<W>(bt, sh, lane);
+    // ------------------------------ the plan, the copies --------------------
+    q4_feed<W, C::kStages, D>(bt, pool, sh, qw_smem + C::kTiles, lane);
   } else if (warp == kQWIssue) {
     // ------------------------------ MMA issuer -----------------------------
     // (the whole warp walks, one elected lane issues: tree_wide.cu says why)
@@ -197,8 +194,8 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     while (ok) {
       const int place = items % kQ4Queue;
       if (!arrived(&sh.item_full[place], (items / kQ4Queue) & 1, 0x3F810)) break;
-      const int end = sh.item_end[place];
-      const int n = __shfl_sync(0xffffffffu, sh.item[place].t1 - sh.item[place].t0, 0);
+      const int end = sh.item[place].end;
+      const int n = __shfl_sync(0xffffffffu, sh.item[place].it.t1 - sh.item[place].it.t0, 0);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.item_empty[place]);
       if (end) break;
@@ -248,58 +245,27 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQWConvertRegs));
     const int cw = warp - 8;
     uint8_t* ring = qw_smem + C::kTiles + cw * C::kStages * C::kStage;
-    const int page_mask = bt.table ? (1 << bt.page_shift) - 1 : INT_MAX;
-    uint32_t f_seg = 0, f_stage = 0, in_ring = 0;
-    int f_step = 0, f_t1 = 0;
-    bool f_end = false;
-    // Brings the warp's next step if the plan is that far (tree_q4_kernel has the same).
-    auto bring = [&]() {
-      while (f_step >= f_t1) {
-        if (f_end || !mbar_test(&sh.seg_full[f_seg % kQ4Queue], (f_seg / kQ4Queue) & 1)) return;
-        const Q4Seg<W>& seg = sh.seg[f_seg % kQ4Queue];
-        f_end = seg.end != 0;
-        if (f_end) return;
-        f_step = seg.t0 + (cw + W - seg.g0 % W) % W;
-        f_t1 = seg.t1;
-        ++f_seg;
-      }
-      const Q4Seg<W>& seg = sh.seg[(f_seg - 1) % kQ4Queue];
-      const int i = f_step - seg.t0;
-      const int page = seg.pages[0][i];
-      if (lane == 0) {
-        uint64_t* bar = &sh.full[cw][f_stage];
-        mbar_arrive_expect_tx(bar, page >= 0 ? C::kGranule : 0);
-        if (page >= 0)
-          bulk_load(ring + f_stage * C::kStage, q4::granule(pool, D, page, seg.it.kvh, (f_step * 16) & page_mask),
-                    C::kGranule, bar);
-      }
-      f_step += W;
-      ++in_ring;
-      if (++f_stage == C::kStages) f_stage = 0;
-    };
-    uint32_t stage = 0, phase = 0;
-    uint32_t f_items = 0;  // items done
+    uint32_t stage = 0, phase = 0, items = 0;
     bool ok = true;
-    for (uint32_t c_seg = 0; ok; ++c_seg) {
-      if (!arrived(&sh.seg_full[c_seg % kQ4Queue], (c_seg / kQ4Queue) & 1, 0x3F870)) break;
-      const Q4Seg<W>& seg = sh.seg[c_seg % kQ4Queue];
-      if (seg.end) break;
-      while (in_ring < C::kStages) {
-        const uint32_t had = in_ring;
-        bring();
-        if (in_ring == had) break;
-      }
-      const int rows = seg.it.len + seg.it.n, len = seg.it.len;
-      const bool tree = seg.it.n > 1;
-      for (int st = seg.t0 + (cw + W - seg.g0 % W) % W; st < seg.t1; st += W) {
-        if (in_ring == 0) bring();
-        const uint32_t tile = (seg.g0 + st - seg.t0) / TS;
+    for (; ok; ++items) {
+      const int place = items % kQ4Queue;
+      if (!arrived(&sh.item_full[place], (items / kQ4Queue) & 1, 0x3F870)) break;
+      const Q4Item& entry = sh.item[place];
+      if (entry.end) break;
+      const int len = entry.it.len, rows = len + entry.it.n, g0 = entry.g0;
+      const int s0 = entry.it.t0 * TS, steps = entry.it.t1 * TS - s0;
+      const bool tree = entry.it.n > 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.item_empty[place]);
+      for (int i = (cw + W - g0 % W) % W; i < steps; i += W) {
+        const int st = s0 + i;
+        const uint32_t tile = (g0 + i) / TS;
         const uint32_t slot = tile % kQWSlots, round = tile / kQWSlots;
-        const bool gone = seg.pages[0][st - seg.t0] < 0;
         if (!arrived(&sh.full[cw][stage], phase, 0x3F880)) {
           ok = false;
           break;
         }
+        const bool gone = sh.gone[cw][stage];
         const int part = lane >> 4, r = lane & 15;   // two lanes to a row
         const uint8_t* g = ring + stage * C::kStage;
         const int at = st * 16 + r;                  // row of the cache
@@ -321,11 +287,11 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
               // a NaN that some rows do not see: taken out here, put back at the item's end
               if ((dv[i] & 0x7fffu) > 0x7c00u) {
                 dv[i] &= 0xffff0000u;
-                sh.special[f_items & 7] = 1;
+                sh.special[items & 7] = 1;
               }
               if ((dv[i] & 0x7fff0000u) > 0x7c000000u) {
                 dv[i] &= 0x0000ffffu;
-                sh.special[f_items & 7] = 1;
+                sh.special[items & 7] = 1;
               }
             }
           }
@@ -397,18 +363,13 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.v_full[slot]);
-        // the stage is read: a next step
-        --in_ring;
-        bring();
+        // (the stage is read by then)
+        if (lane == 0) mbar_arrive(&sh.empty[cw][stage]);
         if (++stage == C::kStages) {
           stage = 0;
           phase ^= 1;
         }
       }
-      if (!ok) break;
-      f_items += seg.last;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.seg_empty[c_seg % kQ4Queue]);
     }
   } else if (warp < 8) {
     // ------------------------------ softmax ----------------------------------
@@ -435,8 +396,8 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       const int place = items % kQ4Queue;
       // (waited for whatever ran out before: all eight warps come here, so all leave)
       if (!arrived(&sh.item_full[place], (items / kQ4Queue) & 1, 0x3F8B0)) break;
-      end = sh.item_end[place];
-      const Item it = sh.item[place];
+      end = sh.item[place].end;
+      const Item it = sh.item[place].it;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.item_empty[place]);
       if (end) break;
