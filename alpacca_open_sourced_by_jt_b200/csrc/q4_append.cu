@@ -10,11 +10,13 @@
 // paged.cu does.
 //
 // Bound by reading the projections and writing q and the pool, and nearly as much by
-// its instructions.  A thread takes eight pairs of a head, which it rotates by itself:
-// 16 consecutive dims, or for neox rows 8 and the 8 that are half the rotation further
-// on, so two words of codes; D / 16 lanes a head (with 8 dims a thread the sum, the
-// root and the addresses of a head weigh twice as much: 72 us for 8191 tokens, 32/8
-// heads x 128, bf16).  The cosines and sines of a token serve all of a thread's heads.
+// instructions and L1's data path.  A thread takes eight pairs of a head, which it rotates
+// by itself: 16 consecutive dims, or for neox rows 8 and the 8 that are half the rotation
+// further on, so two words of codes; D / 16 lanes a head (with 8 dims a thread the sum, the
+// root and the addresses of a head weigh twice as much).  It keeps its head over the tokens,
+// so that addresses and roles are found once: 8191 tokens, 32/8 heads x 128, bf16: 53 us
+// (3.8 TB/s), 72 with the heads in the inner loop; into 4 bits, 64 wide, and read back 37
+// us, 56.  Not kept: rows, cosines and sines through rings in shared memory (51 and 42 us).
 
 #include <cfloat>
 
@@ -82,7 +84,9 @@ __device__ __forceinline__ uint32_t largest8(const float* x) {
 }
 
 constexpr int kThreads = 256;
-constexpr int kAppendThreads = 384, kResident = 2;  // most threads, CTAs per SM of norm_append_kernel
+// Most threads, CTAs per SM of norm_append_kernel: 80 registers each (with 64 the rows on
+// their way are spilled).
+constexpr int kAppendThreads = 384, kResident = 2;
 
 // 8 elements as loaded.
 template <typename TS>

@@ -10,12 +10,23 @@
 // takes the first token v with r(0) + .. + r(v) > d sum r: over all u and d the
 // next token then has the model's distribution, whatever was drafted.
 //
+// Where a residual has no weight left (draft rows that do not sum to 1), the row's
+// largest token is taken, and the path goes on to a child that has it.
+//
 // Only rows on the path decide anything, so only those are read: a cluster of CTAs
 // walks one request, each CTA a slice of the vocabulary, and meets over
 // distributed shared memory once per row.  The decisions compare sums of 32-bit
-// exponentials (2^-22) held in 64 bits; the draw, whose outcome hangs on sums at
-// borders some 10^-5 apart, takes 64-bit exponentials: a second reading of the
-// last row, out of L2.
+// exponentials (2^-21; where less than a sixteenth of such a sum is left, it is taken
+// anew in 64 bits); the draw and the residuals, whose outcome hangs on sums at borders
+// some 10^-5 apart, take 64-bit exponentials: another reading of the row, out of L2.
+//
+// Bound by latency, not by bytes: a row on a path takes some 7 us (2.5 of loads, 1.5 of
+// reductions and the cluster's barrier, 1.5 of the children), a 64-bit sum over it 10 to
+// 14 (chains of some 15 dependent operations a token, four side by side).  64 requests
+// with up to 31 nodes over 128256 f32 logits: 66 us for paths of up to 7 rows; 24 requests
+// with drafts' rows 67; one request of 4 nodes 9.6.  Not kept: the next loads or the
+// children's logits ahead of time (registers: 74 us instead of 66 for the 64), more
+// registers and fewer CTAs an SM (99).
 
 #include <cooperative_groups.h>
 
@@ -671,13 +682,16 @@ int b2a_verify_picks(const void* logits, long long row_stride, int dtype, const 
   if (n_rows == 0) return B2A_OK;
   VF::Args a = {logits, row_stride, draft, draft_row_stride, cu_dev, parents_dev, tokens_dev, uniforms_dev,
                 draws_dev, temperature_dev, picks_dev, B, n_rows, max_nodes, V, 0, 0, 0, 0};
-  // Few rows: a cluster for each, all at once, rather than node after node of a path.
-  a.all_nodes = n_rows > B && static_cast<long long>(n_rows) * VF::kCluster <= 4 * b2a_host::sm_count();
+  // Few rows: a cluster for each, all at once, rather than node after node of a path, as
+  // long as all clusters are resident (rows of 128256 f32: 4 nodes of one request 9.6 us
+  // against 17.1, 8 of each of 4 26 against 27.5; of 8 requests 36 against 31).
+  a.all_nodes = n_rows > B && static_cast<long long>(n_rows) * VF::kCluster <= 2 * b2a_host::sm_count();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(dtype, [&](auto* t) {
     using T = typename std::remove_pointer<decltype(t)>::type;
     // Wider CTAs where all clusters are resident with them (2 of 512 threads an SM, 4 of
-    // 256): 24 requests with drafts' rows 141 us with 256 threads, 94 with 512.
+    // 256): 24 requests with drafts' rows 84 us with 256 threads, 67 with 512, 37 requests
+    // 47 and 44, 64 requests 71 and 82.
     const long long ctas = static_cast<long long>(a.all_nodes ? n_rows : B) * VF::kCluster;
     return ctas <= 2 * b2a_host::sm_count() ? verify_launch<T, 512>(a, st) : verify_launch<T, 256>(a, st);
   });

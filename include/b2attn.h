@@ -663,8 +663,8 @@ int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* pare
  *   d    = m / -8 rounded to 8 significant bits, within +-8160, kept as f16
  *   code = floor(x / d + 8.5) within 0 .. 15
  * it stands for d * (code - 8), which f16 holds exactly, half a step |d| / 2 from x
- * (up to a whole one at the end of the range without the code 16).  Values beyond 65280 saturate; a block with a NaN has d = NaN
- * and stands for NaN.
+ * (up to a whole one at the end of the range, which has no code 16).  Values beyond
+ * 65280 saturate; a block with a NaN has d = NaN and stands for NaN.
  *
  * A 4-bit pool is [n_pages][KV][page_rows / 16] granules of 18 D bytes (K and V
  * of 16 rows of one head), pages page_bytes apart (0: dense), a multiple of 16;
@@ -680,7 +680,8 @@ int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* pare
  *   x = x (+ bias);  s = 1 / sqrt(f32(sum x^2 / D + eps)), the sum in 64 bits;
  *   x = (x * s) * w;  then the rotation
  *   wq, wk    f32 [D] the norms' weights, or NULL: no norm of q, of k
- * q_out is of kv_dtype.  D 64, 128 or 256; n_rot a multiple of 16; all rows, tables, weights and pools 16-byte aligned. */
+ * q_out is of kv_dtype.  D 64, 128 or 256; n_rot a multiple of 16; all rows, tables,
+ * weights and pools 16-byte aligned. */
 int b2a_norm_rope_append_paged(const void* q, long long q_tok_stride, const void* k,
                                long long k_tok_stride, const void* v, long long v_tok_stride,
                                int in_dtype, const float* bq, const float* bk, const float* bv,
@@ -749,8 +750,8 @@ int b2a_tree_commit_q4(const int* picks_dev, const int* tokens_dev, const int* p
  * picks of nodes off the path, of padding rows and of requests left out (numbers
  * out of bounds) are -1, and where a row has no weight at all.  Where a residual
  * has none left (draft rows that do not sum to 1) the largest logit's v is
- * taken.  Decisions: exponentials in 32 bits (relative error 2^-21), sums in 64;
- * the draw and residuals in 64. */
+ * taken, and the path goes on to a child that has it.  Decisions: exponentials in
+ * 32 bits (relative error 2^-21), sums in 64; the draw and residuals in 64. */
 int b2a_verify_picks(const void* logits, long long row_stride, int dtype, const float* draft,
                      long long draft_row_stride, const int* cu_dev, const int* parents_dev,
                      const int* tokens_dev, const float* uniforms_dev, const float* draws_dev,
