@@ -34,7 +34,7 @@
 // a granule at head_dim 64, 350 at 128, 3200 cycles for a step of two at 128 with 15 warps
 // at work.  16 x 32760 rows, 32/8 heads x 128, bf16: one node 160 us (3.8 TB/s; the 16-bit
 // cache's kernel takes 327), 16 query rows 265; x 64 112 us; 64 requests of 200 to 8000
-// rows x 64, pages of 16: 102 us, an item's end and begin (join, q, first data) 4 us each.
+// rows x 64, pages of 16: 96 us, an item's end and begin (join, q, first data) 4 us each.
 // With each warp looking after its own copies 193 and 113 us.
 #include <limits.h>
 #include <math.h>

@@ -14,10 +14,10 @@
 // keys), 25 owns TMEM and issues the MMAs.
 // TMEM: S0, S1 (128 columns each), O (D), Q (D / 2).
 //
-// Bound by instructions: a tile of 128 keys takes some 6900 of them, half for the
-// conversion, which a block of 128 rows repeats, half for the softmax.  16 x 32760 rows,
-// 32/8 heads x 128: 32 rows 312 us (1.9 TB/s), 64 rows 366, 128 rows 454; 8 requests of
-// 9K to 16K rows, up to 512 query rows a KV head: 380 us, 440 TFLOP/s.  With converters
+// Bound by instructions: a tile of 128 keys takes some 5700 of them with 32 rows, half for
+// the conversion, which a block of 128 rows repeats, half for the softmax.  16 x 32760
+// rows, 32/8 heads x 128: 32 rows 303 us (2.0 TB/s), 64 rows 366, 128 rows 454; 8 requests
+// of 9K to 16K rows, up to 512 query rows a KV head: 370 us, 450 TFLOP/s.  With converters
 // that bring their own steps 333 us for 32 rows.
 
 #include <limits.h>

@@ -648,8 +648,11 @@ cudaError_t verify_launch(VF::Args a, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (b2a_host::launch_flags() & B2A_LAUNCH_PDL) ? 2 : 1;
-  cudaError_t e = a.draft ? cudaLaunchKernelEx(&cfg, VF::verify_kernel<T, kThreads, true>, a)
-                          : cudaLaunchKernelEx(&cfg, VF::verify_kernel<T, kThreads, false>, a);
+  // (with what stands in it besides, more than 48 KB from some 1,800,000 tokens on)
+  auto* kernel = a.draft ? &VF::verify_kernel<T, kThreads, true> : &VF::verify_kernel<T, kThreads, false>;
+  static std::atomic<unsigned long long> done[2];
+  cudaError_t e = allow_smem(kernel, 64 * 1024, done[a.draft ? 1 : 0]);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e == cudaSuccess && a.all_nodes)
     e = launch_second(VF::verify_path_kernel, dim3((a.B + VF::kPathWarps - 1) / VF::kPathWarps),
                       dim3(VF::kPathWarps * 32), 0, st, a);

@@ -578,6 +578,8 @@ def tree_decode_q4(q: torch.Tensor, pool: torch.Tensor, lens: torch.Tensor, cu: 
     if workspace is None:
         ws_bytes = _tree_q4_bytes(q.device.index, max_nodes, H, KV, D, max_len)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    elif not workspace.is_cuda or not workspace.is_contiguous():
+        _bad("workspace must be a contiguous CUDA tensor")
     else:
         ws_bytes = workspace.numel() * workspace.element_size()
     _lib.check(_lib.load().b2a_tree_decode_q4(

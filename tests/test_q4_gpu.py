@@ -451,7 +451,8 @@ def test_wrappers_refuse(cuda_dev):
     for kw in (dict(table=s.kw["table"].long()), dict(max_nodes=0), dict(max_nodes=129), dict(scale=0.0),
                dict(scale=math.nan), dict(max_len=10 ** 6), dict(out=torch.empty((2, 8, 64), device=cuda_dev)),
                dict(max_len=2000, table=torch.zeros((1, 200), dtype=torch.int32, device=cuda_dev),
-                    workspace=torch.empty(16, dtype=torch.uint8, device=cuda_dev))):
+                    workspace=torch.empty(16, dtype=torch.uint8, device=cuda_dev)),
+               dict(workspace=torch.empty(1 << 20, dtype=torch.uint8))):
         with pytest.raises(Bad):
             s.run(**kw)
     q, rest = s.q, s.args

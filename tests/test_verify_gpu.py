@@ -96,6 +96,13 @@ def test_picks(cuda_dev, draft, dt, nodes, V, shift):
 
 
 @pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("nodes", [[2], [1, 2, 0, 2]])
+def test_the_largest_vocabulary(cuda_dev, draft, nodes):
+    c, want = settled(lambda rng: make(nodes, 2000000, "bf16", draft, "chain", rng))
+    assert np.array_equal(run(cuda_dev, c, "bf16")[:sum(nodes)], want)
+
+
+@pytest.mark.parametrize("draft", [False, True])
 @pytest.mark.parametrize("nodes", [[6], [20, 30, 4], [3] * 50])
 def test_stars_of_likely_tokens(cuda_dev, draft, nodes):
     """Many children are turned down one after another: what is left gets small."""
