@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
   const float heat = a.temperature ? (a.temperature[b] > FLT_MAX ? FLT_MAX : a.temperature[b]) : 1.f;
   const bool greedy = !(heat > 0.f);
   const double cold = greedy ? 0.0 : 1.0 / static_cast<double>(heat);
-  const double cold_t = fmin(cold * 1.4426950408889634 * kTable, 1e300);
-  const float cold2 = static_cast<float>(fmin(cold * 1.4426950408889634, 1e30));
+  const double cold_t = cold * 1.4426950408889634 * kTable;
+  const float cold2 = static_cast<float>(fmin(cold * 1.4426950408889634, static_cast<double>(FLT_MAX)));
   int buf = 0;
 
   // what the CTAs of the cluster put into s_ex[buf], combined by all of them alike
@@ -286,11 +286,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
     // ---- the children in order ----------------------------------------------------------
     int rejected = 0, next = -1;
     double total = part;  // sum of r (certain drafts); drafts with a row: r is relative to it
-    // (weights below e^-690 are 0; comparing with the logit that has it, a NaN is 0 too)
-    const float least = fmaxf(fmaf(-690.f, heat, top), -FLT_MAX);
-    auto weight = [&](float x) {  // e^((x - M) / T)
-      const double e = exp_below((static_cast<double>(fmaxf(x, least)) - M) * cold_t, s_table);
-      return x >= least ? e : 0.0;
+    // e^((x - M) / T).  Weights below e^-690 are 0, and a NaN's; the exponent itself is
+    // compared: a float next to M may be off by more where T is small.
+    auto weight = [&](float x) {
+      constexpr double least = -690.0 * 1.4426950408889634 * kTable;
+      const double y = (static_cast<double>(x) - M) * cold_t, e = exp_below(y, s_table);
+      return y >= least ? e : 0.0;
     };
     // r(v) after k rejections of drafts with a row, from e^((x - M) / T)
     double per_total = 1.0 / total;

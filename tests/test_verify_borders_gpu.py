@@ -1,0 +1,60 @@
+"""Sampled verification (paged.verify_picks) where a temperature is small against the
+spacing of the logits: equal picks with the definition in 64 bits (q4_ref.verify), whose
+decisions are asserted to be clear."""
+import numpy as np
+import pytest
+
+from tests import q4_ref
+from tests.test_verify_gpu import run
+
+pytestmark = pytest.mark.gpu
+
+
+def below(top, n):
+    """top and the n - 1 floats under it, in order."""
+    x = [np.float32(top)]
+    while len(x) < n:
+        x.append(np.nextafter(x[-1], np.float32(-np.inf), dtype=np.float32))
+    return np.array(x, np.float32)
+
+
+def cold_case(many):
+    """Rows that hold the floats under their largest (twice the largest), with
+    temperatures at which e^-690, the least weight that counts, lies among them; a root
+    with two children, of which the first has next to no weight and the second half."""
+    V = 96
+    rows, heat = [], []
+    for top in (20.0, 1500.0, 0.1, 3.0e-24, -7.0, 1.0e30):
+        x = below(top, V - 1)
+        gap = float(x[0]) - float(x[1])
+        for at in (0.3, 0.5, 0.6, 0.7, 0.9, 1.0, 1.3, 1.5, 2.0, 2.5, 4.0, 6.0, 6.5, 20.0):
+            rows.append(np.concatenate([x[:1], x]))
+            heat.append(gap * at / 690)
+    rows, heat = rows[:many], heat[:many]
+    n = len(rows)
+    rng = np.random.default_rng(4)
+    x = np.zeros((3 * n, V), np.float32)
+    tokens = np.zeros(3 * n, np.int64)
+    for b in range(n):
+        place = rng.permutation(V)  # where each of them stands
+        x[3 * b, place] = rows[b]
+        x[3 * b + 1:3 * b + 3, b % V] = 1.0
+        tokens[3 * b + 1] = place[2 + b % 5]  # one to five floats under the largest
+        tokens[3 * b + 2] = place[b % 2]
+    u = np.tile(np.array([0, 0.3, 0.0], np.float32), n)
+    u[2::3] = np.where(np.arange(n) % 3 == 0, 0.2, 0.9)  # taken, and turned down
+    return dict(x=x, cu=(3 * np.arange(n + 1)).tolist(), parents=[-1, 0, 0] * n, tokens=tokens, u=u,
+                d=(0.2603 + 0.4808 * (np.arange(n) % 2)).astype(np.float32), T=np.array(heat, np.float32), q=None)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("many", [12, 84])  # a cluster per node, and per request
+def test_temperatures_small_against_the_logits_spacing(cuda_dev, many, draft):
+    c = cold_case(many)
+    assert (c["T"] > 0).all()
+    if draft:
+        c["q"] = np.full(c["x"].shape, 1.0 / c["x"].shape[1], np.float32)
+    picks, margin, drawn = q4_ref.verify(c["x"], c["cu"], c["parents"], c["tokens"], c["u"], c["d"], c["T"], c["q"])
+    assert margin > 2e-5 and drawn > 1e-11
+    got = run(cuda_dev, c, "f32", max_nodes=3)
+    assert np.array_equal(got, picks), np.nonzero(got != picks)[0]
