@@ -392,16 +392,30 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
     uint32_t own = 0, theirs = 0;  // tiles this warpgroup and that one have done
     uint32_t pvbase = 0, items = 0;
     int end = 0;
-    bool dead = false;  // a wait ran out: no more waiting, the barriers go on
+    bool dead = false;  // a wait of this warp ran out: no more waiting, the barriers go on
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity, where));
       return !dead;
     };
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(128 * kQWGroups) : "memory"); };
+    // meet(), and whether one of the eight warps says so.  A wait may run out in some warps
+    // only, so what decides which barriers follow is decided here, by all alike.
+    auto any_of = [&](bool says) {
+      uint32_t any;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 p, %1, 0;\n\t"
+          "bar.red.or.pred q, 1, %2, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(any)
+          : "r"(static_cast<uint32_t>(says)), "n"(128 * kQWGroups)
+          : "memory");
+      return any != 0u;
+    };
     while (true) {
       const int place = items % kQ4Queue;
-      // (waited for whatever ran out before: all eight warps come here, so all leave)
-      if (!arrived(&sh.item_full[place], (items / kQ4Queue) & 1, 0x3F8B0)) break;
+      // (waited for whatever ran out before)
+      if (any_of(!arrived(&sh.item_full[place], (items / kQ4Queue) & 1, 0x3F8B0))) break;
       end = sh.item[place].end;
       const Item it = sh.item[place].it;
       __syncwarp();
@@ -583,9 +597,10 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       const float mref = (M == -INFINITY) ? 0.f : M;
       meet();
       sh.x[w][r] = (m == -INFINITY) ? 0.f : l * fast_exp2(m - mref);
-      meet();
-      const float L = sh.x[0][r] + sh.x[1][r];
       wait(&sh.last, items & 1, 0x3F8F0);
+      const bool lost = any_of(dead);
+      dead = lost;
+      const float L = sh.x[0][r] + sh.x[1][r];
       const uint32_t which = items & 7;
       ++items;
       tc_fence_after();
@@ -596,7 +611,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
       const int lo = max(it.t0 * BN - it.len, 0), hi = min(it.t1 * BN - it.len, it.n);
       const uint4 sees = make_uint4(anc[0], anc[1], anc[2], anc[3]);
       float* po = part_o + (static_cast<size_t>(max(slot, 0)) * bt.rows_per_block + r) * D;
-      if (rep_shift == 0 && busy && !dead) {
+      if (rep_shift == 0 && busy && !lost) {
         // the warpgroups write the columns in turn, 32 (a block) at a time
 #pragma unroll 1
         for (int col = w * 32; col < D; col += 32 * kQWGroups) {
@@ -640,7 +655,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
           sh.x[1][r] = L;
         }
         meet();
-        if (w == 0 && !dead) {
+        if (w == 0 && !lost) {
           float top = -INFINITY, sum = 0.f;
           for (int i = rr; i < 128; i += lanes_of) top = fmaxf(top, sh.x[0][i]);
           const float tref = top == -INFINITY ? 0.f : top;
