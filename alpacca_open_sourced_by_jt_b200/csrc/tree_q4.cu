@@ -381,6 +381,10 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           const uint4 u = *reinterpret_cast<const uint4*>(base + 16 * D + t * (8 * NB) + i * 16);
           dk[4 * i] = u.x; dk[4 * i + 1] = u.y; dk[4 * i + 2] = u.z; dk[4 * i + 3] = u.w;
         }
+        const bool no_rows = (no_page >> gr) & 1u;  // of a page outside the pool: zeros (the stage holds anything)
+        if (no_rows)
+#pragma unroll
+          for (int i = 0; i < 2 * NB; ++i) dk[i] = 0u;
         float2 s[NT][2];  // of keys 4t, 4t + 1 | 4t + 2, 4t + 3
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = make_float2(0.f, 0.f);
@@ -429,7 +433,10 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           const uint4 u = *reinterpret_cast<const uint4*>(base + 17 * D + t * (8 * NB) + i * 16);
           dv[4 * i] = u.x; dv[4 * i + 1] = u.y; dv[4 * i + 2] = u.z; dv[4 * i + 3] = u.w;
         }
-        if (tail || no_page) {
+        if (no_rows)
+#pragma unroll
+          for (int i = 0; i < 2 * NB; ++i) dv[i] = 0u;
+        if (tail) {
           // keys that are not there, or that only some rows see, may hold anything
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -440,7 +447,6 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
               bool see = j < 0;
               if (j >= 0 && j < it.n && row_lo + nt * 8 + g < R)
                 see = reinterpret_cast<const uint32_t*>(&sh.sees[warp][nt * 8 + g])[j >> 5] >> (j & 31) & 1u;
-              if ((no_page >> gr) & 1u) see = false;
               float& x = i & 1 ? s[nt][i >> 1].y : s[nt][i >> 1].x;
               if (!see) x = -INFINITY;
               any |= see;
@@ -668,11 +674,11 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       } else {
         const int rr = row_lo + r, nd = rr / bt.group;
         const size_t row = static_cast<size_t>(it.node0 + nd) * bt.H + it.kvh * bt.group + (rr - nd * bt.group);
-        const float f = 1.f / L;  // a node sees itself: L > 0
+        const float f = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= f;
         paged::store8(out + row * D + d, x);
-        if (lse && d == 0) lse[row] = (M + log2f(L)) * kLn2;
+        if (lse && d == 0) lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
       }
     }
     __syncwarp();
