@@ -21,7 +21,8 @@ the model itself would have picked:
     x   += act . Wdown^T b2a_gemm, in place
   logits = RMSNorm(x) . Woutput^T                 b2a_gemm_q8
   penalties, biases, masks, picks                 b2a_constrain_logits
-  where tokens are sampled, which drafts stand    b2a_verify_picks
+  where tokens are sampled, which drafts stand    b2a_verify_picks (the former then
+                                                  only for limits)
   accepted paths, K/V rows into place             b2a_tree_commit, b2a_tree_commit_q4
 
 Prompts go through the same layers in chunks, as chains.  Where the drafts
@@ -188,8 +189,12 @@ class DraftStep:
         tokens = torch.tensor(flat, dtype=torch.int32, device=dev)
         parents = torch.tensor(par, dtype=torch.int32, device=dev)
         logits, plan = self._forward(add, tokens, parents)
-        self.logits, self.picks = paged.constrain_logits(
-            logits, plan.cu, parents, tokens, max_nodes=max(add), out=logits, **limits)
+        self.logits = logits
+        # (sampled without limits: nothing to do to the logits, and no use for all rows' greedy
+        # picks; verify_picks reads the rows on the paths alone)
+        if draws is None or any(x is not None for x in limits.values()):
+            _, self.picks = paged.constrain_logits(
+                logits, plan.cu, parents, tokens, max_nodes=max(add), out=logits, **limits)
         if draws is not None:
             self.picks = paged.verify_picks(self.logits, plan.cu, parents, tokens, uniforms, draws,
                                             max_nodes=max(add), temperature=temperature, draft=draft)
