@@ -16,9 +16,11 @@
 // Only rows on the path decide anything, so only those are read: a cluster of CTAs
 // walks one request, each CTA a slice of the vocabulary, and meets over
 // distributed shared memory once per row.  The decisions compare sums of 32-bit
-// exponentials (2^-21; where less than a sixteenth of such a sum is left, it is taken
-// anew in 64 bits); the draw and the residuals, whose outcome hangs on sums at borders
-// some 10^-5 apart, take 64-bit exponentials: another reading of the row, out of L2.
+// exponentials: up to five multiplied (2^-22 each), arguments of three roundings, 4 or 8
+// added in 32 bits and those in 64, so that a weight e^-y is off by at most 2^-22 (7 + y)
+// of itself; where less than a sixteenth of such a sum is left, it is taken anew in 64
+// bits.  The draw and the residuals, whose outcome hangs on sums at borders some 10^-5
+// apart, take 64-bit exponentials: another reading of the row, out of L2.
 //
 // Bound by latency, not by bytes: a row on a path takes some 7 us (2.5 of loads, 1.5 of
 // reductions and the cluster's barrier, 1.5 of the children), a 64-bit sum over it 10 to
@@ -72,9 +74,9 @@ __device__ __forceinline__ double exp_below(double y, const double* table) {
 }
 
 struct Exchange {
-  double sum;
-  float top, part;  // largest logit, sum of exponentials relative to it
-  int at;           // the largest's lowest place
+  double sum, part;  // part: sum of exponentials relative to
+  float top;         // the largest logit
+  int at;            // the largest's lowest place
 };
 
 template <typename T>
@@ -91,8 +93,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
                                                                   // slice: rejected at this node
   __shared__ double s_table[kTable];
   __shared__ Exchange s_ex[2];
-  __shared__ double s_warp[kWarps];
-  __shared__ float s_top[kWarps], s_part[kWarps];
+  __shared__ double s_warp[kWarps], s_part[kWarps];
+  __shared__ float s_top[kWarps];
   __shared__ int s_at[kWarps];
   __shared__ int s_par[kMaxNodes], s_tok[kMaxNodes], s_pick[kMaxNodes];
   __shared__ float s_u[kMaxNodes];
@@ -168,24 +170,32 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
     const T* row = static_cast<const T*>(a.logits) + (c0 + cur) * a.stride;
     const float* qrow = kDraft ? a.draft + (c0 + cur) * a.draft_stride : nullptr;
     // ---- the row's largest logit, its place, the sum of exponentials -----------------
-    float top = -INFINITY, part = 0.f;
+    // (ref: what part is relative to.  It follows top only when that is more than a factor
+    // of 2 above it, so that a row that rises in small steps does not round part at each.)
+    float top = -INFINITY, ref = -INFINITY;
+    double part = 0.0;
     int place = a.V;
     {
       constexpr int kVec = 16 / sizeof(T), kLoads = 4;
-      auto take = [&](const float* x, int v) {  // kVec logits from v on
+      auto take = [&](const float* x, int v, int apart) {  // kVec logits from v on
         float m = x[0];
 #pragma unroll
         for (int e = 1; e < kVec; ++e) m = fmaxf(m, x[e]);
         if (m > top) {
-          part *= fast_exp2((top - m) * cold2);
           top = m;
+          if ((m - ref) * cold2 > 1.f) {
+            part *= fast_exp2((ref - m) * cold2);
+            ref = m;
+          }
 #pragma unroll
           for (int e = kVec - 1; e >= 0; --e)
-            if (x[e] == m) place = v + e;
+            if (x[e] == m) place = v + e * apart;
         }
         if (top > -INFINITY) {
+          float some = 0.f;
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) part += fast_exp2((x[e] - top) * cold2);
+          for (int e = 0; e < kVec; ++e) some += fast_exp2((x[e] - ref) * cold2);
+          part += some;
         }
       };
       if (reinterpret_cast<uintptr_t>(row) % 16 == 0) {  // (slices are whole groups)
@@ -205,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
 #pragma unroll
             for (int e = 0; e < kVec; ++e)  // (a NaN has weight 0)
               x[e] = fmaxf(ld_elem(reinterpret_cast<const T*>(&u[k]) + e), -INFINITY);
-            take(x, v0 + i * kVec);
+            take(x, v0 + i * kVec, 1);
           }
         }
         for (int v = v0 + groups * kVec + tid; v < v1; v += kThreads) {
@@ -213,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
           x[0] = fmaxf(at(row, v), -INFINITY);
 #pragma unroll
           for (int e = 1; e < kVec; ++e) x[e] = -INFINITY;
-          take(x, v);
+          take(x, v, 1);
         }
       } else {
         for (int v = v0 + tid; v < v1; v += kThreads * kVec) {
@@ -221,20 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
 #pragma unroll
           for (int e = 0; e < kVec; ++e)
             x[e] = v + e * kThreads < v1 ? fmaxf(at(row, v + e * kThreads), -INFINITY) : -INFINITY;
-          float m = x[0];
-#pragma unroll
-          for (int e = 1; e < kVec; ++e) m = fmaxf(m, x[e]);
-          if (m > top) {
-            part *= fast_exp2((top - m) * cold2);
-            top = m;
-#pragma unroll
-            for (int e = kVec - 1; e >= 0; --e)
-              if (x[e] == m) place = v + e * kThreads;
-          }
-          if (top > -INFINITY) {
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) part += fast_exp2((x[e] - top) * cold2);
-          }
+          take(x, v, kThreads);
         }
       }
     }
@@ -245,8 +242,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
       const uint32_t most = __reduce_max_sync(0xffffffffu, key);
       const float all = __uint_as_float((most & 0x80000000u) ? most ^ 0x80000000u : ~most);
       place = __reduce_min_sync(0xffffffffu, top == all ? place : a.V);
-      part = top > -INFINITY ? part * fast_exp2((top - all) * cold2) : 0.f;
-      top = all;
+      part = top > -INFINITY ? part * fast_exp2((ref - all) * cold2) : 0.0;
+      top = ref = all;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     };
@@ -258,8 +255,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
     }
     __syncthreads();
     if (warp == 0) {
-      top = lane < kWarps ? s_top[lane] : -INFINITY;
-      part = lane < kWarps ? s_part[lane] : 0.f;
+      top = ref = lane < kWarps ? s_top[lane] : -INFINITY;
+      part = lane < kWarps ? s_part[lane] : 0.0;
       place = lane < kWarps ? s_at[lane] : a.V;
       join();
       if (lane == 0) {
@@ -271,8 +268,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
     cluster.sync();
     {
       const Exchange* e = cluster.map_shared_rank(&s_ex[buf], lane < ranks ? lane : 0);
-      top = lane < ranks ? e->top : -INFINITY;
-      part = lane < ranks ? e->part : 0.f;
+      top = ref = lane < ranks ? e->top : -INFINITY;
+      part = lane < ranks ? e->part : 0.0;
       place = lane < ranks ? e->at : a.V;
       join();
     }

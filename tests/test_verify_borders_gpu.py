@@ -1,8 +1,9 @@
 """Sampled verification (paged.verify_picks) where a temperature is small against the
-spacing of the logits: equal picks with the definition in 64 bits (q4_ref.verify), whose
-decisions are asserted to be clear."""
+spacing of the logits, and where much of a sum is taken off: equal picks with the
+definition in 64 bits (q4_ref.verify), whose decisions are asserted to be clear."""
 import numpy as np
 import pytest
+import torch
 
 from tests import q4_ref
 from tests.test_verify_gpu import run
@@ -58,3 +59,34 @@ def test_temperatures_small_against_the_logits_spacing(cuda_dev, many, draft):
     assert margin > 2e-5 and drawn > 1e-11
     got = run(cuda_dev, c, "f32", max_nodes=3)
     assert np.array_equal(got, picks), np.nonzero(got != picks)[0]
+
+
+@pytest.mark.parametrize("dt,singles", [("f32", 0), ("f16", 0), ("f16", 36)])
+@pytest.mark.parametrize("side", [-1, 1])
+def test_what_is_left_of_a_long_sum(cuda_dev, dt, singles, side):
+    """Two million like weights behind one that has 10 of 11 parts of the sum and is turned
+    down; the next child's number lies 1e-4 of itself beside its share of what is left.
+    Weights e^-y may be off by 2^-22 (7 + y) of themselves: the large one, ten times what is
+    left, by 1.7e-5 of that, the others (y = 17) by 5.8e-6."""
+    V = 2000000
+    at = 123456
+    ratio = 0.3 / 1.3
+    n = 3 + singles
+    x = np.zeros((n, V), np.float32)
+    x[0, at] = np.log(0.3 * V)
+    x[0, 0] = np.log(10 * 1.3 * V)
+    x = torch.from_numpy(x).to(torch.float16 if dt == "f16" else torch.float32).float().numpy()
+    big, second = np.exp(x[0, [0, at]].astype(np.float64))
+    left = second + V - 2
+    u = np.zeros(n, np.float32)
+    u[1] = 0.99
+    u[2] = second / left * (1 + side * 1e-4)
+    assert abs(second / left - ratio) < 0.01 and left / (left + big) > 1 / 16  # not summed up anew
+    tokens = np.zeros(n, np.int64)
+    tokens[2] = at
+    rng = np.random.default_rng(8)
+    c = dict(x=x, cu=[0] + list(range(3, n + 1)), parents=[-1, 0, 0] + [-1] * singles, tokens=tokens, u=u,
+             d=rng.random(1 + singles).astype(np.float32), T=None, q=None)
+    picks, margin, drawn = q4_ref.verify(x, c["cu"], c["parents"], tokens, u, c["d"], None, None)
+    assert margin > 9e-5 and drawn > 1e-11 and (picks[0] == at) == (side < 0)
+    assert np.array_equal(run(cuda_dev, c, dt, max_nodes=3), picks)
