@@ -16,10 +16,14 @@
 //             operand per block.  -8 sum w comes from an MMA of its own per block
 //             (ones in row `block` of A: all blocks share four accumulators).
 //             f16 w: 2^-12 of each weight, as tree_mma_kernel's P for f16 caches.
-// The softmax runs relative to a number per query row that is at least (within
-// 2^8) the largest score + log2 |d_v|, so w neither overflows nor, where it counts,
-// falls under f16 whatever the scales are.  Scores, sums and accumulators are
-// f32.  Hidden keys have w = 0 whatever their bytes say.
+// The weights p are relative to a number m per query row, and those of a block of V,
+// p d_v, are held times a power of two c of the row and block.  Both follow only where
+// a w would pass 2^15 (or a row's p 2^60): m then goes to the largest score, by whole
+// exponents, and c to where the block's largest product is in [1/2, 1), or to where the
+// products so far had theirs if that is lower.  So no w overflows, and one is under f16's
+// normal numbers, off by up to 2^-25, only if it is 2^13 times smaller than the largest of
+// its own block: what the blocks beside it hold does not matter.  Scores, sums and
+// accumulators are f32.  Hidden keys have w = 0 whatever their bytes say.
 //
 // S has the queries on its rows, so an accumulator is already the B operand of the
 // second product (no transposition), and a lane's four keys of a granule are rows
@@ -38,6 +42,8 @@
 // With each warp looking after its own copies 193 and 113 us.
 #include <limits.h>
 #include <math.h>
+
+#include <cfloat>
 
 #include "b2a_common.cuh"
 #include "q4.cuh"
@@ -104,6 +110,12 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
         "f"(c[3]));
 }
+
+// Powers of two, exponents of floats (normal ones; exponent_bits: any, not negative).
+constexpr int kQ4Top = 100;
+__device__ __forceinline__ int exponent_bits(float x) { return static_cast<int>(__float_as_uint(x) >> 23); }
+__device__ __forceinline__ int exponent_of(float x) { return exponent_bits(x) - 127; }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 // The walk over a CTA's items by a whole warp.  Requests are looked at 32 at a time, one by
 // each lane.
@@ -265,6 +277,7 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
   float qc[NB][NT];       // -8 sum q of a block
   float sscale[NT];
   float o[2 * NB][NT][4], ws[NT][4], m[NT], l[NT];
+  float c[NT][NB];        // a block's weights are held times this power of two
   uint32_t spoilt[NT];    // blocks with a NaN scale that the row sees
   bool have_anc = false;
   while (true) {
@@ -325,9 +338,11 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        m[nt] = -INFINITY;
+        m[nt] = -FLT_MAX;
         l[nt] = 0.f;
         spoilt[nt] = 0u;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) c[nt][b] = power_of_two(kQ4Top);
 #pragma unroll
         for (int e = 0; e < 4; ++e) ws[nt][e] = 0.f;
       }
@@ -456,16 +471,41 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
               for (int b = 0; b < NB / 2; ++b) dv[i * (NB / 2) + b] = 0u;
           }
         }
-        auto top_scale = [&]() {  // the largest |d_v| of the lane's keys, a NaN before all
+        // The weights p and, by block, their products with the scales, rounded to f16.  They are
+        // relative to the row's m and c as they stand, unless one would come near f16's end
+        // (or a scale is NaN): then those of the rows that need it follow, and all is done again.
+        float2 p[NT][2];
+        float sum[NT];
+        uint32_t w[NB][NT][2];
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+          bool grow = false;
           __half2 top = __float2half2_rn(0.f);
 #pragma unroll
-          for (int i = 0; i < NB * 2; ++i)
-            top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&dv[i])));
-          const uint32_t bits = *reinterpret_cast<const uint32_t*>(&top);
-          return max(bits & 0x7fffu, bits >> 16 & 0x7fffu);
-        };
-        uint32_t top16 = top_scale();
-        if (__any_sync(0xffffffffu, top16 > 0x7c00u)) {
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 x = fma2(s[nt][h], make_float2(sscale[nt], sscale[nt]), make_float2(-m[nt], -m[nt]));
+              p[nt][h] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            }
+            sum[nt] = (p[nt][0].x + p[nt][0].y) + (p[nt][1].x + p[nt][1].y);
+            grow |= sum[nt] > 0x1p60f;  // (far from f32's end, for l too)
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const __half* hv = reinterpret_cast<const __half*>(dv) + 2 * h * NB + b;
+              const float2 d = make_float2(__half2float(hv[0]), __half2float(hv[NB]));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const float2 x = mul2(mul2(p[nt][h], make_float2(c[nt][b], c[nt][b])), d);
+                w[b][nt][h] = MmaOp<__half>::pack(x.x, x.y);
+                top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&w[b][nt][h])));
+              }
+            }
+          grow |= ((*reinterpret_cast<const uint32_t*>(&top) + 0x07ff07ffu) & 0x80008000u) != 0u;  // above 2^15, NaN
+          if (again || !__any_sync(0xffffffffu, grow)) break;
           // A NaN scale of a key that is seen: its block's outputs become NaN at the
           // item's end; here it counts as zero.
 #pragma unroll
@@ -480,66 +520,64 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
               for (int nt = 0; nt < NT; ++nt)
                 if ((i & 1 ? s[nt][i >> 1].y : s[nt][i >> 1].x) != -INFINITY) spoilt[nt] |= 1u << b;
             }
-          top16 = top_scale();
-        }
-        // A power of two (its exponent) that is at least the largest |d_v| of the lane's
-        // keys: with whole exponents the weight of a row's only key is exact.
-        const float far = static_cast<float>(min(static_cast<int>(top16 >> 10), 30) - 14);
-        bool grow = false;
-        float mx[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float x = fmaxf(fmaxf(s[nt][0].x, s[nt][0].y), fmaxf(s[nt][1].x, s[nt][1].y));
-          x = fmaf(x, sscale[nt], far);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          mx[nt] = x;
-          grow |= x > m[nt] + 8.f;
-        }
-        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float now = fmaxf(m[nt], mx[nt]);
-            const float alpha = now == -INFINITY ? 0.f : fast_exp2(m[nt] - now);
-            m[nt] = now;
-            l[nt] *= alpha;
-            const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
-#pragma unroll
-            for (int i = 0; i < 2 * NB; ++i) {
-              o[i][nt][0] *= a0;
-              o[i][nt][1] *= a1;
-              o[i][nt][2] *= a0;
-              o[i][nt][3] *= a1;
+            // m follows where a score is more than 2^8 above it, by whole exponents (the weight
+            // of a row's only key is exact)
+            float mx = fmaxf(fmaxf(s[nt][0].x, s[nt][0].y), fmaxf(s[nt][1].x, s[nt][1].y)) * sscale[nt];
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float before = m[nt];
+            int step = 0;
+            if (mx > before + 8.f) {
+              const float up = ceilf(mx - before);
+              step = up < 300.f ? static_cast<int>(up) : 300;
+              m[nt] = up < 300.f ? before + up : mx;
             }
-            ws[nt][0] *= a0;
-            ws[nt][1] *= a1;
+            const float alpha = fast_exp2(before - m[nt]);
+            l[nt] *= alpha;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 x = fma2(s[nt][h], make_float2(sscale[nt], sscale[nt]), make_float2(-m[nt], -m[nt]));
+              p[nt][h] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              // the block's largest product, and the power of two that brings it under 1;
+              // what is there already keeps its place, or goes down with it
+              float most = 0.f;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const __half* hv = reinterpret_cast<const __half*>(dv) + 2 * h * NB + b;
+                const float2 x = mul2(p[nt][h], make_float2(__half2float(hv[0]), __half2float(hv[NB])));
+                most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
+              }
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+              const int e = exponent_of(c[nt][b]), to = max(min(min(e + step, 126 - exponent_bits(most)), kQ4Top), -kQ4Top);
+              c[nt][b] = power_of_two(to);
+              const float f = alpha * (to - e < -126 ? 0.f : power_of_two(to - e));
+              const float a0 = __shfl_sync(0xffffffffu, f, 8 * t), a1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+              for (int i = 2 * b; i < 2 * b + 2; ++i) {
+                o[i][nt][0] *= a0;
+                o[i][nt][1] *= a1;
+                o[i][nt][2] *= a0;
+                o[i][nt][3] *= a1;
+              }
+              if (g == b) {
+                ws[nt][0] *= a0;
+                ws[nt][1] *= a1;
+              }
+            }
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float mref = m[nt] == -INFINITY ? 0.f : m[nt];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 x = fma2(s[nt][h], make_float2(sscale[nt], sscale[nt]), make_float2(-mref, -mref));
-            s[nt][h] = make_float2(fast_exp2(x.x), fast_exp2(x.y));  // the weights, unscaled
-          }
-          l[nt] += (s[nt][0].x + s[nt][0].y) + (s[nt][1].x + s[nt][1].y);
-        }
+        for (int nt = 0; nt < NT; ++nt) l[nt] += sum[nt];
         // ---- output -----------------------------------------------------------------
         const uint8_t* vb = base + 8 * D + (g & 3) * 64 + t * 16;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          uint32_t w[NT][2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const __half* hv = reinterpret_cast<const __half*>(dv) + 2 * h * NB + b;
-            const float2 d = make_float2(__half2float(hv[0]), __half2float(hv[NB]));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const float2 x = mul2(s[nt][h], d);
-              w[nt][h] = MmaOp<__half>::pack(x.x, x.y);
-            }
-          }
           const uint4 u = *reinterpret_cast<const uint4*>(vb + b * 256);
           const uint32_t lo = __byte_perm(u.x, u.y, sel), hi = __byte_perm(u.z, u.w, sel);
           const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
@@ -549,9 +587,9 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           const uint32_t ones[4] = {one, one, one, one};  // (rows 8 to 15 are not used)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(o[2 * b][nt], a0, w[nt][0], w[nt][1], o[2 * b][nt]);
-            mma_f16(o[2 * b + 1][nt], a1, w[nt][0], w[nt][1], o[2 * b + 1][nt]);
-            mma_f16(ws[nt], ones, w[nt][0], w[nt][1], ws[nt]);
+            mma_f16(o[2 * b][nt], a0, w[b][nt][0], w[b][nt][1], o[2 * b][nt]);
+            mma_f16(o[2 * b + 1][nt], a1, w[b][nt][0], w[b][nt][1], o[2 * b + 1][nt]);
+            mma_f16(ws[nt], ones, w[b][nt][0], w[b][nt][1], ws[nt]);
           }
         }
       }
@@ -576,8 +614,10 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        float w0 = -8.f * __shfl_sync(0xffffffffu, ws[nt][0], b * 4 + t);
-        float w1 = -8.f * __shfl_sync(0xffffffffu, ws[nt][1], b * 4 + t);
+        const float back = power_of_two(-exponent_of(c[nt][b]));
+        const float b0 = __shfl_sync(0xffffffffu, back, 8 * t), b1 = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+        float w0 = -8.f * __shfl_sync(0xffffffffu, ws[nt][0], b * 4 + t) * b0;
+        float w1 = -8.f * __shfl_sync(0xffffffffu, ws[nt][1], b * 4 + t) * b1;
         if (seen_nan) {
           if (__shfl_sync(0xffffffffu, spoilt[nt], 8 * t) >> b & 1u) w0 = __uint_as_float(0x7fffffffu);
           if (__shfl_sync(0xffffffffu, spoilt[nt], 8 * t + 4) >> b & 1u) w1 = __uint_as_float(0x7fffffffu);
@@ -585,10 +625,10 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float* x = o[2 * b + i][nt];
-          x[0] = fmaf(x[0], 16777216.f, w0);
-          x[1] = fmaf(x[1], 16777216.f, w1);
-          x[2] = fmaf(x[2], 1048576.f, w0);
-          x[3] = fmaf(x[3], 1048576.f, w1);
+          x[0] = fmaf(x[0], 16777216.f * b0, w0);
+          x[1] = fmaf(x[1], 16777216.f * b1, w1);
+          x[2] = fmaf(x[2], 1048576.f * b0, w0);
+          x[3] = fmaf(x[3], 1048576.f * b1, w1);
         }
       }
     }
@@ -623,12 +663,12 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
 #pragma unroll
       for (int nt = 0; nt < NT && warp + H < W; ++nt) {
         const float m2 = mine_ml[(nt * 8 + g) * 2], l2 = mine_ml[(nt * 8 + g) * 2 + 1];
-        const float now = fmaxf(m[nt], m2), mref = now == -INFINITY ? 0.f : now;
-        const float a = fast_exp2(m[nt] - mref), c = fast_exp2(m2 - mref);
+        const float now = fmaxf(m[nt], m2);
+        const float a = fast_exp2(m[nt] - now), a2 = fast_exp2(m2 - now);
         m[nt] = now;
-        l[nt] = l[nt] * a + l2 * c;
+        l[nt] = l[nt] * a + l2 * a2;
         const float a0 = __shfl_sync(0xffffffffu, a, 8 * t), a1 = __shfl_sync(0xffffffffu, a, 8 * t + 4);
-        const float c0 = __shfl_sync(0xffffffffu, c, 8 * t), c1 = __shfl_sync(0xffffffffu, c, 8 * t + 4);
+        const float c0 = __shfl_sync(0xffffffffu, a2, 8 * t), c1 = __shfl_sync(0xffffffffu, a2, 8 * t + 4);
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) {
           const float* from = mine + nt * 8 * C::kPad + 32 * (i >> 1) + 4 * (i & 1);
@@ -646,19 +686,18 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
     if (!arrived(&sh.joined, items & 1, 0x3F500)) return;
     const int slot = part_slot(it, blockIdx.x);
     const int live = min(RB, R - row_lo);
-    // warps that had no step have m = -inf and l = 0
+    // warps that had no step have m = -FLT_MAX and l = 0
     for (int i = threadIdx.x; i < live * (D / 8); i += W * 32) {
       const int r = i / (D / 8), d = (i - r * (D / 8)) * 8;
-      float M = -INFINITY;
+      float M = -FLT_MAX;
 #pragma unroll
       for (int w = 0; w < H; ++w) M = fmaxf(M, merge_ml[(w * RB + r) * 2]);
-      const float mref = M == -INFINITY ? 0.f : M;
       float L = 0.f, x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = 0.f;
 #pragma unroll 4
       for (int w = 0; w < H; ++w) {
-        const float f = fast_exp2(merge_ml[(w * RB + r) * 2] - mref);
+        const float f = fast_exp2(merge_ml[(w * RB + r) * 2] - M);
         L += merge_ml[(w * RB + r) * 2 + 1] * f;
         const float4 y0 = *reinterpret_cast<const float4*>(merge + (w * RB + r) * C::kPad + d);
         const float4 y1 = *reinterpret_cast<const float4*>(merge + (w * RB + r) * C::kPad + d + 4);

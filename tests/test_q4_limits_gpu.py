@@ -1,5 +1,6 @@
 """Attention over the 4-bit cache (paged.tree_decode_q4) at its limits, against 64 bits
-over the values that the pool stands for: rows of pages outside the pool.
+over the values that the pool stands for: rows of pages outside the pool, V blocks of
+unlike sizes beside one another.
 
 Bounds (u the unit roundoff of the output's type, w = sum p |v|): u |out| for the output,
 half a step of the type's least numbers where that is more;
@@ -122,3 +123,37 @@ def test_rows_of_pages_outside_the_pool_are_zeros(cuda_dev, H, KV, D, nodes):
             assert np.array_equal(a[:nodes], b[:nodes]) and np.array_equal(a[2 * nodes:], b[2 * nodes:])
         if len(bad) == last + 1:
             assert (out[nodes:2 * nodes] == 0).all() and np.isfinite(lse).all()
+
+
+# ---- scales ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("D,H,nodes", [(64, 8, 1), (128, 8, 1), (128, 8, 4), (256, 4, 1), (256, 4, 3), (128, 8, 16)])
+def test_blocks_of_unlike_sizes(cuda_dev, dt, D, H, nodes):
+    """A block's outputs are as near whatever the blocks beside it hold: all rows' first
+    block large, one key's alone, every key's blocks of a size of their own, blocks of
+    zeros."""
+    rng = np.random.default_rng(D + nodes)
+    KV, rows = 2, [1500, 333 + nodes]
+    k = normal(rng, rows, KV, D)
+    for kind in ("first", "outlier", "all", "zeros"):
+        v = normal(rng, rows, KV, D)
+        for x in v:
+            blocks = x.reshape(len(x), KV, D // 32, 32)
+            if kind == "first":
+                blocks[:, :, 0] *= 1e4
+                blocks[:, :, 1] *= 1e-2
+            elif kind == "outlier":
+                blocks[:, :, 1] *= 1e-2
+                blocks[len(x) // 3, :, 0] = 6e4
+            elif kind == "all":
+                blocks *= 10.0 ** rng.uniform(-3, 4, (1, 1, D // 32, 1))
+            else:
+                blocks[:, :, 0] *= 1e4
+                blocks[:, :, 1] = 0
+                blocks[7, :, 1] = 1e-2
+        # (the largest values end at 65280: f16 outputs stay finite)
+        for x in v:
+            np.clip(x, -6e4, 6e4, out=x)
+        s = Batch(cuda_dev, dt, H, k, v, [nodes, nodes], 32, seed=3)
+        s.check(*s.outputs())
