@@ -71,7 +71,6 @@ struct alignas(128) Q4Shared {  // (the rings stand behind it)
   uint64_t handed, joined, read;                   // at an item's end
   uint4 sees[W][16];                               // the nodes that a warp's rows see
   Q4Item item[kQ4Queue];
-  uint8_t gone[W][S];                              // bit i: granule i of the step has no page
 };
 
 template <int D, int NT>
@@ -164,6 +163,12 @@ struct Q4Walk {
   }
 };
 
+template <int D>
+__device__ __forceinline__ void q4_blank(uint8_t* granule) {
+#pragma unroll 1
+  for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(granule + 16 * D)[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 // The feeding warp: items to the queue, and each step's granules to the ring of the warp
 // that takes it, a step a lane.  Step number g goes to warp g % W; the slots of a batch of
 // steps are all different, so no lane waits for a copy that another is to make.
@@ -206,9 +211,14 @@ __device__ __forceinline__ void q4_feed(const Batch& bt, const q4::Pool& pool, S
         const uint32_t turn = static_cast<uint32_t>(g + i), w = turn % W, use = turn / W, s = use % S;
         if (use >= S) ok = mbar_wait(&sh.empty[w][s], (use / S - 1) & 1, 0x3F200) != 0;
         if (ok) {
-          sh.gone[w][s] = (has0 ? 0 : 1) | (two && !has1 ? 2 : 0);
           uint64_t* bar = &sh.full[w][s];
           uint8_t* dst = rings + (w * S + s) * (SK / 16 * kGranule);
+          if (one != has0 || two != has1) {
+            // rows of a page outside the pool: zeros for their scales, with whatever codes
+            if (one != has0) q4_blank<D>(dst);
+            if (two != has1) q4_blank<D>(dst + kGranule);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (copies come here again)
+          }
           mbar_arrive_expect_tx(bar, (has0 + has1) * kGranule);
           if (has0)
             bulk_load(dst, q4::granule(pool, D, p0, it.kvh, row & page_mask), has1 && !split ? 2 * kGranule : kGranule, bar);
@@ -355,7 +365,6 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
       const uint8_t* base = ring + stage * C::kStage;
       int row0 = (it.t0 + i_step) * kQ4Keys;
       const bool tail = row0 + kQ4Keys > it.len;
-      const uint32_t no_page = sh.gone[warp][stage];
       if (tail && !have_anc) {
         // the nodes that the rows see: a lane per row
         have_anc = true;
@@ -396,10 +405,6 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           const uint4 u = *reinterpret_cast<const uint4*>(base + 16 * D + t * (8 * NB) + i * 16);
           dk[4 * i] = u.x; dk[4 * i + 1] = u.y; dk[4 * i + 2] = u.z; dk[4 * i + 3] = u.w;
         }
-        const bool no_rows = (no_page >> gr) & 1u;  // of a page outside the pool: zeros (the stage holds anything)
-        if (no_rows)
-#pragma unroll
-          for (int i = 0; i < 2 * NB; ++i) dk[i] = 0u;
         float2 s[NT][2];  // of keys 4t, 4t + 1 | 4t + 2, 4t + 3
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = make_float2(0.f, 0.f);
@@ -448,28 +453,29 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           const uint4 u = *reinterpret_cast<const uint4*>(base + 17 * D + t * (8 * NB) + i * 16);
           dv[4 * i] = u.x; dv[4 * i + 1] = u.y; dv[4 * i + 2] = u.z; dv[4 * i + 3] = u.w;
         }
-        if (no_rows)
-#pragma unroll
-          for (int i = 0; i < 2 * NB; ++i) dv[i] = 0u;
         if (tail) {
           // keys that are not there, or that only some rows see, may hold anything
+          uint32_t any = 0u;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = row0 + 4 * t + i - it.len;
-            bool any = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              bool see = j < 0;
-              if (j >= 0 && j < it.n && row_lo + nt * 8 + g < R)
-                see = reinterpret_cast<const uint32_t*>(&sh.sees[warp][nt * 8 + g])[j >> 5] >> (j & 31) & 1u;
-              float& x = i & 1 ? s[nt][i >> 1].y : s[nt][i >> 1].x;
-              if (!see) x = -INFINITY;
-              any |= see;
+          for (int nt = 0; nt < NT; ++nt) {
+            const int j0 = row0 + 4 * t - it.len, at = j0 >> 5;  // tree row of the first key, its word
+            uint32_t vis = 0xfu;
+            if (j0 > -4) {
+              const uint32_t* words = reinterpret_cast<const uint32_t*>(&sh.sees[warp][nt * 8 + g]);
+              const uint32_t w0 = at < 0 ? ~0u : at < kWords ? words[at] : 0u, w1 = at + 1 < kWords ? words[at + 1] : 0u;
+              vis = __funnelshift_r(w0, w1, j0 & 31);
             }
-            if (!any)
+            if (!(vis & 1u)) s[nt][0].x = -INFINITY;
+            if (!(vis & 2u)) s[nt][0].y = -INFINITY;
+            if (!(vis & 4u)) s[nt][1].x = -INFINITY;
+            if (!(vis & 8u)) s[nt][1].y = -INFINITY;
+            any |= vis;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!((any >> i) & 1u))
 #pragma unroll
               for (int b = 0; b < NB / 2; ++b) dv[i * (NB / 2) + b] = 0u;
-          }
         }
         // The weights p and, by block, their products with the scales, rounded to f16.  They are
         // relative to the row's m and c as they stand, unless one would come near f16's end

@@ -52,7 +52,6 @@ struct alignas(128) QWShared {
   uint32_t tmem;
   int special[8];  // an item's tree rows held NaN (converters are less than 8 items ahead)
   Q4Item item[kQ4Queue];
-  uint8_t gone[kQWConvert][S];  // a step without a page or without rows
   float x[kQWGroups][128];  // maxima, at an item's end sums, between the warpgroups
   float o[128][33];         // rows of O, where several lanes share a query row
 };
@@ -271,11 +270,10 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
           ok = false;
           break;
         }
-        const bool gone = sh.gone[cw][stage];
         const int part = lane >> 4, r = lane & 15;   // two lanes to a row
         const uint8_t* g = ring + stage * C::kStage;
         const int at = st * 16 + r;                  // row of the cache
-        const bool none = at >= rows || gone;
+        const bool none = at >= rows;
         // the row in a tile, swizzled: chunk c is at `swz` with c & 7 in bits 4 to 6 flipped
         const uint32_t key = (st % TS) * 16 + r, swz = key * 128 + ((key & 7) << 4);
         // scales of K and V, [block] f16; of rows that are not there 0
@@ -285,7 +283,7 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
           dk[i] = *reinterpret_cast<const uint32_t*>(g + 16 * D + r * (2 * NB) + i * 4);
           dv[i] = *reinterpret_cast<const uint32_t*>(g + 17 * D + r * (2 * NB) + i * 4);
         }
-        if (st * 16 + 16 > len || gone) {  // rows of the tree, or past the last
+        if (st * 16 + 16 > len) {  // rows of the tree, or past the last
 #pragma unroll
           for (int i = 0; i < NB / 2; ++i) {
             if (none) dk[i] = dv[i] = 0u;
