@@ -183,7 +183,8 @@ class DraftStep:
                                ("temperature", temperature, self.B)):
                 paged._f32(name, t, n)
             if draft is not None and (draft.dtype is not torch.float32 or not draft.is_cuda or
-                                      draft.shape != (len(flat), self.m.V) or draft.stride(1) != 1):
+                                      draft.shape != (len(flat), self.m.V) or draft.stride(1) != 1 or
+                                      (len(flat) > 1 and draft.stride(0) < self.m.V)):
                 raise _lib.B2AShapeError(_lib.ERR_SHAPE, "draft must be a CUDA f32 tensor, a row per node")
         dev = self.m.device
         tokens = torch.tensor(flat, dtype=torch.int32, device=dev)

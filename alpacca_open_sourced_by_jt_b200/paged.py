@@ -95,6 +95,8 @@ def _pool(k: torch.Tensor, v: torch.Tensor, dims: int = 4):
     R, KV, D = shape[-3:]
     if stride[-1] != 1 or stride[-2] != D or (R > 1 and stride[-3] != KV * D):
         _bad("each page must be contiguous")
+    if shape[-4] > 1 and stride[-4] < R * KV * D:  # (0, an expanded page, is "dense" to the C call)
+        _bad("the pages of a pool must not overlap")
     return shape, stride
 
 
@@ -277,7 +279,8 @@ def tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, len
     (P, R, KV, D), pstride = _pool(k_pool, v_pool)
     dt, qs = q.dtype, q.stride()
     n, H, Dq = q.shape
-    if not q.is_cuda or qs[2] != 1 or qs[1] != D or Dq != D or k_pool.dtype is not dt:
+    if not q.is_cuda or qs[2] != 1 or qs[1] != D or Dq != D or k_pool.dtype is not dt or (
+            n > 1 and qs[0] < H * D):
         _bad("q must be a CUDA tensor (n, H, D), contiguous per token, in the pools' type")
     B = lens.numel()
     _i32("lens", lens)
@@ -464,6 +467,8 @@ def _q4(pool: torch.Tensor, dims: int = 4):
     if width % 18 or stride[-1] != 1 or (G > 1 and stride[-2] != width) or (
             KV > 1 and stride[-3] != G * width):
         _bad("each page of a 4-bit pool must be contiguous, 18 * D bytes per 16 rows of a head")
+    if P > 1 and stride[-4] < KV * G * width:
+        _bad("the pages of a pool must not overlap")
     return P, 16 * G, KV, width // 18, (stride[-4] if P > 1 else KV * G * width)
 
 
@@ -560,7 +565,7 @@ def tree_decode_q4(q: torch.Tensor, pool: torch.Tensor, lens: torch.Tensor, cu: 
     P, R, KV, D, page_bytes = _q4(pool)
     dt, qs = q.dtype, q.stride()
     n, H, Dq = q.shape
-    if not q.is_cuda or qs[2] != 1 or qs[1] != D or Dq != D:
+    if not q.is_cuda or qs[2] != 1 or qs[1] != D or Dq != D or (n > 1 and qs[0] < H * D):
         _bad("q must be a CUDA tensor (n, H, D), contiguous per token, as the pool's rows")
     B = lens.numel()
     _i32("lens", lens)

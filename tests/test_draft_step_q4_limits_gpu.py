@@ -39,3 +39,16 @@ def test_sampled_steps_read_the_rows_on_their_paths_only(cuda_dev, monkeypatch):
     assert len(calls) == 1 and got == [[35], [35]]
     s.verify([([t[-1]], [-1]) for t in got])
     assert len(calls) == 2
+
+
+def test_a_broadcast_draft_is_refused_before_the_step_takes_pages(cuda_dev):
+    from alpacca_open_sourced_by_jt_b200 import _lib
+    s = make(cuda_dev, "norm", requests=1, n_pages=8, page_rows=16, max_len=64, kv_bits=4)
+    last = s.prefill([list(range(15))])
+    state = (s.ring_state.tolist(), s.held.tolist(), s.lens.tolist())
+    tree = ([last[0], 5, 6], [-1, 0, 0])  # (its rows begin a page)
+    row = torch.full((1, s.m.V), 1 / s.m.V, device=cuda_dev)
+    with pytest.raises(_lib.B2AShapeError):
+        s.verify([tree], **numbers(cuda_dev, 3, 1, 0), draft=row.expand(3, -1))
+    assert state == (s.ring_state.tolist(), s.held.tolist(), s.lens.tolist())
+    assert len(s.verify([tree], **numbers(cuda_dev, 3, 1, 0), draft=row.repeat(3, 1))) == 1
