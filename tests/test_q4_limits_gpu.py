@@ -1,6 +1,6 @@
 """Attention over the 4-bit cache (paged.tree_decode_q4) at its limits, against 64 bits
 over the values that the pool stands for: rows of pages outside the pool, V blocks of
-unlike sizes beside one another.
+unlike sizes beside one another, long contexts in which every granule of 16 rows counts.
 
 Bounds (u the unit roundoff of the output's type, w = sum p |v|): u |out| for the output,
 half a step of the type's least numbers where that is more;
@@ -157,3 +157,52 @@ def test_blocks_of_unlike_sizes(cuda_dev, dt, D, H, nodes):
             np.clip(x, -6e4, 6e4, out=x)
         s = Batch(cuda_dev, dt, H, k, v, [nodes, nodes], 32, seed=3)
         s.check(*s.outputs())
+
+
+# ---- long contexts -------------------------------------------------------------------
+
+LONG = [  # D, H, KV, rows, nodes, page: query rows a KV head
+    (64, 8, 2, [20012, 3, 31007], [1, 1, 1], 16),       # 4
+    (128, 8, 2, [24577, 4096], [1, 1], 64),
+    (64, 8, 2, [20015, 9000], [4, 2], 32),              # 16
+    (128, 16, 2, [16385, 40], [8, 3], 16),              # 64: two lanes a row
+    (64, 8, 2, [20019, 3], [8, 1], 16),                 # 32: four
+    (128, 16, 2, [15000, 700], [16, 2], 128),           # 128: one
+    (256, 8, 2, [20001], [1], 64),
+    (256, 8, 2, [9001, 30], [5, 2], 16),                # 20, by blocks of 8
+]
+
+
+@pytest.mark.parametrize("D,H,KV,rows,nodes,page", LONG)
+def test_every_granule_of_a_long_context_counts(cuda_dev, D, H, KV, rows, nodes, page):
+    """V is zero but for one dim of each row, the granule's number modulo D: a granule that
+    were left out, or taken twice, would change a sum over some 20 to 150 of them, all of
+    one sign, by more than the bound's 1e-3 of it."""
+    from alpacca_open_sourced_by_jt_b200 import _lib
+    rng = np.random.default_rng(D + rows[0])
+    k = normal(rng, rows, KV, D)
+    v = []
+    for r in rows:
+        x = np.zeros((r, KV, D), np.float32)
+        x[np.arange(r), :, np.arange(r) // 16 % D] = -rng.uniform(0.5, 1.5, (r, KV))
+        v.append(x)
+    s = Batch(cuda_dev, "bf16" if D == 128 else "f16", H, k, v, nodes, page, seed=1)
+    out, lse = s.outputs()
+    s.check(out, lse)
+    assert (out[0] < -1e-5).all() and len({float(x) for x in s.vd[0].ravel()}) > 10
+    # the bound tells a lost granule: without any one of them some sum is off by more
+    q = s.q.double().cpu().numpy()
+    p = np.exp(s.kh[0][:, 0] @ q[0, 0] * s.scale)
+    p[s.lens[0] + 1:] = 0
+    p /= p.sum()
+    own = np.zeros(D)
+    part = np.add.reduceat(-p * s.vh[0][:, 0].sum(-1), np.arange(0, rows[0], 16))
+    np.add.at(own, np.arange(len(part)) % D, part)
+    whole = -(-(s.lens[0] + 1) // 16) - 1  # (granules of the prefix)
+    share = part[:whole] / own[np.arange(whole) % D]
+    small = rows[0] * 2.0 ** -21 * (p[:, None] * s.vd[0][:, 0]).max() / own.min()
+    assert share.min() > 2 * (UNIT[s.dt] + 2.0 ** -11 + 5e-4 + small), (share.min(), small)
+    for _ in range(5):  # and is the same, call after call
+        again = s.outputs()
+        assert np.array_equal(again[0], out) and np.array_equal(again[1], lse)
+    _lib.raise_device_error()

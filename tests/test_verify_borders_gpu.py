@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import q4_ref
-from tests.test_verify_gpu import run
+from tests.test_verify_gpu import make, run, wanted
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,21 @@ def test_what_is_left_of_a_long_sum(cuda_dev, dt, singles, side):
     picks, margin, drawn = q4_ref.verify(x, c["cu"], c["parents"], tokens, u, c["d"], None, None)
     assert margin > 9e-5 and drawn > 1e-11 and (picks[0] == at) == (side < 0)
     assert np.array_equal(run(cuda_dev, c, dt, max_nodes=3), picks)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("nodes", [[6], [20, 30, 4], [3] * 50])
+def test_stars_with_high_numbers(cuda_dev, draft, nodes):
+    """Children of a root, likely tokens, nearly all turned down: four cases whose
+    decisions are clear."""
+    seen = 0
+    for seed in range(200):
+        c = make(nodes, 400, "f32", draft, "star", np.random.default_rng(seed), agree=1.0)
+        c["u"] = np.maximum(c["u"], np.float32(0.9))
+        picks, margin, drawn = wanted(c)
+        if margin > 2e-5 and drawn > 1e-11:
+            assert np.array_equal(run(cuda_dev, c, "f32"), picks)
+            seen += 1
+            if seen == 4:
+                return
+    raise AssertionError(f"{seen} clear cases")
