@@ -447,6 +447,24 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           }
         }
         // ---- softmax ----------------------------------------------------------------
+        uint32_t shown = 0xfu;  // which of the lane's keys a row sees
+        if (tail) {
+          // keys that are not there, or that only some rows see, may hold anything
+          shown = 0u;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int j0 = row0 + 4 * t - it.len, at = j0 >> 5;  // tree row of the first key, its word
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(&sh.sees[warp][nt * 8 + g]);
+            const uint32_t w0 = at < 0 ? ~0u : at < kWords ? words[at] : 0u,
+                           w1 = at + 1 < 0 ? ~0u : at + 1 < kWords ? words[at + 1] : 0u;
+            const uint32_t vis = __funnelshift_r(w0, w1, j0 & 31);
+            if (!(vis & 1u)) s[nt][0].x = -INFINITY;
+            if (!(vis & 2u)) s[nt][0].y = -INFINITY;
+            if (!(vis & 4u)) s[nt][1].x = -INFINITY;
+            if (!(vis & 8u)) s[nt][1].y = -INFINITY;
+            shown |= vis;
+          }
+        }
         uint32_t dv[NB * 2];  // [key][block] f16
 #pragma unroll
         for (int i = 0; i < NB / 2; ++i) {
@@ -454,26 +472,9 @@ __global__ void __launch_bounds__(Q4Cfg<D, NT>::kThreads, 1) tree_q4_kernel(
           dv[4 * i] = u.x; dv[4 * i + 1] = u.y; dv[4 * i + 2] = u.z; dv[4 * i + 3] = u.w;
         }
         if (tail) {
-          // keys that are not there, or that only some rows see, may hold anything
-          uint32_t any = 0u;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int j0 = row0 + 4 * t - it.len, at = j0 >> 5;  // tree row of the first key, its word
-            uint32_t vis = 0xfu;
-            if (j0 > -4) {
-              const uint32_t* words = reinterpret_cast<const uint32_t*>(&sh.sees[warp][nt * 8 + g]);
-              const uint32_t w0 = at < 0 ? ~0u : at < kWords ? words[at] : 0u, w1 = at + 1 < kWords ? words[at + 1] : 0u;
-              vis = __funnelshift_r(w0, w1, j0 & 31);
-            }
-            if (!(vis & 1u)) s[nt][0].x = -INFINITY;
-            if (!(vis & 2u)) s[nt][0].y = -INFINITY;
-            if (!(vis & 4u)) s[nt][1].x = -INFINITY;
-            if (!(vis & 8u)) s[nt][1].y = -INFINITY;
-            any |= vis;
-          }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (!((any >> i) & 1u))
+            if (!((shown >> i) & 1u))
 #pragma unroll
               for (int b = 0; b < NB / 2; ++b) dv[i * (NB / 2) + b] = 0u;
         }
