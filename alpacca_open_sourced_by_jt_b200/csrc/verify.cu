@@ -16,19 +16,20 @@
 // Only rows on the path decide anything, so only those are read: a cluster of CTAs
 // walks one request, each CTA a slice of the vocabulary, and meets over
 // distributed shared memory once per row.  The decisions compare sums of 32-bit
-// exponentials: up to five multiplied (2^-22 each), arguments of three roundings, 4 or 8
-// added in 32 bits and those in 64, so that a weight e^-y is off by at most 2^-22 (7 + y)
-// of itself; where less than a sixteenth of such a sum is left, it is taken anew in 64
-// bits.  The draw and the residuals, whose outcome hangs on sums at borders some 10^-5
+// exponentials: up to five multiplied (2^-22 each), arguments of three roundings, 16 or 32
+// added in 32 bits (7 roundings deep) and those in 64, so that a sum of weights e^-y is
+// off by at most 2^-22 (7 + y) of each; where less than a sixteenth of such a sum is left,
+// it is taken anew in 64 bits.  The draw and the residuals, whose outcome hangs on sums at borders some 10^-5
 // apart, take 64-bit exponentials: another reading of the row, out of L2.
 //
 // Bound by latency, not by bytes: a row on a path takes some 7 us (2.5 of loads, 1.5 of
 // reductions and the cluster's barrier, 1.5 of the children), a 64-bit sum over it 10 to
 // 14 (chains of some 15 dependent operations a token, four side by side).  64 requests
-// with up to 31 nodes over 128256 f32 logits: 66 us for paths of up to 7 rows; 24 requests
-// with drafts' rows 67; one request of 4 nodes 9.6.  Not kept: the next loads or the
-// children's logits ahead of time (registers: 74 us instead of 66 for the 64), more
-// registers and fewer CTAs an SM (99).
+// with up to 31 nodes over 128256 f32 logits: 50 to 73 us, by the longest path, 60 on
+// average over eight draws of the inputs; 24 requests with drafts' rows 57 to 75, 65; one
+// request of 4 nodes 9 to 19.  With sums in 32 bits throughout 58 us for the 64.  Not kept:
+// the next loads or the children's logits ahead of time (registers: 12 % more for the 64),
+// more registers and fewer CTAs an SM (half as much again).
 
 #include <cooperative_groups.h>
 
@@ -174,6 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
     // of 2 above it, so that a row that rises in small steps does not round part at each.)
     float top = -INFINITY, ref = -INFINITY;
     double part = 0.0;
+    float some = 0.f;  // (of up to kLoads groups, then added to part)
     int place = a.V;
     {
       constexpr int kVec = 16 / sizeof(T), kLoads = 4;
@@ -184,7 +186,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
         if (m > top) {
           top = m;
           if ((m - ref) * cold2 > 1.f) {
-            part *= fast_exp2((ref - m) * cold2);
+            const float f = fast_exp2((ref - m) * cold2);
+            part *= f;
+            some *= f;
             ref = m;
           }
 #pragma unroll
@@ -192,10 +196,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
             if (x[e] == m) place = v + e * apart;
         }
         if (top > -INFINITY) {
-          float some = 0.f;
+          float y[kVec];
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) some += fast_exp2((x[e] - ref) * cold2);
-          part += some;
+          for (int e = 0; e < kVec; ++e) y[e] = fast_exp2((x[e] - ref) * cold2);
+#pragma unroll
+          for (int k = 1; k < kVec; k *= 2)
+#pragma unroll
+            for (int e = 0; e < kVec; e += 2 * k) y[e] += y[e + k];
+          some += y[0];
         }
       };
       if (reinterpret_cast<uintptr_t>(row) % 16 == 0) {  // (slices are whole groups)
@@ -217,6 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
               x[e] = fmaxf(ld_elem(reinterpret_cast<const T*>(&u[k]) + e), -INFINITY);
             take(x, v0 + i * kVec, 1);
           }
+          part += some;
+          some = 0.f;
         }
         for (int v = v0 + groups * kVec + tid; v < v1; v += kThreads) {
           float x[kVec];
@@ -225,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
           for (int e = 1; e < kVec; ++e) x[e] = -INFINITY;
           take(x, v, 1);
         }
+        part += some;
       } else {
         for (int v = v0 + tid; v < v1; v += kThreads * kVec) {
           float x[kVec];
@@ -232,6 +243,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) verify_kernel(const
           for (int e = 0; e < kVec; ++e)
             x[e] = v + e * kThreads < v1 ? fmaxf(at(row, v + e * kThreads), -INFINITY) : -INFINITY;
           take(x, v, kThreads);
+          part += some;
+          some = 0.f;
         }
       }
     }
@@ -684,15 +697,15 @@ int b2a_verify_picks(const void* logits, long long row_stride, int dtype, const 
   VF::Args a = {logits, row_stride, draft, draft_row_stride, cu_dev, parents_dev, tokens_dev, uniforms_dev,
                 draws_dev, temperature_dev, picks_dev, B, n_rows, max_nodes, V, 0, 0, 0, 0};
   // Few rows: a cluster for each, all at once, rather than node after node of a path, as
-  // long as all clusters are resident (rows of 128256 f32: 4 nodes of one request 9.6 us
-  // against 17.1, 8 of each of 4 26 against 27.5; of 8 requests 36 against 31).
+  // long as all clusters are resident (rows of 128256 f32: 4 nodes of one request 8.6 us
+  // against 14.8, 8 of each of 4 24.7 against 29.0; of 8 requests 36.7 against 28.8).
   a.all_nodes = n_rows > B && static_cast<long long>(n_rows) * VF::kCluster <= 2 * b2a_host::sm_count();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(dtype, [&](auto* t) {
     using T = typename std::remove_pointer<decltype(t)>::type;
     // Wider CTAs where all clusters are resident with them (2 of 512 threads an SM, 4 of
-    // 256): 24 requests with drafts' rows 84 us with 256 threads, 67 with 512, 37 requests
-    // 47 and 44, 64 requests 71 and 82.
+    // 256): 24 requests with drafts' rows 77 us with 256 threads, 65 with 512, 37 requests
+    // of 8 nodes 41 with either, 64 requests 52 and 64.
     const long long ctas = static_cast<long long>(a.all_nodes ? n_rows : B) * VF::kCluster;
     return ctas <= 2 * b2a_host::sm_count() ? verify_launch<T, 512>(a, st) : verify_launch<T, 256>(a, st);
   });

@@ -755,8 +755,8 @@ int b2a_tree_commit_q4(const int* picks_dev, const int* tokens_dev, const int* p
  * out of bounds) are -1, and where a row has no weight at all.  Where a residual
  * has none left (draft rows that do not sum to 1) the largest logit's v is
  * taken, and the path goes on to a child that has it.  Decisions: exponentials in
- * 32 bits (a weight e^-y is off by at most 2^-22 (7 + y) of itself), sums in 64; the
- * draw and residuals in 64. */
+ * 32 bits, their sums in 64 (a sum of weights e^-y is off by at most 2^-22 (7 + y) of
+ * each); the draw and residuals in 64. */
 int b2a_verify_picks(const void* logits, long long row_stride, int dtype, const float* draft,
                      long long draft_row_stride, const int* cu_dev, const int* parents_dev,
                      const int* tokens_dev, const float* uniforms_dev, const float* draws_dev,

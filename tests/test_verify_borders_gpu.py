@@ -66,8 +66,8 @@ def test_temperatures_small_against_the_logits_spacing(cuda_dev, many, draft):
 def test_what_is_left_of_a_long_sum(cuda_dev, dt, singles, side):
     """Two million like weights behind one that has 10 of 11 parts of the sum and is turned
     down; the next child's number lies 1e-4 of itself beside its share of what is left.
-    Weights e^-y may be off by 2^-22 (7 + y) of themselves: the large one, ten times what is
-    left, by 1.7e-5 of that, the others (y = 17) by 5.8e-6."""
+    A sum of weights e^-y is off by at most 2^-22 (7 + y) of each: for the large one, ten
+    times what is left, 1.7e-5 of that, for the others (y = 17) 5.8e-6."""
     V = 2000000
     at = 123456
     ratio = 0.3 / 1.3
