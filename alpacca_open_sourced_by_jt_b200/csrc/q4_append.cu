@@ -9,14 +9,14 @@
 // values next to a border.  Products and sums are rounded one by one, as
 // paged.cu does.
 //
-// Bound by reading the projections and writing q and the pool, and nearly as much by
-// instructions and L1's data path.  A thread takes eight pairs of a head, which it rotates
+// Bound by reading the projections and writing q and the pool, and nearly as much by the
+// latency of its instructions (55 % of the issue slots used, L1's data path 60 %).  A thread takes eight pairs of a head, which it rotates
 // by itself: 16 consecutive dims, or for neox rows 8 and the 8 that are half the rotation
 // further on, so two words of codes; D / 16 lanes a head (with 8 dims a thread the sum, the
 // root and the addresses of a head weigh twice as much).  It keeps its head over the tokens,
 // so that addresses and roles are found once: 8191 tokens, 32/8 heads x 128, bf16: 53 us
-// (3.8 TB/s), 72 with the heads in the inner loop; into 4 bits, 64 wide, and read back 37
-// us, 56.  Not kept: rows, cosines and sines through rings in shared memory (51 and 42 us).
+// (3.8 TB/s), 72 with the heads in the inner loop; into 4 bits, 64 wide, and read back 36
+// us (6 of them the reading back), 56.  Not kept: rows, cosines and sines through rings in shared memory (51 and 42 us).
 
 #include <cfloat>
 

@@ -6,8 +6,8 @@
 // converted: a code is a f16 subnormal as it stands in its word (mask, no
 // arithmetic), the block scales go onto f32 numbers.
 //   scores    S = Q.K^T on m16n8k16 MMAs, block by block of 32 dims:
-//             s += d_k[key][block] * (sum q c - 8 sum q), the second term as the
-//             MMA's initial accumulator.  Codes of odd word places are 16 times
+//             s += d_k[key][block] (sum q c) + d_k[key][block] (-8 sum q), two keys
+//             in an operation.  Codes of odd word places are 16 times
 //             larger (2^-20): q is 16 times smaller there.  Each row of q is
 //             scaled by a power of two to a largest element in [2^14, 2^15), so
 //             f16 holds bf16 q's too; elements 2^28 times smaller than the row's
@@ -34,12 +34,12 @@
 // pages have 16 rows, a step a lane.  The others take the steps in turn, each through a
 // ring of its own, so they meet only at an item's end.
 //
-// Bound by instructions and their latency, behind HBM by a factor of 1.7: some 175 of them
-// a granule at head_dim 64, 350 at 128, 3200 cycles for a step of two at 128 with 15 warps
-// at work.  16 x 32760 rows, 32/8 heads x 128, bf16: one node 160 us (3.8 TB/s; the 16-bit
-// cache's kernel takes 327), 16 query rows 265; x 64 112 us; 64 requests of 200 to 8000
-// rows x 64, pages of 16: 96 us, an item's end and begin (join, q, first data) 4 us each.
-// With each warp looking after its own copies 193 and 113 us.
+// Bound by latency with the 15 warps that the registers leave, behind HBM by a factor of
+// 1.7: 367 instructions a granule at head_dim 128 (28 of them MMAs), 52 % of the issue slots
+// used and no pipe above 36 %.  16 x 32760 rows, 32/8 heads x 128, bf16: one node 162 us (3.7
+// TB/s; the 16-bit cache's kernel takes 327), 16 query rows 270; x 64 103 us and 162; 64
+// requests of 200 to 8000 rows x 64, pages of 16: 94 us, an item's end and begin (join, q,
+// first data) 4 us each.  With each warp looking after its own copies a fifth more.
 #include <limits.h>
 #include <math.h>
 
@@ -78,7 +78,7 @@ struct Q4Cfg {
   static constexpr int NB = D / 32;
   static constexpr int kGranule = q4::granule_bytes(D);
   static constexpr int kStage = 2 * kGranule;
-  // (15 warps have 128 registers each, 7 have 255: one node 16 x 32760 rows 160 us and 214)
+  // (15 warps have 128 registers each, 7 have 255: one node 16 x 32760 rows 162 us and 209)
   static constexpr int kWarps = NT == 1 && D <= 128 ? 15 : 7;
   static constexpr int RB = 8 * NT;
   static constexpr int kPad = D + 4;
@@ -163,6 +163,7 @@ struct Q4Walk {
   }
 };
 
+// Zeros for a granule's scales: its rows are then zeros, whatever its codes.
 template <int D>
 __device__ __forceinline__ void q4_blank(uint8_t* granule) {
 #pragma unroll 1

@@ -14,11 +14,12 @@
 // keys), 25 owns TMEM and issues the MMAs.
 // TMEM: S0, S1 (128 columns each), O (D), Q (D / 2).
 //
-// Bound by instructions: a tile of 128 keys takes some 5700 of them with 32 rows, half for
+// Bound by instructions and the waits between them (54 % of the issue slots used, no pipe
+// above 40 %): a tile of 128 keys takes some 5700 with 32 rows, half for
 // the conversion, which a block of 128 rows repeats, half for the softmax.  16 x 32760
-// rows, 32/8 heads x 128: 32 rows 303 us (2.0 TB/s), 64 rows 366, 128 rows 454; 8 requests
-// of 9K to 16K rows, up to 512 query rows a KV head: 370 us, 450 TFLOP/s.  With converters
-// that bring their own steps 333 us for 32 rows.
+// rows, 32/8 heads x 128: 32 rows 302 us (2.0 TB/s), 64 rows 354, 128 rows 451; 8 requests
+// of 9K to 16K rows, up to 512 query rows a KV head: 366 us, 450 TFLOP/s.  With converters
+// that bring their own steps a tenth more for 32 rows.
 
 #include <limits.h>
 
@@ -722,11 +723,11 @@ __global__ void __launch_bounds__(kQWThreads, 1) tree_q4_wide_kernel(
 namespace {
 
 // Which kernel, by the most rows a KV head can have, and the rows of an item.  16 x 32760
-// rows, 32/8 heads x 128: 16 rows 291 us with warp-level MMAs, 330 on tcgen05; 32 rows
-// (two blocks of 16) 533 against 333.
+// rows, 32/8 heads x 128: 16 rows 270 us with warp-level MMAs, 299 on tcgen05; 32 rows
+// (two blocks of 16) 485 against 302.
 bool tree_q4_is_wide(int rows, int D) { return rows > 16 && D <= 128; }
-// (the wide kernel: as many lanes of 128 to a row as the most rows leave; 32 rows 440 us with
-// one lane to a row, 333 with four; 64 rows 452, with two 380)
+// (the wide kernel: as many lanes of 128 to a row as the most rows leave; 32 rows 428 us with
+// one lane to a row, 339 with two, 302 with four; 64 rows 439, with two 354)
 int tree_q4_rep(int rows) { return rows <= 32 ? 2 : rows <= 64 ? 1 : 0; }
 int tree_q4_rows(int rows, int D, int group) {
   if (tree_q4_is_wide(rows, D)) return (128 >> tree_q4_rep(rows)) / group * group;

@@ -655,7 +655,8 @@ int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* pare
  * step of the section above with a cache of 4 bits:
  *   b2a_page_plan          as above
  *   per layer: b2a_rope_append_q4, b2a_tree_decode_q4
- *   b2a_constrain_logits, then b2a_verify_picks where tokens are sampled
+ *   b2a_constrain_logits, then b2a_verify_picks where tokens are sampled (which needs
+ *                          the former for penalties, biases and masks only)
  *   b2a_tree_commit_q4     takes either's picks
  *
  * A 4-bit block is 32 consecutive values of a row: with m the value of largest
@@ -663,8 +664,11 @@ int b2a_tree_commit(const int* picks_dev, const int* tokens_dev, const int* pare
  *   d    = m / -8 rounded to 8 significant bits, within +-8160, kept as f16
  *   code = floor(x / d + 8.5) within 0 .. 15
  * it stands for d * (code - 8), which f16 holds exactly, half a step |d| / 2 from x
- * (up to a whole one at the end of the range, which has no code 16).  Values beyond
- * 65280 saturate; a block with a NaN has d = NaN and stands for NaN.
+ * (up to a whole one at the end of the range, which has no code 16) and what d's own
+ * rounding makes of it: 2^-8 of the value, where d is under f16's normal numbers up to
+ * 2^-22.  Values beyond 65280 saturate; a block with a NaN has d = NaN and stands for
+ * NaN.  (The rule is that of GGUF's Q4_0 blocks; the scale's bits, its range and the
+ * layout are not.)
  *
  * A 4-bit pool is [n_pages][KV][page_rows / 16] granules of 18 D bytes (K and V
  * of 16 rows of one head), pages page_bytes apart (0: dense), a multiple of 16;
@@ -708,8 +712,8 @@ int b2a_q4_rows(const void* pool, int n_pages, int page_rows, long long page_byt
                 void* k_out, void* v_out, int out_dtype, int n_tok, int KV, int D, void* stream);
 
 /* b2a_tree_decode over a 4-bit pool: q and out of dtype F16 or BF16.  f32 scores
- * (q is scaled by a power of two to f16, exact but for elements 2^28 times smaller
- * than their row's largest), sums and accumulators.  For the product with V the
+ * (q, up to 2^110, is scaled by a power of two to f16, exact but for elements 2^28 times
+ * smaller than their row's largest), sums and accumulators.  For the product with V the
  * weights are rounded to f16: off by 2^-12 of themselves, or by 2^-25 on a scale on
  * which the row's largest is 1/2 or more.  With up to 16 query rows a KV head (D 256:
  * any number) the weights times V's scales are, each block of 32 dims on a scale of its
