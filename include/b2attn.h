@@ -711,13 +711,15 @@ int b2a_rope_append_q4(const void* q, long long q_tok_stride, const void* k, lon
 int b2a_q4_rows(const void* pool, int n_pages, int page_rows, long long page_bytes, const int* slot_dev,
                 void* k_out, void* v_out, int out_dtype, int n_tok, int KV, int D, void* stream);
 
-/* b2a_tree_decode over a 4-bit pool: q and out of dtype F16 or BF16.  f32 scores
- * (q, up to 2^110, is scaled by a power of two to f16, exact but for elements 2^28 times
- * smaller than their row's largest), sums and accumulators.  For the product with V the
+/* b2a_tree_decode over a 4-bit pool: q and out of dtype F16 or BF16.  f32 scores,
+ * sums and accumulators.  q, up to 2^110, is scaled by a power of two to f16, exact but
+ * for elements 2^28 times smaller than their row's largest.  For the product with V the
  * weights are rounded to f16: off by 2^-12 of themselves, or by 2^-25 on a scale on
  * which the row's largest is 1/2 or more.  With up to 16 query rows a KV head (D 256:
- * any number) the weights times V's scales are, each block of 32 dims on a scale of its
- * own.  Rows of a page outside the pool (recorded) stand as zeros, as they do in
+ * any number) codes go into the products as f16 subnormals, of whose sums the MMAs
+ * keep fewer bits: 2^-13 of sum w d, w the weights or |q|, d the blocks' scales; the
+ * weights are rounded times V's scales, each block of 32 dims on a scale of its own.
+ * Rows of a page outside the pool (recorded) stand as zeros, as they do in
  * b2a_tree_decode: score 0, and their share of the sum. */
 size_t b2a_tree_decode_q4_workspace_bytes(int max_nodes, int H, int KV, int D, int max_len);
 int b2a_tree_decode_q4(const void* q, long long q_tok_stride, const void* pool, int n_pages,

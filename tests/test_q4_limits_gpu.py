@@ -159,6 +159,31 @@ def test_blocks_of_unlike_sizes(cuda_dev, dt, D, H, nodes):
         s.check(*s.outputs())
 
 
+@pytest.mark.parametrize("D,H,nodes", [(64, 8, 1), (128, 8, 4), (256, 8, 1), (256, 4, 3), (128, 8, 16)])
+def test_dims_without_values(cuda_dev, D, H, nodes):
+    """Every other dim's codes stand for 0 in blocks with large scales.  With few query rows
+    codes are f16 subnormals c 2^-24 or c 2^-20: an MMA lines its products up by the encoded
+    exponent 2^-14 and keeps 23 bits of that, 2^-13 or 2^-17 of sum w in codes; 8 sum w, of
+    normal numbers, is taken off: 2^-13 of sum p d in all, a tenth more for the accumulators'
+    own 24 bits.  With more rows the cache's values are multiplied: 0."""
+    for rows in (9 + nodes, 41, 300, 3000):
+        rng = np.random.default_rng(rows)
+        k, v = normal(rng, [rows], 2, D), normal(rng, [rows], 2, D)
+        v[0][..., 1::2] = 0
+        v[0][..., ::32] = 8 * rng.uniform(1, 2, (rows, 2, D // 32))
+        s = Batch(cuda_dev, "bf16", H, k, v, [nodes], 16, seed=rows)
+        assert (s.vh[0][..., 1::2] == 0).all()
+        out, lse = s.outputs()
+        q, group = s.q.double().cpu().numpy(), H // 2
+        for i in range(nodes):
+            at = list(range(s.lens[0])) + [s.lens[0] + j for j in ref.chain_of(s.parents, i)]
+            for h in range(H):
+                p = np.exp(s.kh[0][at, h // group] @ q[i, h] * s.scale)
+                much = ((p / p.sum()) @ s.vd[0][at, h // group]).repeat(32)[1::2]
+                room = 0 if nodes * group > 16 and D < 256 else 1.1 * 2.0 ** -13
+                assert (np.abs(out[i, h, 1::2]) <= room * much).all()
+
+
 # ---- long contexts -------------------------------------------------------------------
 
 LONG = [  # D, H, KV, rows, nodes, page: query rows a KV head
