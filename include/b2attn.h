@@ -750,7 +750,7 @@ int b2a_tree_commit_q4(const int* picks_dev, const int* tokens_dev, const int* p
  * depend on the random numbers, and with draft each child was drawn
  * independently from its parent's row.
  *   logits     [n_rows][V] F32, F16 or BF16, rows row_stride apart; -inf and NaN
- *              have weight 0
+ *              have weight 0, and so has what is under e^-690 of the largest
  *   draft      f32 [n_rows][V] probabilities, draft_row_stride apart, or NULL
  *   tokens     int32 [n_rows] the nodes' tokens; one outside [0, V) is passed over
  *   uniforms   f32 [n_rows] in [0, 1): a node's own (node 0's is not used)
